@@ -15,10 +15,17 @@ p = i + (n_k - n_q) (queries end where the keys end), and delta = p - j.
 
 import functools
 import math
+import os
+import sys
 
 import torch
 
 own = False
+
+# the package's root, as tests and examples put it on the path
+PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "deepfold-linear_b200")
+if PACKAGE not in sys.path:
+    sys.path.insert(0, PACKAGE)
 
 TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 
