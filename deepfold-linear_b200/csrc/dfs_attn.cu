@@ -1,0 +1,134 @@
+// dfs_attn.cu -- C entry points of the local attention (include/dfsink.h):
+// argument checks, workspace layout and the choice of kernels.
+#include <cmath>
+
+#include "dfs_attn.cuh"
+
+using namespace dfs;
+
+namespace {
+
+constexpr int kMaxHeadDim = 64;
+constexpr int kMaxRows = 1 << 28;   // positions and distances stay inside 32 bits
+constexpr int kWindowAll = 1 << 30;
+
+bool type_ok(int t) { return t == DFS_BF16 || t == DFS_F16 || t == DFS_F32; }
+
+// DFS_OK, or why the problem cannot run
+int problem_status(const dfs_attn_problem* p, const dfs_relbias* b) {
+  if (!p || p->B < 0 || p->H < 0 || p->H_kv < 0 || p->n_q < 0 || p->n_k < 0 || p->d < 1 || !type_ok(p->dtype) ||
+      p->window < 0 || p->sinks < 0 || !std::isfinite(p->scale))
+    return DFS_ERR_INVALID_ARGUMENT;
+  if (p->H > 0 && (p->H_kv == 0 || p->H % p->H_kv != 0)) return DFS_ERR_INVALID_ARGUMENT;
+  if (b && b->weight &&
+      (!b->lut || b->num_buckets < 1 || b->max_distance < 0 || b->max_distance > DFS_MAX_BUCKET_DISTANCE ||
+       !type_ok(b->dtype)))
+    return DFS_ERR_INVALID_ARGUMENT;
+  if (p->d > kMaxHeadDim || p->n_q > kMaxRows || p->n_k > kMaxRows || p->q_start > kMaxRows ||
+      p->q_start < -kMaxRows || p->B > 65535 || p->H > 65535)
+    return DFS_ERR_UNSUPPORTED;
+  return DFS_OK;
+}
+
+Strided strided(const dfs_strided& s) { return {static_cast<char*>(s.ptr), s.stride_b, s.stride_h, s.stride_n}; }
+
+AttnParams params(const dfs_attn_problem* p, const dfs_attn_args* a) {
+  AttnParams P = {};
+  P.q = strided(a->q);
+  P.k = strided(a->k);
+  P.v = strided(a->v);
+  P.o = strided(a->o);
+  P.d_o = strided(a->d_o);
+  P.d_q = strided(a->d_q);
+  P.d_k = strided(a->d_k);
+  P.d_v = strided(a->d_v);
+  P.lse = a->lse;
+  P.mask = a->mask;
+  P.w = a->bias.weight;
+  P.lut = a->bias.lut;
+  P.nb = a->bias.num_buckets;
+  P.D = a->bias.weight ? a->bias.max_distance : 0;
+  P.wdtype = a->bias.dtype;
+  P.status = a->status;
+  P.B = p->B;
+  P.H = p->H;
+  P.Hkv = p->H_kv;
+  P.G = p->H_kv > 0 ? p->H / p->H_kv : 1;
+  P.nq = p->n_q;
+  P.nk = p->n_k;
+  P.d = p->d;
+  P.causal = p->causal != 0;
+  P.window = p->window == 0 ? kWindowAll : p->window < kWindowAll ? p->window : kWindowAll;
+  P.sinks = p->sinks;
+  P.qs = p->q_start;
+  P.scale = p->scale;
+  P.scale2 = p->scale * kLog2e;
+  return P;
+}
+
+size_t round256(size_t x) { return (x + 255) / 256 * 256; }
+size_t dsum_bytes(const dfs_attn_problem* p) {
+  return round256(sizeof(float) * static_cast<size_t>(p->B) * p->H * p->n_q);
+}
+int dw_parts(const dfs_attn_problem* p) {
+  const int t = attn_q_tile(p->dtype);
+  return p->B * ((p->n_q + t - 1) / t);
+}
+int rc(cudaError_t e) { return e == cudaSuccess ? DFS_OK : DFS_ERR_CUDA; }
+
+}  // namespace
+
+extern "C" int dfs_window_attn_fwd(const dfs_attn_problem* p, const dfs_attn_args* a, void* stream) {
+  if (!a) return DFS_ERR_INVALID_ARGUMENT;
+  const int s = problem_status(p, &a->bias);
+  if (s != DFS_OK) return s;
+  if (p->B == 0 || p->H == 0 || p->n_q == 0) return DFS_OK;
+  if (!a->q.ptr || !a->o.ptr || (p->n_k > 0 && (!a->k.ptr || !a->v.ptr))) return DFS_ERR_INVALID_ARGUMENT;
+  return rc(launch_attn_simt_fwd(params(p, a), p->dtype, static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" size_t dfs_window_attn_bwd_work(const dfs_attn_problem* p, const dfs_relbias* b) {
+  if (problem_status(p, b) != DFS_OK) return 0;
+  size_t n = dsum_bytes(p);
+  if (b && b->weight) n += sizeof(float) * static_cast<size_t>(p->H) * dw_parts(p) * (2 * b->max_distance + 1);
+  return n;
+}
+
+extern "C" int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_args* a, void* work, size_t work_bytes,
+                                   void* stream) {
+  if (!a) return DFS_ERR_INVALID_ARGUMENT;
+  const int s = problem_status(p, &a->bias);
+  if (s != DFS_OK) return s;
+  if (p->B == 0 || p->H == 0) return DFS_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool dw = a->d_weight != nullptr && a->bias.weight != nullptr;
+  if (a->d_weight && !a->bias.weight) return DFS_ERR_INVALID_ARGUMENT;
+  if ((p->n_q > 0 && (!a->q.ptr || !a->o.ptr || !a->d_o.ptr || !a->d_q.ptr || !a->lse || !work)) ||
+      (p->n_k > 0 && (!a->k.ptr || !a->v.ptr || !a->d_k.ptr || !a->d_v.ptr)))
+    return DFS_ERR_INVALID_ARGUMENT;
+  if (work_bytes < dfs_window_attn_bwd_work(p, dw ? &a->bias : nullptr)) return DFS_ERR_WORKSPACE;
+  AttnParams P = params(p, a);
+  P.dsum = static_cast<float*>(work);
+  if (dw) P.dw_part = reinterpret_cast<float*>(static_cast<char*>(work) + dsum_bytes(p));
+  if (p->n_q > 0 || p->n_k > 0) {
+    const int r = rc(launch_attn_simt_bwd(P, p->dtype, st));
+    if (r != DFS_OK) return r;
+  }
+  if (!dw) return DFS_OK;
+  return rc(launch_bucket_sums(P.dw_part, p->H, dw_parts(p), P.D, P.lut, P.nb, P.wdtype, a->d_weight, st));
+}
+
+extern "C" int dfs_window_attn_decode(const dfs_attn_problem* p, const dfs_attn_args* a, const int32_t* lengths,
+                                      void* stream) {
+  if (!a) return DFS_ERR_INVALID_ARGUMENT;
+  const int s = problem_status(p, &a->bias);
+  if (s != DFS_OK) return s;
+  if (p->n_q != 1) return DFS_ERR_INVALID_ARGUMENT;
+  if (p->B == 0 || p->H == 0) return DFS_OK;
+  if (!a->q.ptr || !a->o.ptr || !lengths || (p->n_k > 0 && (!a->k.ptr || !a->v.ptr))) return DFS_ERR_INVALID_ARGUMENT;
+  AttnParams P = params(p, a);
+  P.causal = 1;
+  P.mask = nullptr;
+  P.lengths = lengths;
+  return rc(launch_decode(P, p->dtype, static_cast<cudaStream_t>(stream)));
+}

@@ -1,0 +1,90 @@
+// dfs_attn.cuh -- what the local-attention kernels share: launch parameters, the
+// rule of which key a query sees, element types, and the expanded bias table.
+#pragma once
+
+#include "dfs_device.cuh"
+
+namespace dfs {
+
+struct Strided {
+  char* p;              // element (b, h, n, c) at p + (b sb + h sh + n sn + c) * size
+  int64_t sb, sh, sn;   // in elements; 64 bits: a long cache passes 2^31 elements
+};
+
+struct AttnParams {
+  Strided q, k, v, o, d_o, d_q, d_k, d_v;
+  float* lse;           // (B,H,n_q) log2 units, +inf for a row that sees nothing
+  float* dsum;          // (B,H,n_q) D_i = sum_c dO_ic O_ic (backward workspace)
+  const uint8_t* mask;  // (B,n_k) or null
+  const void* w;        // (H, nb) bias weights of type wdtype, or null
+  const int32_t* lut;   // (2 D + 1)
+  float* dw_part;       // (H, parts, 2 D + 1) sums of dS by distance, or null
+  int32_t* status;
+  const int32_t* lengths;  // decode: (B,)
+  int nb, D, wdtype;
+  int B, H, Hkv, G, nq, nk, d;
+  int causal, window, sinks, qs;
+  float scale, scale2;  // scale; scale * log2(e)
+};
+
+// Visible apart from the mask.  A window of "all" is INT_MAX/2 by the host.
+DFS_DEV bool key_near(int delta, int j, int causal, int window, int sinks) {
+  if (causal ? delta < 0 : false) return false;
+  return (delta < window && -delta < window) || j < sinks;
+}
+
+// Keys [lo, hi) that positions p0..p1 may see through the window (sinks apart).
+DFS_DEV void near_keys(const AttnParams& P, int p0, int p1, int& lo, int& hi) {
+  lo = max(0, p0 - P.window + 1);
+  hi = P.causal ? min(P.nk, p1 + 1) : min(P.nk, p1 + P.window);
+  hi = max(hi, 0);
+  lo = min(lo, hi);
+}
+// Sink keys [0, n) that the last position p1 may see.
+DFS_DEV int sink_keys(const AttnParams& P, int p1) {
+  const int n = P.causal ? min(P.sinks, p1 + 1) : P.sinks;
+  return max(0, min(n, P.nk));
+}
+
+template <typename T>
+DFS_DEV float to_f32(T x);
+template <>
+DFS_DEV float to_f32<float>(float x) { return x; }
+template <>
+DFS_DEV float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+DFS_DEV float to_f32<__half>(__half x) { return __half2float(x); }
+template <typename T>
+DFS_DEV T from_f32(float x);
+template <>
+DFS_DEV float from_f32<float>(float x) { return x; }
+template <>
+DFS_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16(x); }
+template <>
+DFS_DEV __half from_f32<__half>(float x) { return __float2half(x); }
+
+template <typename T>
+DFS_DEV T* row_ptr(const Strided& s, int b, int h, int64_t n) {
+  return reinterpret_cast<T*>(s.p) + b * s.sb + h * s.sh + n * s.sn;
+}
+
+// tab[delta + D] = weight[h, lut[delta + D]] * mul for the whole table (a block's threads).
+DFS_DEV void load_bias_table(float* tab, const void* w, const int32_t* lut, int D, int nb, int wdtype, int h,
+                             float mul, int tid, int nthreads) {
+  for (int x = tid; x < 2 * D + 1; x += nthreads) {
+    const int b = min(max(lut[x], 0), nb - 1);
+    tab[x] = load_as_f32<void>(w, static_cast<size_t>(h) * nb + b, wdtype) * mul;
+  }
+}
+
+constexpr int kBucketThreads = 512;
+
+// launchers (host)
+cudaError_t launch_bucket_sums(const float* part, int H, int parts, int D, const int32_t* lut, int nb, int dtype,
+                               void* out, cudaStream_t st);
+cudaError_t launch_attn_simt_fwd(const AttnParams& P, int dtype, cudaStream_t st);
+cudaError_t launch_attn_simt_bwd(const AttnParams& P, int dtype, cudaStream_t st);
+cudaError_t launch_decode(const AttnParams& P, int dtype, cudaStream_t st);
+int attn_q_tile(int dtype);  // query rows of one entry of dw_part
+
+}  // namespace dfs

@@ -29,6 +29,7 @@
 #include <string>
 #include <vector>
 
+#include "dfs_torch.h"
 #include "dfsink.h"
 
 namespace {
@@ -36,25 +37,7 @@ namespace {
 using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-
-// Errors are thrown as std::runtime_error (pybind11 raises RuntimeError) with
-// the message built here: a TORCH_CHECK whose message formats a number crashed
-// the process in this torch build, inside any extension.
-[[noreturn]] void fail(const std::string& msg) { throw std::runtime_error(msg); }
-void require(bool ok, const char* msg) {
-  if (!ok) fail(msg);
-}
-
-void check_rc(int rc, const char* what) {
-  if (rc != DFS_OK)
-    fail(std::string(what) + " failed: " + dfs_status_string(rc) + " (code " + std::to_string(rc) + ")");
-}
-
-int dtype_code(at::ScalarType t) {
-  if (t == at::kBFloat16) return DFS_BF16;
-  if (t == at::kHalf) return DFS_F16;
-  return DFS_F32;
-}
+using namespace dfs_torch;
 
 Tensor f32(const c10::optional<Tensor>& t) {
   if (!t.has_value() || !t->defined()) return Tensor();
@@ -73,22 +56,6 @@ std::vector<Tensor>& last_report() {
   static auto* r = new std::vector<Tensor>();
   return *r;
 }
-
-// Makes a device current for a scope and restores the previous one, with the
-// plain runtime calls.
-struct DeviceSwitch {
-  int prev = -1;
-  explicit DeviceSwitch(const at::Device& dev) {
-    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev != dev.index()) cudaSetDevice(dev.index());
-  }
-  ~DeviceSwitch() {
-    int cur = -1;
-    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-  }
-  DeviceSwitch(const DeviceSwitch&) = delete;
-  DeviceSwitch& operator=(const DeviceSwitch&) = delete;
-};
 
 // ---------------------------------------------------------------- device status
 // One sticky int32 status word per device: every forward and backward call
@@ -173,8 +140,9 @@ void check_device_status(const at::Device& dev) { g_seen.fetch_or(poll_device_st
 // For Python: the status bits of the current device (see poll_device_status)
 // together with the bits kept by the checks inside calls; all are cleared.
 int take_status(bool wait) {
-  const int v = poll_device_status(at::Device(at::kCUDA, c10::cuda::current_device()), wait);
-  return v | g_seen.exchange(0);
+  const at::Device dev(at::kCUDA, c10::cuda::current_device());
+  const int v = poll_device_status(dev, wait);
+  return v | g_seen.exchange(0) | attn_take_status(dev);
 }
 
 // DFS_TERM_* bits of the optional inputs a call passes (the streamed kernels
@@ -754,6 +722,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("compute_bins", &compute_bins_cuda, "compute_bins of the reference on the device: (B, N, N) int32");
   m.def("balanced_transport", &balanced_transport_autograd,
         "BalancedTransportFn.apply: returns [x_centroid], or [x_centroid, h_centroid] with V");
+  bind_window_attn(m);
   m.def("last_report", []() { return last_report(); },
         "[report (2, B*H) int32: CG iterations, then the residuals' fp32 bits; status, fwd_status] of the most "
         "recent backward (status: the device's sticky status word, the OR of every call's bits since the last "

@@ -24,8 +24,8 @@ LIB_DIR = os.path.join(PKG_DIR, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libdfsink.so")
 SOURCES = ["dfs_abi.cu", "dfs_fwd.cu", "dfs_bwd.cu", "dfs_stream.cu", "dfs_stream_bwd.cu", "dfs_stream_tma.cu",
            "dfs_stream_bwd_tma.cu", "dfs_selftest.cu", "dfs_noalloc.cu", "dfs_pad.cu", "dfs_dense.cu",
-           "dfs_dense_grad.cu", "dfs_peer.cu"]
-HEADERS = ["dfs_device.cuh", "dfs_kernels.cuh", "dfs_slab.cuh", "dfs_tma.cuh"]
+           "dfs_dense_grad.cu", "dfs_peer.cu", "dfs_relbias.cu", "dfs_attn_simt.cu", "dfs_attn.cu"]
+HEADERS = ["dfs_device.cuh", "dfs_kernels.cuh", "dfs_slab.cuh", "dfs_tma.cuh", "dfs_attn.cuh"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-Xcompiler", "-fPIC"]
@@ -78,6 +78,30 @@ class DfsBwdArgs(ctypes.Structure):
         "chain_id", "global_idx", "bond_matrix")]
 
 
+class DfsRelBias(ctypes.Structure):
+    _fields_ = [("weight", _P), ("lut", _P), ("num_buckets", ctypes.c_int32), ("max_distance", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+DFS_MAX_BUCKET_DISTANCE = 1024
+
+
+class DfsAttnProblem(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "H", "H_kv", "n_q", "n_k", "d", "dtype", "causal", "window",
+                                              "sinks", "q_start")] + [("scale", ctypes.c_float)]
+
+
+class DfsStrided(ctypes.Structure):
+    _fields_ = [("ptr", _P), ("stride_b", ctypes.c_int64), ("stride_h", ctypes.c_int64),
+                ("stride_n", ctypes.c_int64)]
+
+
+class DfsAttnArgs(ctypes.Structure):
+    _fields_ = [("q", DfsStrided), ("k", DfsStrided), ("v", DfsStrided), ("o", DfsStrided), ("lse", _P),
+                ("mask", _P), ("bias", DfsRelBias), ("d_o", DfsStrided), ("d_q", DfsStrided),
+                ("d_k", DfsStrided), ("d_v", DfsStrided), ("d_weight", _P), ("status", _P)]
+
+
 class DfsIpcHandle(ctypes.Structure):
     _fields_ = [("bytes", ctypes.c_ubyte * 64)]
 
@@ -95,7 +119,9 @@ EXPORTED_SYMBOLS = ("dfs_abi_version", "dfs_status_string", "dfs_max_n", "dfs_wo
                     "dfs_peer_alloc", "dfs_peer_open", "dfs_peer_close", "dfs_peer_free", "dfs_stream_op_peer",
                     "dfs_compute_bins", "dfs_peer_gather_rows", "dfs_stream_cg_loop_peer",
                     "dfs_dense_iterate", "dfs_dense_work_bytes", "dfs_dense_solve_bwd", "dfs_dense_solve_bwd_scratch",
-                    "dfs_dense_transport_bwd")
+                    "dfs_dense_transport_bwd", "dfs_relbias_fwd", "dfs_relbias_bwd", "dfs_relbias_bwd_work",
+                    "dfs_window_attn_fwd", "dfs_window_attn_bwd", "dfs_window_attn_bwd_work",
+                    "dfs_window_attn_decode")
 
 # phases of the streamed path for row-sharded runs (include/dfsink.h)
 DFS_OP_FWD_INIT, DFS_OP_FWD_ROWS, DFS_OP_FWD_COLS, DFS_OP_FWD_OUT = 0, 1, 2, 3
@@ -164,7 +190,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
 
 TORCH_EXT_NAME = "dfsink_torch"
 TORCH_EXT_PATH = os.path.join(LIB_DIR, TORCH_EXT_NAME + ".so")
-TORCH_EXT_SOURCE = os.path.join(CSRC_DIR, "dfs_torch.cpp")
+TORCH_EXT_SOURCES = [os.path.join(CSRC_DIR, f) for f in ("dfs_torch.cpp", "dfs_torch_attn.cpp")]
 _ext = None
 
 
@@ -172,7 +198,7 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     """Compile the native autograd glue (``dfsink_torch.so``, linked to
     ``libdfsink.so``) into the package with torch's extension builder."""
     build_library(verbose=verbose)
-    deps = [TORCH_EXT_SOURCE, LIB_PATH, os.path.join(INCLUDE_DIR, "dfsink.h")]
+    deps = TORCH_EXT_SOURCES + [os.path.join(CSRC_DIR, "dfs_torch.h"), LIB_PATH, os.path.join(INCLUDE_DIR, "dfsink.h")]
     if (not force and os.path.exists(TORCH_EXT_PATH)
             and all(os.path.getmtime(f) <= os.path.getmtime(TORCH_EXT_PATH) for f in deps)):
         return TORCH_EXT_PATH
@@ -183,7 +209,7 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     # the extension finds libdfsink.so beside itself ($ORIGIN, escaped for ninja ("$$") and
     # for the shell that runs the link ("\\$"))
     ldflags = [f"-L{LIB_DIR}", "-ldfsink", "-Wl,-rpath,\\$$ORIGIN:\\$$ORIGIN/.."]
-    cpp_extension.load(name=TORCH_EXT_NAME, sources=[TORCH_EXT_SOURCE], extra_include_paths=[INCLUDE_DIR],
+    cpp_extension.load(name=TORCH_EXT_NAME, sources=TORCH_EXT_SOURCES, extra_include_paths=[INCLUDE_DIR],
                        extra_cflags=["-O2"], extra_ldflags=ldflags, build_directory=bdir, with_cuda=True,
                        verbose=verbose, is_python_module=True)
     tmp = TORCH_EXT_PATH + ".tmp.%d" % os.getpid()
@@ -280,6 +306,21 @@ def lib() -> ctypes.CDLL:
             L.dfs_dense_transport_bwd.argtypes = [_I, _I, _I] + [_P] * 5
             L.dfs_compute_bins.restype = ctypes.c_int
             L.dfs_compute_bins.argtypes = [ctypes.c_int, ctypes.c_int, _P, _P, _P, _P, _P]
+            _RB, _AP, _AA = ctypes.POINTER(DfsRelBias), ctypes.POINTER(DfsAttnProblem), ctypes.POINTER(DfsAttnArgs)
+            L.dfs_relbias_fwd.restype = ctypes.c_int
+            L.dfs_relbias_fwd.argtypes = [_I, _I, _I, _I, _RB, _P, _P]
+            L.dfs_relbias_bwd_work.restype = ctypes.c_size_t
+            L.dfs_relbias_bwd_work.argtypes = [_I, _I, _I, _RB]
+            L.dfs_relbias_bwd.restype = ctypes.c_int
+            L.dfs_relbias_bwd.argtypes = [_I, _I, _I, _I, _RB, _P, _P, _P, ctypes.c_size_t, _P]
+            L.dfs_window_attn_fwd.restype = ctypes.c_int
+            L.dfs_window_attn_fwd.argtypes = [_AP, _AA, _P]
+            L.dfs_window_attn_bwd_work.restype = ctypes.c_size_t
+            L.dfs_window_attn_bwd_work.argtypes = [_AP, _RB]
+            L.dfs_window_attn_bwd.restype = ctypes.c_int
+            L.dfs_window_attn_bwd.argtypes = [_AP, _AA, _P, ctypes.c_size_t, _P]
+            L.dfs_window_attn_decode.restype = ctypes.c_int
+            L.dfs_window_attn_decode.argtypes = [_AP, _AA, _P, _P]
             L.dfs_selftest_mma.restype = ctypes.c_int
             L.dfs_selftest_mma.argtypes = [ctypes.c_int, _P, _P, _P, ctypes.c_int, ctypes.c_int,
                                            ctypes.c_int, _P]

@@ -405,6 +405,77 @@ int dfs_stream_cg_loop_peer(const dfs_problem* p, const dfs_cg_params* cg, const
                             int row_end, void* workspace, size_t workspace_bytes, const dfs_peer_set* peers,
                             size_t counter_offset, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Local softmax attention with a learned relative position bias.
+ *
+ * A query i stands at position p = i + q_start, a key j at position j; delta =
+ * p - j.  The bias of a pair is weight[h, lut[clamp(delta, -D, D) + D]] with D =
+ * max_distance: `lut` holds the bucket of every distance, the ends stand for all
+ * distances beyond them.
+ * --------------------------------------------------------------------------- */
+#define DFS_MAX_BUCKET_DISTANCE 1024
+typedef struct {
+  const void* weight;      /* (H, num_buckets) of `dtype`, or NULL: no bias             */
+  const int32_t* lut;      /* (2 max_distance + 1) buckets in [0, num_buckets), device  */
+  int32_t num_buckets;
+  int32_t max_distance;    /* 0 .. DFS_MAX_BUCKET_DISTANCE                              */
+  int32_t dtype;           /* DFS_BF16 / DFS_F16 / DFS_F32                              */
+  int32_t reserved;
+} dfs_relbias;
+
+/* bias[h, i, j] (H, n_q, n_k) of the weight's type, dense row-major. */
+int dfs_relbias_fwd(int H, int n_q, int n_k, int q_start, const dfs_relbias* b, void* out, void* stream);
+/* d_weight (H, num_buckets) of the weight's type from d_bias (H, n_q, n_k) of the same type, dense
+ * row-major: sums in fp32 and in a fixed order.  b->weight may be NULL.  work: dfs_relbias_bwd_work bytes. */
+size_t dfs_relbias_bwd_work(int H, int n_q, int n_k, const dfs_relbias* b);
+int dfs_relbias_bwd(int H, int n_q, int n_k, int q_start, const dfs_relbias* b, const void* d_bias, void* d_weight,
+                    void* work, size_t work_bytes, void* stream);
+
+/* A key is visible to a query when its mask byte is nonzero, it is not in the
+ * future (causal: delta >= 0), and it is near (causal: delta < window; else
+ * |delta| < window) or one of the first `sinks` keys.  o = softmax over the
+ * visible keys of (scale q.k + bias) times v; a query that sees no key gives 0.
+ * Keys hidden by the mask are never used, whatever they hold; keys hidden by
+ * the window or by causality must be finite. */
+typedef struct {
+  int32_t B, H, H_kv;      /* query heads; key / value heads (H % H_kv == 0)            */
+  int32_t n_q, n_k, d;     /* 1 <= d <= 64                                              */
+  int32_t dtype;           /* of q, k, v, o and their gradients                         */
+  int32_t causal;          /* nonzero: delta >= 0 only                                  */
+  int32_t window;          /* > 0, or 0: every key is near                              */
+  int32_t sinks;           /* >= 0                                                      */
+  int32_t q_start;         /* position of query 0 (n_k - n_q: both end together)        */
+  float scale;             /* of q.k                                                    */
+} dfs_attn_problem;
+
+typedef struct {           /* (B, heads, n, d) with unit stride along d; strides in elements */
+  void* ptr;
+  int64_t stride_b, stride_h, stride_n;
+} dfs_strided;
+
+typedef struct {
+  dfs_strided q, k, v, o;
+  float* lse;              /* (B,H,n_q): log2 of the row's sum (+inf: no visible key); written  */
+                           /* by the forward unless NULL, read by the backward                  */
+  const uint8_t* mask;     /* (B,n_k) 1 = real key, 0 = hidden; or NULL                         */
+  dfs_relbias bias;
+  /* backward only: gradients of o (in) and of q, k, v, bias.weight (out; d_weight may be NULL) */
+  dfs_strided d_o, d_q, d_k, d_v;
+  void* d_weight;
+  int32_t* status;         /* device int32, error bits OR-ed in; or NULL                        */
+} dfs_attn_args;
+
+int dfs_window_attn_fwd(const dfs_attn_problem* p, const dfs_attn_args* a, void* stream);
+/* Bytes of device workspace of the backward (0 for invalid problems). */
+size_t dfs_window_attn_bwd_work(const dfs_attn_problem* p, const dfs_relbias* b);
+int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_args* a, void* work, size_t work_bytes, void* stream);
+
+/* The newest token of each sequence over a cache: n_q = 1, causal, and query b
+ * stands at position lengths[b] - 1 (int32, device; clamped to [0, n_k]; 0 gives 0).
+ * Reads the cache rows of the sinks and the window only; causal, q_start, lse,
+ * mask and the gradients are ignored. */
+int dfs_window_attn_decode(const dfs_attn_problem* p, const dfs_attn_args* a, const int32_t* lengths, void* stream);
+
 /* TEST-ONLY entry point, not part of the operator surface: runs one of the
  * three tcgen05 MMA operand layouts the kernels use on caller-provided data
  * (D = A B^T, M = 64), so the test suite can check each layout against a
