@@ -2,7 +2,7 @@
 // argument checks, workspace layout and the choice of kernels.
 #include <cmath>
 
-#include "dfs_attn.cuh"
+#include "dfs_attn_tc.cuh"
 
 using namespace dfs;
 
@@ -70,9 +70,23 @@ size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 size_t dsum_bytes(const dfs_attn_problem* p) {
   return round256(sizeof(float) * static_cast<size_t>(p->B) * p->H * p->n_q);
 }
-int dw_parts(const dfs_attn_problem* p) {
-  const int t = attn_q_tile(p->dtype);
-  return p->B * ((p->n_q + t - 1) / t);
+// rows of dw_part per head: a key tile of a batch element each
+int dw_parts(const dfs_attn_problem* p, int tile) { return p->B * ((p->n_k + tile - 1) / tile); }
+constexpr int kSmallestTile = 64;
+
+// Whether an operand can be staged by TMA (and stored in 16-byte pieces): its address and the strides of
+// its extents above 1 are multiples of 16 bytes.
+bool staged(const dfs_strided& s, int n, int heads, int B) {
+  auto ok = [](int64_t stride, int extent) { return extent <= 1 || (stride > 0 && stride % 8 == 0); };
+  return (reinterpret_cast<uintptr_t>(s.ptr) & 15u) == 0 && ok(s.stride_n, n) && ok(s.stride_h, heads) &&
+         ok(s.stride_b, B);
+}
+// The tensor-core kernels: 16-bit operands that TMA can stage.  fp32 operands keep all their bits on the
+// SIMT kernels; a scale that is not positive would turn the running maximum of raw products around.
+bool tensor_cores(const dfs_attn_problem* p, const dfs_attn_args* a) {
+  return p->dtype != DFS_F32 && p->d % 8 == 0 && p->scale > 0.0f && p->n_q > 0 && p->n_k > 0 && tmap_available() &&
+         staged(a->q, p->n_q, p->H, p->B) && staged(a->o, p->n_q, p->H, p->B) &&
+         staged(a->k, p->n_k, p->H_kv, p->B) && staged(a->v, p->n_k, p->H_kv, p->B);
 }
 int rc(cudaError_t e) { return e == cudaSuccess ? DFS_OK : DFS_ERR_CUDA; }
 
@@ -84,13 +98,15 @@ extern "C" int dfs_window_attn_fwd(const dfs_attn_problem* p, const dfs_attn_arg
   if (s != DFS_OK) return s;
   if (p->B == 0 || p->H == 0 || p->n_q == 0) return DFS_OK;
   if (!a->q.ptr || !a->o.ptr || (p->n_k > 0 && (!a->k.ptr || !a->v.ptr))) return DFS_ERR_INVALID_ARGUMENT;
-  return rc(launch_attn_simt_fwd(params(p, a), p->dtype, static_cast<cudaStream_t>(stream)));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const AttnParams P = params(p, a);
+  return rc(tensor_cores(p, a) ? launch_attn_tc_fwd(P, p->dtype, st) : launch_attn_simt_fwd(P, p->dtype, st));
 }
 
 extern "C" size_t dfs_window_attn_bwd_work(const dfs_attn_problem* p, const dfs_relbias* b) {
   if (problem_status(p, b) != DFS_OK) return 0;
   size_t n = dsum_bytes(p);
-  if (b && b->weight) n += sizeof(float) * static_cast<size_t>(p->H) * dw_parts(p) * (2 * b->max_distance + 1);
+  if (b && b->weight) n += sizeof(float) * static_cast<size_t>(p->H) * dw_parts(p, kSmallestTile) * (2 * b->max_distance + 1);
   return n;
 }
 
@@ -109,13 +125,14 @@ extern "C" int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_arg
   if (work_bytes < dfs_window_attn_bwd_work(p, dw ? &a->bias : nullptr)) return DFS_ERR_WORKSPACE;
   AttnParams P = params(p, a);
   P.dsum = static_cast<float*>(work);
+  P.parts = dw_parts(p, kSmallestTile);
   if (dw) P.dw_part = reinterpret_cast<float*>(static_cast<char*>(work) + dsum_bytes(p));
   if (p->n_q > 0 || p->n_k > 0) {
     const int r = rc(launch_attn_simt_bwd(P, p->dtype, st));
     if (r != DFS_OK) return r;
   }
   if (!dw) return DFS_OK;
-  return rc(launch_bucket_sums(P.dw_part, p->H, dw_parts(p), P.D, P.lut, P.nb, P.wdtype, a->d_weight, st));
+  return rc(launch_bucket_sums(P.dw_part, p->H, P.parts, P.D, P.lut, P.nb, P.wdtype, a->d_weight, st));
 }
 
 extern "C" int dfs_window_attn_decode(const dfs_attn_problem* p, const dfs_attn_args* a, const int32_t* lengths,

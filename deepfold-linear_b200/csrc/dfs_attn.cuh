@@ -14,7 +14,7 @@ struct Strided {
 struct AttnParams {
   Strided q, k, v, o, d_o, d_q, d_k, d_v;
   float* lse;           // (B,H,n_q) log2 units, +inf for a row that sees nothing
-  float* dsum;          // (B,H,n_q) D_i = sum_c dO_ic O_ic (backward workspace)
+  float* dsum;          // (B,H,n_q) D_i = sum_j p_ij dP_ij (backward workspace)
   const uint8_t* mask;  // (B,n_k) or null
   const void* w;        // (H, nb) bias weights of type wdtype, or null
   const int32_t* lut;   // (2 D + 1)
@@ -22,6 +22,7 @@ struct AttnParams {
   int32_t* status;
   const int32_t* lengths;  // decode: (B,)
   int nb, D, wdtype;
+  int parts;            // key tiles of all batch elements: rows of dw_part per head
   int B, H, Hkv, G, nq, nk, d;
   int causal, window, sinks, qs;
   float scale, scale2;  // scale; scale * log2(e)
@@ -85,6 +86,5 @@ cudaError_t launch_bucket_sums(const float* part, int H, int parts, int D, const
 cudaError_t launch_attn_simt_fwd(const AttnParams& P, int dtype, cudaStream_t st);
 cudaError_t launch_attn_simt_bwd(const AttnParams& P, int dtype, cudaStream_t st);
 cudaError_t launch_decode(const AttnParams& P, int dtype, cudaStream_t st);
-int attn_q_tile(int dtype);  // query rows of one entry of dw_part
 
 }  // namespace dfs

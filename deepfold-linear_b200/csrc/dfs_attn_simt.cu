@@ -153,21 +153,19 @@ __global__ void __launch_bounds__(kNT) simt_fwd_kernel(AttnParams P) {
   }
 }
 
-// dQ of 64 queries, D_i for the key pass, and the sums of dS by distance.
+// dQ of 64 queries, and D_i for the key pass.  Here D_i = sum_c dO_ic O_ic comes
+// from the rounded O; the key pass gets D_i + sum_j dS_ij, which is sum_j p_ij dP_ij
+// in fp32 (sum_j p_ij = 1).  The sums of dS by bucket need that: they cancel
+// within a row, and from a bfloat16 O alone they were 4e-3 off.
 template <typename E>
 __global__ void __launch_bounds__(kNT) simt_dq_kernel(AttnParams P) {
   extern __shared__ __align__(16) float sm[];
   float *Qt = sm, *dOt = Qt + kTile, *Kt = dOt + kTile, *Kr = Kt + kTile, *Vt = Kr + kTile, *dSt = Vt + kTile;
   float* tab = dSt + kTile;                 // 2 D + 1
-  const int W = 2 * P.D + 1;
-  float* acc = tab + (P.w ? W : 0);         // 2 D + 1
-  __shared__ float Drow[kT], ends[2][4];
+  __shared__ float Drow[kT];
   const int h = blockIdx.y, b = blockIdx.z, hk = h / P.G, tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
   const int i0 = blockIdx.x * kT;
-  const bool dw = P.dw_part != nullptr;
   if (P.w) load_bias_table(tab, P.w, P.lut, P.D, P.nb, P.wdtype, h, kLog2e, tid, kNT);
-  if (dw)
-    for (int x = tid; x < W; x += kNT) acc[x] = 0.0f;
   const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
   load_tile<E>(P.q, b, h, i0, P.nq, P.d, nullptr, Qt, nullptr, tid);
   load_tile<E>(P.d_o, b, h, i0, P.nq, P.d, nullptr, dOt, nullptr, tid);
@@ -178,20 +176,19 @@ __global__ void __launch_bounds__(kNT) simt_dq_kernel(AttnParams P) {
     if (i < P.nq) {
       const E* orow = row_ptr<E>(P.o, b, h, i);
       for (int c = 0; c < P.d; ++c) s = fmaf(dOt[c * kLd + tid], to_f32<E>(orow[c]), s);
-      P.dsum[(static_cast<size_t>(b) * P.H + h) * P.nq + i] = s;
     }
     Drow[tid] = s;
   }
   __syncthreads();
-  float lse[4], Di[4], dq[4][4];
+  float lse[4], Di[4], rest[4], dq[4][4];
   zero(dq);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int i = i0 + 4 * ty + r;
     lse[r] = i < P.nq ? P.lse[(static_cast<size_t>(b) * P.H + h) * P.nq + i] : INFINITY;
     Di[r] = Drow[4 * ty + r];
+    rest[r] = 0.0f;
   }
-  float lo = 0.0f, hi = 0.0f;  // this thread's sums of the distances beyond the table's ends
   const KeyTiles tiles(P, i0 + P.qs, min(i0 + kT, P.nq) - 1 + P.qs);
   for (int x = 0; x < tiles.count(); ++x) {
     const int j0 = tiles[x] * kT;
@@ -209,49 +206,39 @@ __global__ void __launch_bounds__(kNT) simt_dq_kernel(AttnParams P) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float p = exp2f(logit2(P, P.w ? tab : nullptr, mask, s[r][c], i0 + 4 * ty + r, j0 + 4 * tx + c) - lse[r]);
-        dSt[(4 * tx + c) * kLd + 4 * ty + r] = p * (dp[r][c] - Di[r]);
+        const float ds = p * (dp[r][c] - Di[r]);
+        rest[r] += ds;
+        dSt[(4 * tx + c) * kLd + 4 * ty + r] = ds;
       }
     __syncthreads();
     tile_product(dSt, Kr, kT, ty, tx, dq);
-    if (dw && tid < 2 * kT - 1) {  // thread tid owns the tile's diagonal e = row - column
-      const int e = tid - (kT - 1);
-      float t = 0.0f;
-      for (int r = max(0, e); r < min(kT, kT + e); ++r) t += dSt[(r - e) * kLd + r];
-      const int delta = i0 + P.qs - j0 + e;
-      if (delta <= -P.D) lo += t;
-      else if (delta >= P.D) hi += t;
-      else acc[delta + P.D] += t;
-    }
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) rest[r] += __shfl_xor_sync(0xffffffffu, rest[r], w);
     const int i = i0 + 4 * ty + r;
     if (i >= P.nq) continue;
+    if (tx == 0) P.dsum[(static_cast<size_t>(b) * P.H + h) * P.nq + i] = Di[r] + rest[r];
     E* row = row_ptr<E>(P.d_q, b, h, i);
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       if (4 * tx + c < P.d) row[4 * tx + c] = from_f32<E>(dq[r][c] * P.scale);
   }
-  if (dw) {
-    if (P.D == 0) hi += lo, lo = 0.0f;
-    lo = warp_sum(lo);
-    hi = warp_sum(hi);
-    if (tid < 128 && (tid & 31) == 0) ends[0][tid / 32] = lo, ends[1][tid / 32] = hi;
-    __syncthreads();
-    if (tid < 2 && (P.D > 0 || tid == 1))
-      acc[tid == 0 ? 0 : 2 * P.D] = ends[tid][0] + ends[tid][1] + ends[tid][2] + ends[tid][3];
-    __syncthreads();
-    float* dst = P.dw_part + ((static_cast<size_t>(h) * P.B + b) * gridDim.x + blockIdx.x) * W;
-    for (int x = tid; x < W; x += kNT) dst[x] = acc[x];
-  }
 }
 
-// dK and dV of 64 keys: the queries of every head of the group that see them.
+// dK and dV of 64 keys: the queries of every head of the group that see them;
+// and, per head, the sums of dS by distance (a thread per diagonal of a tile, so
+// every sum has one order).
 template <typename E>
 __global__ void __launch_bounds__(kNT) simt_dkv_kernel(AttnParams P) {
   extern __shared__ __align__(16) float sm[];
   float *Kt = sm, *Vt = Kt + kTile, *Qt = Vt + kTile, *Qr = Qt + kTile, *dOt = Qr + kTile, *dOr = dOt + kTile;
   float *Pt = dOr + kTile, *dSt = Pt + kTile, *tab = dSt + kTile;
+  const int W = 2 * P.D + 1;
+  float* acc = tab + (P.w ? W : 0);  // 2 D + 1
+  __shared__ float ends[2][4];
+  const bool dw = P.dw_part != nullptr;
   const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
   const int j0 = blockIdx.x * kT, j1 = min(j0 + kT, P.nk);
   const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
@@ -274,6 +261,9 @@ __global__ void __launch_bounds__(kNT) simt_dkv_kernel(AttnParams P) {
       __syncthreads();
       load_bias_table(tab, P.w, P.lut, P.D, P.nb, P.wdtype, h, kLog2e, tid, kNT);
     }
+    if (dw)
+      for (int x = tid; x < W; x += kNT) acc[x] = 0.0f;
+    float lo = 0.0f, hi = 0.0f;  // this thread's sums of the distances beyond the table's ends
     const float* lse = P.lse + (static_cast<size_t>(b) * P.H + h) * P.nq;
     const float* Dv = P.dsum + (static_cast<size_t>(b) * P.H + h) * P.nq;
     for (int i0 = i_lo / kT * kT; i0 < i_hi; i0 += kT) {
@@ -300,6 +290,29 @@ __global__ void __launch_bounds__(kNT) simt_dkv_kernel(AttnParams P) {
       __syncthreads();
       tile_product(Pt, dOr, kT, ty, tx, dv);
       tile_product(dSt, Qr, kT, ty, tx, dk);
+      if (dw && tid < 2 * kT - 1) {  // thread tid owns the tile's diagonal e = query - key
+        const int e = tid - (kT - 1);
+        float t = 0.0f;
+        for (int i = max(0, e); i < min(kT, kT + e); ++i) t += dSt[i * kLd + i - e];
+        const int delta = i0 + P.qs - j0 + e;
+        if (delta <= -P.D) lo += t;
+        else if (delta >= P.D) hi += t;
+        else acc[delta + P.D] += t;
+      }
+    }
+    if (dw) {
+      if (P.D == 0) hi += lo, lo = 0.0f;
+      lo = warp_sum(lo);
+      hi = warp_sum(hi);
+      __syncthreads();
+      if (tid < 128 && (tid & 31) == 0) ends[0][tid / 32] = lo, ends[1][tid / 32] = hi;
+      __syncthreads();
+      if (tid < 2 && (P.D > 0 || tid == 1))
+        acc[tid == 0 ? 0 : 2 * P.D] = ends[tid][0] + ends[tid][1] + ends[tid][2] + ends[tid][3];
+      __syncthreads();
+      float* dst = P.dw_part + (static_cast<size_t>(h) * P.parts + b * gridDim.x + blockIdx.x) * W;
+      for (int x = tid; x < W; x += kNT) dst[x] = acc[x];
+      __syncthreads();
     }
   }
 #pragma unroll
@@ -336,17 +349,15 @@ cudaError_t bwd(const AttnParams& P, cudaStream_t st) {
   const size_t acc = P.dw_part ? (2 * P.D + 1) * sizeof(float) : 0;
   if (P.nq > 0) {
     const cudaError_t e = launch(simt_dq_kernel<E>, dim3((P.nq + kT - 1) / kT, P.H, P.B),
-                                 6 * kTile * sizeof(float) + table_bytes(P) + acc, st, P);
+                                 6 * kTile * sizeof(float) + table_bytes(P), st, P);
     if (e != cudaSuccess) return e;
   }
   if (P.nk == 0) return cudaSuccess;
-  return launch(simt_dkv_kernel<E>, dim3((P.nk + kT - 1) / kT, P.Hkv, P.B), 8 * kTile * sizeof(float) + table_bytes(P),
+  return launch(simt_dkv_kernel<E>, dim3((P.nk + kT - 1) / kT, P.Hkv, P.B), 8 * kTile * sizeof(float) + table_bytes(P) + acc,
                 st, P);
 }
 
 }  // namespace
-
-int attn_q_tile(int) { return kT; }
 
 cudaError_t launch_attn_simt_fwd(const AttnParams& P, int dtype, cudaStream_t st) {
   return dtype == DFS_F32 ? fwd<float>(P, st) : dtype == DFS_BF16 ? fwd<__nv_bfloat16>(P, st) : fwd<__half>(P, st);

@@ -1,0 +1,163 @@
+// dfs_attn_tc.cuh -- shared by the tensor-core local-attention kernels: operand
+// staging, TMEM operands, tile information, bias tables.
+#pragma once
+
+#include "dfs_attn.cuh"
+#include "dfs_tma.cuh"
+
+namespace dfs {
+
+constexpr int kTcRows = 128;              // tile edge, queries and keys
+constexpr int kTcTileBytes = 128 * 128;   // 128 rows of 64 16-bit elements, 128-byte swizzle
+
+struct TcParams {
+  CUtensorMap q, k, v, d_o;
+  AttnParams a;
+};
+
+// instruction descriptor, kind::f16; b_mn: B is stored with its N index contiguous
+__host__ __device__ constexpr uint32_t tc_idesc(int M, int N, bool bf16, bool b_mn) {
+  return idesc_f16(M, N, bf16) | (static_cast<uint32_t>(b_mn) << 16);
+}
+
+// D(tmem) (+)= A(tmem) * B(smem): A's 16-bit elements lie two to a 32-bit column
+DFS_DEV void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accum));
+}
+
+// 128 x N product over d: both operands K-major tiles of 128-byte rows
+DFS_DEV void tc_mma_kk(uint32_t d_tmem, uint32_t a_s, uint32_t b_s, uint32_t idesc, int ksteps) {
+  for (int k = 0; k < ksteps; ++k)
+    mma_f16(d_tmem, sw128_desc(a_s + 32 * k, 16, 1024), sw128_desc(b_s + 32 * k, 16, 1024), idesc, k > 0);
+}
+// 128 x dp product over 128 rows of B: A in TMEM, B a tile whose rows are the contraction index
+DFS_DEV void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_s, uint32_t idesc, bool accum) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    mma_f16_ts(d_tmem, a_tmem + 8 * k, sw128_desc(b_s + 2048 * k, 1024, 1024), idesc, accum || k > 0);
+}
+
+DFS_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+DFS_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+DFS_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* tm, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+
+template <bool BF16>
+DFS_DEV uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if (BF16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <bool BF16>
+DFS_DEV float2 unpack16(uint32_t x) {
+  if (BF16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  const __half2 h = *reinterpret_cast<const __half2*>(&x);
+  return __half22float2(h);
+}
+
+DFS_DEV float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+
+// A wait that gave up: tell the host (status may be mapped host memory: a plain store)
+DFS_DEV void report_timeout(int32_t* status) {
+  if (status != nullptr) *reinterpret_cast<volatile int32_t*>(status) = DFS_ERR_DEVICE_TIMEOUT;
+}
+
+// Bits c of [0, 128) with a <= c < b, as four words
+DFS_DEV uint32_t range_word(int a, int b, int w) {
+  const int lo = min(max(a - 32 * w, 0), 32), hi = min(max(b - 32 * w, 0), 32);
+  const uint32_t below_hi = hi == 32 ? 0xffffffffu : (1u << hi) - 1u;
+  const uint32_t below_lo = lo == 32 ? 0xffffffffu : (1u << lo) - 1u;
+  return below_hi & ~below_lo;
+}
+
+// The bias table widened by its end values, so that a tile whose distances
+// reach into the table needs no clamp: tab[delta + ext], ext = D + 255.
+DFS_DEV int bias_ext(int D) { return D + 255; }
+DFS_DEV void load_bias_ext(float* tab, const AttnParams& P, int h, int tid, int nthreads) {
+  const int E = bias_ext(P.D);
+  for (int x = tid; x < 2 * E + 1; x += nthreads) {
+    const int at = min(max(x - E, -P.D), P.D) + P.D;
+    const int b = min(max(P.lut[at], 0), P.nb - 1);
+    tab[x] = load_as_f32<void>(P.w, static_cast<size_t>(h) * P.nb + b, P.wdtype) * kLog2e;
+  }
+}
+inline size_t bias_ext_bytes(const AttnParams& P) { return P.w ? (2 * (P.D + 255) + 1) * sizeof(float) : 0; }
+
+// One tile as the producer announces it: first key (or query) row, -1 for the
+// end; the key mask's bits.
+struct TileInfo {
+  int at, head;
+  uint32_t bits[4];
+};
+
+// Mask bits of keys [j0, j0 + 128) (a full warp; all lanes get the four words)
+DFS_DEV void key_bits(const uint8_t* mask, int j0, int nk, int lane, uint32_t (&bits)[4]) {
+  uint32_t nib = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int j = j0 + 4 * lane + e;
+    if (j < nk && (mask == nullptr || mask[j] != 0)) nib |= 1u << e;
+  }
+  const uint32_t part = nib << (4 * (lane & 7));
+#pragma unroll
+  for (int w = 0; w < 4; ++w) bits[w] = __reduce_or_sync(0xffffffffu, (lane >> 3) == w ? part : 0u);
+}
+
+// Key tiles of 128 seen by positions p0..p1: the sink tiles [0, ns), then the window's [t0, t1).
+struct TcKeyTiles {
+  int ns, t0, t1;
+  DFS_DEV TcKeyTiles(const AttnParams& P, int p0, int p1) {
+    int lo, hi;
+    near_keys(P, p0, p1, lo, hi);
+    t0 = lo / kTcRows;
+    t1 = hi > lo ? (hi + kTcRows - 1) / kTcRows : t0;
+    ns = (sink_keys(P, p1) + kTcRows - 1) / kTcRows;
+    if (hi > lo) ns = min(ns, t0);
+  }
+  DFS_DEV int count() const { return ns + (t1 - t0); }
+  DFS_DEV int operator[](int x) const { return x < ns ? x : t0 + (x - ns); }
+};
+
+// Whether every pair of queries at p0..p0+127 and keys j0..j0+127 is visible, the mask apart.
+DFS_DEV bool all_visible(const AttnParams& P, int p0, int j0) {
+  const int p1 = p0 + kTcRows - 1, j1 = j0 + kTcRows - 1;
+  if (j1 >= P.nk || (P.causal && p0 < j1)) return false;
+  return (p1 - j0 < P.window && j1 - p0 < P.window) || j1 < P.sinks;
+}
+// Visible keys of the tile at j0 for position p, the mask apart: bits of word w.
+DFS_DEV uint32_t row_bits(const AttnParams& P, int p, int j0, int w) {
+  const int top = min(P.causal ? p + 1 : P.nk, P.nk);
+  const int near_top = min(top, p + P.window);
+  return range_word(p - P.window + 1 - j0, near_top - j0, w) | range_word(0, min(P.sinks, top) - j0, w);
+}
+
+// A strided (B, heads, n, d) operand of 16-bit elements as {d, n, heads, B}, boxes of 64 x 128.
+bool tc_tmap(CUtensorMap* tm, const Strided& s, bool bf16, int d, int n, int heads, int B);
+
+cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st);
+cudaError_t launch_attn_tc_bwd(const AttnParams& P, int dtype, cudaStream_t st);
+
+}  // namespace dfs

@@ -738,6 +738,28 @@ bool make_tmap(CUtensorMap* tm, const void* ptr, int dtype, int inner, int rows,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_tmap_4d(CUtensorMap* tm, const void* ptr, int dtype, int inner, int rows, int heads, int B,
+                  int64_t row_stride, int64_t head_stride, int64_t batch_stride, int box_inner, int box_rows) {
+  if (ptr == nullptr || (reinterpret_cast<uintptr_t>(ptr) & 15u) != 0 || box_inner * 2 != 128) return false;
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows),
+                              static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(B)};
+  // the stride of an extent of 1 is never used: any multiple of 16 bytes serves
+  const int64_t own[3] = {rows > 1 ? row_stride : 64, heads > 1 ? head_stride : 64, B > 1 ? batch_stride : 64};
+  cuuint64_t strides[3];
+  for (int k = 0; k < 3; ++k) {
+    if (own[k] <= 0 || own[k] % 8 != 0) return false;
+    strides[k] = static_cast<cuuint64_t>(own[k]) * 2;
+  }
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_rows), 1u, 1u};
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  return fn(tm, dtype == DFS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+            const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 namespace {
 
 template <int MODE, int DT, int D, bool TERMS>

@@ -166,6 +166,12 @@ cudaError_t launch_dependent(void (*kern)(Params...), dim3 grid, dim3 block, siz
 // 128-byte swizzle (box_inner x element size must be 128 bytes).  False when
 // the address is not 16-byte aligned or the driver refuses the map.
 bool make_tmap(CUtensorMap* tm, const void* ptr, int dtype, int inner, int rows, int BH, int box_inner, int box_rows);
+// Tensor map of a strided (B, heads, rows, inner) tensor of 16-bit elements
+// (strides in elements, unit along inner) as {inner, rows, heads, B}, boxes of
+// box_inner x box_rows, 128-byte swizzle, zeros outside.  False when the address
+// or a stride is not a multiple of 16 bytes or the driver refuses the map.
+bool make_tmap_4d(CUtensorMap* tm, const void* ptr, int dtype, int inner, int rows, int heads, int B,
+                  int64_t row_stride, int64_t head_stride, int64_t batch_stride, int box_inner, int box_rows);
 // True when cuTensorMapEncodeTiled could be obtained from the driver.
 bool tmap_available();
 

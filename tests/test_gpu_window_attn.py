@@ -1,7 +1,7 @@
 """Local attention and its position bias on the GPU against the float64 oracle.
 
-Tolerances, from the arithmetic: u is the operands' unit roundoff (2^-9 bfloat16,
-2^-12 float16, 2^-24 float32).  An output is rounded once (u), and sums products
+Tolerances, from the arithmetic: u bounds the root mean square of a rounding's
+relative error (2^-9 bfloat16, 2^-12 float16; 2^-24 float32).  An output is rounded once (u), and sums products
 of probabilities rounded once (u, relative to a sum of terms of either sign,
 whose 2-norm over random data is that of the result): 2 u, twice that allowed.
 A gradient has one more rounded factor (dS, or o within D): 3 u, twice that
