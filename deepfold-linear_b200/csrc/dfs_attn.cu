@@ -125,10 +125,12 @@ extern "C" int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_arg
   if (work_bytes < dfs_window_attn_bwd_work(p, dw ? &a->bias : nullptr)) return DFS_ERR_WORKSPACE;
   AttnParams P = params(p, a);
   P.dsum = static_cast<float*>(work);
-  P.parts = dw_parts(p, kSmallestTile);
+  const bool tc = tensor_cores(p, a) && staged(a->d_o, p->n_q, p->H, p->B) && staged(a->d_q, p->n_q, p->H, p->B) &&
+                  staged(a->d_k, p->n_k, p->H_kv, p->B) && staged(a->d_v, p->n_k, p->H_kv, p->B);
+  P.parts = dw_parts(p, tc ? kTcRows : kSmallestTile);
   if (dw) P.dw_part = reinterpret_cast<float*>(static_cast<char*>(work) + dsum_bytes(p));
   if (p->n_q > 0 || p->n_k > 0) {
-    const int r = rc(launch_attn_simt_bwd(P, p->dtype, st));
+    const int r = rc(tc ? launch_attn_tc_bwd(P, p->dtype, st) : launch_attn_simt_bwd(P, p->dtype, st));
     if (r != DFS_OK) return r;
   }
   if (!dw) return DFS_OK;
