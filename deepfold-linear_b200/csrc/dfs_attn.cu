@@ -1,5 +1,6 @@
 // dfs_attn.cu -- C entry points of the local attention (include/dfsink.h):
 // argument checks, workspace layout and the choice of kernels.
+#include <algorithm>
 #include <cmath>
 
 #include "dfs_attn_tc.cuh"
@@ -43,6 +44,7 @@ AttnParams params(const dfs_attn_problem* p, const dfs_attn_args* a) {
   P.d_k = strided(a->d_k);
   P.d_v = strided(a->d_v);
   P.lse = a->lse;
+  P.o_lo = p->dtype != DFS_F32 ? static_cast<char*>(a->o_lo) : nullptr;
   P.mask = a->mask;
   P.w = a->bias.weight;
   P.lut = a->bias.lut;
@@ -76,15 +78,17 @@ constexpr int kSmallestTile = 64;
 
 // Whether an operand can be staged by TMA (and stored in 16-byte pieces): its address and the strides of
 // its extents above 1 are multiples of 16 bytes.
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool staged(const dfs_strided& s, int n, int heads, int B) {
   auto ok = [](int64_t stride, int extent) { return extent <= 1 || (stride > 0 && stride % 8 == 0); };
-  return (reinterpret_cast<uintptr_t>(s.ptr) & 15u) == 0 && ok(s.stride_n, n) && ok(s.stride_h, heads) &&
+  return aligned16(s.ptr) && ok(s.stride_n, n) && ok(s.stride_h, heads) &&
          ok(s.stride_b, B);
 }
 // The tensor-core kernels: 16-bit operands that TMA can stage.  fp32 operands keep all their bits on the
 // SIMT kernels; a scale that is not positive would turn the running maximum of raw products around.
 bool tensor_cores(const dfs_attn_problem* p, const dfs_attn_args* a) {
-  return p->dtype != DFS_F32 && p->d % 8 == 0 && p->scale > 0.0f && p->n_q > 0 && p->n_k > 0 && tmap_available() &&
+  const int64_t tiles = (std::max(p->n_q, p->n_k) + kTcRows - 1) / kTcRows;
+  return tiles * p->B * p->H < (int64_t{1} << 31) && p->dtype != DFS_F32 && p->d % 8 == 0 && p->scale > 0.0f && p->n_q > 0 && p->n_k > 0 && tmap_available() && aligned16(a->o_lo) &&
          staged(a->q, p->n_q, p->H, p->B) && staged(a->o, p->n_q, p->H, p->B) &&
          staged(a->k, p->n_k, p->H_kv, p->B) && staged(a->v, p->n_k, p->H_kv, p->B);
 }

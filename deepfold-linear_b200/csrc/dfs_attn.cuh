@@ -13,6 +13,7 @@ struct Strided {
 
 struct AttnParams {
   Strided q, k, v, o, d_o, d_q, d_k, d_v;
+  char* o_lo;           // laid out as o: o's rounding error, or null
   float* lse;           // (B,H,n_q) log2 units, +inf for a row that sees nothing
   float* dsum;          // (B,H,n_q) D_i = sum_j p_ij dP_ij (backward workspace)
   const uint8_t* mask;  // (B,n_k) or null

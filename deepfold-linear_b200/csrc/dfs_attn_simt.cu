@@ -145,16 +145,21 @@ __global__ void __launch_bounds__(kNT) simt_fwd_kernel(AttnParams P) {
     if (i >= P.nq) continue;
     const float inv = l[r] > 0.0f ? 1.0f / l[r] : 0.0f;
     E* row = row_ptr<E>(P.o, b, h, i);
+    E* rest = P.o_lo ? reinterpret_cast<E*>(P.o_lo) + (row - reinterpret_cast<E*>(P.o.p)) : nullptr;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      if (4 * tx + c < P.d) row[4 * tx + c] = from_f32<E>(o[r][c] * inv);
+      if (4 * tx + c < P.d) {
+        const float v = o[r][c] * inv;
+        row[4 * tx + c] = from_f32<E>(v);
+        if (rest) rest[4 * tx + c] = from_f32<E>(v - to_f32<E>(from_f32<E>(v)));
+      }
     if (P.lse && tx == 0)
       P.lse[(static_cast<size_t>(b) * P.H + h) * P.nq + i] = l[r] > 0.0f ? m[r] + log2f(l[r]) : INFINITY;
   }
 }
 
 // dQ of 64 queries, and D_i for the key pass.  Here D_i = sum_c dO_ic O_ic comes
-// from the rounded O; the key pass gets D_i + sum_j dS_ij, which is sum_j p_ij dP_ij
+// from O (with what its rounding took, where the forward kept that); the key pass gets D_i + sum_j dS_ij, which is sum_j p_ij dP_ij
 // in fp32 (sum_j p_ij = 1).  The sums of dS by bucket need that: they cancel
 // within a row, and from a bfloat16 O alone they were 4e-3 off.
 template <typename E>
@@ -175,7 +180,9 @@ __global__ void __launch_bounds__(kNT) simt_dq_kernel(AttnParams P) {
     const int i = i0 + tid;
     if (i < P.nq) {
       const E* orow = row_ptr<E>(P.o, b, h, i);
-      for (int c = 0; c < P.d; ++c) s = fmaf(dOt[c * kLd + tid], to_f32<E>(orow[c]), s);
+      const E* rest = P.o_lo ? reinterpret_cast<const E*>(P.o_lo) + (orow - reinterpret_cast<const E*>(P.o.p)) : nullptr;
+      for (int c = 0; c < P.d; ++c)
+        s = fmaf(dOt[c * kLd + tid], to_f32<E>(orow[c]) + (rest ? to_f32<E>(rest[c]) : 0.0f), s);
     }
     Drow[tid] = s;
   }

@@ -29,16 +29,31 @@ DFS_DEV void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accum));
 }
 
-// 128 x N product over d: both operands K-major tiles of 128-byte rows
-DFS_DEV void tc_mma_kk(uint32_t d_tmem, uint32_t a_s, uint32_t b_s, uint32_t idesc, int ksteps) {
-  for (int k = 0; k < ksteps; ++k)
-    mma_f16(d_tmem, sw128_desc(a_s + 32 * k, 16, 1024), sw128_desc(b_s + 32 * k, 16, 1024), idesc, k > 0);
+// One lane of a converged warp.  The compiler keeps what that lane computes in
+// uniform registers, where the MMA takes its descriptors from; a branch on the
+// lane number moved each there one by one, and issuing 8 MMAs took 600 clocks.
+DFS_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
-// 128 x dp product over 128 rows of B: A in TMEM, B a tile whose rows are the contraction index
-DFS_DEV void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_s, uint32_t idesc, bool accum) {
+DFS_DEV int warp_index() { return __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x / 32), 0); }
+
+// Descriptors of a tile at `s`: rows as the M or N index (a step of 16 along d is
+// +2 in the address field), or as the contraction index (16 rows: +128).
+DFS_DEV uint64_t tc_desc(uint32_t s) { return sw128_desc(s, 1024, 1024); }
+
+// 128 x 128 product over d of two tiles
+DFS_DEV void tc_mma_kk(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, int ksteps) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    mma_f16_ts(d_tmem, a_tmem + 8 * k, sw128_desc(b_s + 2048 * k, 1024, 1024), idesc, accum || k > 0);
+  for (int k = 0; k < 4; ++k)
+    if (k < ksteps) mma_f16(d_tmem, a + 2 * k, b + 2 * k, idesc, k > 0);
+}
+// 128 x dp product over the 128 rows of B: A in TMEM
+DFS_DEV void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, bool accum) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) mma_f16_ts(d_tmem, a_tmem + 8 * k, b + 128 * k, idesc, accum || k > 0);
 }
 
 DFS_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -51,6 +66,35 @@ DFS_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+DFS_DEV void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+}
+DFS_DEV void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+DFS_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+DFS_DEV void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+DFS_DEV void tmem_wait_ld16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 DFS_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -78,7 +122,85 @@ DFS_DEV float2 unpack16(uint32_t x) {
   return __half22float2(h);
 }
 
-DFS_DEV float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+// Packed fp32 pairs, denormals flushed (an exponential that underflowed is 0).
+DFS_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.ftz.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+DFS_DEV float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.ftz.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+DFS_DEV float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.ftz.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+DFS_DEV float2 both(float x) { return make_float2(x, x); }
+
+// 2^x of a pair on the FMA pipes (the MUFU gives 16 a clock per SM, and these
+// kernels wait for it): x = j + f, j = round(x) by adding 1.5 * 2^23 (j lands in
+// the low mantissa bits), 2^f on [-1/2, 1/2] by a degree-4 polynomial (relative
+// minimax fit by reweighted least squares: 2.7e-6 off at most, far below the
+// 16-bit rounding of what it feeds), 2^j by adding j to the exponent.  At and
+// below -126 the result is a denormal (2^f there is just under 1), which the packed operations above take as
+// 0; NaN stays non-finite.
+DFS_DEV float2 exp2_poly(float2 x) {
+  float2 c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c.x) : "f"(x.x), "f"(-126.0f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c.y) : "f"(x.y), "f"(-126.0f));
+  const float2 t = add2(c, both(12582912.0f));
+  const float2 f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), c);
+  float2 p = fma2(both(0.00957009662f), f, both(0.0559178591f));
+  p = fma2(p, f, both(0.240247443f));
+  p = fma2(p, f, both(0.693121791f));
+  p = fma2(p, f, both(0.999999285f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+// Pair number c of a row's chunk of 16 pairs: about one in three on the FMA pipes.
+template <int kEvery>
+DFS_DEV float2 exp2_pair(float2 x, int c) {
+  return kEvery > 0 && c % kEvery == kEvery - 1 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+}
+
+// Wait for the phase with the given parity; false once about two seconds of clock
+// cycles have passed.  The clock is only looked at every 1024 tries: reading it
+// on the way through a wait that is about to end costs more than the wait.
+DFS_DEV bool tc_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  long long t0 = 0;
+  for (uint32_t it = 1;; ++it) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((it & 1023u) == 0) {
+      const long long now = clock64();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > 4000000000ll) return false;
+    }
+  }
+}
 
 // A wait that gave up: tell the host (status may be mapped host memory: a plain store)
 DFS_DEV void report_timeout(int32_t* status) {
@@ -141,21 +263,35 @@ struct TcKeyTiles {
   DFS_DEV int operator[](int x) const { return x < ns ? x : t0 + (x - ns); }
 };
 
-// Whether every pair of queries at p0..p0+127 and keys j0..j0+127 is visible, the mask apart.
-DFS_DEV bool all_visible(const AttnParams& P, int p0, int j0) {
-  const int p1 = p0 + kTcRows - 1, j1 = j0 + kTcRows - 1;
+// Whether every pair of the 32 queries at p0.. and the 32 keys at j0.. is visible, the mask apart.
+DFS_DEV bool block_visible(const AttnParams& P, int p0, int j0) {
+  const int p1 = p0 + 31, j1 = j0 + 31;
   if (j1 >= P.nk || (P.causal && p0 < j1)) return false;
   return (p1 - j0 < P.window && j1 - p0 < P.window) || j1 < P.sinks;
 }
-// Visible keys of the tile at j0 for position p, the mask apart: bits of word w.
-DFS_DEV uint32_t row_bits(const AttnParams& P, int p, int j0, int w) {
+// Visible keys j0..j0+31 for position p, the mask apart.
+DFS_DEV uint32_t key_word(const AttnParams& P, int p, int j0) {
   const int top = min(P.causal ? p + 1 : P.nk, P.nk);
-  const int near_top = min(top, p + P.window);
-  return range_word(p - P.window + 1 - j0, near_top - j0, w) | range_word(0, min(P.sinks, top) - j0, w);
+  return range_word(p - P.window + 1 - j0, min(top, p + P.window) - j0, 0) | range_word(0, min(P.sinks, top) - j0, 0);
 }
-
+// Visible queries at positions p0..p0+31 for key j, the mask apart.
+DFS_DEV uint32_t query_word(const AttnParams& P, int j, int p0) {
+  uint32_t v = range_word(P.causal ? j - p0 : j - P.window + 1 - p0, j + P.window - p0, 0);
+  if (j < P.sinks) v |= range_word(P.causal ? j - p0 : 0, 32, 0);
+  return v;
+}
+// Where the distances of a block of 32 x 32 lie: 1 beyond the table's far end, -1 beyond the other, 0 in it.
+DFS_DEV int block_side(const AttnParams& P, int p0, int j0) {
+  return p0 - j0 - 31 >= P.D ? 1 : p0 - j0 + 31 <= -P.D ? -1 : 0;
+}
 // A strided (B, heads, n, d) operand of 16-bit elements as {d, n, heads, B}, boxes of 64 x 128.
 bool tc_tmap(CUtensorMap* tm, const Strided& s, bool bf16, int d, int n, int heads, int B);
+
+// One CTA per tile of each (head, batch element), heads fastest and tiles slowest:
+// the CTAs with the most tiles to walk start first, over all heads.  (Tiles
+// fastest left a head's longest CTA among the last: 35 % of SM time idle at
+// N = 4096, causal.)
+inline unsigned tc_grid(int n, int heads, int B) { return static_cast<unsigned>((n + kTcRows - 1) / kTcRows) * heads * B; }
 
 cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st);
 cudaError_t launch_attn_tc_bwd(const AttnParams& P, int dtype, cudaStream_t st);

@@ -3,7 +3,7 @@
 // Two passes, neither with atomics, so gradients repeat bit for bit:
 //   dQ pass   one CTA per 128 queries of a head, over the key tiles they see:
 //             S = Q K^T, dP = dO V^T, p = 2^(S - lse), dS = p (dP - D), dQ += dS K;
-//             D comes from the rounded O, and D + sum_j dS_ij = sum_j p_ij dP_ij (in
+//             D comes from O (and what its rounding took), and D + sum_j dS_ij = sum_j p_ij dP_ij (in
 //             fp32) goes to the key pass, whose bias sums cancel within a row;
 //   dK/dV pass  one CTA per 128 keys of a key head, over the query tiles (of every
 //             head of the group) that see them, on transposed tiles: S^T = K Q^T,
@@ -12,16 +12,21 @@
 // instead of 7 and one exponential instead of two, but 32 KB of fp32 atomics (in
 // varying order) a tile pair.
 //
-// Both: warps 0-7 work element by element (a TMEM row and half of a tile's columns
-// each), warp 8 issues the MMAs (the next tile's S and dP while this one's
-// elements are worked on), warp 9 stages tiles by TMA and announces them.
+// Both: warps 0-15 work element by element (a TMEM row and a quarter of a tile's
+// columns per thread: blocks of 32 x 32 per warp, skipped where all is hidden),
+// warp 16 issues the MMAs (the next tile's S and dP while this one's elements are
+// worked on), warp 17 stages tiles by TMA and announces them.  The exponentials
+// (1024 clocks a tile on the MUFU) go in part to the FMA pipes; four element warps
+// a scheduler cover the latencies of TMEM, barriers and dependent arithmetic.
 #include "dfs_attn_tc.cuh"
 
 namespace dfs {
 namespace {
 
-constexpr int kBwdThreads = 320;
-constexpr int kWork = 256;     // threads of the element warps
+constexpr int kBwdThreads = 576;
+constexpr int kWork = 512;     // threads of the element warps
+constexpr int kMmaWarp = 16, kTmaWarp = 17;
+constexpr int kPolyEvery = 3;
 constexpr int kStages = 3, kInfo = 4;
 
 // TMEM columns (512 allocated)
@@ -32,13 +37,13 @@ struct BwdShared {
   uint64_t s_full, s_free, ds_ready, acc_done;
   TileInfo info[kInfo];
   alignas(16) float stat[kStages][2][kTcRows];  // dK/dV pass: lse and D of the stage's queries
-  float half[2][kTcRows];           // dQ pass: two half rows' sums
+  float part[4][kTcRows];           // dQ pass: a row's four partial sums
   float ends[2][kWork / 32];
-  float diag[2][kWork / 32][96];    // dK/dV pass: a warp's strip's diagonals, two tiles in turn
+  float diag[2][kWork / 32][64];    // dK/dV pass: the diagonals of a warp's block, two tiles in turn
   uint32_t tmem;
 };
 
-DFS_DEV void work_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+DFS_DEV void work_barrier() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
 
 template <bool BF16>
 struct E16 {
@@ -49,13 +54,13 @@ struct E16<true> {
   using T = __nv_bfloat16;
 };
 
-// 32 of a row's gradient values, scaled, to global memory (columns c0.. of d)
+// 16 of a row's gradient values, scaled, to global memory (columns c0.. of d)
 template <bool BF16>
-DFS_DEV void store_row32(const Strided& s, int b, int h, int row, int c0, int d, const uint32_t (&v)[32], float mul,
+DFS_DEV void store_row16(const Strided& s, int b, int h, int row, int c0, int d, const uint32_t (&v)[16], float mul,
                          bool zero) {
   auto* dst = row_ptr<typename E16<BF16>::T>(s, b, h, row) + c0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
+  for (int e = 0; e < 2; ++e)
     if (c0 + 8 * e < d) {
       uint32_t r[4];
 #pragma unroll
@@ -75,9 +80,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
   const uint32_t sQ = base, sO = sQ + kTcTileBytes, sK = sO + kTcTileBytes, sV = sK + kStages * kTcTileBytes;
   BwdShared& S = *reinterpret_cast<BwdShared*>(gen + (2 + 2 * kStages) * kTcTileBytes);
   float* tab = reinterpret_cast<float*>(&S + 1);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int h = blockIdx.y, b = blockIdx.z, hk = h / P.G;
-  const int i0 = (gridDim.x - 1 - blockIdx.x) * kTcRows, p0 = i0 + P.qs;
+  const int warp = warp_index(), lane = threadIdx.x % 32;
+  const int h = blockIdx.x % P.H, b = blockIdx.x / P.H % P.B, hk = h / P.G;
+  const int i0 = ((P.nq - 1) / kTcRows - static_cast<int>(blockIdx.x / P.H / P.B)) * kTcRows;  // causal: longest first
+  const int p0 = i0 + P.qs;
   bool err = false;
   if (threadIdx.x == 0) {
     mbar_init(&S.own_full, 1);
@@ -88,14 +94,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
     mbar_init(&S.acc_done, 1);
     fence_mbar_init();
   }
-  if (warp == 8) tmem_alloc(&S.tmem, 512);
+  if (warp == kMmaWarp) tmem_alloc(&S.tmem, 512);
   if (P.w) load_bias_ext(tab, P, h, threadIdx.x, kBwdThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = S.tmem;
 
-  if (warp == 9) {  // ---- producer
+  if (warp == kTmaWarp) {  // ---- producer
     const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
     const TcKeyTiles tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
     if (lane == 0) {
@@ -112,7 +118,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
         if ((bits[0] | bits[1] | bits[2] | bits[3]) == 0) continue;
       }
       const int s = t % kStages;
-      if (!mbar_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
+      if (!tc_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
       if (lane == 0) {
         TileInfo& f = S.info[t % kInfo];
         f.at = j0;
@@ -128,13 +134,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
       }
       ++t;
     }
-  } else if (warp == 8) {  // ---- MMA
+  } else if (warp == kMmaWarp) {  // ---- MMA
     const int dp = (P.d + 15) / 16 * 16;
     const uint32_t id_s = tc_idesc(128, 128, BF16, false), id_a = tc_idesc(128, dp, BF16, true);
-    err = !mbar_wait(&S.own_full, 0);
+    err = !tc_wait(&S.own_full, 0);
     auto start = [&](int t, bool& end) {
       const int s = t % kStages;
-      if (!mbar_wait(&S.full[s], (t / kStages) & 1)) return false;
+      if (!tc_wait(&S.full[s], (t / kStages) & 1)) return false;
       const TileInfo& f = S.info[t % kInfo];
       end = f.at < 0;
       if (!end && P.mask != nullptr) {
@@ -151,14 +157,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
         fence_async_smem();
         __syncwarp();
       }
-      if (t > 0 && !mbar_wait(&S.s_free, (t - 1) & 1)) return false;
+      if (t > 0 && !tc_wait(&S.s_free, (t - 1) & 1)) return false;
       tc_fence_after();
-      if (lane == 0) {
+      if (elect_one()) {
         if (end) {
           mbar_arrive(&S.s_full);
         } else {
-          tc_mma_kk(tm + kColS, sQ, sK + s * kTcTileBytes, id_s, dp / 16);
-          tc_mma_kk(tm + kColDP, sO, sV + s * kTcTileBytes, id_s, dp / 16);
+          tc_mma_kk(tm + kColS, tc_desc(sQ), tc_desc(sK + s * kTcTileBytes), id_s, dp / 16);
+          tc_mma_kk(tm + kColDP, tc_desc(sO), tc_desc(sV + s * kTcTileBytes), id_s, dp / 16);
           mma_commit(&S.s_full);
         }
       }
@@ -170,130 +176,121 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
     for (int t = 0; !end && !err; ++t) {
       bool next_end = false;
       if (!start(t + 1, next_end)) { err = true; break; }
-      if (!mbar_wait(&S.ds_ready, t & 1)) { err = true; break; }
+      if (!tc_wait(&S.ds_ready, t & 1)) { err = true; break; }
       tc_fence_after();
-      if (lane == 0) {
-        tc_mma_ts(tm + kColA, tm + kColDS, sK + (t % kStages) * kTcTileBytes, id_a, t > 0);
+      if (elect_one()) {
+        tc_mma_ts(tm + kColA, tm + kColDS, tc_desc(sK + (t % kStages) * kTcTileBytes), id_a, t > 0);
         mma_commit(&S.empty[t % kStages]);
         mma_commit(&S.acc_done);
       }
       __syncwarp();
       end = next_end;
     }
-  } else {  // ---- elements: warp w has TMEM lanes 32 (w % 4).. and columns 64 (w / 4)..
-    const int row = (warp % 4) * 32 + lane, ch = warp / 4, i = i0 + row, p = p0 + row;
-    const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
-    const int E = bias_ext(P.D);
+  } else {  // ---- elements: warp w has TMEM lanes 32 (w % 4).. and columns 32 (w / 4)..
+    const int wq = warp % 4, cg = warp / 4, row = wq * 32 + lane, i = i0 + row, p = p0 + row, pw = p0 + 32 * wq;
+    const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
+    const int E = bias_ext(P.D), c0 = 16 * cg;  // c0: this thread's columns of d
     using T16 = typename E16<BF16>::T;
     const size_t stat = (static_cast<size_t>(b) * P.H + h) * P.nq + i;
     float D = 0.0f;
     if (i < P.nq) {
-      const T16* orow = row_ptr<T16>(P.o, b, h, i) + 32 * ch;
-      const T16* drow = row_ptr<T16>(P.d_o, b, h, i) + 32 * ch;
+      const T16* orow = row_ptr<T16>(P.o, b, h, i) + c0;
+      const T16* rest = P.o_lo ? reinterpret_cast<const T16*>(P.o_lo) + (orow - reinterpret_cast<const T16*>(P.o.p))
+                               : nullptr;
+      const T16* drow = row_ptr<T16>(P.d_o, b, h, i) + c0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (32 * ch + 8 * e < P.d) {
+      for (int e = 0; e < 2; ++e)
+        if (c0 + 8 * e < P.d) {
           const uint4 x = *reinterpret_cast<const uint4*>(orow + 8 * e), y = *reinterpret_cast<const uint4*>(drow + 8 * e);
-          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+          const uint4 z = rest ? *reinterpret_cast<const uint4*>(rest + 8 * e) : make_uint4(0, 0, 0, 0);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const float2 f = unpack16<BF16>(xs[u]), g = unpack16<BF16>(ys[u]);
-            D = fmaf(f.x, g.x, fmaf(f.y, g.y, D));
+            const float2 f = unpack16<BF16>(xs[u]), g = unpack16<BF16>(ys[u]), r = unpack16<BF16>(zs[u]);
+            D = fmaf(f.x + r.x, g.x, fmaf(f.y + r.y, g.y, D));
           }
         }
     }
-    S.half[ch][row] = D;
+    S.part[cg][row] = D;
     work_barrier();
-    D = S.half[0][row] + S.half[1][row];
+    D = (S.part[0][row] + S.part[1][row]) + (S.part[2][row] + S.part[3][row]);
     const float lse = i < P.nq ? P.lse[stat] : INFINITY;
-    float2 rest = make_float2(0.0f, 0.0f);
+    float2 rest = both(0.0f);
     int t = 0;
     for (;; ++t) {
-      if (!mbar_wait(&S.s_full, t & 1)) { err = true; break; }
-      const int j0 = S.info[t % kInfo].at;
-      if (j0 < 0) break;
-      uint32_t bits[4];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) bits[w] = S.info[t % kInfo].bits[w];
+      if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
+      const TileInfo& f = S.info[t % kInfo];
+      const int at = f.at, j0 = at + 32 * cg;
+      if (at < 0) break;
+      const uint32_t bits = f.bits[cg];
       tc_fence_after();
-      uint32_t sr[2][32], dr[2][32];
-#pragma unroll
-      for (int w = 0; w < 2; ++w) tmem_ld32_async(tm + lanes + kColS + 64 * ch + 32 * w, sr[w]);
-#pragma unroll
-      for (int w = 0; w < 2; ++w) tmem_ld32_async(tm + lanes + kColDP + 64 * ch + 32 * w, dr[w]);
-#pragma unroll
-      for (int w = 0; w < 2; ++w) tmem_wait_ld(sr[w]);
-#pragma unroll
-      for (int w = 0; w < 2; ++w) tmem_wait_ld(dr[w]);
+      uint32_t sr[32], dr[32], pk[16];
+      tmem_ld32_async(tm + lanes + kColS + 32 * cg, sr);
+      tmem_ld32_async(tm + lanes + kColDP + 32 * cg, dr);
+      const bool whole = bits == ~0u && block_visible(P, pw, j0);
+      const uint32_t vis = whole ? ~0u : bits & key_word(P, p, j0);
+      const bool live = whole || __any_sync(0xffffffffu, vis != 0);
+      const int side = P.w ? block_side(P, pw, j0) : 2;
+      tmem_wait_ld(sr);
+      tmem_wait_ld(dr);
       tc_fence_before();
       mbar_arrive(&S.s_free);
-      float mul = P.scale2, off = -lse;
-      if (P.w) {
-        const int dlo = p0 - j0 - 127, dhi = p0 - j0 + 127;
-        if (dlo >= P.D) {
-          off = tab[E + P.D] - lse;
-        } else if (dhi <= -P.D) {
-          off = tab[E - P.D] - lse;
-        } else {
-          const float* at = tab + (E + p - j0 - 64 * ch);
+      if (live) {
+        if (side == 0) {
+          const float* tb = tab + (E + p - j0);
 #pragma unroll
-          for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              sr[w][c] = __float_as_uint(fmaf(__uint_as_float(sr[w][c]), P.scale2, at[-(32 * w + c)]));
-          mul = 1.0f;
+          for (int c = 0; c < 32; ++c) sr[c] = __float_as_uint(fmaf(__uint_as_float(sr[c]), P.scale2, tb[-c]));
         }
-      }
-      if (!all_visible(P, p0, j0) || (bits[0] & bits[1] & bits[2] & bits[3]) != ~0u) {
-        // a hidden key's logit is -inf, and its dP (0 or, from hidden memory, anything) is 0
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint32_t vis = (ch ? bits[2 + w] : bits[w]) & row_bits(P, p, j0, 2 * ch + w);
+        if (!whole) {
+          // a hidden key's logit is -inf, and its dP (from hidden memory: anything) 0
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
             const bool on = (vis >> c) & 1u;
-            sr[w][c] = on ? sr[w][c] : 0xff800000u;
-            dr[w][c] = on ? dr[w][c] : 0u;
+            sr[c] = on ? sr[c] : 0xff800000u;
+            dr[c] = on ? dr[c] : 0u;
           }
         }
-      }
-      if (t > 0 && !mbar_wait(&S.acc_done, (t - 1) & 1)) { err = true; break; }
-      uint32_t pk[32];
+        const float2 mul = both(side == 0 ? 1.0f : P.scale2);
+        const float2 off = both((side == 1 ? tab[E + P.D] : side == -1 ? tab[E - P.D] : 0.0f) - lse);
 #pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        const int w = c / 16, e = 2 * (c % 16);
-        float2 x = make_float2(__uint_as_float(sr[w][e]), __uint_as_float(sr[w][e + 1]));
-        x = fma2(x, make_float2(mul, mul), make_float2(off, off));
-        x = make_float2(ex2(x.x), ex2(x.y));
-        const float2 dp = make_float2(__uint_as_float(dr[w][e]), __uint_as_float(dr[w][e + 1]));
-        const float2 ds = __fmul2_rn(x, __fadd2_rn(dp, make_float2(-D, -D)));
-        rest = __fadd2_rn(rest, ds);
-        pk[c] = pack16<BF16>(ds.x, ds.y);
+        for (int c = 0; c < 16; ++c) {
+          const float2 s = make_float2(__uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1]));
+          const float2 dp = make_float2(__uint_as_float(dr[2 * c]), __uint_as_float(dr[2 * c + 1]));
+          const float2 ds = mul2(exp2_pair<kPolyEvery>(fma2(s, mul, off), c), add2(dp, both(-D)));
+          rest = add2(rest, ds);
+          pk[c] = pack16<BF16>(ds.x, ds.y);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) pk[c] = 0;
       }
-      tmem_st32(tm + lanes + kColDS + 32 * ch, pk);
+      if (t > 0 && !tc_wait(&S.acc_done, (t - 1) & 1)) { err = true; break; }
+      tmem_st16(tm + lanes + kColDS + 16 * cg, pk);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&S.ds_ready);
     }
-    if (!err && t > 0) err = !mbar_wait(&S.acc_done, (t - 1) & 1);
+    if (!err && t > 0) err = !tc_wait(&S.acc_done, (t - 1) & 1);
     tc_fence_after();
-    uint32_t v[32];
-    const int c0 = 32 * ch;
-    if (t > 0 && c0 < P.d) {
-      tmem_ld32_async(tm + lanes + kColA + c0, v);
-      tmem_wait_ld(v);
+    if (c0 < P.d) {
+      uint32_t v[16];
+      if (t > 0) {
+        tmem_ld16_async(tm + lanes + kColA + c0, v);
+        tmem_wait_ld16(v);
+      }
+      if (i < P.nq) store_row16<BF16>(P.d_q, b, h, i, c0, P.d, v, P.scale, t == 0);
     }
-    if (i < P.nq && c0 < P.d) store_row32<BF16>(P.d_q, b, h, i, c0, P.d, v, P.scale, t == 0);
     work_barrier();
-    S.half[ch][row] = rest.x + rest.y;
+    S.part[cg][row] = rest.x + rest.y;
     work_barrier();
-    if (ch == 0 && i < P.nq) P.dsum[stat] = D + (S.half[0][row] + S.half[1][row]);
+    if (cg == 0 && i < P.nq)
+      P.dsum[stat] = D + ((S.part[0][row] + S.part[1][row]) + (S.part[2][row] + S.part[3][row]));
   }
   if (err) report_timeout(P.status);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tm, 512);
+  if (warp == kMmaWarp) tmem_dealloc(tm, 512);
 }
 
 template <bool BF16>
@@ -307,8 +304,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
   float* tab = reinterpret_cast<float*>(&S + 1);
   const int W = 2 * P.D + 1;
   float* acc = tab + (P.w ? 2 * bias_ext(P.D) + 1 : 0);  // W sums by distance
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int hk = blockIdx.y, b = blockIdx.z, j0 = blockIdx.x * kTcRows;
+  const int warp = warp_index(), lane = threadIdx.x % 32;
+  const int hk = blockIdx.x % P.Hkv, b = blockIdx.x / P.Hkv % P.B, tile = blockIdx.x / P.Hkv / P.B;
+  const int j0 = tile * kTcRows;  // the sinks' tiles, which all queries see, first
   bool err = false;
   if (threadIdx.x == 0) {
     mbar_init(&S.own_full, 1);
@@ -319,7 +317,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
     mbar_init(&S.acc_done, 1);
     fence_mbar_init();
   }
-  if (warp == 8) tmem_alloc(&S.tmem, 512);
+  if (warp == kMmaWarp) tmem_alloc(&S.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -335,7 +333,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
   i_lo = max(i_lo, 0) / kTcRows;
   i_hi = (min(i_hi, P.nq) + kTcRows - 1) / kTcRows;  // in tiles
 
-  if (warp == 9) {  // ---- producer
+  if (warp == kTmaWarp) {  // ---- producer
     uint32_t bits[4];
     key_bits(P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr, j0, P.nk, lane, bits);
     const int per = (bits[0] | bits[1] | bits[2] | bits[3]) == 0 ? 0 : max(0, i_hi - i_lo);
@@ -358,7 +356,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
           st[1][e] = i < P.nq ? P.dsum[at + i] : 0.0f;
         }
       }
-      if (!mbar_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
+      if (!tc_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
       if (i0 >= 0) {
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -380,22 +378,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
         }
       }
     }
-  } else if (warp == 8) {  // ---- MMA
+  } else if (warp == kMmaWarp) {  // ---- MMA
     const int dp = (P.d + 15) / 16 * 16;
     const uint32_t id_s = tc_idesc(128, 128, BF16, false), id_a = tc_idesc(128, dp, BF16, true);
-    err = !mbar_wait(&S.own_full, 0);
+    err = !tc_wait(&S.own_full, 0);
     auto start = [&](int t, bool& end) {
       const int s = t % kStages;
-      if (!mbar_wait(&S.full[s], (t / kStages) & 1)) return false;
+      if (!tc_wait(&S.full[s], (t / kStages) & 1)) return false;
       end = S.info[t % kInfo].at < 0;
-      if (t > 0 && !mbar_wait(&S.s_free, (t - 1) & 1)) return false;
+      if (t > 0 && !tc_wait(&S.s_free, (t - 1) & 1)) return false;
       tc_fence_after();
-      if (lane == 0) {
+      if (elect_one()) {
         if (end) {
           mbar_arrive(&S.s_full);
         } else {
-          tc_mma_kk(tm + kColS, sK, sQ + s * kTcTileBytes, id_s, dp / 16);
-          tc_mma_kk(tm + kColDP, sV, sO + s * kTcTileBytes, id_s, dp / 16);
+          tc_mma_kk(tm + kColS, tc_desc(sK), tc_desc(sQ + s * kTcTileBytes), id_s, dp / 16);
+          tc_mma_kk(tm + kColDP, tc_desc(sV), tc_desc(sO + s * kTcTileBytes), id_s, dp / 16);
           mma_commit(&S.s_full);
         }
       }
@@ -407,21 +405,21 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
     for (int t = 0; !end && !err; ++t) {
       bool next_end = false;
       if (!start(t + 1, next_end)) { err = true; break; }
-      if (!mbar_wait(&S.ds_ready, t & 1)) { err = true; break; }
+      if (!tc_wait(&S.ds_ready, t & 1)) { err = true; break; }
       tc_fence_after();
-      if (lane == 0) {
+      if (elect_one()) {
         const int s = t % kStages;
-        tc_mma_ts(tm + kColA, tm + kColP, sO + s * kTcTileBytes, id_a, t > 0);
-        tc_mma_ts(tm + kColB, tm + kColDS, sQ + s * kTcTileBytes, id_a, t > 0);
+        tc_mma_ts(tm + kColA, tm + kColP, tc_desc(sO + s * kTcTileBytes), id_a, t > 0);
+        tc_mma_ts(tm + kColB, tm + kColDS, tc_desc(sQ + s * kTcTileBytes), id_a, t > 0);
         mma_commit(&S.empty[s]);
         mma_commit(&S.acc_done);
       }
       __syncwarp();
       end = next_end;
     }
-  } else {  // ---- elements: a key row and half of the tile's queries per thread
-    const int row = (warp % 4) * 32 + lane, ch = warp / 4, j = j0 + row, tid = threadIdx.x;
-    const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+  } else {  // ---- elements: a key row and a quarter of the tile's queries per thread
+    const int wq = warp % 4, cg = warp / 4, row = wq * 32 + lane, j = j0 + row, jw = j0 + 32 * wq, tid = threadIdx.x;
+    const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
     const int E = bias_ext(P.D);
     const bool dw = P.dw_part != nullptr;
     float lo = 0.0f, hi = 0.0f;  // sums of dS beyond the table's ends
@@ -438,20 +436,20 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
         acc[tid == 0 ? 0 : 2 * P.D] += s;
       }
       work_barrier();
-      float* dst = P.dw_part + (static_cast<size_t>(hk * P.G + head) * P.parts + b * gridDim.x + blockIdx.x) * W;
+      float* dst = P.dw_part + (static_cast<size_t>(hk * P.G + head) * P.parts + b * (P.parts / P.B) + tile) * W;
       for (int x = tid; x < W; x += kWork) dst[x] = acc[x];
       lo = hi = 0.0f;
     };
     // the heads from `from` on have no tile here: their sums are zero
     auto zero_heads = [&](int from) {
       for (int g = from; g < P.G; ++g) {
-        float* dst = P.dw_part + (static_cast<size_t>(hk * P.G + g) * P.parts + b * gridDim.x + blockIdx.x) * W;
+        float* dst = P.dw_part + (static_cast<size_t>(hk * P.G + g) * P.parts + b * (P.parts / P.B) + tile) * W;
         for (int x = tid; x < W; x += kWork) dst[x] = 0.0f;
       }
     };
     int t = 0;
     for (;; ++t) {
-      if (!mbar_wait(&S.s_full, t & 1)) { err = true; break; }
+      if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
       const int i0 = S.info[t % kInfo].at, g = S.info[t % kInfo].head;
       if (i0 < 0) break;
       if (g != head) {
@@ -463,123 +461,107 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
           for (int x = tid; x < W; x += kWork) acc[x] = 0.0f;
         work_barrier();
       }
-      const uint32_t kbits = S.info[t % kInfo].bits[warp % 4];
-      const bool whole = (S.info[t % kInfo].bits[0] & S.info[t % kInfo].bits[1] & S.info[t % kInfo].bits[2] &
-                          S.info[t % kInfo].bits[3]) == ~0u;
-      const float* lse = S.stat[t % kStages][0] + 64 * ch;
-      const float* Dv = S.stat[t % kStages][1] + 64 * ch;
+      const uint32_t kbits = S.info[t % kInfo].bits[wq];
+      const float* lse = S.stat[t % kStages][0] + 32 * cg;
+      const float* Dv = S.stat[t % kStages][1] + 32 * cg;
+      const int p0 = i0 + P.qs, pw = p0 + 32 * cg;
       tc_fence_after();
-      uint32_t sr[2][32], dr[2][32];
-#pragma unroll
-      for (int w = 0; w < 2; ++w) tmem_ld32_async(tm + lanes + kColS + 64 * ch + 32 * w, sr[w]);
-#pragma unroll
-      for (int w = 0; w < 2; ++w) tmem_ld32_async(tm + lanes + kColDP + 64 * ch + 32 * w, dr[w]);
-#pragma unroll
-      for (int w = 0; w < 2; ++w) tmem_wait_ld(sr[w]);
-#pragma unroll
-      for (int w = 0; w < 2; ++w) tmem_wait_ld(dr[w]);
+      uint32_t sr[32], dr[32], pk[16];
+      tmem_ld32_async(tm + lanes + kColS + 32 * cg, sr);
+      tmem_ld32_async(tm + lanes + kColDP + 32 * cg, dr);
+      const bool whole = kbits == ~0u && block_visible(P, pw, jw);
+      const uint32_t vis = whole ? ~0u : (kbits >> lane) & 1u ? query_word(P, j, pw) : 0u;
+      const bool live = whole || __any_sync(0xffffffffu, vis != 0);
+      const int side = P.w ? block_side(P, pw, jw) : 2;
+      tmem_wait_ld(sr);
+      tmem_wait_ld(dr);
       tc_fence_before();
       mbar_arrive(&S.s_free);
-      const int p0 = i0 + P.qs;
-      float mul = P.scale2, add = 0.0f;
-      int side = 0;  // where the tile's distances lie: in the table, or beyond an end
-      const int dlo = p0 - j0 - 127, dhi = p0 - j0 + 127;
-      if (P.w) {
-        if (dlo >= P.D) {
-          add = tab[E + P.D];
-          side = 1;
-        } else if (dhi <= -P.D) {
-          add = tab[E - P.D];
-          side = -1;
-        } else {
-          const float* at = tab + (E + p0 + 64 * ch - j);
+      if (live) {
+        if (side == 0) {
+          const float* tb = tab + (E + pw - j);
 #pragma unroll
-          for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              sr[w][c] = __float_as_uint(fmaf(__uint_as_float(sr[w][c]), P.scale2, at[32 * w + c]));
-          mul = 1.0f;
+          for (int c = 0; c < 32; ++c) sr[c] = __float_as_uint(fmaf(__uint_as_float(sr[c]), P.scale2, tb[c]));
         }
-      }
-      if (!all_visible(P, p0, j0) || !whole) {
-        // queries [a, b) of the tile see this key through the window, all from `from` on as a sink
-        const bool on = (kbits >> lane) & 1u;
-        const int a = P.causal ? j - p0 : j - P.window + 1 - p0, z = j + P.window - p0;
-        const int from = P.causal ? j - p0 : 0;
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          uint32_t vis = range_word(a, z, 2 * ch + w);
-          if (j < P.sinks) vis |= range_word(from, kTcRows, 2 * ch + w);
-          if (!on) vis = 0;
+        if (!whole) {
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
-            const bool k = (vis >> c) & 1u;
-            sr[w][c] = k ? sr[w][c] : 0xff800000u;
-            dr[w][c] = k ? dr[w][c] : 0u;
+            const bool on = (vis >> c) & 1u;
+            sr[c] = on ? sr[c] : 0xff800000u;
+            dr[c] = on ? dr[c] : 0u;
           }
         }
-      }
-      if (t > 0 && !mbar_wait(&S.acc_done, (t - 1) & 1)) { err = true; break; }
-      uint32_t pk[32];
+        const float2 mul = both(side == 0 ? 1.0f : P.scale2);
+        const float2 add = both(side == 1 ? tab[E + P.D] : side == -1 ? tab[E - P.D] : 0.0f);
 #pragma unroll
-      for (int c = 0; c < 32; c += 2) {  // four queries
-        const int w = c / 16, e = 2 * (c % 16);
-        const float4 ls = *reinterpret_cast<const float4*>(lse + 2 * c);
-        const float4 dd = *reinterpret_cast<const float4*>(Dv + 2 * c);
-        const float2 l2[2] = {make_float2(ls.x, ls.y), make_float2(ls.z, ls.w)};
-        const float2 d2[2] = {make_float2(dd.x, dd.y), make_float2(dd.z, dd.w)};
+        for (int c = 0; c < 16; c += 2) {  // four queries
+          const float4 ls = *reinterpret_cast<const float4*>(lse + 2 * c);
+          const float4 dd = *reinterpret_cast<const float4*>(Dv + 2 * c);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float2 x = make_float2(__uint_as_float(sr[w][e + 2 * u]), __uint_as_float(sr[w][e + 2 * u + 1]));
-          x = fma2(x, make_float2(mul, mul), fma2(l2[u], make_float2(-1.0f, -1.0f), make_float2(add, add)));
-          x = make_float2(ex2(x.x), ex2(x.y));
-          pk[c + u] = pack16<BF16>(x.x, x.y);
-          const float2 dp = make_float2(__uint_as_float(dr[w][e + 2 * u]), __uint_as_float(dr[w][e + 2 * u + 1]));
-          const float2 ds = __fmul2_rn(x, fma2(d2[u], make_float2(-1.0f, -1.0f), dp));
-          dr[w][e + 2 * u] = __float_as_uint(ds.x);
-          dr[w][e + 2 * u + 1] = __float_as_uint(ds.y);
+          for (int u = 0; u < 2; ++u) {
+            const float2 l2 = u ? make_float2(ls.z, ls.w) : make_float2(ls.x, ls.y);
+            const float2 d2 = u ? make_float2(dd.z, dd.w) : make_float2(dd.x, dd.y);
+            const int e = 2 * (c + u);
+            const float2 s = make_float2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
+            const float2 dp = make_float2(__uint_as_float(dr[e]), __uint_as_float(dr[e + 1]));
+            const float2 x = exp2_pair<kPolyEvery>(fma2(s, mul, fma2(l2, both(-1.0f), add)), c + u);
+            const float2 ds = mul2(x, fma2(d2, both(-1.0f), dp));
+            pk[c + u] = pack16<BF16>(x.x, x.y);
+            dr[e] = __float_as_uint(ds.x);
+            dr[e + 1] = __float_as_uint(ds.y);
+          }
         }
-      }
-      tmem_st32(tm + lanes + kColP + 32 * ch, pk);
+      } else {
 #pragma unroll
-      for (int c = 0; c < 32; ++c)
-        pk[c] = pack16<BF16>(__uint_as_float(dr[c / 16][2 * (c % 16)]), __uint_as_float(dr[c / 16][2 * (c % 16) + 1]));
-      tmem_st32(tm + lanes + kColDS + 32 * ch, pk);
+        for (int c = 0; c < 16; ++c) pk[c] = 0;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) dr[c] = 0;
+      }
+      if (t > 0 && !tc_wait(&S.acc_done, (t - 1) & 1)) { err = true; break; }
+      tmem_st16(tm + lanes + kColP + 16 * cg, pk);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) pk[c] = pack16<BF16>(__uint_as_float(dr[2 * c]), __uint_as_float(dr[2 * c + 1]));
+      tmem_st16(tm + lanes + kColDS + 16 * cg, pk);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&S.ds_ready);
       if (dw) {
-        if (side != 0) {
-          float2 s2 = make_float2(0.0f, 0.0f);
+        const int dlo = p0 - j0 - 127, dhi = p0 - j0 + 127;  // the tile's distances
+        if (dlo >= P.D || dhi <= -P.D) {
+          float2 s2 = both(0.0f);
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            s2 = __fadd2_rn(s2, make_float2(__uint_as_float(dr[c / 16][2 * (c % 16)]),
-                                            __uint_as_float(dr[c / 16][2 * (c % 16) + 1])));
-          if (side > 0) hi += s2.x + s2.y;
+          for (int c = 0; c < 16; ++c)
+            s2 = add2(s2, make_float2(__uint_as_float(dr[2 * c]), __uint_as_float(dr[2 * c + 1])));
+          if (dlo >= P.D) hi += s2.x + s2.y;
           else lo += s2.x + s2.y;
         } else {
-          // Diagonals of this warp's strip (32 keys x 64 queries): the running sum of a diagonal moves one
-          // lane up as the query advances, and is complete once lane 31 has added its element.
+          // Diagonals of this warp's block of 32 keys x 32 queries: the running sum of a diagonal moves one lane
+          // up as the query advances, and is complete once lane 31 has added its element.
           float* out = S.diag[strip][warp];
           float run = 0.0f;
+          if (live) {
 #pragma unroll
-          for (int c = 0; c < 64; ++c) {
-            run += __uint_as_float(dr[c / 32][c % 32]);
-            if (c < 63) {
-              if (lane == 31) out[c] = run;
-              run = __shfl_up_sync(0xffffffffu, run, 1);
-              if (lane == 0) run = 0.0f;
+            for (int c = 0; c < 32; ++c) {
+              run += __uint_as_float(dr[c]);
+              if (c < 31) {
+                if (lane == 31) out[c] = run;
+                run = __shfl_up_sync(0xffffffffu, run, 1);
+                if (lane == 0) run = 0.0f;
+              }
             }
+          } else {
+            out[lane] = 0.0f;  // slots 0..30 (slot 31 is lane 31's below)
+            __syncwarp();
           }
-          out[94 - lane] = run;  // slot x + 31 for diagonal x = query - key of the strip
+          out[62 - lane] = run;  // slot x + 31 for diagonal x = query - key of the block
           work_barrier();
           if (tid < 2 * kTcRows - 1) {
             const int e = tid - (kTcRows - 1);  // query - key within the tile
             float s = 0.0f;
 #pragma unroll
             for (int w = 0; w < kWork / 32; ++w) {
-              const int x = e - 64 * (w / 4) + 32 * (w % 4) + 31;
-              if (x >= 0 && x < 95) s += S.diag[strip][w][x];
+              const int x = e - 32 * (w / 4) + 32 * (w % 4) + 31;
+              if (x >= 0 && x < 63) s += S.diag[strip][w][x];
             }
             const int delta = p0 - j0 + e;
             if (delta <= -P.D) lo += s;
@@ -594,28 +576,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
       if (head >= 0) flush();
       zero_heads(head + 1);
     }
-    if (!err && t > 0) err = !mbar_wait(&S.acc_done, (t - 1) & 1);
+    if (!err && t > 0) err = !tc_wait(&S.acc_done, (t - 1) & 1);
     tc_fence_after();
-    const int c0 = 32 * ch;
+    const int c0 = 16 * cg;
     if (c0 < P.d) {
-      uint32_t v[32];
+      uint32_t v[16];
       if (t > 0) {
-        tmem_ld32_async(tm + lanes + kColA + c0, v);
-        tmem_wait_ld(v);
+        tmem_ld16_async(tm + lanes + kColA + c0, v);
+        tmem_wait_ld16(v);
       }
-      if (j < P.nk) store_row32<BF16>(P.d_v, b, hk, j, c0, P.d, v, 1.0f, t == 0);
+      if (j < P.nk) store_row16<BF16>(P.d_v, b, hk, j, c0, P.d, v, 1.0f, t == 0);
       if (t > 0) {
-        tmem_ld32_async(tm + lanes + kColB + c0, v);
-        tmem_wait_ld(v);
+        tmem_ld16_async(tm + lanes + kColB + c0, v);
+        tmem_wait_ld16(v);
       }
-      if (j < P.nk) store_row32<BF16>(P.d_k, b, hk, j, c0, P.d, v, P.scale, t == 0);
+      if (j < P.nk) store_row16<BF16>(P.d_k, b, hk, j, c0, P.d, v, P.scale, t == 0);
     }
   }
   if (err) report_timeout(P.status);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tm, 512);
+  if (warp == kMmaWarp) tmem_dealloc(tm, 512);
 }
 
 }  // namespace
@@ -635,9 +617,9 @@ cudaError_t launch_attn_tc_bwd(const AttnParams& P, int dtype, cudaStream_t st) 
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
-  dq<<<dim3((P.nq + kTcRows - 1) / kTcRows, P.H, P.B), kBwdThreads, smem, st>>>(T);
+  dq<<<tc_grid(P.nq, P.H, P.B), kBwdThreads, smem, st>>>(T);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  dkv<<<dim3((P.nk + kTcRows - 1) / kTcRows, P.Hkv, P.B), kBwdThreads, smem, st>>>(T);
+  dkv<<<tc_grid(P.nk, P.Hkv, P.B), kBwdThreads, smem, st>>>(T);
   return cudaGetLastError();
 }
 

@@ -144,7 +144,7 @@ Problem make_problem(const Tensor& Q, const Tensor& K, const Tensor& V, const op
   return r;
 }
 
-dfs_attn_args args_of(const Problem& r, const Tensor& o, const Tensor& lse) {
+dfs_attn_args args_of(const Problem& r, const Tensor& o, const Tensor& lse, const Tensor& o_lo) {
   dfs_attn_args a{};
   a.q = strided(r.q);
   a.k = strided(r.k);
@@ -153,16 +153,19 @@ dfs_attn_args args_of(const Problem& r, const Tensor& o, const Tensor& lse) {
   a.lse = lse.defined() ? lse.data_ptr<float>() : nullptr;
   a.mask = r.mask.defined() ? static_cast<const uint8_t*>(r.mask.data_ptr()) : nullptr;
   a.bias = bias_of(r.w, r.lut, r.max_distance);
+  a.o_lo = o_lo.defined() ? o_lo.data_ptr() : nullptr;
   return a;
 }
 
 cudaStream_t stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
-Tensor run_forward(const Problem& r, bool keep, Tensor* lse) {
+// keep: what the backward needs, lse and (16-bit types) what the rounding of o took
+Tensor run_forward(const Problem& r, bool keep, Tensor* lse, Tensor* o_lo) {
   const DeviceSwitch guard(r.q.device());
   Tensor o = like(r.q);
   if (keep) *lse = at::empty({r.q.size(0), r.q.size(1), r.q.size(2)}, r.q.options().dtype(at::kFloat));
-  dfs_attn_args a = args_of(r, o, keep ? *lse : Tensor());
+  if (keep && r.p.dtype != DFS_F32) *o_lo = like(r.q);
+  dfs_attn_args a = args_of(r, o, keep ? *lse : Tensor(), keep ? *o_lo : Tensor());
   a.status = checked_status(r.q.device());
   check_rc(dfs_window_attn_fwd(&r.p, &a, stream_of(r.q)), "dfs_window_attn_fwd");
   return o;
@@ -173,9 +176,9 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
                         optional<Tensor> mask, optional<Tensor> lut, int64_t max_distance, int64_t window, int64_t sinks, bool causal,
                         int64_t q_start, double scale) {
     const Problem r = make_problem(Q, K, V, mask, weight, lut, max_distance, window, sinks, causal, q_start, scale);
-    Tensor lse;
-    Tensor o = run_forward(r, true, &lse);
-    ctx->save_for_backward({r.q, r.k, r.v, r.mask, r.w, r.lut, o, lse});
+    Tensor lse, o_lo;
+    Tensor o = run_forward(r, true, &lse, &o_lo);
+    ctx->save_for_backward({r.q, r.k, r.v, r.mask, r.w, r.lut, o, lse, o_lo});
     ctx->saved_data["max_distance"] = max_distance;
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
@@ -194,13 +197,13 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
                                    ctx->saved_data["max_distance"].toInt(), ctx->saved_data["window"].toInt(),
                                    ctx->saved_data["sinks"].toInt(), ctx->saved_data["causal"].toBool(),
                                    ctx->saved_data["q_start"].toInt(), ctx->saved_data["scale"].toDouble());
-    const Tensor &o = s[6], &lse = s[7];
+    const Tensor &o = s[6], &lse = s[7], &o_lo = s[8];
     const DeviceSwitch guard(r.q.device());
     const Tensor dO = walkable(grads[0].to(r.q.scalar_type()));
     Tensor dq = like(r.q), dk = like(r.k), dv = like(r.v), dw;
     const bool want_w = r.w.defined() && ctx->needs_input_grad(3);  // the edge after Q, K, V where there is one
     if (want_w) dw = at::empty_like(r.w);
-    dfs_attn_args a = args_of(r, o, lse);
+    dfs_attn_args a = args_of(r, o, lse, o_lo);
     a.d_o = strided(dO);
     a.d_q = strided(dq);
     a.d_k = strided(dk);
@@ -228,7 +231,7 @@ Tensor window_attn(Tensor Q, Tensor K, Tensor V, optional<Tensor> mask, optional
     return WindowAttnFn::apply(Q, K, V, has_w ? weight : c10::nullopt, mask, lut, max_distance, window, sinks,
                                causal, q_start, scale);
   return run_forward(make_problem(Q, K, V, mask, weight, lut, max_distance, window, sinks, causal, q_start, scale), false,
-                     nullptr);
+                     nullptr, nullptr);
 }
 
 Tensor window_attn_decode(Tensor q, Tensor K, Tensor V, Tensor lengths, optional<Tensor> weight, optional<Tensor> lut,
@@ -242,7 +245,7 @@ Tensor window_attn_decode(Tensor q, Tensor K, Tensor V, Tensor lengths, optional
   const Tensor len = lengths.contiguous().to(at::kInt);
   const DeviceSwitch guard(q.device());
   Tensor o = at::empty(q.sizes(), q.options());
-  dfs_attn_args a = args_of(r, o.unsqueeze(2), Tensor());
+  dfs_attn_args a = args_of(r, o.unsqueeze(2), Tensor(), Tensor());
   a.status = checked_status(q.device());
   check_rc(dfs_window_attn_decode(&r.p, &a, len.data_ptr<int32_t>(), stream_of(q)), "dfs_window_attn_decode");
   return o;

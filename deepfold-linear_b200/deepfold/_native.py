@@ -99,7 +99,7 @@ class DfsStrided(ctypes.Structure):
 
 class DfsAttnArgs(ctypes.Structure):
     _fields_ = [("q", DfsStrided), ("k", DfsStrided), ("v", DfsStrided), ("o", DfsStrided), ("lse", _P),
-                ("mask", _P), ("bias", DfsRelBias), ("d_o", DfsStrided), ("d_q", DfsStrided),
+                ("mask", _P), ("bias", DfsRelBias), ("o_lo", _P), ("d_o", DfsStrided), ("d_q", DfsStrided),
                 ("d_k", DfsStrided), ("d_v", DfsStrided), ("d_weight", _P), ("status", _P)]
 
 

@@ -459,6 +459,8 @@ typedef struct {
                            /* by the forward unless NULL, read by the backward                  */
   const uint8_t* mask;     /* (B,n_k) 1 = real key, 0 = hidden; or NULL                         */
   dfs_relbias bias;
+  void* o_lo;              /* laid out as o: what the rounding of o took (16-bit types), written by */
+                           /* the forward and read by the backward; or NULL in both              */
   /* backward only: gradients of o (in) and of q, k, v, bias.weight (out; d_weight may be NULL) */
   dfs_strided d_o, d_q, d_k, d_v;
   void* d_weight;

@@ -75,7 +75,7 @@ def test_struct_sizes_match_header_layout():
     assert ctypes.sizeof(nat.DfsRelBias) == 32
     assert ctypes.sizeof(nat.DfsAttnProblem) == 48
     assert ctypes.sizeof(nat.DfsStrided) == 32
-    assert ctypes.sizeof(nat.DfsAttnArgs) == 8 * 32 + 32 + 4 * 8
+    assert ctypes.sizeof(nat.DfsAttnArgs) == 8 * 32 + 32 + 5 * 8
 
 
 def attn(**kw):
