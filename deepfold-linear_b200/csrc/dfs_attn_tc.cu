@@ -13,12 +13,17 @@
 // clocks, the two products 512.  So part of them run on the FMA pipes, and two
 // CTAs share an SM (256 of its 512 TMEM columns each), with 16 element warps
 // between them to cover TMEM and barrier latencies.
+#include <type_traits>
+
 #include "dfs_attn_tc.cuh"
 
 namespace dfs {
 namespace {
 
-constexpr int kFwdThreads = 320;
+// 384 threads x 80 registers at launch = 256 x 104 (elements) + 128 x 32 (MMA, TMA and two idle warps)
+constexpr int kFwdThreads = 384;
+constexpr int kElementRegs = 104, kOtherRegs = 32;
+static_assert(256 * kElementRegs + 128 * kOtherRegs <= kFwdThreads * 80, "register shares");
 constexpr int kWork = 256;  // threads of the element warps
 constexpr int kKStages = 3, kVStages = 2, kInfo = 4;
 // the running maximum may lag by this much (log2) before O is rescaled: P stays
@@ -71,6 +76,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
   tc_fence_after();
   const uint32_t tm = S.tmem;
 
+  if (warp >= 8) regs_down<kOtherRegs>();
   if (warp == 9) {  // ---- producer
     const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
     const TcKeyTiles tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
@@ -93,6 +99,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
         f.at = j0;
 #pragma unroll
         for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
+        describe_tile(P, f, p0, j0);
         if (j0 < 0) {
           mbar_arrive(&S.k_full[ks]);
         } else {
@@ -163,41 +170,35 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
       __syncwarp();
       end = next_end;
     }
-  } else {  // ---- elements: warp w has rows 32 (w % 4).. and columns 64 (w / 4)..
+  } else if (warp < 8) {  // ---- elements: warp w has rows 32 (w % 4).. and columns 64 (w / 4)..
+    regs_up<kElementRegs>();
     const int wq = warp % 4, ch = warp / 4;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
     const int row = wq * 32 + lane, i = i0 + row, p = p0 + row, pw = p0 + wq * 32;
     const int E = bias_ext(P.D), c0 = 32 * ch;  // c0: this thread's columns of O
     float m = -INFINITY;
     float2 l = make_float2(0.0f, 0.0f);
-    int t = 0;
-    for (;; ++t) {
-      if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
-      const TileInfo& f = S.info[t % kInfo];
-      const int at = f.at;
-      if (at < 0) break;
-      const int j0 = at + 64 * ch;
-      const uint32_t bits[2] = {f.bits[2 * ch], f.bits[2 * ch + 1]};
-      tc_fence_after();
-      uint32_t sr[2][32];
-      tmem_ld32_async(tm + lanes + kColS + 64 * ch, sr[0]);
-      tmem_ld32_async(tm + lanes + kColS + 64 * ch + 32, sr[1]);
-      // per block of 32 x 32: whether any pair is visible, and the logits (log2 units) as mul s + add
-      bool live[2], whole[2];
-      uint32_t vis[2];
-      float mul[2], add[2];
+    const float far_hi = P.w ? tab[E + P.D] : 0.0f, far_lo = P.w ? tab[E - P.D] : 0.0f;
+    // One tile, S on its way to sr.  Plain tiles (all but a row's first and last few) need no look at masks
+    // or distances; the others are taken apart into blocks of 32 x 32.
+    auto step = [&](auto is_plain, int t, uint32_t (&sr)[2][32], int j0, const uint32_t (&bits)[2], float far) -> bool {
+      constexpr bool kPlain = decltype(is_plain)::value;
+      bool live[2] = {true, true}, whole[2] = {true, true};
+      uint32_t vis[2] = {~0u, ~0u};
+      float mul[2] = {P.scale2, P.scale2}, add[2] = {far, far};  // logits (log2 units) are mul s + add
+      int side[2] = {1, 1};
+      if (!kPlain) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        whole[u] = bits[u] == ~0u && block_visible(P, pw, j0 + 32 * u);
-        vis[u] = ~0u;
-        live[u] = true;
-        if (!whole[u]) {
-          vis[u] = bits[u] & key_word(P, p, j0 + 32 * u);
-          live[u] = __any_sync(0xffffffffu, vis[u] != 0);
+        for (int u = 0; u < 2; ++u) {
+          whole[u] = bits[u] == ~0u && block_visible(P, pw, j0 + 32 * u);
+          if (!whole[u]) {
+            vis[u] = bits[u] & key_word(P, p, j0 + 32 * u);
+            live[u] = __any_sync(0xffffffffu, vis[u] != 0);
+          }
+          side[u] = P.w ? block_side(P, pw, j0 + 32 * u) : 2;
+          mul[u] = side[u] == 0 ? 1.0f : P.scale2;
+          add[u] = side[u] == 1 ? far_hi : side[u] == -1 ? far_lo : 0.0f;
         }
-        const int side = block_side(P, pw, j0 + 32 * u);
-        mul[u] = P.w && side == 0 ? 1.0f : P.scale2;
-        add[u] = P.w && side != 0 ? tab[E + (side > 0 ? P.D : -P.D)] : 0.0f;
       }
       tmem_wait_ld(sr[0]);
       tmem_wait_ld(sr[1]);
@@ -206,25 +207,24 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
       float top = -INFINITY;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        if (!live[u]) continue;
-        if (P.w && block_side(P, pw, j0 + 32 * u) == 0) {
-          const float* tb = tab + (E + p - j0 - 32 * u);
+        if (!kPlain) {
+          if (!live[u]) continue;
+          if (side[u] == 0) {
+            const float* tb = tab + (E + p - j0 - 32 * u);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) sr[u][c] = __float_as_uint(fmaf(__uint_as_float(sr[u][c]), P.scale2, tb[-c]));
+            for (int c = 0; c < 32; ++c) sr[u][c] = __float_as_uint(fmaf(__uint_as_float(sr[u][c]), P.scale2, tb[-c]));
+          }
+          if (!whole[u]) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) sr[u][c] = (vis[u] >> c) & 1u ? sr[u][c] : 0xff800000u;
+          }
         }
-        if (!whole[u]) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) sr[u][c] = (vis[u] >> c) & 1u ? sr[u][c] : 0xff800000u;
-        }
-        float v[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(sr[u][c]);
-        top = fmaxf(top, fmaf(max32(v), mul[u], add[u]));
+        top = fmaxf(top, fmaf(max32u(sr[u]), mul[u], add[u]));
       }
       S.top[t & 1][ch][row] = top;
       asm volatile("bar.sync %0, 64;" ::"r"(1 + wq) : "memory");
       top = fmaxf(top, S.top[t & 1][ch ^ 1][row]);
-      if (t > 0 && !tc_wait(&S.pv_done, (t - 1) & 1)) { err = true; break; }
+      if (t > 0 && !tc_wait(&S.pv_done, (t - 1) & 1)) return false;
       const bool raise = top > m + kLag || (m == -INFINITY && top > -INFINITY);
       if (__any_sync(0xffffffffu, raise)) {
         const float mn = raise ? top : m;
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t pk[16];
-        if (live[u]) {
+        if (kPlain || live[u]) {
           const float2 mu = both(mul[u]), off = both(add[u] - ref);
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
@@ -265,6 +265,27 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&S.p_ready);
+      return true;
+    };
+    int t = 0;
+    for (;; ++t) {
+      if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
+      const TileInfo& f = S.info[t % kInfo];
+      const int at = f.at;
+      if (at < 0) break;
+      const bool plain = f.plain;
+      const int tile_side = f.side;
+      const int j0 = at + 64 * ch;
+      const uint32_t bits[2] = {f.bits[2 * ch], f.bits[2 * ch + 1]};
+      tc_fence_after();
+      uint32_t sr[2][32];
+      tmem_ld32_async(tm + lanes + kColS + 64 * ch, sr[0]);
+      tmem_ld32_async(tm + lanes + kColS + 64 * ch + 32, sr[1]);
+      if (plain)
+        err = !step(std::true_type(), t, sr, j0, bits, tile_side > 0 ? far_hi : tile_side < 0 ? far_lo : 0.0f);
+      else
+        err = !step(std::false_type(), t, sr, j0, bits, 0.0f);
+      if (err) break;
     }
     if (!err && t > 0) err = !tc_wait(&S.pv_done, (t - 1) & 1);
     tc_fence_after();
@@ -326,7 +347,7 @@ cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st) 
   T.d_o = T.q;
   const size_t smem = 1024 + (1 + kKStages + kVStages) * kTcTileBytes + sizeof(FwdShared) + bias_ext_bytes(P);
   auto kern = bf16 ? tc_fwd_kernel<true> : tc_fwd_kernel<false>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  const cudaError_t e = prepare_split(kern, smem, kFwdThreads, 256 * kElementRegs + 128 * kOtherRegs);
   if (e != cudaSuccess) return e;
   kern<<<tc_grid(P.nq, P.H, P.B), kFwdThreads, smem, st>>>(T);
   return cudaGetLastError();

@@ -29,6 +29,17 @@ DFS_DEV void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accum));
 }
 
+// maximum of 32 values held as bits
+DFS_DEV float max32u(const uint32_t (&v)[32]) {
+  float a[3];
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    a[i] = fmax3(__uint_as_float(v[3 * i]), __uint_as_float(v[3 * i + 1]), __uint_as_float(v[3 * i + 2]));
+#pragma unroll
+  for (int i = 9; i + 1 < 32; i += 2) a[(i / 2) % 3] = fmax3(a[(i / 2) % 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+  return fmaxf(fmax3(a[0], a[1], a[2]), __uint_as_float(v[31]));
+}
+
 // One lane of a converged warp.  The compiler keeps what that lane computes in
 // uniform registers, where the MMA takes its descriptors from; a branch on the
 // lane number moved each there one by one, and issuing 8 MMAs took 600 clocks.
@@ -178,9 +189,9 @@ DFS_DEV float2 exp2_pair(float2 x, int c) {
   return kEvery > 0 && c % kEvery == kEvery - 1 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
 }
 
-// Wait for the phase with the given parity; false once about two seconds of clock
-// cycles have passed.  The clock is only looked at every 1024 tries: reading it
-// on the way through a wait that is about to end costs more than the wait.
+// Wait for the phase with the given parity; false once four billion clocks (some two
+// seconds) have passed.  The clock is read on every 1024th try only, never on the
+// way through a short wait.  (A sleep hint on the try made waits wake late.)
 DFS_DEV bool tc_wait(uint64_t* bar, uint32_t parity) {
   const uint32_t addr = smem_u32(bar);
   long long t0 = 0;
@@ -201,6 +212,13 @@ DFS_DEV bool tc_wait(uint64_t* bar, uint32_t parity) {
     }
   }
 }
+
+// Registers of this warpgroup (four warps) from here on.  The shares of a block
+// must not add up to more than it was launched with.
+template <int N>
+DFS_DEV void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+DFS_DEV void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // A wait that gave up: tell the host (status may be mapped host memory: a plain store)
 DFS_DEV void report_timeout(int32_t* status) {
@@ -229,9 +247,10 @@ DFS_DEV void load_bias_ext(float* tab, const AttnParams& P, int h, int tid, int 
 inline size_t bias_ext_bytes(const AttnParams& P) { return P.w ? (2 * (P.D + 255) + 1) * sizeof(float) : 0; }
 
 // One tile as the producer announces it: first key (or query) row, -1 for the
-// end; the key mask's bits.
+// end; whether it is plain (all pairs visible, one bias for all) and where its
+// distances lie (block_side); the key mask's bits.
 struct TileInfo {
-  int at, head;
+  int at, plain, side, head;
   uint32_t bits[4];
 };
 
@@ -263,9 +282,9 @@ struct TcKeyTiles {
   DFS_DEV int operator[](int x) const { return x < ns ? x : t0 + (x - ns); }
 };
 
-// Whether every pair of the 32 queries at p0.. and the 32 keys at j0.. is visible, the mask apart.
-DFS_DEV bool block_visible(const AttnParams& P, int p0, int j0) {
-  const int p1 = p0 + 31, j1 = j0 + 31;
+// Whether every pair of a square block (queries from position p0, keys from j0) is visible, the mask apart.
+DFS_DEV bool block_visible(const AttnParams& P, int p0, int j0, int edge = 32) {
+  const int p1 = p0 + edge - 1, j1 = j0 + edge - 1;
   if (j1 >= P.nk || (P.causal && p0 < j1)) return false;
   return (p1 - j0 < P.window && j1 - p0 < P.window) || j1 < P.sinks;
 }
@@ -280,9 +299,15 @@ DFS_DEV uint32_t query_word(const AttnParams& P, int j, int p0) {
   if (j < P.sinks) v |= range_word(P.causal ? j - p0 : 0, 32, 0);
   return v;
 }
-// Where the distances of a block of 32 x 32 lie: 1 beyond the table's far end, -1 beyond the other, 0 in it.
-DFS_DEV int block_side(const AttnParams& P, int p0, int j0) {
-  return p0 - j0 - 31 >= P.D ? 1 : p0 - j0 + 31 <= -P.D ? -1 : 0;
+// Where the distances of a square block of pairs lie: 1 beyond the table's far end, -1 beyond the other, 0 in it.
+DFS_DEV int block_side(const AttnParams& P, int p0, int j0, int edge = 32) {
+  return p0 - j0 - (edge - 1) >= P.D ? 1 : p0 - j0 + (edge - 1) <= -P.D ? -1 : 0;
+}
+// What the producer says of the tile of 128 queries at p0 and 128 keys at j0 (its mask bits are set already).
+DFS_DEV void describe_tile(const AttnParams& P, TileInfo& f, int p0, int j0) {
+  f.side = P.w ? block_side(P, p0, j0, kTcRows) : 0;
+  f.plain = (f.bits[0] & f.bits[1] & f.bits[2] & f.bits[3]) == ~0u && (P.w == nullptr || f.side != 0) &&
+            block_visible(P, p0, j0, kTcRows);
 }
 // A strided (B, heads, n, d) operand of 16-bit elements as {d, n, heads, B}, boxes of 64 x 128.
 bool tc_tmap(CUtensorMap* tm, const Strided& s, bool bf16, int d, int n, int heads, int B);
@@ -292,6 +317,17 @@ bool tc_tmap(CUtensorMap* tm, const Strided& s, bool bf16, int d, int n, int hea
 // fastest left a head's longest CTA among the last: 35 % of SM time idle at
 // N = 4096, causal.)
 inline unsigned tc_grid(int n, int heads, int B) { return static_cast<unsigned>((n + kTcRows - 1) / kTcRows) * heads * B; }
+
+// Dynamic shared memory of a kernel, and that its register split fits what it is launched with (an increase
+// that the block's own registers cannot serve would wait forever).
+template <typename K>
+cudaError_t prepare_split(K kern, size_t smem, int threads, int share) {
+  cudaFuncAttributes at;
+  cudaError_t e = cudaFuncGetAttributes(&at, kern);
+  if (e != cudaSuccess) return e;
+  if ((at.numRegs + 7) / 8 * 8 * threads < share) return cudaErrorInvalidConfiguration;
+  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+}
 
 cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st);
 cudaError_t launch_attn_tc_bwd(const AttnParams& P, int dtype, cudaStream_t st);

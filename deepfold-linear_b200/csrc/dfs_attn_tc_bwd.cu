@@ -18,12 +18,17 @@
 // worked on), warp 17 stages tiles by TMA and announces them.  The exponentials
 // (1024 clocks a tile on the MUFU) go in part to the FMA pipes; four element warps
 // a scheduler cover the latencies of TMEM, barriers and dependent arithmetic.
+#include <type_traits>
+
 #include "dfs_attn_tc.cuh"
 
 namespace dfs {
 namespace {
 
-constexpr int kBwdThreads = 576;
+// 640 threads x 96 registers at launch = 512 x 112 (elements) + 128 x 32 (MMA, TMA and two idle warps)
+constexpr int kBwdThreads = 640;
+constexpr int kElementRegs = 112, kOtherRegs = 32;
+static_assert(512 * kElementRegs + 128 * kOtherRegs <= kBwdThreads * 96, "register shares");
 constexpr int kWork = 512;     // threads of the element warps
 constexpr int kMmaWarp = 16, kTmaWarp = 17;
 constexpr int kPolyEvery = 3;
@@ -36,7 +41,7 @@ struct BwdShared {
   uint64_t own_full, full[kStages], empty[kStages];
   uint64_t s_full, s_free, ds_ready, acc_done;
   TileInfo info[kInfo];
-  alignas(16) float stat[kStages][2][kTcRows];  // dK/dV pass: lse and D of the stage's queries
+  alignas(16) float stat[kStages][2][kTcRows];  // dK/dV pass: -lse and -D of the stage's queries
   float part[4][kTcRows];           // dQ pass: a row's four partial sums
   float ends[2][kWork / 32];
   float diag[2][kWork / 32][64];    // dK/dV pass: the diagonals of a warp's block, two tiles in turn
@@ -101,6 +106,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
   tc_fence_after();
   const uint32_t tm = S.tmem;
 
+  if (warp >= kMmaWarp) regs_down<kOtherRegs>();
   if (warp == kTmaWarp) {  // ---- producer
     const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
     const TcKeyTiles tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
@@ -124,6 +130,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
         f.at = j0;
 #pragma unroll
         for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
+        describe_tile(P, f, p0, j0);
         if (j0 < 0) {
           mbar_arrive(&S.full[s]);
         } else {
@@ -186,7 +193,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
       __syncwarp();
       end = next_end;
     }
-  } else {  // ---- elements: warp w has TMEM lanes 32 (w % 4).. and columns 32 (w / 4)..
+  } else if (warp < kMmaWarp) {  // ---- elements: warp w has TMEM lanes 32 (w % 4).. and columns 32 (w / 4)..
+    regs_up<kElementRegs>();
     const int wq = warp % 4, cg = warp / 4, row = wq * 32 + lane, i = i0 + row, p = p0 + row, pw = p0 + 32 * wq;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
     const int E = bias_ext(P.D), c0 = 16 * cg;  // c0: this thread's columns of d
@@ -216,32 +224,37 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
     D = (S.part[0][row] + S.part[1][row]) + (S.part[2][row] + S.part[3][row]);
     const float lse = i < P.nq ? P.lse[stat] : INFINITY;
     float2 rest = both(0.0f);
-    int t = 0;
-    for (;; ++t) {
-      if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
-      const TileInfo& f = S.info[t % kInfo];
-      const int at = f.at, j0 = at + 32 * cg;
-      if (at < 0) break;
-      const uint32_t bits = f.bits[cg];
-      tc_fence_after();
-      uint32_t sr[32], dr[32], pk[16];
-      tmem_ld32_async(tm + lanes + kColS + 32 * cg, sr);
-      tmem_ld32_async(tm + lanes + kColDP + 32 * cg, dr);
-      const bool whole = bits == ~0u && block_visible(P, pw, j0);
-      const uint32_t vis = whole ? ~0u : bits & key_word(P, p, j0);
-      const bool live = whole || __any_sync(0xffffffffu, vis != 0);
-      const int side = P.w ? block_side(P, pw, j0) : 2;
+    const float far_hi = P.w ? tab[E + P.D] : 0.0f, far_lo = P.w ? tab[E - P.D] : 0.0f;
+    // One tile, S and dP on their way to sr and dr (plain tiles: see TileInfo).
+    auto step = [&](auto is_plain, int t, uint32_t (&sr)[32], uint32_t (&dr)[32], int j0, uint32_t bits,
+                    float far) -> bool {
+      constexpr bool kPlain = decltype(is_plain)::value;
+      bool whole = true, live = true;
+      uint32_t vis = ~0u;
+      int side = 1;
+      float mul = P.scale2;
+      if (!kPlain) {
+        whole = bits == ~0u && block_visible(P, pw, j0);
+        if (!whole) {
+          vis = bits & key_word(P, p, j0);
+          live = __any_sync(0xffffffffu, vis != 0);
+        }
+        side = P.w ? block_side(P, pw, j0) : 2;
+        far = side == 1 ? far_hi : side == -1 ? far_lo : 0.0f;
+        if (side == 0) mul = 1.0f;
+      }
       tmem_wait_ld(sr);
       tmem_wait_ld(dr);
       tc_fence_before();
       mbar_arrive(&S.s_free);
-      if (live) {
-        if (side == 0) {
+      uint32_t pk[16];
+      if (kPlain || live) {
+        if (!kPlain && side == 0) {
           const float* tb = tab + (E + p - j0);
 #pragma unroll
           for (int c = 0; c < 32; ++c) sr[c] = __float_as_uint(fmaf(__uint_as_float(sr[c]), P.scale2, tb[-c]));
         }
-        if (!whole) {
+        if (!kPlain && !whole) {
           // a hidden key's logit is -inf, and its dP (from hidden memory: anything) 0
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
@@ -250,13 +263,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
             dr[c] = on ? dr[c] : 0u;
           }
         }
-        const float2 mul = both(side == 0 ? 1.0f : P.scale2);
-        const float2 off = both((side == 1 ? tab[E + P.D] : side == -1 ? tab[E - P.D] : 0.0f) - lse);
+        const float2 mul_2 = both(mul), off = both(far - lse);
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
           const float2 s = make_float2(__uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1]));
           const float2 dp = make_float2(__uint_as_float(dr[2 * c]), __uint_as_float(dr[2 * c + 1]));
-          const float2 ds = mul2(exp2_pair<kPolyEvery>(fma2(s, mul, off), c), add2(dp, both(-D)));
+          const float2 ds = mul2(exp2_pair<kPolyEvery>(fma2(s, mul_2, off), c), add2(dp, both(-D)));
           rest = add2(rest, ds);
           pk[c] = pack16<BF16>(ds.x, ds.y);
         }
@@ -264,11 +276,30 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
 #pragma unroll
         for (int c = 0; c < 16; ++c) pk[c] = 0;
       }
-      if (t > 0 && !tc_wait(&S.acc_done, (t - 1) & 1)) { err = true; break; }
+      if (t > 0 && !tc_wait(&S.acc_done, (t - 1) & 1)) return false;
       tmem_st16(tm + lanes + kColDS + 16 * cg, pk);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&S.ds_ready);
+      return true;
+    };
+    int t = 0;
+    for (;; ++t) {
+      if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
+      const TileInfo& f = S.info[t % kInfo];
+      const int at = f.at, j0 = at + 32 * cg;
+      if (at < 0) break;
+      const int plain = f.plain, tile_side = f.side;
+      const uint32_t bits = f.bits[cg];
+      tc_fence_after();
+      uint32_t sr[32], dr[32];
+      tmem_ld32_async(tm + lanes + kColS + 32 * cg, sr);
+      tmem_ld32_async(tm + lanes + kColDP + 32 * cg, dr);
+      if (plain)
+        err = !step(std::true_type(), t, sr, dr, j0, bits, tile_side > 0 ? far_hi : tile_side < 0 ? far_lo : 0.0f);
+      else
+        err = !step(std::false_type(), t, sr, dr, j0, bits, 0.0f);
+      if (err) break;
     }
     if (!err && t > 0) err = !tc_wait(&S.acc_done, (t - 1) & 1);
     tc_fence_after();
@@ -333,6 +364,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
   i_lo = max(i_lo, 0) / kTcRows;
   i_hi = (min(i_hi, P.nq) + kTcRows - 1) / kTcRows;  // in tiles
 
+  if (warp >= kMmaWarp) regs_down<kOtherRegs>();
   if (warp == kTmaWarp) {  // ---- producer
     uint32_t bits[4];
     key_bits(P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr, j0, P.nk, lane, bits);
@@ -352,8 +384,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = i0 + 4 * lane + e;
-          st[0][e] = i < P.nq ? P.lse[at + i] : INFINITY;
-          st[1][e] = i < P.nq ? P.dsum[at + i] : 0.0f;
+          st[0][e] = i < P.nq ? -P.lse[at + i] : -INFINITY;
+          st[1][e] = i < P.nq ? -P.dsum[at + i] : 0.0f;
         }
       }
       if (!tc_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
@@ -369,6 +401,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
         f.head = g;
 #pragma unroll
         for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
+        describe_tile(P, f, i0 + P.qs, j0);
         if (i0 < 0) {
           mbar_arrive(&S.full[s]);
         } else {
@@ -417,13 +450,89 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
       __syncwarp();
       end = next_end;
     }
-  } else {  // ---- elements: a key row and a quarter of the tile's queries per thread
+  } else if (warp < kMmaWarp) {  // ---- elements: a key row and a quarter of the tile's queries per thread
+    regs_up<kElementRegs>();
     const int wq = warp % 4, cg = warp / 4, row = wq * 32 + lane, j = j0 + row, jw = j0 + 32 * wq, tid = threadIdx.x;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
     const int E = bias_ext(P.D);
     const bool dw = P.dw_part != nullptr;
     float lo = 0.0f, hi = 0.0f;  // sums of dS beyond the table's ends
     int head = -1, strip = 0;
+    float far_hi = 0.0f, far_lo = 0.0f;
+    // One tile, S^T and dP^T on their way to sr and dr; leaves dS in dr.
+    auto step = [&](auto is_plain, int t, uint32_t (&sr)[32], uint32_t (&dr)[32], int pw, uint32_t kbits, float far,
+                    bool& live) -> bool {
+      constexpr bool kPlain = decltype(is_plain)::value;
+      const float* lse = S.stat[t % kStages][0] + 32 * cg;
+      const float* Dv = S.stat[t % kStages][1] + 32 * cg;
+      bool whole = true;
+      uint32_t vis = ~0u;
+      int side = 1;
+      float mul = P.scale2;
+      if (!kPlain) {
+        whole = kbits == ~0u && block_visible(P, pw, jw);
+        if (!whole) {
+          vis = (kbits >> lane) & 1u ? query_word(P, j, pw) : 0u;
+          live = __any_sync(0xffffffffu, vis != 0);
+        }
+        side = P.w ? block_side(P, pw, jw) : 2;
+        far = side == 1 ? far_hi : side == -1 ? far_lo : 0.0f;
+        if (side == 0) mul = 1.0f;
+      }
+      tmem_wait_ld(sr);
+      tmem_wait_ld(dr);
+      tc_fence_before();
+      mbar_arrive(&S.s_free);
+      uint32_t pk[16];
+      if (kPlain || live) {
+        if (!kPlain && side == 0) {
+          const float* tb = tab + (E + pw - j);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) sr[c] = __float_as_uint(fmaf(__uint_as_float(sr[c]), P.scale2, tb[c]));
+        }
+        if (!kPlain && !whole) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const bool on = (vis >> c) & 1u;
+            sr[c] = on ? sr[c] : 0xff800000u;
+            dr[c] = on ? dr[c] : 0u;
+          }
+        }
+        const float2 mul_2 = both(mul), far_2 = both(far);
+#pragma unroll
+        for (int c = 0; c < 16; c += 2) {  // four queries
+          const float4 ls = *reinterpret_cast<const float4*>(lse + 2 * c);
+          const float4 dd = *reinterpret_cast<const float4*>(Dv + 2 * c);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float2 l2 = u ? make_float2(ls.z, ls.w) : make_float2(ls.x, ls.y);
+            const float2 d2 = u ? make_float2(dd.z, dd.w) : make_float2(dd.x, dd.y);
+            const int e = 2 * (c + u);
+            const float2 s = make_float2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
+            const float2 dp = make_float2(__uint_as_float(dr[e]), __uint_as_float(dr[e + 1]));
+            const float2 x = exp2_pair<kPolyEvery>(fma2(s, mul_2, add2(l2, far_2)), c + u);
+            const float2 ds = mul2(x, add2(dp, d2));
+            pk[c + u] = pack16<BF16>(x.x, x.y);
+            dr[e] = __float_as_uint(ds.x);
+            dr[e + 1] = __float_as_uint(ds.y);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) pk[c] = 0;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) dr[c] = 0;
+      }
+      if (t > 0 && !tc_wait(&S.acc_done, (t - 1) & 1)) return false;
+      tmem_st16(tm + lanes + kColP + 16 * cg, pk);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) pk[c] = pack16<BF16>(__uint_as_float(dr[2 * c]), __uint_as_float(dr[2 * c + 1]));
+      tmem_st16(tm + lanes + kColDS + 16 * cg, pk);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&S.ds_ready);
+      return true;
+    };
     // this head's sums by distance, to memory (the element threads together)
     auto flush = [&]() {
       if (P.D == 0) hi += lo, lo = 0.0f;
@@ -460,79 +569,30 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
         if (dw)
           for (int x = tid; x < W; x += kWork) acc[x] = 0.0f;
         work_barrier();
+        if (P.w) far_hi = tab[E + P.D], far_lo = tab[E - P.D];
       }
-      const uint32_t kbits = S.info[t % kInfo].bits[wq];
-      const float* lse = S.stat[t % kStages][0] + 32 * cg;
-      const float* Dv = S.stat[t % kStages][1] + 32 * cg;
-      const int p0 = i0 + P.qs, pw = p0 + 32 * cg;
+      const TileInfo& f = S.info[t % kInfo];
+      const uint32_t kbits = f.bits[wq];
+      const int plain = f.plain, tile_side = f.side;
+      const int p0 = i0 + P.qs;
       tc_fence_after();
-      uint32_t sr[32], dr[32], pk[16];
+      uint32_t sr[32], dr[32];
       tmem_ld32_async(tm + lanes + kColS + 32 * cg, sr);
       tmem_ld32_async(tm + lanes + kColDP + 32 * cg, dr);
-      const bool whole = kbits == ~0u && block_visible(P, pw, jw);
-      const uint32_t vis = whole ? ~0u : (kbits >> lane) & 1u ? query_word(P, j, pw) : 0u;
-      const bool live = whole || __any_sync(0xffffffffu, vis != 0);
-      const int side = P.w ? block_side(P, pw, jw) : 2;
-      tmem_wait_ld(sr);
-      tmem_wait_ld(dr);
-      tc_fence_before();
-      mbar_arrive(&S.s_free);
-      if (live) {
-        if (side == 0) {
-          const float* tb = tab + (E + pw - j);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) sr[c] = __float_as_uint(fmaf(__uint_as_float(sr[c]), P.scale2, tb[c]));
-        }
-        if (!whole) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const bool on = (vis >> c) & 1u;
-            sr[c] = on ? sr[c] : 0xff800000u;
-            dr[c] = on ? dr[c] : 0u;
-          }
-        }
-        const float2 mul = both(side == 0 ? 1.0f : P.scale2);
-        const float2 add = both(side == 1 ? tab[E + P.D] : side == -1 ? tab[E - P.D] : 0.0f);
-#pragma unroll
-        for (int c = 0; c < 16; c += 2) {  // four queries
-          const float4 ls = *reinterpret_cast<const float4*>(lse + 2 * c);
-          const float4 dd = *reinterpret_cast<const float4*>(Dv + 2 * c);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float2 l2 = u ? make_float2(ls.z, ls.w) : make_float2(ls.x, ls.y);
-            const float2 d2 = u ? make_float2(dd.z, dd.w) : make_float2(dd.x, dd.y);
-            const int e = 2 * (c + u);
-            const float2 s = make_float2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
-            const float2 dp = make_float2(__uint_as_float(dr[e]), __uint_as_float(dr[e + 1]));
-            const float2 x = exp2_pair<kPolyEvery>(fma2(s, mul, fma2(l2, both(-1.0f), add)), c + u);
-            const float2 ds = mul2(x, fma2(d2, both(-1.0f), dp));
-            pk[c + u] = pack16<BF16>(x.x, x.y);
-            dr[e] = __float_as_uint(ds.x);
-            dr[e + 1] = __float_as_uint(ds.y);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < 16; ++c) pk[c] = 0;
-#pragma unroll
-        for (int c = 0; c < 32; ++c) dr[c] = 0;
-      }
-      if (t > 0 && !tc_wait(&S.acc_done, (t - 1) & 1)) { err = true; break; }
-      tmem_st16(tm + lanes + kColP + 16 * cg, pk);
-#pragma unroll
-      for (int c = 0; c < 16; ++c) pk[c] = pack16<BF16>(__uint_as_float(dr[2 * c]), __uint_as_float(dr[2 * c + 1]));
-      tmem_st16(tm + lanes + kColDS + 16 * cg, pk);
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&S.ds_ready);
+      bool live = true;
+      if (plain)
+        err = !step(std::true_type(), t, sr, dr, p0 + 32 * cg, kbits,
+                    tile_side > 0 ? far_hi : tile_side < 0 ? far_lo : 0.0f, live);
+      else
+        err = !step(std::false_type(), t, sr, dr, p0 + 32 * cg, kbits, 0.0f, live);
+      if (err) break;
       if (dw) {
-        const int dlo = p0 - j0 - 127, dhi = p0 - j0 + 127;  // the tile's distances
-        if (dlo >= P.D || dhi <= -P.D) {
+        if (tile_side != 0) {
           float2 s2 = both(0.0f);
 #pragma unroll
           for (int c = 0; c < 16; ++c)
             s2 = add2(s2, make_float2(__uint_as_float(dr[2 * c]), __uint_as_float(dr[2 * c + 1])));
-          if (dlo >= P.D) hi += s2.x + s2.y;
+          if (tile_side > 0) hi += s2.x + s2.y;
           else lo += s2.x + s2.y;
         } else {
           // Diagonals of this warp's block of 32 keys x 32 queries: the running sum of a diagonal moves one lane
@@ -613,9 +673,9 @@ cudaError_t launch_attn_tc_bwd(const AttnParams& P, int dtype, cudaStream_t st) 
                       (P.w ? (2 * P.D + 1) * sizeof(float) : 0);
   auto dq = bf16 ? tc_dq_kernel<true> : tc_dq_kernel<false>;
   auto dkv = bf16 ? tc_dkv_kernel<true> : tc_dkv_kernel<false>;
-  cudaError_t e = cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  const int share = 512 * kElementRegs + 128 * kOtherRegs;
+  cudaError_t e = prepare_split(dq, smem, kBwdThreads, share);
+  if (e == cudaSuccess) e = prepare_split(dkv, smem, kBwdThreads, share);
   if (e != cudaSuccess) return e;
   dq<<<tc_grid(P.nq, P.H, P.B), kBwdThreads, smem, st>>>(T);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
