@@ -87,5 +87,6 @@ cudaError_t launch_bucket_sums(const float* part, int H, int parts, int D, const
 cudaError_t launch_attn_simt_fwd(const AttnParams& P, int dtype, cudaStream_t st);
 cudaError_t launch_attn_simt_bwd(const AttnParams& P, int dtype, cudaStream_t st);
 cudaError_t launch_decode(const AttnParams& P, int dtype, cudaStream_t st);
+cudaError_t launch_decode_mma(const AttnParams& P, int dtype, cudaStream_t st);  // 16-bit, 16-byte rows
 
 }  // namespace dfs
