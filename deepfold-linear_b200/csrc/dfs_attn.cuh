@@ -79,8 +79,6 @@ DFS_DEV void load_bias_table(float* tab, const void* w, const int32_t* lut, int 
   }
 }
 
-constexpr int kBucketThreads = 512;
-
 // launchers (host)
 cudaError_t launch_bucket_sums(const float* part, int H, int parts, int D, const int32_t* lut, int nb, int dtype,
                                void* out, cudaStream_t st);
