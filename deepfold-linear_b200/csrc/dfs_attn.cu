@@ -154,8 +154,9 @@ extern "C" int dfs_window_attn_decode(const dfs_attn_problem* p, const dfs_attn_
   P.mask = nullptr;
   P.lengths = lengths;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // 16-byte copies of cache rows, 4-byte reads of q
-  const bool rows = p->dtype != DFS_F32 && p->d % 8 == 0 && staged(a->q, 1, p->H, p->B) &&
+  // cache tiles staged by TMA, 4-byte reads of q
+  const bool rows = p->dtype != DFS_F32 && p->d % 8 == 0 && p->n_k > 0 && tmap_available() &&
+                    staged(a->q, 1, p->H, p->B) &&
                     staged(a->k, p->n_k, p->H_kv, p->B) && staged(a->v, p->n_k, p->H_kv, p->B);
   return rc(rows ? launch_decode_mma(P, p->dtype, st) : launch_decode(P, p->dtype, st));
 }

@@ -3,40 +3,40 @@
 //
 // Reading the visible cache rows is all the time there is: 256 bytes of K and V
 // a key at d = 64 for 4 d operations a query head.  A cluster of up to 8 CTAs
-// shares one key head of one sequence and splits its visible keys (the sinks,
-// then the window, as one list) into equal runs; each CTA copies tiles of 64 keys
-// through a ring of shared-memory stages and its 4 warps take 16 keys each:
-// S = Q K^T and O += P V for the group's heads as mma.sync m16n8k16 (16 heads by
-// 8 keys; the tensor-core rate does not matter here, the small shape does).  Every
-// warp keeps its own maximum and sum; warps join through shared memory, CTAs
-// through distributed shared memory, in a fixed order and without a second launch.
+// shares one key head of one sequence and splits the tiles of 128 keys that hold
+// visible ones (the sinks' and the window's) into equal runs.  In a CTA one warp
+// keeps TMA copies in flight through a ring of stages and four warps take 32 keys
+// of a tile each: S = Q K^T and O += P V for the group's heads as mma.sync
+// m16n8k16 (16 heads by 8 keys; the tensor-core rate does not matter here, the
+// small shape does).  Every warp keeps its own maximum and sum; warps join through
+// shared memory, CTAs through distributed shared memory, in a fixed order and
+// without a second launch.  (Copies by the threads themselves, 16 bytes each, cost
+// 440 instructions a warp per 64 keys and held the reads to 4.2 TB/s.)
+#include <algorithm>
 #include <type_traits>
 
-#include "dfs_attn.cuh"
+#include "dfs_attn_tc.cuh"
 
 namespace dfs {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kKeys = 64;          // keys of a tile
-constexpr int kStages = 3;
+constexpr int kThreads = 160;      // four warps of products, one of copies
+constexpr int kStages = 2;         // of K and V tiles: 64 KB, three CTAs an SM
 constexpr int kHeads = 16;         // query heads of a CTA: the rows of an m16n8k16 product
-constexpr int kPitch = 72;         // elements of a staged row: 144 bytes keep ldmatrix free of conflicts
-constexpr int kTileElems = kKeys * kPitch;
 constexpr int kMaxSplit = 8;
 
 struct DecodeShared {
+  uint64_t full[kStages], empty[kStages];
   float m[4][kHeads], l[4][kHeads];       // the warps' maxima and sums
   float cm[kHeads], cl[kHeads];           // the CTA's, read by the cluster
   float o[kHeads][68];                    // the CTA's sums of P V, read by the cluster
 };
 
-DFS_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {  // bytes 16, or 0: zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-DFS_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-DFS_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+struct DecodeParams {
+  CUtensorMap k, v;
+  AttnParams a;
+  int split, chunks;
+};
 
 DFS_DEV void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -57,55 +57,56 @@ DFS_DEV void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <bool BF16>
-DFS_DEV uint32_t pack(float lo, float hi) {
-  uint32_t r;
-  if (BF16)
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
+// Byte of 16-byte piece c of row r of a tile (128-byte rows, 128-byte swizzle)
+DFS_DEV uint32_t piece_at(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
 // grid (split, key heads x head chunks, batch), clusters of `split` CTAs
 template <typename E>
-__global__ void __launch_bounds__(kThreads) decode_mma_kernel(AttnParams P, int split, int chunks) {
+__global__ void __launch_bounds__(kThreads) decode_mma_kernel(const __grid_constant__ DecodeParams T) {
   constexpr bool BF16 = std::is_same<E, __nv_bfloat16>::value;
-  extern __shared__ __align__(16) unsigned char raw[];
-  E* stage = reinterpret_cast<E*>(raw);  // [kStages][2][kKeys][kPitch]: K, V
-  DecodeShared& S = *reinterpret_cast<DecodeShared*>(raw + kStages * 2 * kTileElems * sizeof(E));
+  extern __shared__ unsigned char raw[];
+  const AttnParams& P = T.a;
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  unsigned char* gen = raw + (base - smem_u32(raw));
+  DecodeShared& S = *reinterpret_cast<DecodeShared*>(gen + kStages * 2 * kTcTileBytes);
   float* tab = reinterpret_cast<float*>(&S + 1);  // [heads][D + 1] bias of delta = 0 .. D
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, rank = blockIdx.x;
-  const int hk = blockIdx.y / chunks, g0 = blockIdx.y % chunks * kHeads, b = blockIdx.z;
+  const int tid = threadIdx.x, warp = warp_index(), lane = tid % 32, rank = blockIdx.x, split = T.split;
+  const int hk = blockIdx.y / T.chunks, g0 = blockIdx.y % T.chunks * kHeads, b = blockIdx.z;
   const int ng = min(kHeads, P.G - g0), h0 = hk * P.G + g0;
   const int len = min(max(P.lengths[b], 0), P.nk), p = len - 1;
-  const int lo = max(0, len - P.window), ns = min(P.sinks, lo), total = ns + (len - lo);
-  const int tiles = (total + kKeys - 1) / kKeys, per = (tiles + split - 1) / split;
-  const int t0 = min(rank * per, tiles), t1 = min(t0 + per, tiles);
-  const int ksteps = (P.d + 15) / 16, pieces = 2 * ksteps;
-
-  const E* kb = row_ptr<E>(P.k, b, hk, 0);
-  const E* vb = row_ptr<E>(P.v, b, hk, 0);
-  auto load = [&](int t) {  // one commit group, empty beyond the run
-    if (t < t1) {
-      E* ks = stage + (t - t0) % kStages * 2 * kTileElems;
-      const int c = tid % 8;
-#pragma unroll
-      for (int r = tid / 8; r < kKeys; r += kThreads / 8) {
-        const int x = t * kKeys + r, j = x < ns ? x : lo + (x - ns);
-        if (c < pieces) {
-          const uint32_t bytes = x < total && 8 * c < P.d ? 16u : 0u;  // rows and columns beyond: zeros
-          const int64_t jj = bytes ? j : 0;
-          const int cc = bytes ? 8 * c : 0;
-          cp_async16(smem_u32(ks + r * kPitch + 8 * c), kb + jj * P.k.sn + cc, bytes);
-          cp_async16(smem_u32(ks + kTileElems + r * kPitch + 8 * c), vb + jj * P.v.sn + cc, bytes);
-        }
+  const int lo = max(0, len - P.window), ns = min(P.sinks, lo);  // keys [0, ns) and [lo, len) are visible
+  const int w0 = lo / kTcRows, sink_tiles = min((ns + kTcRows - 1) / kTcRows, w0);
+  const int tiles = len > 0 ? sink_tiles + (len + kTcRows - 1) / kTcRows - w0 : 0;
+  const int per = (tiles + split - 1) / split, t0 = min(rank * per, tiles), t1 = min(t0 + per, tiles);
+  auto tile_key = [&](int t) { return (t < sink_tiles ? t : w0 + (t - sink_tiles)) * kTcRows; };
+  const int ksteps = (P.d + 15) / 16;
+  bool err = false;
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(&S.full[s], 1), mbar_init(&S.empty[s], 4);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const int t_near = t1 - 1;  // the run's newest tile
+  const bool near_run = P.w && t1 > t0 && p - min(tile_key(t_near) + kTcRows - 1, p) < P.D;
+  if (warp == 4) {
+    for (int t = t0; t < t1; ++t) {
+      const int s = (t - t0) % kStages;
+      if (!tc_wait(&S.empty[s], (((t - t0) / kStages) & 1) ^ 1)) { err = true; break; }
+      if (lane == 0) {
+        const uint32_t bar = smem_u32(&S.full[s]), dst = base + s * 2 * kTcTileBytes;
+        mbar_arrive_expect_tx(bar, 2 * kTcTileBytes);
+        tma_load_4d(dst, &T.k, 0, tile_key(t), hk, b, bar);
+        tma_load_4d(dst + kTcTileBytes, &T.v, 0, tile_key(t), hk, b, bar);
       }
+      __syncwarp();
     }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) load(t0 + s);
+  }
+  // the table where this run comes near the query (the copies are on their way)
+  if (near_run && warp < 4)
+    for (int x = tid; x < ng * (P.D + 1); x += 128) {
+      const int bk = min(max(P.lut[P.D + x % (P.D + 1)], 0), P.nb - 1);
+      tab[x] = load_as_f32<void>(P.w, static_cast<size_t>(h0 + x / (P.D + 1)) * P.nb + bk, P.wdtype) * kLog2e;
+    }
 
   // Q as the A operand: rows lane / 4 and + 8, columns 2 (lane % 4).. of each k step
   const int g = lane / 4, q2 = 2 * (lane % 4);
@@ -120,19 +121,13 @@ __global__ void __launch_bounds__(kThreads) decode_mma_kernel(AttnParams P, int 
     }
   // the far bias of this thread's two heads; the table where this run comes near the query
   float far[2] = {0.0f, 0.0f};
-  const int last = t1 > t0 ? min(t1 * kKeys, total) - 1 : -1;  // the run's newest key
-  const bool near_run = P.w && last >= 0 && p - (last < ns ? last : lo + (last - ns)) < P.D;
   if (P.w) {
     const int bk = min(max(P.lut[2 * P.D], 0), P.nb - 1);
 #pragma unroll
     for (int r = 0; r < 2; ++r)
       if (g + 8 * r < ng) far[r] = load_as_f32<void>(P.w, static_cast<size_t>(h0 + g + 8 * r) * P.nb + bk, P.wdtype) * kLog2e;
   }
-  if (near_run)
-    for (int x = tid; x < ng * (P.D + 1); x += kThreads) {
-      const int bk = min(max(P.lut[P.D + x % (P.D + 1)], 0), P.nb - 1);
-      tab[x] = load_as_f32<void>(P.w, static_cast<size_t>(h0 + x / (P.D + 1)) * P.nb + bk, P.wdtype) * kLog2e;
-    }
+  if (near_run && warp < 4) asm volatile("bar.sync 1, 128;" ::: "memory");
 
   float o[8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -140,76 +135,105 @@ __global__ void __launch_bounds__(kThreads) decode_mma_kernel(AttnParams P, int 
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
 
-  for (int t = t0; t < t1; ++t) {
-    cp_async_wait<kStages - 2>();
-    __syncthreads();  // tile t is in; everybody is done with tile t - 1
-    load(t + kStages - 1);
-    const E* ks = stage + (t - t0) % kStages * 2 * kTileElems + 16 * warp * kPitch;
-    const E* vs = ks + kTileElems;
-    float s[2][4] = {};
+  for (int t = t0; warp < 4 && t < t1; ++t) {
+    const int st = (t - t0) % kStages;
+    if (!tc_wait(&S.full[st], ((t - t0) / kStages) & 1)) { err = true; break; }
+    const int j0 = tile_key(t) + 32 * warp;  // this warp's 32 keys
+    const uint32_t ks = base + st * 2 * kTcTileBytes + 32 * warp * 128, vs = ks + kTcTileBytes;
+    const bool edge = j0 + 32 > len || (j0 < lo && j0 + 32 > ns);  // some key of the 32 is hidden
+    if (edge) {
+      // a hidden row may hold anything, and 0 x NaN is NaN: zero its V
+      unsigned char* vt = gen + (st * 2 + 1) * kTcTileBytes + 32 * warp * 128;
+      for (int r = lane / 8; r < 32; r += 4)
+        if (j0 + r >= len || (j0 + r < lo && j0 + r >= ns))
+          *reinterpret_cast<uint4*>(vt + r * 128 + lane % 8 * 16) = make_uint4(0, 0, 0, 0);
+      fence_async_smem();  // before the stage's next copy
+      __syncwarp();
+    }
+    float s[4][4] = {};
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (k < ksteps) {
-        uint32_t kf[4];
-        ldsm4(smem_u32(ks + ((lane / 16) * 8 + lane % 8) * kPitch + 16 * k + (lane / 8 % 2) * 8), kf);
-        mma16<BF16>(s[0], qa[k], kf[0], kf[1]);
-        mma16<BF16>(s[1], qa[k], kf[2], kf[3]);
-      }
-    const int x0 = t * kKeys + 16 * warp + q2;
-    const int xl = min(t * kKeys + 16 * warp + 15, total - 1);
-    const bool near = near_run && p - (xl < ns ? xl : lo + (xl - ns)) < P.D;
-    float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int x = x0 + 8 * n + (e & 1), r = e >> 1;
-        float bias = far[r];
-        if (near && x < total && g + 8 * r < ng) {
-          const int j = x < ns ? x : lo + (x - ns);
-          bias = tab[(g + 8 * r) * (P.D + 1) + min(p - j, P.D)];
+        for (int n = 0; n < 2; ++n) {
+          uint32_t kf[4];
+          ldsm4(ks + piece_at(16 * n + (lane / 16) * 8 + lane % 8, 2 * k + lane / 8 % 2), kf);
+          mma16<BF16>(s[2 * n], qa[k], kf[0], kf[1]);
+          mma16<BF16>(s[2 * n + 1], qa[k], kf[2], kf[3]);
         }
-        s[n][e] = x < total ? fmaf(s[n][e], P.scale2, bias) : -INFINITY;
-        top[r] = fmaxf(top[r], s[n][e]);
       }
-    uint32_t pa[4];
+    const bool near = near_run && p - min(j0 + 31, p) < P.D;
+    float top[2] = {-INFINITY, -INFINITY};
+    if (near) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + 8 * n + q2 + (e & 1), row = min(g + 8 * (e >> 1), ng - 1);
+          s[n][e] = fmaf(s[n][e], P.scale2, tab[row * (P.D + 1) + min(max(p - j, 0), P.D)]);
+        }
+    } else {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e], P.scale2, far[e >> 1]);
+    }
+    if (edge) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + 8 * n + q2 + (e & 1);
+          if (j >= len || (j < lo && j >= ns)) s[n][e] = -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+    uint32_t pa[2][4];
+    float shrink[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
       const float mn = fmaxf(m[r], top[r]), ref = mn == -INFINITY ? 0.0f : mn;
-      const float shrink = ex2(m[r] - ref);
+      shrink[r] = ex2(m[r] - ref);
       m[r] = mn;
       float sum = 0.0f;
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < 4; ++n) {
         const float a = ex2(s[n][2 * r] - ref), c = ex2(s[n][2 * r + 1] - ref);
         sum += a + c;
-        pa[2 * n + r] = pack<BF16>(a, c);
+        pa[n / 2][2 * (n % 2) + r] = pack16<BF16>(a, c);
       }
-      l[r] = l[r] * shrink + sum;
+      l[r] = l[r] * shrink[r] + sum;
+    }
+    if (__any_sync(0xffffffffu, shrink[0] != 1.0f || shrink[1] != 1.0f)) {
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        o[n][2 * r] *= shrink;
-        o[n][2 * r + 1] *= shrink;
-      }
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] *= shrink[e >> 1];
     }
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
-      if (n < ksteps) {
-        uint32_t vf[4];
-        ldsm4t(smem_u32(vs + (lane % 16) * kPitch + 16 * n + (lane / 16) * 8), vf);
-        mma16<BF16>(o[2 * n], pa, vf[0], vf[1]);
-        mma16<BF16>(o[2 * n + 1], pa, vf[2], vf[3]);
-      }
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        if (n < ksteps) {
+          uint32_t vf[4];
+          ldsm4t(vs + piece_at(16 * k + lane % 16, 2 * n + lane / 16), vf);
+          mma16<BF16>(o[2 * n], pa[k], vf[0], vf[1]);
+          mma16<BF16>(o[2 * n + 1], pa[k], vf[2], vf[3]);
+        }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&S.empty[st]);
   }
-  cp_async_wait<0>();
   // join the warps: maxima and sums, then each warp in turn adds its part
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    if (lane % 4 == 0) {
+    if (warp < 4 && lane % 4 == 0) {
       S.m[warp][g + 8 * r] = m[r];
       S.l[warp][g + 8 * r] = l[r];
     }
@@ -264,37 +288,43 @@ __global__ void __launch_bounds__(kThreads) decode_mma_kernel(AttnParams P, int 
     }
     row_ptr<E>(P.o, b, h0 + head, 0)[c] = from_f32<E>(sum > 0.0f ? acc / sum : 0.0f);
   }
+  if (err) report_timeout(P.status);
   if (split > 1) cluster_sync();  // nobody leaves while its memory is read
 }
 
 template <typename E>
 cudaError_t launch(const AttnParams& P, cudaStream_t st) {
-  const int chunks = (P.G + kHeads - 1) / kHeads, heads = P.G < kHeads ? P.G : kHeads;
-  // CTAs: about four an SM (as many as its shared memory holds), so that short batches are split and large
-  // ones are not, with a tile of keys for each at least
-  const long problems = static_cast<long>(P.B) * P.Hkv * chunks;
-  const long seen = P.window < P.nk ? static_cast<long>(P.window) + P.sinks : P.nk;
-  const long tiles = ((seen < P.nk ? seen : P.nk) + kKeys - 1) / kKeys;
-  int split = 1;
-  while (split < kMaxSplit && split * problems < 4 * 148 && 2 * split <= tiles) split *= 2;
-  const size_t smem = kStages * 2 * kTileElems * sizeof(E) + sizeof(DecodeShared) +
-                      (P.w ? heads * (P.D + 1) * sizeof(float) : 0);
+  DecodeParams T;
+  T.a = P;
+  const bool bf16 = std::is_same<E, __nv_bfloat16>::value;
+  if (!tc_tmap(&T.k, P.k, bf16, P.d, P.nk, P.Hkv, P.B) || !tc_tmap(&T.v, P.v, bf16, P.d, P.nk, P.Hkv, P.B))
+    return cudaErrorInvalidValue;
+  T.chunks = (P.G + kHeads - 1) / kHeads;
+  // Splits: until the CTAs fill the three an SM that fit, while each has a tile of keys; so short batches are
+  // split and large ones are not.
+  const long problems = static_cast<long>(P.B) * P.Hkv * T.chunks;
+  const long seen = std::min<long>(static_cast<long>(P.window) + P.sinks, P.nk);
+  const long tiles = (seen + kTcRows - 1) / kTcRows;
+  T.split = 1;
+  while (T.split < kMaxSplit && T.split * problems < 3 * 148 && 2 * T.split <= tiles) T.split *= 2;
+  const size_t smem = 1024 + kStages * 2 * kTcTileBytes + sizeof(DecodeShared) +
+                      (P.w ? std::min(P.G, kHeads) * (P.D + 1) * sizeof(float) : 0);
   auto kern = decode_mma_kernel<E>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(split, P.Hkv * chunks, P.B);
+  cfg.gridDim = dim3(T.split, P.Hkv * T.chunks, P.B);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.x = T.split;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, P, split, chunks);
+  return cudaLaunchKernelEx(&cfg, kern, T);
 }
 
 }  // namespace

@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads) relbias_bwd_kernel(RelParams P, cons
     const T* at = head + static_cast<size_t>(i) * P.nk + j;
     const int a = static_cast<int>(reinterpret_cast<uintptr_t>(at) / sizeof(T) % V);  // the same for the whole warp
     auto piece = [&](const T* q) -> uint4 {
-      if (q >= dB && q + V <= end) return __ldg(reinterpret_cast<const uint4*>(q));
+      if (q >= dB && q + V <= end) return __ldcs(reinterpret_cast<const uint4*>(q));
       union { uint4 q; T e[V]; } v;
       v.q = make_uint4(0, 0, 0, 0);
 #pragma unroll
@@ -229,43 +229,70 @@ __global__ void __launch_bounds__(kThreads) relbias_bwd_kernel(RelParams P, cons
   const bool far = d_lo >= D || d_hi <= -D;
   if (lane == 0) is_near[warp] = some && !far;
   if (some) {
-    float run[V];
+    float2 run[V / 2];
 #pragma unroll
-    for (int e = 0; e < V; ++e) run[e] = 0.0f;
+    for (int e = 0; e < V / 2; ++e) run[e] = make_float2(0.0f, 0.0f);
     float* out = strips + warp * len;
-    for (int i = i0; i < i1; i += 8) {
-      uint4 x[8];
+    auto add_row = [&](uint4 x) {
+      float v[V];
+      unpack<T>(x, v);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) x[r] = i + r < i1 ? fetch(i + r) : make_uint4(0, 0, 0, 0);
+      for (int e = 0; e < V / 2; ++e) run[e] = __fadd2_rn(run[e], make_float2(v[2 * e], v[2 * e + 1]));
+    };
+    // the sums of a near strip move on by one column between two rows
+    auto move_on = [&]() {
+      const float in = __shfl_up_sync(0xffffffffu, run[V / 2 - 1].y, 1);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        float v[V];
-        unpack<T>(x[r], v);
+      for (int e = V / 2 - 1; e > 0; --e) run[e] = make_float2(run[e - 1].y, run[e].x);
+      run[0] = make_float2(lane == 0 ? 0.0f : in, run[0].x);
+    };
+    // rows that need no care: whole in columns, and on 16-byte boundaries like their neighbours
+    const bool easy = s0 + C <= P.nk && P.nk % V == 0 && (reinterpret_cast<uintptr_t>(dB) & 15u) == 0;
+    int i = i0;
+    if (easy) {
+      const T* at = head + static_cast<size_t>(i0) * P.nk + j;
+      const size_t pitch = static_cast<size_t>(P.nk);
+      for (; i + 8 <= i1; i += 8, at += 8 * pitch) {
+        uint4 x[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) x[r] = __ldcs(reinterpret_cast<const uint4*>(at + r * pitch));
         if (far) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) run[e] += v[e];
-        } else if (i + r < i1) {
-          // before this row, the sums have moved on by one column per earlier row
-          if (i + r > i0) {
-            const float in = __shfl_up_sync(0xffffffffu, run[V - 1], 1);
+          for (int r = 0; r < 8; ++r) add_row(x[r]);
+        } else {
 #pragma unroll
-            for (int e = V - 1; e > 0; --e) run[e] = run[e - 1];
-            run[0] = lane == 0 ? 0.0f : in;
+          for (int r = 0; r < 8; ++r) {
+            if (i + r > i0) move_on();
+            add_row(x[r]);
+            if (lane == 31) out[i + r - i0] = run[V / 2 - 1].y;  // slot s: diagonal i0 - (s0 + C - 1) + s
           }
-#pragma unroll
-          for (int e = 0; e < V; ++e) run[e] += v[e];
-          if (lane == 31) out[i + r - i0] = run[V - 1];  // slot s: diagonal i0 - (s0 + C - 1) + s
         }
+      }
+    }
+    for (; i < i1; i += 4) {
+      uint4 x[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = i + r < i1 ? fetch(i + r) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (i + r >= i1) break;
+        if (!far && i + r > i0) move_on();
+        add_row(x[r]);
+        if (!far && lane == 31) out[i + r - i0] = run[V / 2 - 1].y;
       }
     }
     if (far) {
       float s = 0.0f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) s += run[e];
+      for (int e = 0; e < V / 2; ++e) s += run[e].x + run[e].y;
       (d_lo >= D ? hi : lo) = s;
     } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) out[i1 - 1 - i0 + (C - 1 - lane * V - e)] = run[e];
+      for (int e = 0; e < V / 2; ++e) {
+        float* last = out + (i1 - 1 - i0 + C - 1 - lane * V - 2 * e);
+        last[0] = run[e].x;
+        last[-1] = run[e].y;
+      }
     }
   }
   __syncthreads();

@@ -94,8 +94,9 @@ def window_attn_decode(q, k_cache, v_cache, lengths, window: int | None = None, 
     key and value are already in the cache.
 
     k_cache, v_cache (B,H_kv,n_max,d), any strides with unit stride along d;
-    lengths (B,) int32 or int64 on the device, clamped to [0, n_max]; rows from
-    lengths[b] on are not read, a length of 0 gives zeros.  Returns (B,H,d).
+    lengths (B,) int32 or int64 on the device, clamped to [0, n_max]; hidden rows
+    (from lengths[b] on, or before the window) are never used, whatever they hold;
+    a length of 0 gives zeros.  Returns (B,H,d).
     Forward only.
     """
     if not q.is_cuda:
