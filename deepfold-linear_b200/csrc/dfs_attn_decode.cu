@@ -103,9 +103,11 @@ __global__ void __launch_bounds__(kThreads) decode_mma_kernel(const __grid_const
   }
   // the table where this run comes near the query (the copies are on their way)
   if (near_run && warp < 4)
-    for (int x = tid; x < ng * (P.D + 1); x += 128) {
-      const int bk = min(max(P.lut[P.D + x % (P.D + 1)], 0), P.nb - 1);
-      tab[x] = load_as_f32<void>(P.w, static_cast<size_t>(h0 + x / (P.D + 1)) * P.nb + bk, P.wdtype) * kLog2e;
+    for (int x = tid; x <= P.D; x += 128) {
+      const int bk = min(max(P.lut[P.D + x], 0), P.nb - 1);
+#pragma unroll 4
+      for (int r = 0; r < ng; ++r)
+        tab[r * (P.D + 1) + x] = load_as_f32<void>(P.w, static_cast<size_t>(h0 + r) * P.nb + bk, P.wdtype) * kLog2e;
     }
 
   // Q as the A operand: rows lane / 4 and + 8, columns 2 (lane % 4).. of each k step
@@ -300,17 +302,16 @@ cudaError_t launch(const AttnParams& P, cudaStream_t st) {
   if (!tc_tmap(&T.k, P.k, bf16, P.d, P.nk, P.Hkv, P.B) || !tc_tmap(&T.v, P.v, bf16, P.d, P.nk, P.Hkv, P.B))
     return cudaErrorInvalidValue;
   T.chunks = (P.G + kHeads - 1) / kHeads;
-  // Splits: until the CTAs fill the three an SM that fit, while each has a tile of keys; so short batches are
-  // split and large ones are not.
+  // Splits: until there are twice the CTAs that fit at once (three an SM), so that ragged lengths even out,
+  // while each has a tile of keys; short batches are split and large ones are not.
   const long problems = static_cast<long>(P.B) * P.Hkv * T.chunks;
   const long seen = std::min<long>(static_cast<long>(P.window) + P.sinks, P.nk);
   const long tiles = (seen + kTcRows - 1) / kTcRows;
   T.split = 1;
-  while (T.split < kMaxSplit && T.split * problems < 3 * 148 && 2 * T.split <= tiles) T.split *= 2;
+  while (T.split < kMaxSplit && T.split * problems < 6 * 148 && 2 * T.split <= tiles) T.split *= 2;
   const size_t smem = 1024 + kStages * 2 * kTcTileBytes + sizeof(DecodeShared) +
                       (P.w ? std::min(P.G, kHeads) * (P.D + 1) * sizeof(float) : 0);
-  auto kern = decode_mma_kernel<E>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  const cudaError_t e = prepare_kernel<decode_mma_kernel<E>>(smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(T.split, P.Hkv * T.chunks, P.B);
@@ -323,8 +324,8 @@ cudaError_t launch(const AttnParams& P, cudaStream_t st) {
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, T);
+  cfg.numAttrs = T.split > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, decode_mma_kernel<E>, T);
 }
 
 }  // namespace

@@ -346,10 +346,15 @@ cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st) 
     return cudaErrorInvalidValue;
   T.d_o = T.q;
   const size_t smem = 1024 + (1 + kKStages + kVStages) * kTcTileBytes + sizeof(FwdShared) + bias_ext_bytes(P);
-  auto kern = bf16 ? tc_fwd_kernel<true> : tc_fwd_kernel<false>;
-  const cudaError_t e = prepare_split(kern, smem, kFwdThreads, 256 * kElementRegs + 128 * kOtherRegs);
+  const int share = 256 * kElementRegs + 128 * kOtherRegs;
+  const unsigned grid = tc_grid(P.nq, P.H, P.B);
+  const cudaError_t e = bf16 ? prepare_kernel<tc_fwd_kernel<true>>(smem, kFwdThreads, share)
+                             : prepare_kernel<tc_fwd_kernel<false>>(smem, kFwdThreads, share);
   if (e != cudaSuccess) return e;
-  kern<<<tc_grid(P.nq, P.H, P.B), kFwdThreads, smem, st>>>(T);
+  if (bf16)
+    tc_fwd_kernel<true><<<grid, kFwdThreads, smem, st>>>(T);
+  else
+    tc_fwd_kernel<false><<<grid, kFwdThreads, smem, st>>>(T);
   return cudaGetLastError();
 }
 

@@ -2,6 +2,8 @@
 // staging, TMEM operands, tile information, bias tables.
 #pragma once
 
+#include <atomic>
+
 #include "dfs_attn.cuh"
 #include "dfs_tma.cuh"
 
@@ -237,11 +239,21 @@ DFS_DEV uint32_t range_word(int a, int b, int w) {
 // reach into the table needs no clamp: tab[delta + ext], ext = D + 255.
 DFS_DEV int bias_ext(int D) { return D + 255; }
 DFS_DEV void load_bias_ext(float* tab, const AttnParams& P, int h, int tid, int nthreads) {
-  const int E = bias_ext(P.D);
-  for (int x = tid; x < 2 * E + 1; x += nthreads) {
-    const int at = min(max(x - E, -P.D), P.D) + P.D;
-    const int b = min(max(P.lut[at], 0), P.nb - 1);
-    tab[x] = load_as_f32<void>(P.w, static_cast<size_t>(h) * P.nb + b, P.wdtype) * kLog2e;
+  const int E = bias_ext(P.D), W = 2 * E + 1;
+  for (int x0 = tid; x0 < W; x0 += 4 * nthreads) {  // four entries' look-ups in flight: each is two dependent loads
+    int b[4];
+    float v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int at = min(max(x0 + u * nthreads - E, -P.D), P.D) + P.D;
+      b[u] = P.lut[at];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      v[u] = load_as_f32<void>(P.w, static_cast<size_t>(h) * P.nb + min(max(b[u], 0), P.nb - 1), P.wdtype);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (x0 + u * nthreads < W) tab[x0 + u * nthreads] = v[u] * kLog2e;
   }
 }
 inline size_t bias_ext_bytes(const AttnParams& P) { return P.w ? (2 * (P.D + 255) + 1) * sizeof(float) : 0; }
@@ -318,15 +330,25 @@ bool tc_tmap(CUtensorMap* tm, const Strided& s, bool bf16, int d, int n, int hea
 // N = 4096, causal.)
 inline unsigned tc_grid(int n, int heads, int B) { return static_cast<unsigned>((n + kTcRows - 1) / kTcRows) * heads * B; }
 
-// Dynamic shared memory of a kernel, and that its register split fits what it is launched with (an increase
+// Dynamic shared memory of kernel K, raised once per device to the largest asked for (the call costs host
+// time); and, where the kernel splits its registers, that the shares fit what it is launched with (an increase
 // that the block's own registers cannot serve would wait forever).
-template <typename K>
-cudaError_t prepare_split(K kern, size_t smem, int threads, int share) {
-  cudaFuncAttributes at;
-  cudaError_t e = cudaFuncGetAttributes(&at, kern);
+template <auto K>
+cudaError_t prepare_kernel(size_t smem, int threads = 0, int share = 0) {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<size_t> ready[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if ((at.numRegs + 7) / 8 * 8 * threads < share) return cudaErrorInvalidConfiguration;
-  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (dev < kMaxDevices && ready[dev].load(std::memory_order_relaxed) >= smem) return cudaSuccess;
+  if (share > 0) {
+    cudaFuncAttributes at;
+    if ((e = cudaFuncGetAttributes(&at, K)) != cudaSuccess) return e;
+    if ((at.numRegs + 7) / 8 * 8 * threads < share) return cudaErrorInvalidConfiguration;
+  }
+  e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e == cudaSuccess && dev < kMaxDevices) ready[dev].store(smem, std::memory_order_relaxed);
+  return e;
 }
 
 cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st);

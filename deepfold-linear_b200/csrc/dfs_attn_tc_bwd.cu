@@ -662,6 +662,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
 
 }  // namespace
 
+template <bool BF16>
+static cudaError_t launch_bwd(const TcParams& T, size_t smem, cudaStream_t st) {
+  const AttnParams& P = T.a;
+  const int share = 512 * kElementRegs + 128 * kOtherRegs;
+  cudaError_t e = prepare_kernel<tc_dq_kernel<BF16>>(smem, kBwdThreads, share);
+  if (e == cudaSuccess) e = prepare_kernel<tc_dkv_kernel<BF16>>(smem, kBwdThreads, share);
+  if (e != cudaSuccess) return e;
+  tc_dq_kernel<BF16><<<tc_grid(P.nq, P.H, P.B), kBwdThreads, smem, st>>>(T);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  tc_dkv_kernel<BF16><<<tc_grid(P.nk, P.Hkv, P.B), kBwdThreads, smem, st>>>(T);
+  return cudaGetLastError();
+}
+
 cudaError_t launch_attn_tc_bwd(const AttnParams& P, int dtype, cudaStream_t st) {
   const bool bf16 = dtype == DFS_BF16;
   TcParams T;
@@ -671,16 +684,7 @@ cudaError_t launch_attn_tc_bwd(const AttnParams& P, int dtype, cudaStream_t st) 
     return cudaErrorInvalidValue;
   const size_t smem = 1024 + (2 + 2 * kStages) * kTcTileBytes + sizeof(BwdShared) + bias_ext_bytes(P) +
                       (P.w ? (2 * P.D + 1) * sizeof(float) : 0);
-  auto dq = bf16 ? tc_dq_kernel<true> : tc_dq_kernel<false>;
-  auto dkv = bf16 ? tc_dkv_kernel<true> : tc_dkv_kernel<false>;
-  const int share = 512 * kElementRegs + 128 * kOtherRegs;
-  cudaError_t e = prepare_split(dq, smem, kBwdThreads, share);
-  if (e == cudaSuccess) e = prepare_split(dkv, smem, kBwdThreads, share);
-  if (e != cudaSuccess) return e;
-  dq<<<tc_grid(P.nq, P.H, P.B), kBwdThreads, smem, st>>>(T);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  dkv<<<tc_grid(P.nk, P.Hkv, P.B), kBwdThreads, smem, st>>>(T);
-  return cudaGetLastError();
+  return bf16 ? launch_bwd<true>(T, smem, st) : launch_bwd<false>(T, smem, st);
 }
 
 }  // namespace dfs

@@ -72,7 +72,10 @@ Tensor walkable(const Tensor& t) {
 // An output laid out as `t` is.
 Tensor like(const Tensor& t) { return t.numel() ? at::empty_like(t) : at::empty(t.sizes(), t.options()); }
 
-dfs_strided strided(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+// (B, heads, n, d); a (B, heads, d) tensor has one row per head
+dfs_strided strided(const Tensor& t) {
+  return {t.data_ptr(), t.stride(0), t.stride(1), t.dim() == 4 ? t.stride(2) : 0};
+}
 
 dfs_relbias bias_of(const Tensor& w, const Tensor& lut, int64_t max_distance) {
   dfs_relbias b{};
@@ -105,11 +108,11 @@ Problem make_problem(const Tensor& Q, const Tensor& K, const Tensor& V, const op
                      int64_t sinks, bool causal, int64_t q_start, double scale) {
   require(Q.is_cuda() && K.is_cuda() && V.is_cuda(), "deepfold B200 attention runs on CUDA tensors only (no CPU path)");
   require(K.device() == Q.device() && V.device() == Q.device(), "Q, K, V must be on one device");
-  require(Q.dim() == 4 && K.dim() == 4 && V.sizes() == K.sizes() && K.size(0) == Q.size(0) && K.size(3) == Q.size(3),
+  require(K.dim() == 4 && V.sizes() == K.sizes() && K.size(0) == Q.size(0) && K.size(3) == Q.size(-1),
           "Q must be (B, H, n_q, d); K and V (B, H_kv, n_k, d)");
   require(float_type(Q) && K.scalar_type() == Q.scalar_type() && V.scalar_type() == Q.scalar_type(),
           "Q, K, V must share one type: bfloat16, float16 or float32");
-  const int64_t B = Q.size(0), H = Q.size(1), Hkv = K.size(1), d = Q.size(3);
+  const int64_t B = Q.size(0), H = Q.size(1), Hkv = K.size(1), d = Q.size(-1);
   require(H == 0 || (Hkv > 0 && H % Hkv == 0), "the query heads must be a multiple of the key heads");
   require(d >= 1 && d <= 64, "head dims 1 to 64 are supported");
   Problem r;
@@ -132,7 +135,7 @@ Problem make_problem(const Tensor& Q, const Tensor& K, const Tensor& V, const op
   p.B = narrow32(B, "B");
   p.H = narrow32(H, "H");
   p.H_kv = narrow32(Hkv, "H_kv");
-  p.n_q = narrow32(Q.size(2), "n_q");
+  p.n_q = Q.dim() == 4 ? narrow32(Q.size(2), "n_q") : 1;
   p.n_k = narrow32(K.size(2), "n_k");
   p.d = static_cast<int32_t>(d);
   p.dtype = dtype_code(Q.scalar_type());
@@ -227,6 +230,7 @@ Tensor window_attn(Tensor Q, Tensor K, Tensor V, optional<Tensor> mask, optional
   const bool has_w = weight.has_value() && weight->defined();
   const bool grad = at::GradMode::is_enabled() && (Q.requires_grad() || K.requires_grad() || V.requires_grad() ||
                                                    (has_w && weight->requires_grad()));
+  require(Q.dim() == 4, "Q must be (B, H, n_q, d)");
   if (grad)
     return WindowAttnFn::apply(Q, K, V, has_w ? weight : c10::nullopt, mask, lut, max_distance, window, sinks,
                                causal, q_start, scale);
@@ -237,7 +241,7 @@ Tensor window_attn(Tensor Q, Tensor K, Tensor V, optional<Tensor> mask, optional
 Tensor window_attn_decode(Tensor q, Tensor K, Tensor V, Tensor lengths, optional<Tensor> weight, optional<Tensor> lut,
                           int64_t max_distance, int64_t window, int64_t sinks, double scale) {
   require(q.dim() == 3, "q must be (B, H, d)");
-  const Problem r = make_problem(q.unsqueeze(2), K, V, c10::nullopt, weight, lut, max_distance, window, sinks, true, 0,
+  const Problem r = make_problem(q, K, V, c10::nullopt, weight, lut, max_distance, window, sinks, true, 0,
                                  scale);
   require(lengths.is_cuda() && lengths.device() == q.device() && lengths.dim() == 1 && lengths.size(0) == q.size(0) &&
               (lengths.scalar_type() == at::kInt || lengths.scalar_type() == at::kLong),
@@ -245,7 +249,7 @@ Tensor window_attn_decode(Tensor q, Tensor K, Tensor V, Tensor lengths, optional
   const Tensor len = lengths.contiguous().to(at::kInt);
   const DeviceSwitch guard(q.device());
   Tensor o = at::empty(q.sizes(), q.options());
-  dfs_attn_args a = args_of(r, o.unsqueeze(2), Tensor(), Tensor());
+  dfs_attn_args a = args_of(r, o, Tensor(), Tensor());
   a.status = checked_status(q.device());
   check_rc(dfs_window_attn_decode(&r.p, &a, len.data_ptr<int32_t>(), stream_of(q)), "dfs_window_attn_decode");
   return o;

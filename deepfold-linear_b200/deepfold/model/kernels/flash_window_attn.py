@@ -102,7 +102,8 @@ def window_attn_decode(q, k_cache, v_cache, lengths, window: int | None = None, 
     if not q.is_cuda:
         return window_attn_decode(_gpu(q), _gpu(k_cache), _gpu(v_cache), _gpu(lengths), window, sinks,
                                   _gpu(pos_weight), buckets, scale).cpu()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k_cache, v_cache, pos_weight)):
+    if (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad
+            or (pos_weight is not None and pos_weight.requires_grad)) and torch.is_grad_enabled():
         raise NotImplementedError("window_attn_decode is forward only: call it under torch.no_grad(), or "
                                   "flash_window_attn for gradients")
     window, scale, lut, distance = _options(q.shape[-1], window, sinks, scale, pos_weight, buckets, q.device)

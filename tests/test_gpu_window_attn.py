@@ -15,6 +15,7 @@ import numpy as np
 import pytest
 import torch
 
+from deepfold import _native as nat
 from deepfold.model.kernels.flash_window_attn import flash_window_attn, window_attn_decode
 from deepfold.model.position_encoding import RelativeBuckets, relative_position_bias
 from oracle import window_attn_oracle as orc
@@ -220,6 +221,23 @@ def test_results_repeat_bit_for_bit_and_on_another_stream():
         second = step()
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(first, second))
+
+
+def test_first_cuda_work_of_a_host_thread():
+    """A thread that has made no CUDA call yet, its tensors from the allocator's cache: the tensor maps are
+    encoded by the driver, which needs the thread's context bound first."""
+    import threading
+    x = inputs(1, 2, 2, 200, 200, 32, BF16, 15)
+    want = flash_window_attn(x["q"], x["k"], x["v"], window=50)
+    spare = [torch.empty_like(want) for _ in range(8)]
+    del spare
+    torch.cuda.synchronize()
+    got = []
+    t = threading.Thread(target=lambda: got.append(nat.ext().window_attn(x["q"], x["k"], x["v"], None, None, None, 0,
+                                                                         50, 0, True, 0, 32 ** -0.5)))
+    t.start()
+    t.join()
+    assert len(got) == 1 and torch.equal(got[0], want)
 
 
 def test_empty_sizes():
