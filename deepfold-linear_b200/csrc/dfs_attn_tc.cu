@@ -59,119 +59,133 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
   const int i0 = ((P.nq - 1) / kTcRows - static_cast<int>(blockIdx.x / P.H / P.B)) * kTcRows;  // causal: longest first
   const int p0 = i0 + P.qs;
   bool err = false;
-  if (threadIdx.x == 0) {
-    mbar_init(&S.q_full, 1);
-    for (int s = 0; s < kKStages; ++s) mbar_init(&S.k_full[s], 1), mbar_init(&S.k_empty[s], 1);
-    for (int s = 0; s < kVStages; ++s) mbar_init(&S.v_full[s], 1), mbar_init(&S.v_empty[s], 1);
-    mbar_init(&S.s_full, 1);
-    mbar_init(&S.s_free, kWork);
-    mbar_init(&S.p_ready, kWork);
-    mbar_init(&S.pv_done, 1);
-    fence_mbar_init();
-  }
-  if (warp == 8) tmem_alloc(&S.tmem, 256);
-  if (P.w) load_bias_ext(tab, P, h, threadIdx.x, kFwdThreads);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tm = S.tmem;
-
-  if (warp >= 8) regs_down<kOtherRegs>();
-  if (warp == 9) {  // ---- producer
-    const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
-    const TcKeyTiles tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
-    if (lane == 0) {
-      mbar_arrive_expect_tx(smem_u32(&S.q_full), kTcTileBytes);
-      tma_load_4d(sQ, &T.q, 0, i0, h, b, smem_u32(&S.q_full));
-    }
-    int t = 0;
-    for (int x = 0; x <= tiles.count(); ++x) {
-      const int j0 = x < tiles.count() ? tiles[x] * kTcRows : -1;
-      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
-      if (j0 >= 0 && mask != nullptr) {
-        key_bits(mask, j0, P.nk, lane, bits);
-        if ((bits[0] | bits[1] | bits[2] | bits[3]) == 0) continue;
-      }
-      const int ks = t % kKStages, vs = t % kVStages;
-      if (!tc_wait(&S.k_empty[ks], ((t / kKStages) & 1) ^ 1)) { err = true; break; }
+  if (warp >= 8) {
+    regs_down<kOtherRegs>();  // one instruction for the whole warpgroup
+    if (warp == 9) {  // ---- producer
       if (lane == 0) {
-        TileInfo& f = S.info[t % kInfo];
-        f.at = j0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
-        describe_tile(P, f, p0, j0);
-        if (j0 < 0) {
-          mbar_arrive(&S.k_full[ks]);
-        } else {
-          mbar_arrive_expect_tx(smem_u32(&S.k_full[ks]), kTcTileBytes);
-          tma_load_4d(sK + ks * kTcTileBytes, &T.k, 0, j0, hk, b, smem_u32(&S.k_full[ks]));
-        }
-      }
-      if (j0 < 0) break;
-      if (!tc_wait(&S.v_empty[vs], ((t / kVStages) & 1) ^ 1)) { err = true; break; }
-      if (lane == 0) {
-        mbar_arrive_expect_tx(smem_u32(&S.v_full[vs]), kTcTileBytes);
-        tma_load_4d(sV + vs * kTcTileBytes, &T.v, 0, j0, hk, b, smem_u32(&S.v_full[vs]));
-      }
-      ++t;
-    }
-  } else if (warp == 8) {  // ---- MMA
-    const uint32_t id_s = tc_idesc(128, 128, BF16, false);
-    const int dp = (P.d + 15) / 16 * 16;
-    const uint32_t id_o = tc_idesc(128, dp, BF16, true);
-    err = !tc_wait(&S.q_full, 0);
-    // announce tile t: its S, or the end
-    auto start = [&](int t, bool& end) {
-      const int ks = t % kKStages;
-      if (!tc_wait(&S.k_full[ks], (t / kKStages) & 1)) return false;
-      end = S.info[t % kInfo].at < 0;
-      if (t > 0 && !tc_wait(&S.s_free, (t - 1) & 1)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        if (end) {
-          mbar_arrive(&S.s_full);
-        } else {
-          tc_mma_kk(tm + kColS, tc_desc(sQ), tc_desc(sK + ks * kTcTileBytes), id_s, dp / 16);
-          mma_commit(&S.k_empty[ks]);
-          mma_commit(&S.s_full);
-        }
+        prefetch_tmap(&T.q);
+        prefetch_tmap(&T.k);
+        prefetch_tmap(&T.v);
+        mbar_init(&S.q_full, 1);
+        for (int s = 0; s < kKStages; ++s) mbar_init(&S.k_full[s], 1), mbar_init(&S.k_empty[s], 1);
+        for (int s = 0; s < kVStages; ++s) mbar_init(&S.v_full[s], 1), mbar_init(&S.v_empty[s], 1);
+        mbar_init(&S.s_full, 1);
+        mbar_init(&S.s_free, kWork);
+        mbar_init(&S.p_ready, kWork);
+        mbar_init(&S.pv_done, 1);
+        fence_mbar_init();
       }
       __syncwarp();
-      return true;
-    };
-    bool end = false;
-    if (!err) err = !start(0, end);
-    for (int t = 0; !end && !err; ++t) {
-      uint32_t bits[4];
+      setup_arrive<kFwdThreads>();
+      const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
+      const TcKeyTiles tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(smem_u32(&S.q_full), kTcTileBytes);
+        tma_load_4d(sQ, &T.q, 0, i0, h, b, smem_u32(&S.q_full));
+      }
+      int t = 0;
+      for (int x = 0; x <= tiles.count(); ++x) {
+        const int j0 = x < tiles.count() ? tiles[x] * kTcRows : -1;
+        uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+        if (j0 >= 0 && mask != nullptr) {
+          key_bits(mask, j0, P.nk, lane, bits);
+          if ((bits[0] | bits[1] | bits[2] | bits[3]) == 0) continue;
+        }
+        const int ks = t % kKStages, vs = t % kVStages;
+        if (!tc_wait(&S.k_empty[ks], ((t / kKStages) & 1) ^ 1)) { err = true; break; }
+        if (lane == 0) {
+          TileInfo& f = S.info[t % kInfo];
+          f.at = j0;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) bits[w] = S.info[t % kInfo].bits[w];
-      bool next_end = false;
-      if (!start(t + 1, next_end)) { err = true; break; }
-      const int vs = t % kVStages;
-      if (!tc_wait(&S.v_full[vs], (t / kVStages) & 1)) { err = true; break; }
-      if (P.mask != nullptr && (bits[0] & bits[1] & bits[2] & bits[3]) != ~0u) {
-        // a hidden key's V may hold anything, and 0 x NaN is NaN: zero its row
-        unsigned char* vt = gen + (1 + kKStages + vs) * kTcTileBytes;
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          for (int r = lane / 8; r < 32; r += 4)
-            if (!((bits[w] >> r) & 1u))
-              *reinterpret_cast<uint4*>(vt + (32 * w + r) * 128 + (lane % 8) * 16) = make_uint4(0, 0, 0, 0);
-        fence_async_smem();
+          for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
+          describe_tile(P, f, p0, j0);
+          if (j0 < 0) {
+            mbar_arrive(&S.k_full[ks]);
+          } else {
+            mbar_arrive_expect_tx(smem_u32(&S.k_full[ks]), kTcTileBytes);
+            tma_load_4d(sK + ks * kTcTileBytes, &T.k, 0, j0, hk, b, smem_u32(&S.k_full[ks]));
+          }
+        }
+        if (j0 < 0) break;
+        if (!tc_wait(&S.v_empty[vs], ((t / kVStages) & 1) ^ 1)) { err = true; break; }
+        if (lane == 0) {
+          mbar_arrive_expect_tx(smem_u32(&S.v_full[vs]), kTcTileBytes);
+          tma_load_4d(sV + vs * kTcTileBytes, &T.v, 0, j0, hk, b, smem_u32(&S.v_full[vs]));
+        }
+        ++t;
+      }
+    } else if (warp == 8) {  // ---- MMA
+      tmem_alloc(&S.tmem, 256);
+      tc_fence_before();
+      setup_wait<kFwdThreads>();
+      tc_fence_after();
+      const uint32_t tm = S.tmem;
+      const uint32_t id_s = tc_idesc(128, 128, BF16, false);
+      const int dp = (P.d + 15) / 16 * 16;
+      const uint32_t id_o = tc_idesc(128, dp, BF16, true);
+      err = !tc_wait(&S.q_full, 0);
+      // announce tile t: its S, or the end
+      auto start = [&](int t, bool& end) {
+        const int ks = t % kKStages;
+        if (!tc_wait(&S.k_full[ks], (t / kKStages) & 1)) return false;
+        end = S.info[t % kInfo].at < 0;
+        if (t > 0 && !tc_wait(&S.s_free, (t - 1) & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          if (end) {
+            mbar_arrive(&S.s_full);
+          } else {
+            tc_mma_kk(tm + kColS, tc_desc(sQ), tc_desc(sK + ks * kTcTileBytes), id_s, dp / 16);
+            mma_commit(&S.k_empty[ks]);
+            mma_commit(&S.s_full);
+          }
+        }
         __syncwarp();
+        return true;
+      };
+      bool end = false;
+      if (!err) err = !start(0, end);
+      for (int t = 0; !end && !err; ++t) {
+        uint32_t bits[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) bits[w] = S.info[t % kInfo].bits[w];
+        bool next_end = false;
+        if (!start(t + 1, next_end)) { err = true; break; }
+        const int vs = t % kVStages;
+        if (!tc_wait(&S.v_full[vs], (t / kVStages) & 1)) { err = true; break; }
+        if (P.mask != nullptr && (bits[0] & bits[1] & bits[2] & bits[3]) != ~0u) {
+          // a hidden key's V may hold anything, and 0 x NaN is NaN: zero its row
+          unsigned char* vt = gen + (1 + kKStages + vs) * kTcTileBytes;
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            for (int r = lane / 8; r < 32; r += 4)
+              if (!((bits[w] >> r) & 1u))
+                *reinterpret_cast<uint4*>(vt + (32 * w + r) * 128 + (lane % 8) * 16) = make_uint4(0, 0, 0, 0);
+          fence_async_smem();
+          __syncwarp();
+        }
+        if (!tc_wait(&S.p_ready, t & 1)) { err = true; break; }
+        tc_fence_after();
+        if (elect_one()) {
+          tc_mma_ts(tm + kColO, tm + kColP, tc_desc(sV + vs * kTcTileBytes), id_o, t > 0);
+          mma_commit(&S.v_empty[vs]);
+          mma_commit(&S.pv_done);
+        }
+        __syncwarp();
+        end = next_end;
       }
-      if (!tc_wait(&S.p_ready, t & 1)) { err = true; break; }
-      tc_fence_after();
-      if (elect_one()) {
-        tc_mma_ts(tm + kColO, tm + kColP, tc_desc(sV + vs * kTcTileBytes), id_o, t > 0);
-        mma_commit(&S.v_empty[vs]);
-        mma_commit(&S.pv_done);
-      }
-      __syncwarp();
-      end = next_end;
+    } else if (warp != 8) {  // ---- the warpgroup's idle warps
+      setup_wait<kFwdThreads>();
     }
-  } else if (warp < 8) {  // ---- elements: warp w has rows 32 (w % 4).. and columns 64 (w / 4)..
+  } else {  // ---- elements: warp w has rows 32 (w % 4).. and columns 64 (w / 4)..
+    setup_wait<kFwdThreads>();
+    tc_fence_after();
     regs_up<kElementRegs>();
+    const uint32_t tm = S.tmem;
+    if (P.w) {
+      load_bias_ext(tab, P, h, threadIdx.x, kWork);
+      asm volatile("bar.sync 5, 256;" ::: "memory");
+    }
     const int wq = warp % 4, ch = warp / 4;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
     const int row = wq * 32 + lane, i = i0 + row, p = p0 + row, pw = p0 + wq * 32;
@@ -328,7 +342,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tm, 256);
+  if (warp == 8) tmem_dealloc(S.tmem, 256);
 }
 
 }  // namespace

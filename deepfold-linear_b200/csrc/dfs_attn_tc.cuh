@@ -31,6 +31,17 @@ DFS_DEV void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accum));
 }
 
+// The setup barrier of a block: the TMA warp, which initialises the mbarriers, only
+// arrives and starts its copies at once; everybody else waits for the mbarriers,
+// the TMEM address and each other.
+template <int N>
+DFS_DEV void setup_arrive() { asm volatile("bar.arrive 8, %0;" ::"n"(N) : "memory"); }
+template <int N>
+DFS_DEV void setup_wait() { asm volatile("bar.sync 8, %0;" ::"n"(N) : "memory"); }
+DFS_DEV void prefetch_tmap(const CUtensorMap* tm) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tm)) : "memory");
+}
+
 // maximum of 32 values held as bits
 DFS_DEV float max32u(const uint32_t (&v)[32]) {
   float a[3];

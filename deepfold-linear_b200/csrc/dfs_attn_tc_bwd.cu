@@ -90,111 +90,124 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
   const int i0 = ((P.nq - 1) / kTcRows - static_cast<int>(blockIdx.x / P.H / P.B)) * kTcRows;  // causal: longest first
   const int p0 = i0 + P.qs;
   bool err = false;
-  if (threadIdx.x == 0) {
-    mbar_init(&S.own_full, 1);
-    for (int s = 0; s < kStages; ++s) mbar_init(&S.full[s], 1), mbar_init(&S.empty[s], 1);
-    mbar_init(&S.s_full, 1);
-    mbar_init(&S.s_free, kWork);
-    mbar_init(&S.ds_ready, kWork);
-    mbar_init(&S.acc_done, 1);
-    fence_mbar_init();
-  }
-  if (warp == kMmaWarp) tmem_alloc(&S.tmem, 512);
-  if (P.w) load_bias_ext(tab, P, h, threadIdx.x, kBwdThreads);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tm = S.tmem;
 
-  if (warp >= kMmaWarp) regs_down<kOtherRegs>();
-  if (warp == kTmaWarp) {  // ---- producer
-    const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
-    const TcKeyTiles tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
-    if (lane == 0) {
-      mbar_arrive_expect_tx(smem_u32(&S.own_full), 2 * kTcTileBytes);
-      tma_load_4d(sQ, &T.q, 0, i0, h, b, smem_u32(&S.own_full));
-      tma_load_4d(sO, &T.d_o, 0, i0, h, b, smem_u32(&S.own_full));
-    }
-    int t = 0;
-    for (int x = 0; x <= tiles.count(); ++x) {
-      const int j0 = x < tiles.count() ? tiles[x] * kTcRows : -1;
-      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
-      if (j0 >= 0 && mask != nullptr) {
-        key_bits(mask, j0, P.nk, lane, bits);
-        if ((bits[0] | bits[1] | bits[2] | bits[3]) == 0) continue;
-      }
-      const int s = t % kStages;
-      if (!tc_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
+  if (warp >= kMmaWarp) {
+    regs_down<kOtherRegs>();  // one instruction for the whole warpgroup
+    if (warp == kTmaWarp) {  // ---- producer
       if (lane == 0) {
-        TileInfo& f = S.info[t % kInfo];
-        f.at = j0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
-        describe_tile(P, f, p0, j0);
-        if (j0 < 0) {
-          mbar_arrive(&S.full[s]);
-        } else {
-          mbar_arrive_expect_tx(smem_u32(&S.full[s]), 2 * kTcTileBytes);
-          tma_load_4d(sK + s * kTcTileBytes, &T.k, 0, j0, hk, b, smem_u32(&S.full[s]));
-          tma_load_4d(sV + s * kTcTileBytes, &T.v, 0, j0, hk, b, smem_u32(&S.full[s]));
-        }
+        prefetch_tmap(&T.q);
+        prefetch_tmap(&T.k);
+        prefetch_tmap(&T.v);
+        prefetch_tmap(&T.d_o);
+        mbar_init(&S.own_full, 1);
+        for (int s = 0; s < kStages; ++s) mbar_init(&S.full[s], 1), mbar_init(&S.empty[s], 1);
+        mbar_init(&S.s_full, 1);
+        mbar_init(&S.s_free, kWork);
+        mbar_init(&S.ds_ready, kWork);
+        mbar_init(&S.acc_done, 1);
+        fence_mbar_init();
       }
-      ++t;
-    }
-  } else if (warp == kMmaWarp) {  // ---- MMA
-    const int dp = (P.d + 15) / 16 * 16;
-    const uint32_t id_s = tc_idesc(128, 128, BF16, false), id_a = tc_idesc(128, dp, BF16, true);
-    err = !tc_wait(&S.own_full, 0);
-    auto start = [&](int t, bool& end) {
-      const int s = t % kStages;
-      if (!tc_wait(&S.full[s], (t / kStages) & 1)) return false;
-      const TileInfo& f = S.info[t % kInfo];
-      end = f.at < 0;
-      if (!end && P.mask != nullptr) {
-        // a hidden key's K may hold anything, and 0 x NaN is NaN in dS K: zero its row
-        unsigned char* kt = gen + (2 + s) * kTcTileBytes;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t bw = f.bits[w];
-          if (bw != ~0u)
-            for (int r = lane / 8; r < 32; r += 4)
-              if (!((bw >> r) & 1u))
-                *reinterpret_cast<uint4*>(kt + (32 * w + r) * 128 + (lane % 8) * 16) = make_uint4(0, 0, 0, 0);
+      __syncwarp();
+      setup_arrive<kBwdThreads>();
+      const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
+      const TcKeyTiles tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(smem_u32(&S.own_full), 2 * kTcTileBytes);
+        tma_load_4d(sQ, &T.q, 0, i0, h, b, smem_u32(&S.own_full));
+        tma_load_4d(sO, &T.d_o, 0, i0, h, b, smem_u32(&S.own_full));
+      }
+      int t = 0;
+      for (int x = 0; x <= tiles.count(); ++x) {
+        const int j0 = x < tiles.count() ? tiles[x] * kTcRows : -1;
+        uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+        if (j0 >= 0 && mask != nullptr) {
+          key_bits(mask, j0, P.nk, lane, bits);
+          if ((bits[0] | bits[1] | bits[2] | bits[3]) == 0) continue;
         }
-        fence_async_smem();
+        const int s = t % kStages;
+        if (!tc_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
+        if (lane == 0) {
+          TileInfo& f = S.info[t % kInfo];
+          f.at = j0;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
+          describe_tile(P, f, p0, j0);
+          if (j0 < 0) {
+            mbar_arrive(&S.full[s]);
+          } else {
+            mbar_arrive_expect_tx(smem_u32(&S.full[s]), 2 * kTcTileBytes);
+            tma_load_4d(sK + s * kTcTileBytes, &T.k, 0, j0, hk, b, smem_u32(&S.full[s]));
+            tma_load_4d(sV + s * kTcTileBytes, &T.v, 0, j0, hk, b, smem_u32(&S.full[s]));
+          }
+        }
+        ++t;
+      }
+    } else if (warp == kMmaWarp) {  // ---- MMA
+      tmem_alloc(&S.tmem, 512);
+      tc_fence_before();
+      setup_wait<kBwdThreads>();
+      tc_fence_after();
+      const uint32_t tm = S.tmem;
+      const int dp = (P.d + 15) / 16 * 16;
+      const uint32_t id_s = tc_idesc(128, 128, BF16, false), id_a = tc_idesc(128, dp, BF16, true);
+      err = !tc_wait(&S.own_full, 0);
+      auto start = [&](int t, bool& end) {
+        const int s = t % kStages;
+        if (!tc_wait(&S.full[s], (t / kStages) & 1)) return false;
+        const TileInfo& f = S.info[t % kInfo];
+        end = f.at < 0;
+        if (!end && P.mask != nullptr) {
+          // a hidden key's K may hold anything, and 0 x NaN is NaN in dS K: zero its row
+          unsigned char* kt = gen + (2 + s) * kTcTileBytes;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t bw = f.bits[w];
+            if (bw != ~0u)
+              for (int r = lane / 8; r < 32; r += 4)
+                if (!((bw >> r) & 1u))
+                  *reinterpret_cast<uint4*>(kt + (32 * w + r) * 128 + (lane % 8) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_async_smem();
+          __syncwarp();
+        }
+        if (t > 0 && !tc_wait(&S.s_free, (t - 1) & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          if (end) {
+            mbar_arrive(&S.s_full);
+          } else {
+            tc_mma_kk(tm + kColS, tc_desc(sQ), tc_desc(sK + s * kTcTileBytes), id_s, dp / 16);
+            tc_mma_kk(tm + kColDP, tc_desc(sO), tc_desc(sV + s * kTcTileBytes), id_s, dp / 16);
+            mma_commit(&S.s_full);
+          }
+        }
         __syncwarp();
-      }
-      if (t > 0 && !tc_wait(&S.s_free, (t - 1) & 1)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        if (end) {
-          mbar_arrive(&S.s_full);
-        } else {
-          tc_mma_kk(tm + kColS, tc_desc(sQ), tc_desc(sK + s * kTcTileBytes), id_s, dp / 16);
-          tc_mma_kk(tm + kColDP, tc_desc(sO), tc_desc(sV + s * kTcTileBytes), id_s, dp / 16);
-          mma_commit(&S.s_full);
+        return true;
+      };
+      bool end = false;
+      if (!err) err = !start(0, end);
+      for (int t = 0; !end && !err; ++t) {
+        bool next_end = false;
+        if (!start(t + 1, next_end)) { err = true; break; }
+        if (!tc_wait(&S.ds_ready, t & 1)) { err = true; break; }
+        tc_fence_after();
+        if (elect_one()) {
+          tc_mma_ts(tm + kColA, tm + kColDS, tc_desc(sK + (t % kStages) * kTcTileBytes), id_a, t > 0);
+          mma_commit(&S.empty[t % kStages]);
+          mma_commit(&S.acc_done);
         }
+        __syncwarp();
+        end = next_end;
       }
-      __syncwarp();
-      return true;
-    };
-    bool end = false;
-    if (!err) err = !start(0, end);
-    for (int t = 0; !end && !err; ++t) {
-      bool next_end = false;
-      if (!start(t + 1, next_end)) { err = true; break; }
-      if (!tc_wait(&S.ds_ready, t & 1)) { err = true; break; }
-      tc_fence_after();
-      if (elect_one()) {
-        tc_mma_ts(tm + kColA, tm + kColDS, tc_desc(sK + (t % kStages) * kTcTileBytes), id_a, t > 0);
-        mma_commit(&S.empty[t % kStages]);
-        mma_commit(&S.acc_done);
-      }
-      __syncwarp();
-      end = next_end;
+    } else if (warp != kMmaWarp) {  // ---- the warpgroup's idle warps
+      setup_wait<kBwdThreads>();
     }
-  } else if (warp < kMmaWarp) {  // ---- elements: warp w has TMEM lanes 32 (w % 4).. and columns 32 (w / 4)..
+  } else {  // ---- elements: warp w has TMEM lanes 32 (w % 4).. and columns 32 (w / 4)..
+    setup_wait<kBwdThreads>();
+    tc_fence_after();
     regs_up<kElementRegs>();
+    const uint32_t tm = S.tmem;
+    if (P.w) load_bias_ext(tab, P, h, threadIdx.x, kWork);  // read after the barrier below
     const int wq = warp % 4, cg = warp / 4, row = wq * 32 + lane, i = i0 + row, p = p0 + row, pw = p0 + 32 * wq;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
     const int E = bias_ext(P.D), c0 = 16 * cg;  // c0: this thread's columns of d
@@ -321,7 +334,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp) tmem_dealloc(tm, 512);
+  if (warp == kMmaWarp) tmem_dealloc(S.tmem, 512);
 }
 
 template <bool BF16>
@@ -339,20 +352,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
   const int hk = blockIdx.x % P.Hkv, b = blockIdx.x / P.Hkv % P.B, tile = blockIdx.x / P.Hkv / P.B;
   const int j0 = tile * kTcRows;  // the sinks' tiles, which all queries see, first
   bool err = false;
-  if (threadIdx.x == 0) {
-    mbar_init(&S.own_full, 1);
-    for (int s = 0; s < kStages; ++s) mbar_init(&S.full[s], 1), mbar_init(&S.empty[s], 1);
-    mbar_init(&S.s_full, 1);
-    mbar_init(&S.s_free, kWork);
-    mbar_init(&S.ds_ready, kWork);
-    mbar_init(&S.acc_done, 1);
-    fence_mbar_init();
-  }
-  if (warp == kMmaWarp) tmem_alloc(&S.tmem, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tm = S.tmem;
 
   // queries that see some key of the tile: [i_lo, i_hi)
   int i_lo = P.causal ? j0 - P.qs : j0 - P.window + 1 - P.qs;
@@ -364,94 +363,121 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
   i_lo = max(i_lo, 0) / kTcRows;
   i_hi = (min(i_hi, P.nq) + kTcRows - 1) / kTcRows;  // in tiles
 
-  if (warp >= kMmaWarp) regs_down<kOtherRegs>();
-  if (warp == kTmaWarp) {  // ---- producer
-    uint32_t bits[4];
-    key_bits(P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr, j0, P.nk, lane, bits);
-    const int per = (bits[0] | bits[1] | bits[2] | bits[3]) == 0 ? 0 : max(0, i_hi - i_lo);
-    if (lane == 0) {
-      mbar_arrive_expect_tx(smem_u32(&S.own_full), 2 * kTcTileBytes);
-      tma_load_4d(sK, &T.k, 0, j0, hk, b, smem_u32(&S.own_full));
-      tma_load_4d(sV, &T.v, 0, j0, hk, b, smem_u32(&S.own_full));
-    }
-    const int total = per * P.G;
-    for (int t = 0; t <= total; ++t) {
-      const int s = t % kStages;
-      const int g = t < total ? t / per : 0, h = hk * P.G + g, i0 = t < total ? (i_lo + t % per) * kTcRows : -1;
-      float st[2][4];
-      if (i0 >= 0) {
-        const size_t at = (static_cast<size_t>(b) * P.H + h) * P.nq;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = i0 + 4 * lane + e;
-          st[0][e] = i < P.nq ? -P.lse[at + i] : -INFINITY;
-          st[1][e] = i < P.nq ? -P.dsum[at + i] : 0.0f;
-        }
-      }
-      if (!tc_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
-      if (i0 >= 0) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          *reinterpret_cast<float4*>(&S.stat[s][k][4 * lane]) = make_float4(st[k][0], st[k][1], st[k][2], st[k][3]);
-      }
-      __syncwarp();
+  if (warp >= kMmaWarp) {
+    regs_down<kOtherRegs>();  // one instruction for the whole warpgroup
+    if (warp == kTmaWarp) {  // ---- producer
       if (lane == 0) {
-        TileInfo& f = S.info[t % kInfo];
-        f.at = i0;
-        f.head = g;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
-        describe_tile(P, f, i0 + P.qs, j0);
-        if (i0 < 0) {
-          mbar_arrive(&S.full[s]);
-        } else {
-          mbar_arrive_expect_tx(smem_u32(&S.full[s]), 2 * kTcTileBytes);
-          tma_load_4d(sQ + s * kTcTileBytes, &T.q, 0, i0, h, b, smem_u32(&S.full[s]));
-          tma_load_4d(sO + s * kTcTileBytes, &T.d_o, 0, i0, h, b, smem_u32(&S.full[s]));
-        }
-      }
-    }
-  } else if (warp == kMmaWarp) {  // ---- MMA
-    const int dp = (P.d + 15) / 16 * 16;
-    const uint32_t id_s = tc_idesc(128, 128, BF16, false), id_a = tc_idesc(128, dp, BF16, true);
-    err = !tc_wait(&S.own_full, 0);
-    auto start = [&](int t, bool& end) {
-      const int s = t % kStages;
-      if (!tc_wait(&S.full[s], (t / kStages) & 1)) return false;
-      end = S.info[t % kInfo].at < 0;
-      if (t > 0 && !tc_wait(&S.s_free, (t - 1) & 1)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        if (end) {
-          mbar_arrive(&S.s_full);
-        } else {
-          tc_mma_kk(tm + kColS, tc_desc(sK), tc_desc(sQ + s * kTcTileBytes), id_s, dp / 16);
-          tc_mma_kk(tm + kColDP, tc_desc(sV), tc_desc(sO + s * kTcTileBytes), id_s, dp / 16);
-          mma_commit(&S.s_full);
-        }
+        prefetch_tmap(&T.q);
+        prefetch_tmap(&T.k);
+        prefetch_tmap(&T.v);
+        prefetch_tmap(&T.d_o);
+        mbar_init(&S.own_full, 1);
+        for (int s = 0; s < kStages; ++s) mbar_init(&S.full[s], 1), mbar_init(&S.empty[s], 1);
+        mbar_init(&S.s_full, 1);
+        mbar_init(&S.s_free, kWork);
+        mbar_init(&S.ds_ready, kWork);
+        mbar_init(&S.acc_done, 1);
+        fence_mbar_init();
       }
       __syncwarp();
-      return true;
-    };
-    bool end = false;
-    if (!err) err = !start(0, end);
-    for (int t = 0; !end && !err; ++t) {
-      bool next_end = false;
-      if (!start(t + 1, next_end)) { err = true; break; }
-      if (!tc_wait(&S.ds_ready, t & 1)) { err = true; break; }
-      tc_fence_after();
-      if (elect_one()) {
+      setup_arrive<kBwdThreads>();
+      uint32_t bits[4];
+      key_bits(P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr, j0, P.nk, lane, bits);
+      const int per = (bits[0] | bits[1] | bits[2] | bits[3]) == 0 ? 0 : max(0, i_hi - i_lo);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(smem_u32(&S.own_full), 2 * kTcTileBytes);
+        tma_load_4d(sK, &T.k, 0, j0, hk, b, smem_u32(&S.own_full));
+        tma_load_4d(sV, &T.v, 0, j0, hk, b, smem_u32(&S.own_full));
+      }
+      const int total = per * P.G;
+      for (int t = 0; t <= total; ++t) {
         const int s = t % kStages;
-        tc_mma_ts(tm + kColA, tm + kColP, tc_desc(sO + s * kTcTileBytes), id_a, t > 0);
-        tc_mma_ts(tm + kColB, tm + kColDS, tc_desc(sQ + s * kTcTileBytes), id_a, t > 0);
-        mma_commit(&S.empty[s]);
-        mma_commit(&S.acc_done);
+        const int g = t < total ? t / per : 0, h = hk * P.G + g, i0 = t < total ? (i_lo + t % per) * kTcRows : -1;
+        float st[2][4];
+        if (i0 >= 0) {
+          const size_t at = (static_cast<size_t>(b) * P.H + h) * P.nq;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = i0 + 4 * lane + e;
+            st[0][e] = i < P.nq ? -P.lse[at + i] : -INFINITY;
+            st[1][e] = i < P.nq ? -P.dsum[at + i] : 0.0f;
+          }
+        }
+        if (!tc_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
+        if (i0 >= 0) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            *reinterpret_cast<float4*>(&S.stat[s][k][4 * lane]) = make_float4(st[k][0], st[k][1], st[k][2], st[k][3]);
+        }
+        __syncwarp();
+        if (lane == 0) {
+          TileInfo& f = S.info[t % kInfo];
+          f.at = i0;
+          f.head = g;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
+          describe_tile(P, f, i0 + P.qs, j0);
+          if (i0 < 0) {
+            mbar_arrive(&S.full[s]);
+          } else {
+            mbar_arrive_expect_tx(smem_u32(&S.full[s]), 2 * kTcTileBytes);
+            tma_load_4d(sQ + s * kTcTileBytes, &T.q, 0, i0, h, b, smem_u32(&S.full[s]));
+            tma_load_4d(sO + s * kTcTileBytes, &T.d_o, 0, i0, h, b, smem_u32(&S.full[s]));
+          }
+        }
       }
-      __syncwarp();
-      end = next_end;
+    } else if (warp == kMmaWarp) {  // ---- MMA
+      tmem_alloc(&S.tmem, 512);
+      tc_fence_before();
+      setup_wait<kBwdThreads>();
+      tc_fence_after();
+      const uint32_t tm = S.tmem;
+      const int dp = (P.d + 15) / 16 * 16;
+      const uint32_t id_s = tc_idesc(128, 128, BF16, false), id_a = tc_idesc(128, dp, BF16, true);
+      err = !tc_wait(&S.own_full, 0);
+      auto start = [&](int t, bool& end) {
+        const int s = t % kStages;
+        if (!tc_wait(&S.full[s], (t / kStages) & 1)) return false;
+        end = S.info[t % kInfo].at < 0;
+        if (t > 0 && !tc_wait(&S.s_free, (t - 1) & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          if (end) {
+            mbar_arrive(&S.s_full);
+          } else {
+            tc_mma_kk(tm + kColS, tc_desc(sK), tc_desc(sQ + s * kTcTileBytes), id_s, dp / 16);
+            tc_mma_kk(tm + kColDP, tc_desc(sV), tc_desc(sO + s * kTcTileBytes), id_s, dp / 16);
+            mma_commit(&S.s_full);
+          }
+        }
+        __syncwarp();
+        return true;
+      };
+      bool end = false;
+      if (!err) err = !start(0, end);
+      for (int t = 0; !end && !err; ++t) {
+        bool next_end = false;
+        if (!start(t + 1, next_end)) { err = true; break; }
+        if (!tc_wait(&S.ds_ready, t & 1)) { err = true; break; }
+        tc_fence_after();
+        if (elect_one()) {
+          const int s = t % kStages;
+          tc_mma_ts(tm + kColA, tm + kColP, tc_desc(sO + s * kTcTileBytes), id_a, t > 0);
+          tc_mma_ts(tm + kColB, tm + kColDS, tc_desc(sQ + s * kTcTileBytes), id_a, t > 0);
+          mma_commit(&S.empty[s]);
+          mma_commit(&S.acc_done);
+        }
+        __syncwarp();
+        end = next_end;
+      }
+    } else if (warp != kMmaWarp) {  // ---- the warpgroup's idle warps
+      setup_wait<kBwdThreads>();
     }
-  } else if (warp < kMmaWarp) {  // ---- elements: a key row and a quarter of the tile's queries per thread
+  } else {  // ---- elements: a key row and a quarter of the tile's queries per thread
+    setup_wait<kBwdThreads>();
+    tc_fence_after();
     regs_up<kElementRegs>();
+    const uint32_t tm = S.tmem;
     const int wq = warp % 4, cg = warp / 4, row = wq * 32 + lane, j = j0 + row, jw = j0 + 32 * wq, tid = threadIdx.x;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
     const int E = bias_ext(P.D);
@@ -657,7 +683,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp) tmem_dealloc(tm, 512);
+  if (warp == kMmaWarp) tmem_dealloc(S.tmem, 512);
 }
 
 }  // namespace
