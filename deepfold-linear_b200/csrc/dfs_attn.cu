@@ -72,9 +72,31 @@ size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 size_t dsum_bytes(const dfs_attn_problem* p) {
   return round256(sizeof(float) * static_cast<size_t>(p->B) * p->H * p->n_q);
 }
-// rows of dw_part per head: a key tile of a batch element each
-int dw_parts(const dfs_attn_problem* p, int tile) { return p->B * ((p->n_k + tile - 1) / tile); }
-constexpr int kSmallestTile = 64;
+// The backward's key pass: units of work of a batch element and key head.  Every query sees the sinks, so the
+// CTAs of their key tiles would walk all query tiles, with the others done long before; where the queries beyond
+// the window are many, they are cut into segments of their own of about an ordinary tile's length.
+struct KeyUnits {
+  int tiles, sink_tiles, far_segs, far_len;
+  int count() const { return tiles + sink_tiles * far_segs; }
+};
+KeyUnits key_units(const dfs_attn_problem* p, int tile, int q_tile) {
+  KeyUnits u{(p->n_k + tile - 1) / tile, 0, 0, 0};
+  if (p->window == 0 || p->sinks == 0 || q_tile == 0 || p->H_kv == 0) return u;
+  const int64_t G = p->H / p->H_kv, q_tiles = (p->n_q + q_tile - 1) / q_tile;
+  const int64_t near_end = std::min<int64_t>(std::max<int64_t>(int64_t{std::min(tile, p->n_k)} - 1 + p->window - p->q_start, 0), p->n_q);
+  const int64_t far = (q_tiles - (near_end + q_tile - 1) / q_tile) * G;  // of the first tile, the most
+  const int64_t len = std::max<int64_t>(std::min<int64_t>((int64_t{tile} + p->window) / q_tile + 1, q_tiles) * G, 8);
+  if (far < 2 * len) return u;
+  u.sink_tiles = static_cast<int>((std::min(p->sinks, p->n_k) + tile - 1) / tile);
+  u.far_segs = static_cast<int>((far + len - 1) / len);
+  u.far_len = static_cast<int>(len);
+  return u;
+}
+size_t sink_part_bytes(const dfs_attn_problem* p, const KeyUnits& u) {
+  return sizeof(float) * 128 * static_cast<size_t>(std::min<int>(p->sinks, kTcRows)) * p->B * p->H_kv * u.sink_tiles *
+         (u.far_segs > 0 ? u.far_segs + 1 : 0);
+}
+constexpr int kSimtTile = 64;
 
 // Whether an operand can be staged by TMA (and stored in 16-byte pieces): its address and the strides of
 // its extents above 1 are multiples of 16 bytes.
@@ -87,9 +109,9 @@ bool staged(const dfs_strided& s, int n, int heads, int B) {
 // The tensor-core kernels: 16-bit operands that TMA can stage.  fp32 operands keep all their bits on the
 // SIMT kernels; a scale that is not positive would turn the running maximum of raw products around.
 bool tensor_cores(const dfs_attn_problem* p, const dfs_attn_args* a) {
-  const int64_t tiles = (std::max(p->n_q, p->n_k) + kTcRows - 1) / kTcRows;
-  return tiles * p->B * p->H < (int64_t{1} << 31) && p->dtype != DFS_F32 && p->d % 8 == 0 && p->scale > 0.0f && p->n_q > 0 && p->n_k > 0 && tmap_available() && aligned16(a->o_lo) &&
-         staged(a->q, p->n_q, p->H, p->B) && staged(a->o, p->n_q, p->H, p->B) &&
+  const int64_t tiles = (std::max(p->n_q, p->n_k) + kTcRows - 1) / kTcRows + (p->n_q + kTcHalf - 1) / kTcHalf;
+  return tiles * p->B * p->H < (int64_t{1} << 31) && p->dtype != DFS_F32 && p->d % 8 == 0 && p->scale > 0.0f &&
+         p->n_q > 0 && p->n_k > 0 && tmap_available() && aligned16(a->o_lo) && staged(a->q, p->n_q, p->H, p->B) && staged(a->o, p->n_q, p->H, p->B) &&
          staged(a->k, p->n_k, p->H_kv, p->B) && staged(a->v, p->n_k, p->H_kv, p->B);
 }
 int rc(cudaError_t e) { return e == cudaSuccess ? DFS_OK : DFS_ERR_CUDA; }
@@ -109,8 +131,12 @@ extern "C" int dfs_window_attn_fwd(const dfs_attn_problem* p, const dfs_attn_arg
 
 extern "C" size_t dfs_window_attn_bwd_work(const dfs_attn_problem* p, const dfs_relbias* b) {
   if (problem_status(p, b) != DFS_OK) return 0;
-  size_t n = dsum_bytes(p);
-  if (b && b->weight) n += sizeof(float) * static_cast<size_t>(p->H) * dw_parts(p, kSmallestTile) * (2 * b->max_distance + 1);
+  const KeyUnits u = key_units(p, kTcRows, kTcHalf);
+  size_t n = dsum_bytes(p) + round256(sink_part_bytes(p, u));
+  if (b && b->weight) {
+    const int units = std::max(u.count(), key_units(p, kSimtTile, 0).count());  // whichever kernels run
+    n += sizeof(float) * static_cast<size_t>(p->H) * p->B * units * (2 * b->max_distance + 1);
+  }
   return n;
 }
 
@@ -131,8 +157,14 @@ extern "C" int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_arg
   P.dsum = static_cast<float*>(work);
   const bool tc = tensor_cores(p, a) && staged(a->d_o, p->n_q, p->H, p->B) && staged(a->d_q, p->n_q, p->H, p->B) &&
                   staged(a->d_k, p->n_k, p->H_kv, p->B) && staged(a->d_v, p->n_k, p->H_kv, p->B);
-  P.parts = dw_parts(p, tc ? kTcRows : kSmallestTile);
-  if (dw) P.dw_part = reinterpret_cast<float*>(static_cast<char*>(work) + dsum_bytes(p));
+  const KeyUnits u = tc ? key_units(p, kTcRows, kTcHalf) : key_units(p, kSimtTile, 0);
+  P.parts = p->B * u.count();
+  P.sink_tiles = u.sink_tiles;
+  P.far_segs = u.far_segs;
+  P.far_len = u.far_len;
+  char* at = static_cast<char*>(work) + dsum_bytes(p);
+  P.sink_part = reinterpret_cast<float*>(at);
+  if (dw) P.dw_part = reinterpret_cast<float*>(at + round256(sink_part_bytes(p, u)));
   if (p->n_q > 0 || p->n_k > 0) {
     const int r = rc(tc ? launch_attn_tc_bwd(P, p->dtype, st) : launch_attn_simt_bwd(P, p->dtype, st));
     if (r != DFS_OK) return r;

@@ -20,10 +20,12 @@ struct AttnParams {
   const void* w;        // (H, nb) bias weights of type wdtype, or null
   const int32_t* lut;   // (2 D + 1)
   float* dw_part;       // (H, parts, 2 D + 1) sums of dS by distance, or null
+  float* sink_part;     // fp32 parts of the sink keys' gradients, or null
+  int sink_tiles, far_segs, far_len;  // key tiles that hold sinks; segments of queries beyond the window, steps of each
   int32_t* status;
   const int32_t* lengths;  // decode: (B,)
   int nb, D, wdtype;
-  int parts;            // key tiles of all batch elements: rows of dw_part per head
+  int parts;            // rows of dw_part per head: key tiles (and far segments) of all batch elements
   int B, H, Hkv, G, nq, nk, d;
   int causal, window, sinks, qs;
   float scale, scale2;  // scale; scale * log2(e)

@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
       __syncwarp();
       setup_arrive<kFwdThreads>();
       const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
-      const TcKeyTiles tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
+      const TcKeyTiles<kTcRows> tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
       if (lane == 0) {
         mbar_arrive_expect_tx(smem_u32(&S.q_full), kTcTileBytes);
         tma_load_4d(sQ, &T.q, 0, i0, h, b, smem_u32(&S.q_full));
@@ -93,19 +93,12 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
         }
         const int ks = t % kKStages, vs = t % kVStages;
         if (!tc_wait(&S.k_empty[ks], ((t / kKStages) & 1) ^ 1)) { err = true; break; }
-        if (lane == 0) {
-          TileInfo& f = S.info[t % kInfo];
-          f.at = j0;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
-          describe_tile(P, f, p0, j0);
-          if (j0 < 0) {
-            mbar_arrive(&S.k_full[ks]);
-          } else {
-            mbar_arrive_expect_tx(smem_u32(&S.k_full[ks]), kTcTileBytes);
-            tma_load_4d(sK + ks * kTcTileBytes, &T.k, 0, j0, hk, b, smem_u32(&S.k_full[ks]));
-          }
+        if (lane == 0 && j0 >= 0) {
+          mbar_expect_tx(smem_u32(&S.k_full[ks]), kTcTileBytes);
+          tma_load_4d(sK + ks * kTcTileBytes, &T.k, 0, j0, hk, b, smem_u32(&S.k_full[ks]));
         }
+        describe_tile(P, S.info[t % kInfo], j0, h, p0, j0, kTcRows, kTcRows, bits, lane);
+        if (lane == 0) mbar_arrive(&S.k_full[ks]);
         if (j0 < 0) break;
         if (!tc_wait(&S.v_empty[vs], ((t / kVStages) & 1) ^ 1)) { err = true; break; }
         if (lane == 0) {
@@ -167,7 +160,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
         if (!tc_wait(&S.p_ready, t & 1)) { err = true; break; }
         tc_fence_after();
         if (elect_one()) {
-          tc_mma_ts(tm + kColO, tm + kColP, tc_desc(sV + vs * kTcTileBytes), id_o, t > 0);
+          tc_mma_ts<8>(tm + kColO, tm + kColP, tc_desc(sV + vs * kTcTileBytes), id_o, t > 0);
           mma_commit(&S.v_empty[vs]);
           mma_commit(&S.pv_done);
         }
@@ -188,14 +181,15 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
     }
     const int wq = warp % 4, ch = warp / 4;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
-    const int row = wq * 32 + lane, i = i0 + row, p = p0 + row, pw = p0 + wq * 32;
+    const int row = wq * 32 + lane, i = i0 + row, p = p0 + row;
     const int E = bias_ext(P.D), c0 = 32 * ch;  // c0: this thread's columns of O
     float m = -INFINITY;
     float2 l = make_float2(0.0f, 0.0f);
     const float far_hi = P.w ? tab[E + P.D] : 0.0f, far_lo = P.w ? tab[E - P.D] : 0.0f;
     // One tile, S on its way to sr.  Plain tiles (all but a row's first and last few) need no look at masks
     // or distances; the others are taken apart into blocks of 32 x 32.
-    auto step = [&](auto is_plain, int t, uint32_t (&sr)[2][32], int j0, const uint32_t (&bits)[2], float far) -> bool {
+    auto step = [&](auto is_plain, int t, uint32_t (&sr)[2][32], int j0, const uint32_t (&bits)[2],
+                    const int (&cls)[2], float far) -> bool {
       constexpr bool kPlain = decltype(is_plain)::value;
       bool live[2] = {true, true}, whole[2] = {true, true};
       uint32_t vis[2] = {~0u, ~0u};
@@ -204,12 +198,10 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
       if (!kPlain) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          whole[u] = bits[u] == ~0u && block_visible(P, pw, j0 + 32 * u);
-          if (!whole[u]) {
-            vis[u] = bits[u] & key_word(P, p, j0 + 32 * u);
-            live[u] = __any_sync(0xffffffffu, vis[u] != 0);
-          }
-          side[u] = P.w ? block_side(P, pw, j0 + 32 * u) : 2;
+          live[u] = (cls[u] & 3) != kHidden;
+          whole[u] = (cls[u] & 3) == kWhole;
+          if (live[u] && !whole[u]) vis[u] = bits[u] & key_word(P, p, j0 + 32 * u);
+          side[u] = (cls[u] >> 2) - 1;
           mul[u] = side[u] == 0 ? 1.0f : P.scale2;
           add[u] = side[u] == 1 ? far_hi : side[u] == -1 ? far_lo : 0.0f;
         }
@@ -291,14 +283,15 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
       const int tile_side = f.side;
       const int j0 = at + 64 * ch;
       const uint32_t bits[2] = {f.bits[2 * ch], f.bits[2 * ch + 1]};
+      const int cls[2] = {f.cls[4 * wq + 2 * ch], f.cls[4 * wq + 2 * ch + 1]};
       tc_fence_after();
       uint32_t sr[2][32];
       tmem_ld32_async(tm + lanes + kColS + 64 * ch, sr[0]);
       tmem_ld32_async(tm + lanes + kColS + 64 * ch + 32, sr[1]);
       if (plain)
-        err = !step(std::true_type(), t, sr, j0, bits, tile_side > 0 ? far_hi : tile_side < 0 ? far_lo : 0.0f);
+        err = !step(std::true_type(), t, sr, j0, bits, cls, tile_side > 0 ? far_hi : tile_side < 0 ? far_lo : 0.0f);
       else
-        err = !step(std::false_type(), t, sr, j0, bits, 0.0f);
+        err = !step(std::false_type(), t, sr, j0, bits, cls, 0.0f);
       if (err) break;
     }
     if (!err && t > 0) err = !tc_wait(&S.pv_done, (t - 1) & 1);
@@ -347,8 +340,8 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
 
 }  // namespace
 
-bool tc_tmap(CUtensorMap* tm, const Strided& s, bool bf16, int d, int n, int heads, int B) {
-  return make_tmap_4d(tm, s.p, bf16 ? DFS_BF16 : DFS_F16, d, n, heads, B, s.sn, s.sh, s.sb, 64, kTcRows);
+bool tc_tmap(CUtensorMap* tm, const Strided& s, bool bf16, int d, int n, int heads, int B, int rows) {
+  return make_tmap_4d(tm, s.p, bf16 ? DFS_BF16 : DFS_F16, d, n, heads, B, s.sn, s.sh, s.sb, 64, rows);
 }
 
 cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st) {

@@ -11,6 +11,7 @@ namespace dfs {
 
 constexpr int kTcRows = 128;              // tile edge, queries and keys
 constexpr int kTcTileBytes = 128 * 128;   // 128 rows of 64 16-bit elements, 128-byte swizzle
+constexpr int kTcHalf = 64;               // rows of the backward's streamed tiles
 
 struct TcParams {
   CUtensorMap q, k, v, d_o;
@@ -74,10 +75,13 @@ DFS_DEV void tc_mma_kk(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, 
   for (int k = 0; k < 4; ++k)
     if (k < ksteps) mma_f16(d_tmem, a + 2 * k, b + 2 * k, idesc, k > 0);
 }
-// 128 x dp product over the 128 rows of B: A in TMEM
+// 128 x dp product over the 16 kSteps rows of B: A in TMEM, its 8 columns a step side
+// by side, or (kSpread) two steps at the start of every 32 columns
+template <int kSteps, bool kSpread = false>
 DFS_DEV void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, bool accum) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) mma_f16_ts(d_tmem, a_tmem + 8 * k, b + 128 * k, idesc, accum || k > 0);
+  for (int k = 0; k < kSteps; ++k)
+    mma_f16_ts(d_tmem, a_tmem + (kSpread ? 32 * (k / 2) + 8 * (k % 2) : 8 * k), b + 128 * k, idesc, accum || k > 0);
 }
 
 DFS_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -271,10 +275,14 @@ inline size_t bias_ext_bytes(const AttnParams& P) { return P.w ? (2 * (P.D + 255
 
 // One tile as the producer announces it: first key (or query) row, -1 for the
 // end; whether it is plain (all pairs visible, one bias for all) and where its
-// distances lie (block_side); the key mask's bits.
+// distances lie (block_side); the key mask's bits; and for a tile that is not
+// plain, the class of each of its blocks of 32 x 32, so that the element warps
+// need no look at positions for most of them.
+enum { kHidden = 0, kWhole = 1, kPartial = 2 };
 struct TileInfo {
   int at, plain, side, head;
   uint32_t bits[4];
+  uint8_t cls[16];  // kind | (block_side + 1) << 2
 };
 
 // Mask bits of keys [j0, j0 + 128) (a full warp; all lanes get the four words)
@@ -290,24 +298,25 @@ DFS_DEV void key_bits(const uint8_t* mask, int j0, int nk, int lane, uint32_t (&
   for (int w = 0; w < 4; ++w) bits[w] = __reduce_or_sync(0xffffffffu, (lane >> 3) == w ? part : 0u);
 }
 
-// Key tiles of 128 seen by positions p0..p1: the sink tiles [0, ns), then the window's [t0, t1).
+// Key tiles of kRows seen by positions p0..p1: the sink tiles [0, ns), then the window's [t0, t1).
+template <int kRows>
 struct TcKeyTiles {
   int ns, t0, t1;
   DFS_DEV TcKeyTiles(const AttnParams& P, int p0, int p1) {
     int lo, hi;
     near_keys(P, p0, p1, lo, hi);
-    t0 = lo / kTcRows;
-    t1 = hi > lo ? (hi + kTcRows - 1) / kTcRows : t0;
-    ns = (sink_keys(P, p1) + kTcRows - 1) / kTcRows;
+    t0 = lo / kRows;
+    t1 = hi > lo ? (hi + kRows - 1) / kRows : t0;
+    ns = (sink_keys(P, p1) + kRows - 1) / kRows;
     if (hi > lo) ns = min(ns, t0);
   }
   DFS_DEV int count() const { return ns + (t1 - t0); }
   DFS_DEV int operator[](int x) const { return x < ns ? x : t0 + (x - ns); }
 };
 
-// Whether every pair of a square block (queries from position p0, keys from j0) is visible, the mask apart.
-DFS_DEV bool block_visible(const AttnParams& P, int p0, int j0, int edge = 32) {
-  const int p1 = p0 + edge - 1, j1 = j0 + edge - 1;
+// Whether every pair of np queries from position p0 and nj keys from j0 is visible, the mask apart.
+DFS_DEV bool block_visible(const AttnParams& P, int p0, int j0, int np = 32, int nj = 32) {
+  const int p1 = p0 + np - 1, j1 = j0 + nj - 1;
   if (j1 >= P.nk || (P.causal && p0 < j1)) return false;
   return (p1 - j0 < P.window && j1 - p0 < P.window) || j1 < P.sinks;
 }
@@ -322,18 +331,40 @@ DFS_DEV uint32_t query_word(const AttnParams& P, int j, int p0) {
   if (j < P.sinks) v |= range_word(P.causal ? j - p0 : 0, 32, 0);
   return v;
 }
-// Where the distances of a square block of pairs lie: 1 beyond the table's far end, -1 beyond the other, 0 in it.
-DFS_DEV int block_side(const AttnParams& P, int p0, int j0, int edge = 32) {
-  return p0 - j0 - (edge - 1) >= P.D ? 1 : p0 - j0 + (edge - 1) <= -P.D ? -1 : 0;
+// Where the distances of a block of pairs lie: 1 beyond the table's far end, -1 beyond the other, 0 in it.
+DFS_DEV int block_side(const AttnParams& P, int p0, int j0, int np = 32, int nj = 32) {
+  return p0 - j0 - (nj - 1) >= P.D ? 1 : p0 - j0 + (np - 1) <= -P.D ? -1 : 0;
 }
-// What the producer says of the tile of 128 queries at p0 and 128 keys at j0 (its mask bits are set already).
-DFS_DEV void describe_tile(const AttnParams& P, TileInfo& f, int p0, int j0) {
-  f.side = P.w ? block_side(P, p0, j0, kTcRows) : 0;
-  f.plain = (f.bits[0] & f.bits[1] & f.bits[2] & f.bits[3]) == ~0u && (P.w == nullptr || f.side != 0) &&
-            block_visible(P, p0, j0, kTcRows);
+// Class of the block of 32 queries at p0 and 32 keys at j0 whose mask bits are `bits`.
+DFS_DEV uint8_t block_class(const AttnParams& P, int p0, int j0, uint32_t bits) {
+  const int p1 = p0 + 31, j1 = j0 + 31;
+  const bool out = p0 - j1 >= P.window || j0 - p1 >= P.window;  // of the window, every pair
+  const bool hidden = bits == 0 || j0 >= P.nk || (P.causal && p1 < j0) || (out && j0 >= P.sinks);
+  const int kind = hidden ? kHidden : bits == ~0u && block_visible(P, p0, j0) ? kWhole : kPartial;
+  return static_cast<uint8_t>(kind | ((P.w ? block_side(P, p0, j0) : 1) + 1) << 2);
 }
-// A strided (B, heads, n, d) operand of 16-bit elements as {d, n, heads, B}, boxes of 64 x 128.
-bool tc_tmap(CUtensorMap* tm, const Strided& s, bool bf16, int d, int n, int heads, int B);
+// What the producer (a full warp) says of the tile of np queries at p0 and nj keys at j0 with the given mask bits.
+DFS_DEV void describe_tile(const AttnParams& P, TileInfo& f, int at, int head, int p0, int j0, int np, int nj,
+                           const uint32_t (&bits)[4], int lane) {
+  const int nc = nj / 32;  // blocks along the keys: cls[query block * nc + key block]
+  const uint32_t own = bits[0] * (lane % nc == 0) + bits[1] * (lane % nc == 1) + bits[2] * (lane % nc == 2) +
+                       bits[3] * (lane % nc == 3);
+  if (at >= 0 && lane < np / 32 * nc) f.cls[lane] = block_class(P, p0 + lane / nc * 32, j0 + lane % nc * 32, own);
+  if (lane == 0) {
+    f.at = at;
+    f.head = head;
+    f.side = P.w ? block_side(P, p0, j0, np, nj) : 1;
+    bool all = true;
+    for (int w = 0; w < nc; ++w) all = all && bits[w] == ~0u;
+    f.plain = all && f.side != 0 && block_visible(P, p0, j0, np, nj);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
+  }
+  __syncwarp();
+}
+
+// A strided (B, heads, n, d) operand of 16-bit elements as {d, n, heads, B}, boxes of 64 x rows.
+bool tc_tmap(CUtensorMap* tm, const Strided& s, bool bf16, int d, int n, int heads, int B, int rows = kTcRows);
 
 // One CTA per tile of each (head, batch element), heads fastest and tiles slowest:
 // the CTAs with the most tiles to walk start first, over all heads.  (Tiles

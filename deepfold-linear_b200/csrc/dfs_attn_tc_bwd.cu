@@ -12,12 +12,13 @@
 // instead of 7 and one exponential instead of two, but 32 KB of fp32 atomics (in
 // varying order) a tile pair.
 //
-// Both: warps 0-15 work element by element (a TMEM row and a quarter of a tile's
-// columns per thread: blocks of 32 x 32 per warp, skipped where all is hidden),
-// warp 16 issues the MMAs (the next tile's S and dP while this one's elements are
-// worked on), warp 17 stages tiles by TMA and announces them.  The exponentials
-// (1024 clocks a tile on the MUFU) go in part to the FMA pipes; four element warps
-// a scheduler cover the latencies of TMEM, barriers and dependent arithmetic.
+// Both stream tiles of 64 rows past their own 128 and run two CTAs an SM (256 TMEM
+// columns each), so that one's products, TMEM traffic, start and end overlap the
+// other's arithmetic; with 128-row tiles and one CTA an SM of twice the element
+// warps the same work took about twice as long.  Warps 0-7 work element by element
+// (a TMEM row and half of a tile's columns per thread: blocks of 32 x 32 per warp,
+// skipped where all is hidden), warp 8 issues the MMAs, warp 9 stages tiles by TMA
+// and announces them.  Part of the exponentials go to the FMA pipes.
 #include <type_traits>
 
 #include "dfs_attn_tc.cuh"
@@ -25,30 +26,33 @@
 namespace dfs {
 namespace {
 
-// 640 threads x 96 registers at launch = 512 x 112 (elements) + 128 x 32 (MMA, TMA and two idle warps)
-constexpr int kBwdThreads = 640;
-constexpr int kElementRegs = 112, kOtherRegs = 32;
-static_assert(512 * kElementRegs + 128 * kOtherRegs <= kBwdThreads * 96, "register shares");
-constexpr int kWork = 512;     // threads of the element warps
-constexpr int kMmaWarp = 16, kTmaWarp = 17;
+// 384 threads x 80 registers at launch = 256 x 104 (elements) + 128 x 32 (MMA, TMA and two idle warps)
+constexpr int kBwdThreads = 384;
+constexpr int kElementRegs = 104, kOtherRegs = 32;
+static_assert(256 * kElementRegs + 128 * kOtherRegs <= kBwdThreads * 80, "register shares");
+constexpr int kWork = 256;     // threads of the element warps
+constexpr int kMmaWarp = 8, kTmaWarp = 9;
 constexpr int kPolyEvery = 3;
 constexpr int kStages = 3, kInfo = 4;
+constexpr int kHalfBytes = kTcTileBytes / 2;  // a streamed tile
 
-// TMEM columns (512 allocated)
-constexpr uint32_t kColS = 0, kColDP = 128, kColP = 256, kColDS = 320, kColA = 384, kColB = 448;
+// TMEM columns (256 allocated): S and dP (64 each), then the dQ pass's dQ and dS, or dV and dK.  The dK/dV pass
+// writes P and dS over the S and dP that it has read, a warp within its own 32 columns.
+constexpr uint32_t kColS = 0, kColDP = 64, kColA = 128, kColB = 192;
+constexpr uint32_t kColDS = 192;              // dQ pass
 
 struct BwdShared {
   uint64_t own_full, full[kStages], empty[kStages];
   uint64_t s_full, s_free, ds_ready, acc_done;
   TileInfo info[kInfo];
-  alignas(16) float stat[kStages][2][kTcRows];  // dK/dV pass: -lse and -D of the stage's queries
-  float part[4][kTcRows];           // dQ pass: a row's four partial sums
+  alignas(16) float stat[kStages][2][kTcHalf];  // dK/dV pass: -lse and -D of the stage's queries
+  float part[2][kTcRows];           // dQ pass: a row's two partial sums
   float ends[2][kWork / 32];
   float diag[2][kWork / 32][64];    // dK/dV pass: the diagonals of a warp's block, two tiles in turn
   uint32_t tmem;
 };
 
-DFS_DEV void work_barrier() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+DFS_DEV void work_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 template <bool BF16>
 struct E16 {
@@ -59,13 +63,13 @@ struct E16<true> {
   using T = __nv_bfloat16;
 };
 
-// 16 of a row's gradient values, scaled, to global memory (columns c0.. of d)
+// 32 of a row's gradient values, scaled, to global memory (columns c0.. of d)
 template <bool BF16>
-DFS_DEV void store_row16(const Strided& s, int b, int h, int row, int c0, int d, const uint32_t (&v)[16], float mul,
+DFS_DEV void store_row32(const Strided& s, int b, int h, int row, int c0, int d, const uint32_t (&v)[32], float mul,
                          bool zero) {
   auto* dst = row_ptr<typename E16<BF16>::T>(s, b, h, row) + c0;
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
+  for (int e = 0; e < 4; ++e)
     if (c0 + 8 * e < d) {
       uint32_t r[4];
 #pragma unroll
@@ -77,13 +81,13 @@ DFS_DEV void store_row16(const Strided& s, int b, int h, int row, int c0, int d,
 }
 
 template <bool BF16>
-__global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_constant__ TcParams T) {
+__global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_constant__ TcParams T) {
   extern __shared__ unsigned char raw[];
   const AttnParams& P = T.a;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   unsigned char* gen = raw + (base - smem_u32(raw));
-  const uint32_t sQ = base, sO = sQ + kTcTileBytes, sK = sO + kTcTileBytes, sV = sK + kStages * kTcTileBytes;
-  BwdShared& S = *reinterpret_cast<BwdShared*>(gen + (2 + 2 * kStages) * kTcTileBytes);
+  const uint32_t sQ = base, sO = sQ + kTcTileBytes, sK = sO + kTcTileBytes, sV = sK + kStages * kHalfBytes;
+  BwdShared& S = *reinterpret_cast<BwdShared*>(gen + 2 * kTcTileBytes + 2 * kStages * kHalfBytes);
   float* tab = reinterpret_cast<float*>(&S + 1);
   const int warp = warp_index(), lane = threadIdx.x % 32;
   const int h = blockIdx.x % P.H, b = blockIdx.x / P.H % P.B, hk = h / P.G;
@@ -110,7 +114,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
       __syncwarp();
       setup_arrive<kBwdThreads>();
       const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
-      const TcKeyTiles tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
+      const TcKeyTiles<kTcHalf> tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
       if (lane == 0) {
         mbar_arrive_expect_tx(smem_u32(&S.own_full), 2 * kTcTileBytes);
         tma_load_4d(sQ, &T.q, 0, i0, h, b, smem_u32(&S.own_full));
@@ -118,38 +122,31 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
       }
       int t = 0;
       for (int x = 0; x <= tiles.count(); ++x) {
-        const int j0 = x < tiles.count() ? tiles[x] * kTcRows : -1;
+        const int j0 = x < tiles.count() ? tiles[x] * kTcHalf : -1;
         uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
         if (j0 >= 0 && mask != nullptr) {
           key_bits(mask, j0, P.nk, lane, bits);
-          if ((bits[0] | bits[1] | bits[2] | bits[3]) == 0) continue;
+          if ((bits[0] | bits[1]) == 0) continue;
         }
         const int s = t % kStages;
         if (!tc_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
-        if (lane == 0) {
-          TileInfo& f = S.info[t % kInfo];
-          f.at = j0;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
-          describe_tile(P, f, p0, j0);
-          if (j0 < 0) {
-            mbar_arrive(&S.full[s]);
-          } else {
-            mbar_arrive_expect_tx(smem_u32(&S.full[s]), 2 * kTcTileBytes);
-            tma_load_4d(sK + s * kTcTileBytes, &T.k, 0, j0, hk, b, smem_u32(&S.full[s]));
-            tma_load_4d(sV + s * kTcTileBytes, &T.v, 0, j0, hk, b, smem_u32(&S.full[s]));
-          }
+        if (lane == 0 && j0 >= 0) {
+          mbar_expect_tx(smem_u32(&S.full[s]), 2 * kHalfBytes);
+          tma_load_4d(sK + s * kHalfBytes, &T.k, 0, j0, hk, b, smem_u32(&S.full[s]));
+          tma_load_4d(sV + s * kHalfBytes, &T.v, 0, j0, hk, b, smem_u32(&S.full[s]));
         }
+        describe_tile(P, S.info[t % kInfo], j0, h, p0, j0, kTcRows, kTcHalf, bits, lane);
+        if (lane == 0) mbar_arrive(&S.full[s]);
         ++t;
       }
     } else if (warp == kMmaWarp) {  // ---- MMA
-      tmem_alloc(&S.tmem, 512);
+      tmem_alloc(&S.tmem, 256);
       tc_fence_before();
       setup_wait<kBwdThreads>();
       tc_fence_after();
       const uint32_t tm = S.tmem;
       const int dp = (P.d + 15) / 16 * 16;
-      const uint32_t id_s = tc_idesc(128, 128, BF16, false), id_a = tc_idesc(128, dp, BF16, true);
+      const uint32_t id_s = tc_idesc(128, 64, BF16, false), id_a = tc_idesc(128, dp, BF16, true);
       err = !tc_wait(&S.own_full, 0);
       auto start = [&](int t, bool& end) {
         const int s = t % kStages;
@@ -158,9 +155,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
         end = f.at < 0;
         if (!end && P.mask != nullptr) {
           // a hidden key's K may hold anything, and 0 x NaN is NaN in dS K: zero its row
-          unsigned char* kt = gen + (2 + s) * kTcTileBytes;
+          unsigned char* kt = gen + 2 * kTcTileBytes + s * kHalfBytes;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
+          for (int w = 0; w < 2; ++w) {
             const uint32_t bw = f.bits[w];
             if (bw != ~0u)
               for (int r = lane / 8; r < 32; r += 4)
@@ -176,8 +173,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
           if (end) {
             mbar_arrive(&S.s_full);
           } else {
-            tc_mma_kk(tm + kColS, tc_desc(sQ), tc_desc(sK + s * kTcTileBytes), id_s, dp / 16);
-            tc_mma_kk(tm + kColDP, tc_desc(sO), tc_desc(sV + s * kTcTileBytes), id_s, dp / 16);
+            tc_mma_kk(tm + kColS, tc_desc(sQ), tc_desc(sK + s * kHalfBytes), id_s, dp / 16);
+            tc_mma_kk(tm + kColDP, tc_desc(sO), tc_desc(sV + s * kHalfBytes), id_s, dp / 16);
             mma_commit(&S.s_full);
           }
         }
@@ -192,7 +189,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
         if (!tc_wait(&S.ds_ready, t & 1)) { err = true; break; }
         tc_fence_after();
         if (elect_one()) {
-          tc_mma_ts(tm + kColA, tm + kColDS, tc_desc(sK + (t % kStages) * kTcTileBytes), id_a, t > 0);
+          tc_mma_ts<4>(tm + kColA, tm + kColDS, tc_desc(sK + (t % kStages) * kHalfBytes), id_a, t > 0);
           mma_commit(&S.empty[t % kStages]);
           mma_commit(&S.acc_done);
         }
@@ -208,9 +205,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
     regs_up<kElementRegs>();
     const uint32_t tm = S.tmem;
     if (P.w) load_bias_ext(tab, P, h, threadIdx.x, kWork);  // read after the barrier below
-    const int wq = warp % 4, cg = warp / 4, row = wq * 32 + lane, i = i0 + row, p = p0 + row, pw = p0 + 32 * wq;
+    const int wq = warp % 4, cg = warp / 4, row = wq * 32 + lane, i = i0 + row, p = p0 + row;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
-    const int E = bias_ext(P.D), c0 = 16 * cg;  // c0: this thread's columns of d
+    const int E = bias_ext(P.D), c0 = 32 * cg;  // c0: this thread's columns of d
     using T16 = typename E16<BF16>::T;
     const size_t stat = (static_cast<size_t>(b) * P.H + h) * P.nq + i;
     float D = 0.0f;
@@ -220,7 +217,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
                                : nullptr;
       const T16* drow = row_ptr<T16>(P.d_o, b, h, i) + c0;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int e = 0; e < 4; ++e)
         if (c0 + 8 * e < P.d) {
           const uint4 x = *reinterpret_cast<const uint4*>(orow + 8 * e), y = *reinterpret_cast<const uint4*>(drow + 8 * e);
           const uint4 z = rest ? *reinterpret_cast<const uint4*>(rest + 8 * e) : make_uint4(0, 0, 0, 0);
@@ -234,25 +231,23 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
     }
     S.part[cg][row] = D;
     work_barrier();
-    D = (S.part[0][row] + S.part[1][row]) + (S.part[2][row] + S.part[3][row]);
+    D = S.part[0][row] + S.part[1][row];
     const float lse = i < P.nq ? P.lse[stat] : INFINITY;
     float2 rest = both(0.0f);
     const float far_hi = P.w ? tab[E + P.D] : 0.0f, far_lo = P.w ? tab[E - P.D] : 0.0f;
     // One tile, S and dP on their way to sr and dr (plain tiles: see TileInfo).
     auto step = [&](auto is_plain, int t, uint32_t (&sr)[32], uint32_t (&dr)[32], int j0, uint32_t bits,
-                    float far) -> bool {
+                    int cls, float far) -> bool {
       constexpr bool kPlain = decltype(is_plain)::value;
       bool whole = true, live = true;
       uint32_t vis = ~0u;
       int side = 1;
       float mul = P.scale2;
       if (!kPlain) {
-        whole = bits == ~0u && block_visible(P, pw, j0);
-        if (!whole) {
-          vis = bits & key_word(P, p, j0);
-          live = __any_sync(0xffffffffu, vis != 0);
-        }
-        side = P.w ? block_side(P, pw, j0) : 2;
+        live = (cls & 3) != kHidden;
+        whole = (cls & 3) == kWhole;
+        if (live && !whole) vis = bits & key_word(P, p, j0);
+        side = (cls >> 2) - 1;
         far = side == 1 ? far_hi : side == -1 ? far_lo : 0.0f;
         if (side == 0) mul = 1.0f;
       }
@@ -304,64 +299,78 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dq_kernel(const __grid_cons
       if (at < 0) break;
       const int plain = f.plain, tile_side = f.side;
       const uint32_t bits = f.bits[cg];
+      const int cls = f.cls[2 * wq + cg];
       tc_fence_after();
       uint32_t sr[32], dr[32];
       tmem_ld32_async(tm + lanes + kColS + 32 * cg, sr);
       tmem_ld32_async(tm + lanes + kColDP + 32 * cg, dr);
       if (plain)
-        err = !step(std::true_type(), t, sr, dr, j0, bits, tile_side > 0 ? far_hi : tile_side < 0 ? far_lo : 0.0f);
+        err = !step(std::true_type(), t, sr, dr, j0, bits, cls, tile_side > 0 ? far_hi : tile_side < 0 ? far_lo : 0.0f);
       else
-        err = !step(std::false_type(), t, sr, dr, j0, bits, 0.0f);
+        err = !step(std::false_type(), t, sr, dr, j0, bits, cls, 0.0f);
       if (err) break;
     }
     if (!err && t > 0) err = !tc_wait(&S.acc_done, (t - 1) & 1);
     tc_fence_after();
     if (c0 < P.d) {
-      uint32_t v[16];
+      uint32_t v[32];
       if (t > 0) {
-        tmem_ld16_async(tm + lanes + kColA + c0, v);
-        tmem_wait_ld16(v);
+        tmem_ld32_async(tm + lanes + kColA + c0, v);
+        tmem_wait_ld(v);
       }
-      if (i < P.nq) store_row16<BF16>(P.d_q, b, h, i, c0, P.d, v, P.scale, t == 0);
+      if (i < P.nq) store_row32<BF16>(P.d_q, b, h, i, c0, P.d, v, P.scale, t == 0);
     }
     work_barrier();
     S.part[cg][row] = rest.x + rest.y;
     work_barrier();
     if (cg == 0 && i < P.nq)
-      P.dsum[stat] = D + ((S.part[0][row] + S.part[1][row]) + (S.part[2][row] + S.part[3][row]));
+      P.dsum[stat] = D + (S.part[0][row] + S.part[1][row]);
   }
   if (err) report_timeout(P.status);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp) tmem_dealloc(S.tmem, 512);
+  if (warp == kMmaWarp) tmem_dealloc(S.tmem, 256);
 }
 
 template <bool BF16>
-__global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_constant__ TcParams T) {
+__global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_constant__ TcParams T) {
   extern __shared__ unsigned char raw[];
   const AttnParams& P = T.a;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   unsigned char* gen = raw + (base - smem_u32(raw));
-  const uint32_t sK = base, sV = sK + kTcTileBytes, sQ = sV + kTcTileBytes, sO = sQ + kStages * kTcTileBytes;
-  BwdShared& S = *reinterpret_cast<BwdShared*>(gen + (2 + 2 * kStages) * kTcTileBytes);
+  const uint32_t sK = base, sV = sK + kTcTileBytes, sQ = sV + kTcTileBytes, sO = sQ + kStages * kHalfBytes;
+  BwdShared& S = *reinterpret_cast<BwdShared*>(gen + 2 * kTcTileBytes + 2 * kStages * kHalfBytes);
   float* tab = reinterpret_cast<float*>(&S + 1);
   const int W = 2 * P.D + 1;
   float* acc = tab + (P.w ? 2 * bias_ext(P.D) + 1 : 0);  // W sums by distance
   const int warp = warp_index(), lane = threadIdx.x % 32;
-  const int hk = blockIdx.x % P.Hkv, b = blockIdx.x / P.Hkv % P.B, tile = blockIdx.x / P.Hkv / P.B;
-  const int j0 = tile * kTcRows;  // the sinks' tiles, which all queries see, first
+  const int hk = blockIdx.x % P.Hkv, b = blockIdx.x / P.Hkv % P.B, unit = blockIdx.x / P.Hkv / P.B;
+  // Units: first the far segments of the sinks' tiles (the queries beyond their window, which see the sinks
+  // only; without them those tiles' CTAs would walk every query tile), then the key tiles.
+  const int far_units = P.sink_tiles * P.far_segs;
+  const bool far_unit = unit < far_units;
+  const int tile = far_unit ? unit / P.far_segs : unit - far_units, j0 = tile * kTcRows;
+  const int sink_rows = P.far_segs > 0 ? min(max(P.sinks - j0, 0), kTcRows) : 0;  // rows that are joined afterwards
   bool err = false;
 
-  // queries that see some key of the tile: [i_lo, i_hi)
+  // queries that see some key of the tile, in tiles of queries: [i_lo, i_hi); this unit's steps [first, last)
+  // of (head, query tile)
   int i_lo = P.causal ? j0 - P.qs : j0 - P.window + 1 - P.qs;
   int i_hi = min(j0 + kTcRows, P.nk) - 1 + P.window - P.qs;
   if (j0 < P.sinks) {
-    i_hi = P.nq;
+    if (P.far_segs == 0) i_hi = P.nq;
     if (!P.causal) i_lo = 0;
   }
-  i_lo = max(i_lo, 0) / kTcRows;
-  i_hi = (min(i_hi, P.nq) + kTcRows - 1) / kTcRows;  // in tiles
+  i_lo = max(i_lo, 0) / kTcHalf;
+  i_hi = (max(min(i_hi, P.nq), 0) + kTcHalf - 1) / kTcHalf;
+  if (far_unit) {
+    i_lo = max(i_lo, i_hi);
+    i_hi = (P.nq + kTcHalf - 1) / kTcHalf;
+  }
+  const int per = max(0, i_hi - i_lo);
+  const int first = far_unit ? min(unit % P.far_segs * P.far_len, per * P.G) : 0;
+  const int last = far_unit ? min(first + P.far_len, per * P.G) : per * P.G;
 
   if (warp >= kMmaWarp) {
     regs_down<kOtherRegs>();  // one instruction for the whole warpgroup
@@ -383,70 +392,60 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
       setup_arrive<kBwdThreads>();
       uint32_t bits[4];
       key_bits(P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr, j0, P.nk, lane, bits);
-      const int per = (bits[0] | bits[1] | bits[2] | bits[3]) == 0 ? 0 : max(0, i_hi - i_lo);
+      const int total = (bits[0] | bits[1] | bits[2] | bits[3]) == 0 ? 0 : last - first;
       if (lane == 0) {
         mbar_arrive_expect_tx(smem_u32(&S.own_full), 2 * kTcTileBytes);
         tma_load_4d(sK, &T.k, 0, j0, hk, b, smem_u32(&S.own_full));
         tma_load_4d(sV, &T.v, 0, j0, hk, b, smem_u32(&S.own_full));
       }
-      const int total = per * P.G;
       for (int t = 0; t <= total; ++t) {
         const int s = t % kStages;
-        const int g = t < total ? t / per : 0, h = hk * P.G + g, i0 = t < total ? (i_lo + t % per) * kTcRows : -1;
-        float st[2][4];
+        const int g = t < total ? (first + t) / per : 0, h = hk * P.G + g;
+        const int i0 = t < total ? (i_lo + (first + t) % per) * kTcHalf : -1;
+        float st[2][2];
         if (i0 >= 0) {
           const size_t at = (static_cast<size_t>(b) * P.H + h) * P.nq;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = i0 + 4 * lane + e;
+          for (int e = 0; e < 2; ++e) {
+            const int i = i0 + 2 * lane + e;
             st[0][e] = i < P.nq ? -P.lse[at + i] : -INFINITY;
             st[1][e] = i < P.nq ? -P.dsum[at + i] : 0.0f;
           }
         }
         if (!tc_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
         if (i0 >= 0) {
+          if (lane == 0) {
+            mbar_expect_tx(smem_u32(&S.full[s]), 2 * kHalfBytes);
+            tma_load_4d(sQ + s * kHalfBytes, &T.q, 0, i0, h, b, smem_u32(&S.full[s]));
+            tma_load_4d(sO + s * kHalfBytes, &T.d_o, 0, i0, h, b, smem_u32(&S.full[s]));
+          }
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            *reinterpret_cast<float4*>(&S.stat[s][k][4 * lane]) = make_float4(st[k][0], st[k][1], st[k][2], st[k][3]);
+            *reinterpret_cast<float2*>(&S.stat[s][k][2 * lane]) = make_float2(st[k][0], st[k][1]);
         }
-        __syncwarp();
-        if (lane == 0) {
-          TileInfo& f = S.info[t % kInfo];
-          f.at = i0;
-          f.head = g;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
-          describe_tile(P, f, i0 + P.qs, j0);
-          if (i0 < 0) {
-            mbar_arrive(&S.full[s]);
-          } else {
-            mbar_arrive_expect_tx(smem_u32(&S.full[s]), 2 * kTcTileBytes);
-            tma_load_4d(sQ + s * kTcTileBytes, &T.q, 0, i0, h, b, smem_u32(&S.full[s]));
-            tma_load_4d(sO + s * kTcTileBytes, &T.d_o, 0, i0, h, b, smem_u32(&S.full[s]));
-          }
-        }
+        describe_tile(P, S.info[t % kInfo], i0, g, i0 + P.qs, j0, kTcHalf, kTcRows, bits, lane);
+        if (lane == 0) mbar_arrive(&S.full[s]);
       }
     } else if (warp == kMmaWarp) {  // ---- MMA
-      tmem_alloc(&S.tmem, 512);
+      tmem_alloc(&S.tmem, 256);
       tc_fence_before();
       setup_wait<kBwdThreads>();
       tc_fence_after();
       const uint32_t tm = S.tmem;
       const int dp = (P.d + 15) / 16 * 16;
-      const uint32_t id_s = tc_idesc(128, 128, BF16, false), id_a = tc_idesc(128, dp, BF16, true);
+      const uint32_t id_s = tc_idesc(128, 64, BF16, false), id_a = tc_idesc(128, dp, BF16, true);
       err = !tc_wait(&S.own_full, 0);
       auto start = [&](int t, bool& end) {
         const int s = t % kStages;
         if (!tc_wait(&S.full[s], (t / kStages) & 1)) return false;
         end = S.info[t % kInfo].at < 0;
-        if (t > 0 && !tc_wait(&S.s_free, (t - 1) & 1)) return false;
         tc_fence_after();
         if (elect_one()) {
           if (end) {
             mbar_arrive(&S.s_full);
           } else {
-            tc_mma_kk(tm + kColS, tc_desc(sK), tc_desc(sQ + s * kTcTileBytes), id_s, dp / 16);
-            tc_mma_kk(tm + kColDP, tc_desc(sV), tc_desc(sO + s * kTcTileBytes), id_s, dp / 16);
+            tc_mma_kk(tm + kColS, tc_desc(sK), tc_desc(sQ + s * kHalfBytes), id_s, dp / 16);
+            tc_mma_kk(tm + kColDP, tc_desc(sV), tc_desc(sO + s * kHalfBytes), id_s, dp / 16);
             mma_commit(&S.s_full);
           }
         }
@@ -456,108 +455,36 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
       bool end = false;
       if (!err) err = !start(0, end);
       for (int t = 0; !end && !err; ++t) {
-        bool next_end = false;
-        if (!start(t + 1, next_end)) { err = true; break; }
         if (!tc_wait(&S.ds_ready, t & 1)) { err = true; break; }
         tc_fence_after();
         if (elect_one()) {
           const int s = t % kStages;
-          tc_mma_ts(tm + kColA, tm + kColP, tc_desc(sO + s * kTcTileBytes), id_a, t > 0);
-          tc_mma_ts(tm + kColB, tm + kColDS, tc_desc(sQ + s * kTcTileBytes), id_a, t > 0);
+          tc_mma_ts<4, true>(tm + kColA, tm + kColS, tc_desc(sO + s * kHalfBytes), id_a, t > 0);
+          tc_mma_ts<4, true>(tm + kColB, tm + kColDP, tc_desc(sQ + s * kHalfBytes), id_a, t > 0);
           mma_commit(&S.empty[s]);
           mma_commit(&S.acc_done);
         }
         __syncwarp();
-        end = next_end;
+        // the next S and dP overwrite the P and dS that these products read
+        if (!tc_wait(&S.acc_done, t & 1) || !start(t + 1, end)) { err = true; break; }
       }
     } else if (warp != kMmaWarp) {  // ---- the warpgroup's idle warps
       setup_wait<kBwdThreads>();
     }
-  } else {  // ---- elements: a key row and a quarter of the tile's queries per thread
+  } else {  // ---- elements: a key row and half of the tile's queries per thread
     setup_wait<kBwdThreads>();
     tc_fence_after();
     regs_up<kElementRegs>();
     const uint32_t tm = S.tmem;
-    const int wq = warp % 4, cg = warp / 4, row = wq * 32 + lane, j = j0 + row, jw = j0 + 32 * wq, tid = threadIdx.x;
+    const int wq = warp % 4, cg = warp / 4, row = wq * 32 + lane, j = j0 + row, tid = threadIdx.x;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
     const int E = bias_ext(P.D);
     const bool dw = P.dw_part != nullptr;
     float lo = 0.0f, hi = 0.0f;  // sums of dS beyond the table's ends
     int head = -1, strip = 0;
     float far_hi = 0.0f, far_lo = 0.0f;
-    // One tile, S^T and dP^T on their way to sr and dr; leaves dS in dr.
-    auto step = [&](auto is_plain, int t, uint32_t (&sr)[32], uint32_t (&dr)[32], int pw, uint32_t kbits, float far,
-                    bool& live) -> bool {
-      constexpr bool kPlain = decltype(is_plain)::value;
-      const float* lse = S.stat[t % kStages][0] + 32 * cg;
-      const float* Dv = S.stat[t % kStages][1] + 32 * cg;
-      bool whole = true;
-      uint32_t vis = ~0u;
-      int side = 1;
-      float mul = P.scale2;
-      if (!kPlain) {
-        whole = kbits == ~0u && block_visible(P, pw, jw);
-        if (!whole) {
-          vis = (kbits >> lane) & 1u ? query_word(P, j, pw) : 0u;
-          live = __any_sync(0xffffffffu, vis != 0);
-        }
-        side = P.w ? block_side(P, pw, jw) : 2;
-        far = side == 1 ? far_hi : side == -1 ? far_lo : 0.0f;
-        if (side == 0) mul = 1.0f;
-      }
-      tmem_wait_ld(sr);
-      tmem_wait_ld(dr);
-      tc_fence_before();
-      mbar_arrive(&S.s_free);
-      uint32_t pk[16];
-      if (kPlain || live) {
-        if (!kPlain && side == 0) {
-          const float* tb = tab + (E + pw - j);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) sr[c] = __float_as_uint(fmaf(__uint_as_float(sr[c]), P.scale2, tb[c]));
-        }
-        if (!kPlain && !whole) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const bool on = (vis >> c) & 1u;
-            sr[c] = on ? sr[c] : 0xff800000u;
-            dr[c] = on ? dr[c] : 0u;
-          }
-        }
-        const float2 mul_2 = both(mul), far_2 = both(far);
-#pragma unroll
-        for (int c = 0; c < 16; c += 2) {  // four queries
-          const float4 ls = *reinterpret_cast<const float4*>(lse + 2 * c);
-          const float4 dd = *reinterpret_cast<const float4*>(Dv + 2 * c);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float2 l2 = u ? make_float2(ls.z, ls.w) : make_float2(ls.x, ls.y);
-            const float2 d2 = u ? make_float2(dd.z, dd.w) : make_float2(dd.x, dd.y);
-            const int e = 2 * (c + u);
-            const float2 s = make_float2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
-            const float2 dp = make_float2(__uint_as_float(dr[e]), __uint_as_float(dr[e + 1]));
-            const float2 x = exp2_pair<kPolyEvery>(fma2(s, mul_2, add2(l2, far_2)), c + u);
-            const float2 ds = mul2(x, add2(dp, d2));
-            pk[c + u] = pack16<BF16>(x.x, x.y);
-            dr[e] = __float_as_uint(ds.x);
-            dr[e + 1] = __float_as_uint(ds.y);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < 16; ++c) pk[c] = 0;
-#pragma unroll
-        for (int c = 0; c < 32; ++c) dr[c] = 0;
-      }
-      if (t > 0 && !tc_wait(&S.acc_done, (t - 1) & 1)) return false;
-      tmem_st16(tm + lanes + kColP + 16 * cg, pk);
-#pragma unroll
-      for (int c = 0; c < 16; ++c) pk[c] = pack16<BF16>(__uint_as_float(dr[2 * c]), __uint_as_float(dr[2 * c + 1]));
-      tmem_st16(tm + lanes + kColDS + 16 * cg, pk);
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&S.ds_ready);
-      return true;
+    auto dw_row = [&](int g) {
+      return P.dw_part + (static_cast<size_t>(hk * P.G + g) * P.parts + b * (P.parts / P.B) + unit) * W;
     };
     // this head's sums by distance, to memory (the element threads together)
     auto flush = [&]() {
@@ -571,24 +498,90 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
         acc[tid == 0 ? 0 : 2 * P.D] += s;
       }
       work_barrier();
-      float* dst = P.dw_part + (static_cast<size_t>(hk * P.G + head) * P.parts + b * (P.parts / P.B) + tile) * W;
+      float* dst = dw_row(head);
       for (int x = tid; x < W; x += kWork) dst[x] = acc[x];
       lo = hi = 0.0f;
     };
-    // the heads from `from` on have no tile here: their sums are zero
-    auto zero_heads = [&](int from) {
-      for (int g = from; g < P.G; ++g) {
-        float* dst = P.dw_part + (static_cast<size_t>(hk * P.G + g) * P.parts + b * (P.parts / P.B) + tile) * W;
+    // heads that have no tile here: their sums are zero
+    auto zero_heads = [&](int from, int to) {
+      for (int g = from; g < to; ++g) {
+        float* dst = dw_row(g);
         for (int x = tid; x < W; x += kWork) dst[x] = 0.0f;
+      }
+    };
+    // One block, S^T and dP^T on their way to sr and dr: P and dS to TMEM, over S and dP, and the block's sum of dS
+    // to `sum`; a block that is not plain also leaves dS in dr.
+    auto step = [&](auto is_plain, int t, uint32_t (&sr)[32], uint32_t (&dr)[32], int pw, uint32_t kbits, int cls,
+                    float far, float2& sum) {
+      constexpr bool kPlain = decltype(is_plain)::value;
+      const float* lse = S.stat[t % kStages][0] + 32 * cg;
+      const float* Dv = S.stat[t % kStages][1] + 32 * cg;
+      float mul = P.scale2;
+      uint32_t vis = ~0u;
+      if (!kPlain) {
+        const int side = (cls >> 2) - 1;
+        if ((cls & 3) == kPartial) vis = (kbits >> lane) & 1u ? query_word(P, j, pw) : 0u;
+        far = side == 1 ? far_hi : side == -1 ? far_lo : 0.0f;
+        if (side == 0) mul = 1.0f;
+      }
+      tmem_wait_ld(sr);
+      tmem_wait_ld(dr);
+      if (!kPlain) {
+        if ((cls >> 2) == 1) {
+          const float* tb = tab + (E + pw - j);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) sr[c] = __float_as_uint(fmaf(__uint_as_float(sr[c]), P.scale2, tb[c]));
+        }
+        if ((cls & 3) == kPartial) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const bool on = (vis >> c) & 1u;
+            sr[c] = on ? sr[c] : 0xff800000u;
+            dr[c] = on ? dr[c] : 0u;
+          }
+        }
+      }
+      const float2 mul_2 = both(mul), far_2 = both(far);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {  // 16 queries at a time: registers
+        uint32_t pp[8], ps[8];
+#pragma unroll
+        for (int c = 0; c < 8; c += 2) {
+          const float4 ls = *reinterpret_cast<const float4*>(lse + 16 * hf + 2 * c);
+          const float4 dd = *reinterpret_cast<const float4*>(Dv + 16 * hf + 2 * c);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float2 l2 = u ? make_float2(ls.z, ls.w) : make_float2(ls.x, ls.y);
+            const float2 d2 = u ? make_float2(dd.z, dd.w) : make_float2(dd.x, dd.y);
+            const int e = 16 * hf + 2 * (c + u);
+            const float2 s = make_float2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
+            const float2 dp = make_float2(__uint_as_float(dr[e]), __uint_as_float(dr[e + 1]));
+            const float2 x = exp2_pair<kPolyEvery>(fma2(s, mul_2, add2(l2, far_2)), 8 * hf + c + u);
+            const float2 ds = mul2(x, add2(dp, d2));
+            sum = add2(sum, ds);
+            pp[c + u] = pack16<BF16>(x.x, x.y);
+            ps[c + u] = pack16<BF16>(ds.x, ds.y);
+            if (!kPlain) {
+              dr[e] = __float_as_uint(ds.x);
+              dr[e + 1] = __float_as_uint(ds.y);
+            }
+          }
+        }
+        tmem_st8(tm + lanes + kColS + 32 * cg + 8 * hf, pp);
+        tmem_st8(tm + lanes + kColDP + 32 * cg + 8 * hf, ps);
       }
     };
     int t = 0;
     for (;; ++t) {
       if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
-      const int i0 = S.info[t % kInfo].at, g = S.info[t % kInfo].head;
+      const TileInfo& f = S.info[t % kInfo];
+      const int i0 = f.at, g = f.head;
       if (i0 < 0) break;
       if (g != head) {
-        if (dw && head >= 0) flush();
+        if (dw) {
+          if (head >= 0) flush();
+          zero_heads(head + 1, g);
+        }
         work_barrier();  // nobody reads the old tables any more
         head = g;
         if (P.w) load_bias_ext(tab, P, hk * P.G + g, tid, kWork);
@@ -597,120 +590,158 @@ __global__ void __launch_bounds__(kBwdThreads, 1) tc_dkv_kernel(const __grid_con
         work_barrier();
         if (P.w) far_hi = tab[E + P.D], far_lo = tab[E - P.D];
       }
-      const TileInfo& f = S.info[t % kInfo];
+      const int plain = f.plain, tile_side = f.side, cls = f.cls[4 * cg + wq];
       const uint32_t kbits = f.bits[wq];
-      const int plain = f.plain, tile_side = f.side;
-      const int p0 = i0 + P.qs;
-      tc_fence_after();
+      const int p0 = i0 + P.qs, pw = p0 + 32 * cg;
+      const bool live = plain || (cls & 3) != kHidden;
+      float2 sum = both(0.0f);
       uint32_t sr[32], dr[32];
-      tmem_ld32_async(tm + lanes + kColS + 32 * cg, sr);
-      tmem_ld32_async(tm + lanes + kColDP + 32 * cg, dr);
-      bool live = true;
-      if (plain)
-        err = !step(std::true_type(), t, sr, dr, p0 + 32 * cg, kbits,
-                    tile_side > 0 ? far_hi : tile_side < 0 ? far_lo : 0.0f, live);
-      else
-        err = !step(std::false_type(), t, sr, dr, p0 + 32 * cg, kbits, 0.0f, live);
-      if (err) break;
-      if (dw) {
-        if (tile_side != 0) {
-          float2 s2 = both(0.0f);
-#pragma unroll
-          for (int c = 0; c < 16; ++c)
-            s2 = add2(s2, make_float2(__uint_as_float(dr[2 * c]), __uint_as_float(dr[2 * c + 1])));
-          if (tile_side > 0) hi += s2.x + s2.y;
-          else lo += s2.x + s2.y;
-        } else {
-          // Diagonals of this warp's block of 32 keys x 32 queries: the running sum of a diagonal moves one lane
-          // up as the query advances, and is complete once lane 31 has added its element.
-          float* out = S.diag[strip][warp];
-          float run = 0.0f;
-          if (live) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              run += __uint_as_float(dr[c]);
-              if (c < 31) {
-                if (lane == 31) out[c] = run;
-                run = __shfl_up_sync(0xffffffffu, run, 1);
-                if (lane == 0) run = 0.0f;
-              }
-            }
-          } else {
-            out[lane] = 0.0f;  // slots 0..30 (slot 31 is lane 31's below)
-            __syncwarp();
-          }
-          out[62 - lane] = run;  // slot x + 31 for diagonal x = query - key of the block
-          work_barrier();
-          if (tid < 2 * kTcRows - 1) {
-            const int e = tid - (kTcRows - 1);  // query - key within the tile
-            float s = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWork / 32; ++w) {
-              const int x = e - 32 * (w / 4) + 32 * (w % 4) + 31;
-              if (x >= 0 && x < 63) s += S.diag[strip][w][x];
-            }
-            const int delta = p0 - j0 + e;
-            if (delta <= -P.D) lo += s;
-            else if (delta >= P.D) hi += s;
-            else acc[delta + P.D] += s;
-          }
-          strip ^= 1;
-        }
+      if (live) {
+        tc_fence_after();
+        tmem_ld32_async(tm + lanes + kColS + 32 * cg, sr);
+        tmem_ld32_async(tm + lanes + kColDP + 32 * cg, dr);
+        if (plain)
+          step(std::true_type(), t, sr, dr, pw, kbits, cls, tile_side > 0 ? far_hi : far_lo, sum);
+        else
+          step(std::false_type(), t, sr, dr, pw, kbits, cls, 0.0f, sum);
+      } else {
+        const uint32_t none[16] = {};
+        tc_fence_after();
+        tmem_st16(tm + lanes + kColS + 32 * cg, none);
+        tmem_st16(tm + lanes + kColDP + 32 * cg, none);
       }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&S.ds_ready);
+      if (!dw) continue;
+      if (tile_side != 0) {
+        if (tile_side > 0) hi += sum.x + sum.y;
+        else lo += sum.x + sum.y;
+        continue;
+      }
+      // Diagonals of this warp's block of 32 keys x 32 queries: the running sum of a diagonal moves one lane up
+      // as the query advances, and is complete once lane 31 has added its element.
+      float* out = S.diag[strip][warp];
+      float run = 0.0f;
+      if (live) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          run += __uint_as_float(dr[c]);
+          if (c < 31) {
+            if (lane == 31) out[c] = run;
+            run = __shfl_up_sync(0xffffffffu, run, 1);
+            if (lane == 0) run = 0.0f;
+          }
+        }
+      } else {
+        out[lane] = 0.0f;  // slots 0..30 (slot 31 is lane 31's below)
+        __syncwarp();
+      }
+      out[62 - lane] = run;  // slot x + 31 for diagonal x = query - key of the block
+      work_barrier();
+      if (tid < kTcRows + kTcHalf - 1) {
+        const int e = tid - (kTcRows - 1);  // query - key within the tile
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWork / 32; ++w) {
+          const int x = e - 32 * (w / 4) + 32 * (w % 4) + 31;
+          if (x >= 0 && x < 63) s += S.diag[strip][w][x];
+        }
+        const int delta = p0 - j0 + e;
+        if (delta <= -P.D) lo += s;
+        else if (delta >= P.D) hi += s;
+        else acc[delta + P.D] += s;
+      }
+      strip ^= 1;
     }
     if (dw) {
       if (head >= 0) flush();
-      zero_heads(head + 1);
+      zero_heads(head + 1, P.G);
     }
     if (!err && t > 0) err = !tc_wait(&S.acc_done, (t - 1) & 1);
     tc_fence_after();
-    const int c0 = 16 * cg;
+    const int c0 = 32 * cg;
     if (c0 < P.d) {
-      uint32_t v[16];
-      if (t > 0) {
-        tmem_ld16_async(tm + lanes + kColA + c0, v);
-        tmem_wait_ld16(v);
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {  // dV, dK
+        uint32_t v[32];
+        if (t > 0) {
+          tmem_ld32_async(tm + lanes + (which ? kColB : kColA) + c0, v);
+          tmem_wait_ld(v);
+        }
+        if (j >= P.nk) continue;
+        if (row < sink_rows) {
+          // joined in 32 bits: [key head][sink tile][key tile, segments][sink row][dV, dK][64]
+          const size_t seg = far_unit ? unit % P.far_segs + 1 : 0;
+          float* dst = P.sink_part +
+                       (((static_cast<size_t>(b) * P.Hkv + hk) * P.sink_tiles + tile) * (P.far_segs + 1) + seg) *
+                           (min(P.sinks, kTcRows) * 128) + row * 128 + 64 * which + c0;
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (c0 + e < P.d) dst[e] = t > 0 ? __uint_as_float(v[e]) : 0.0f;
+        } else if (!far_unit) {
+          store_row32<BF16>(which ? P.d_k : P.d_v, b, hk, j, c0, P.d, v, which ? P.scale : 1.0f, t == 0);
+        }
       }
-      if (j < P.nk) store_row16<BF16>(P.d_v, b, hk, j, c0, P.d, v, 1.0f, t == 0);
-      if (t > 0) {
-        tmem_ld16_async(tm + lanes + kColB + c0, v);
-        tmem_wait_ld16(v);
-      }
-      if (j < P.nk) store_row16<BF16>(P.d_k, b, hk, j, c0, P.d, v, P.scale, t == 0);
     }
   }
   if (err) report_timeout(P.status);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp) tmem_dealloc(S.tmem, 512);
+  if (warp == kMmaWarp) tmem_dealloc(S.tmem, 256);
+}
+
+// Joins a sink row's parts (the key tile's own and the far segments', in order).
+// grid (sink tiles, key heads, batch), a thread per value of a row at a time.
+template <bool BF16>
+__global__ void __launch_bounds__(256) sink_join_kernel(AttnParams P) {
+  const int tile = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, j0 = tile * kTcRows;
+  const int rows = min(min(P.sinks, P.nk) - j0, kTcRows), pitch = min(P.sinks, kTcRows) * 128;
+  const float* src = P.sink_part +
+                     ((static_cast<size_t>(b) * P.Hkv + hk) * P.sink_tiles + tile) * (P.far_segs + 1) * pitch;
+  for (int x = threadIdx.x; x < rows * 128; x += 256) {
+    const int row = x / 128, which = x % 128 / 64, c = x % 64;
+    if (c >= P.d) continue;
+    float s = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k <= P.far_segs; ++k) s += src[static_cast<size_t>(k) * pitch + x];
+    using T16 = typename E16<BF16>::T;
+    row_ptr<T16>(which ? P.d_k : P.d_v, b, hk, j0 + row)[c] = from_f32<T16>(which ? s * P.scale : s);
+  }
 }
 
 }  // namespace
 
 template <bool BF16>
-static cudaError_t launch_bwd(const TcParams& T, size_t smem, cudaStream_t st) {
-  const AttnParams& P = T.a;
-  const int share = 512 * kElementRegs + 128 * kOtherRegs;
+static cudaError_t launch_bwd(const AttnParams& P, cudaStream_t st) {
+  TcParams T;
+  T.a = P;
+  auto maps = [&](int q_rows, int k_rows) {
+    return tc_tmap(&T.q, P.q, BF16, P.d, P.nq, P.H, P.B, q_rows) &&
+           tc_tmap(&T.d_o, P.d_o, BF16, P.d, P.nq, P.H, P.B, q_rows) &&
+           tc_tmap(&T.k, P.k, BF16, P.d, P.nk, P.Hkv, P.B, k_rows) &&
+           tc_tmap(&T.v, P.v, BF16, P.d, P.nk, P.Hkv, P.B, k_rows);
+  };
+  const size_t smem = 1024 + 2 * kTcTileBytes + 2 * kStages * kHalfBytes + sizeof(BwdShared) + bias_ext_bytes(P) +
+                      (P.w ? (2 * P.D + 1) * sizeof(float) : 0);
+  const int share = 256 * kElementRegs + 128 * kOtherRegs;
   cudaError_t e = prepare_kernel<tc_dq_kernel<BF16>>(smem, kBwdThreads, share);
   if (e == cudaSuccess) e = prepare_kernel<tc_dkv_kernel<BF16>>(smem, kBwdThreads, share);
   if (e != cudaSuccess) return e;
+  if (!maps(kTcRows, kTcHalf)) return cudaErrorInvalidValue;
   tc_dq_kernel<BF16><<<tc_grid(P.nq, P.H, P.B), kBwdThreads, smem, st>>>(T);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  tc_dkv_kernel<BF16><<<tc_grid(P.nk, P.Hkv, P.B), kBwdThreads, smem, st>>>(T);
+  if (!maps(kTcHalf, kTcRows)) return cudaErrorInvalidValue;
+  const unsigned units = (P.nk + kTcRows - 1) / kTcRows + P.sink_tiles * P.far_segs;
+  tc_dkv_kernel<BF16><<<units * P.Hkv * P.B, kBwdThreads, smem, st>>>(T);
+  if ((e = cudaGetLastError()) != cudaSuccess || P.far_segs == 0) return e;
+  sink_join_kernel<BF16><<<dim3(P.sink_tiles, P.Hkv, P.B), 256, 0, st>>>(P);
   return cudaGetLastError();
 }
 
 cudaError_t launch_attn_tc_bwd(const AttnParams& P, int dtype, cudaStream_t st) {
-  const bool bf16 = dtype == DFS_BF16;
-  TcParams T;
-  T.a = P;
-  if (!tc_tmap(&T.q, P.q, bf16, P.d, P.nq, P.H, P.B) || !tc_tmap(&T.k, P.k, bf16, P.d, P.nk, P.Hkv, P.B) ||
-      !tc_tmap(&T.v, P.v, bf16, P.d, P.nk, P.Hkv, P.B) || !tc_tmap(&T.d_o, P.d_o, bf16, P.d, P.nq, P.H, P.B))
-    return cudaErrorInvalidValue;
-  const size_t smem = 1024 + (2 + 2 * kStages) * kTcTileBytes + sizeof(BwdShared) + bias_ext_bytes(P) +
-                      (P.w ? (2 * P.D + 1) * sizeof(float) : 0);
-  return bf16 ? launch_bwd<true>(T, smem, st) : launch_bwd<false>(T, smem, st);
+  return dtype == DFS_BF16 ? launch_bwd<true>(P, st) : launch_bwd<false>(P, st);
 }
 
 }  // namespace dfs

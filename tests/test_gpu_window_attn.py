@@ -113,6 +113,19 @@ def test_forward_and_gradients(shape, causal, window, sinks, kind, dtype):
     check(x, dtype, buckets, causal=causal, window=window, sinks=sinks, grad=not one_key)
 
 
+@pytest.mark.parametrize("causal,window,sinks,n_q,n_k,q_start,H,H_kv", [
+    (True, 16, 4, 1537, 1537, None, 2, 1),     # many queries beyond the window see the sinks only
+    (False, 30, 3, 1400, 1400, None, 1, 1),
+    (True, 9, 200, 1700, 1700, None, 1, 1),    # sinks over two key tiles
+    (True, 10, 3, 1600, 64, 0, 2, 2),          # few keys, queries far beyond them
+    (False, 12, 2, 1300, 1500, 900, 1, 1)])
+def test_gradients_of_sinks_that_many_queries_see(causal, window, sinks, n_q, n_k, q_start, H, H_kv):
+    x = inputs(1, H, H_kv, n_q, n_k, 32, BF16, 16, nb=32)
+    mask = torch.ones(1, n_k, device="cuda", dtype=torch.bool)
+    mask[0, 1] = False
+    check(x, BF16, BUCKETS["log2"], mask, causal=causal, window=window, sinks=sinks, q_start=q_start)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_masks_with_holes_empty_rows_and_nan_in_the_padding(dtype):
     n = 200
