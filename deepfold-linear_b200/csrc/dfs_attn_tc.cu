@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) tc_fwd_kernel(const __grid_con
           for (int c = 0; c < 16; ++c) {
             const float2 s = make_float2(__uint_as_float(sr[u][2 * c]), __uint_as_float(sr[u][2 * c + 1]));
             const float2 x = exp2_pair<kPolyEvery>(fma2(s, mu, off), c);
-            l = add2(l, x);
+            l = add2_ftz(l, x);
             pk[c] = pack16<BF16>(x.x, x.y);
           }
         } else {

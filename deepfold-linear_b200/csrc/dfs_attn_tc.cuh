@@ -150,17 +150,11 @@ DFS_DEV float2 unpack16(uint32_t x) {
   return __half22float2(h);
 }
 
-// Packed fp32 pairs, denormals flushed (an exponential that underflowed is 0).
-DFS_DEV float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, z, w;\n\t"
-      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
-      "fma.rn.ftz.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-DFS_DEV float2 add2(float2 a, float2 b) {
+// Packed fp32 pairs.  Products and the sums of exponentials flush denormals, so that
+// an exponential that underflowed counts as 0.
+DFS_DEV float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+DFS_DEV float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+DFS_DEV float2 add2_ftz(float2 a, float2 b) {
   float2 d;
   asm("{\n\t.reg .b64 x, y, w;\n\t"
       "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
@@ -206,13 +200,12 @@ DFS_DEV float2 exp2_pair(float2 x, int c) {
   return kEvery > 0 && c % kEvery == kEvery - 1 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
 }
 
-// Wait for the phase with the given parity; false once four billion clocks (some two
-// seconds) have passed.  The clock is read on every 1024th try only, never on the
-// way through a short wait.  (A sleep hint on the try made waits wake late.)
+// Wait for the phase with the given parity; false after some seconds (each try
+// sleeps for a while by itself).  No clock is read and the loop is short: warps
+// wait most of the time, and their tries take issue slots from the others.
 DFS_DEV bool tc_wait(uint64_t* bar, uint32_t parity) {
   const uint32_t addr = smem_u32(bar);
-  long long t0 = 0;
-  for (uint32_t it = 1;; ++it) {
+  for (int tries = 1 << 27; tries > 0; --tries) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -222,12 +215,8 @@ DFS_DEV bool tc_wait(uint64_t* bar, uint32_t parity) {
         : "r"(addr), "r"(parity)
         : "memory");
     if (done) return true;
-    if ((it & 1023u) == 0) {
-      const long long now = clock64();
-      if (t0 == 0) t0 = now;
-      else if (now - t0 > 4000000000ll) return false;
-    }
   }
+  return false;
 }
 
 // Registers of this warpgroup (four warps) from here on.  The shares of a block

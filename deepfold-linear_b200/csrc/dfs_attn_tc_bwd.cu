@@ -435,27 +435,27 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
       const int dp = (P.d + 15) / 16 * 16;
       const uint32_t id_s = tc_idesc(128, 64, BF16, false), id_a = tc_idesc(128, dp, BF16, true);
       err = !tc_wait(&S.own_full, 0);
-      auto start = [&](int t, bool& end) {
-        const int s = t % kStages;
-        if (!tc_wait(&S.full[s], (t / kStages) & 1)) return false;
+      auto wait_tile = [&](int t, bool& end) {
+        if (!tc_wait(&S.full[t % kStages], (t / kStages) & 1)) return false;
         end = S.info[t % kInfo].at < 0;
-        tc_fence_after();
-        if (elect_one()) {
-          if (end) {
-            mbar_arrive(&S.s_full);
-          } else {
-            tc_mma_kk(tm + kColS, tc_desc(sK), tc_desc(sQ + s * kHalfBytes), id_s, dp / 16);
-            tc_mma_kk(tm + kColDP, tc_desc(sV), tc_desc(sO + s * kHalfBytes), id_s, dp / 16);
-            mma_commit(&S.s_full);
-          }
-        }
-        __syncwarp();
         return true;
       };
+      auto start = [&](int t, bool end) {  // one lane: tile t's S and dP, or the end
+        const int s = t % kStages;
+        if (end) {
+          mbar_arrive(&S.s_full);
+        } else {
+          tc_mma_kk(tm + kColS, tc_desc(sK), tc_desc(sQ + s * kHalfBytes), id_s, dp / 16);
+          tc_mma_kk(tm + kColDP, tc_desc(sV), tc_desc(sO + s * kHalfBytes), id_s, dp / 16);
+          mma_commit(&S.s_full);
+        }
+      };
       bool end = false;
-      if (!err) err = !start(0, end);
+      if (!err) err = !wait_tile(0, end);
+      if (!err && elect_one()) start(0, end);
+      __syncwarp();
       for (int t = 0; !end && !err; ++t) {
-        if (!tc_wait(&S.ds_ready, t & 1)) { err = true; break; }
+        if (!wait_tile(t + 1, end) || !tc_wait(&S.ds_ready, t & 1)) { err = true; break; }
         tc_fence_after();
         if (elect_one()) {
           const int s = t % kStages;
@@ -463,10 +463,11 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
           tc_mma_ts<4, true>(tm + kColB, tm + kColDP, tc_desc(sQ + s * kHalfBytes), id_a, t > 0);
           mma_commit(&S.empty[s]);
           mma_commit(&S.acc_done);
+          // The next S and dP overwrite the P and dS that these products read: MMAs of one thread execute in
+          // the order of their issue, and the commit below covers all of them.
+          start(t + 1, end);
         }
         __syncwarp();
-        // the next S and dP overwrite the P and dS that these products read
-        if (!tc_wait(&S.acc_done, t & 1) || !start(t + 1, end)) { err = true; break; }
       }
     } else if (warp != kMmaWarp) {  // ---- the warpgroup's idle warps
       setup_wait<kBwdThreads>();
