@@ -219,6 +219,12 @@ DFS_DEV bool tc_wait(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
+// A warp's arrival, after everything its lanes did before.
+DFS_DEV void warp_arrive(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+
 // Registers of this warpgroup (four warps) from here on.  The shares of a block
 // must not add up to more than it was launched with.
 template <int N>
@@ -264,14 +270,14 @@ inline size_t bias_ext_bytes(const AttnParams& P) { return P.w ? (2 * (P.D + 255
 
 // One tile as the producer announces it: first key (or query) row, -1 for the
 // end; whether it is plain (all pairs visible, one bias for all) and where its
-// distances lie (block_side); the key mask's bits; and for a tile that is not
+// distances lie (1 beyond the bias table's far end, -1 beyond the other, 0 in it); the key mask's bits; and for a tile that is not
 // plain, the class of each of its blocks of 32 x 32, so that the element warps
 // need no look at positions for most of them.
 enum { kHidden = 0, kWhole = 1, kPartial = 2 };
 struct TileInfo {
   int at, plain, side, head;
   uint32_t bits[4];
-  uint8_t cls[16];  // kind | (block_side + 1) << 2
+  uint8_t cls[16];  // kind | (side + 1) << 2
 };
 
 // Mask bits of keys [j0, j0 + 128) (a full warp; all lanes get the four words)
@@ -303,12 +309,6 @@ struct TcKeyTiles {
   DFS_DEV int operator[](int x) const { return x < ns ? x : t0 + (x - ns); }
 };
 
-// Whether every pair of np queries from position p0 and nj keys from j0 is visible, the mask apart.
-DFS_DEV bool block_visible(const AttnParams& P, int p0, int j0, int np = 32, int nj = 32) {
-  const int p1 = p0 + np - 1, j1 = j0 + nj - 1;
-  if (j1 >= P.nk || (P.causal && p0 < j1)) return false;
-  return (p1 - j0 < P.window && j1 - p0 < P.window) || j1 < P.sinks;
-}
 // Visible keys j0..j0+31 for position p, the mask apart.
 DFS_DEV uint32_t key_word(const AttnParams& P, int p, int j0) {
   const int top = min(P.causal ? p + 1 : P.nk, P.nk);
@@ -320,34 +320,55 @@ DFS_DEV uint32_t query_word(const AttnParams& P, int j, int p0) {
   if (j < P.sinks) v |= range_word(P.causal ? j - p0 : 0, 32, 0);
   return v;
 }
-// Where the distances of a block of pairs lie: 1 beyond the table's far end, -1 beyond the other, 0 in it.
-DFS_DEV int block_side(const AttnParams& P, int p0, int j0, int np = 32, int nj = 32) {
-  return p0 - j0 - (nj - 1) >= P.D ? 1 : p0 - j0 + (np - 1) <= -P.D ? -1 : 0;
+// Class of the block of 32 queries from position p0 and 32 keys from j0, whose mask bits are `bits`; o = p0 - j0.
+DFS_DEV int block_class(const AttnParams& P, int o, int j0, uint32_t bits) {
+  const int far = o < 0 ? -o : o;
+  const bool hidden = bits == 0 || j0 >= P.nk || (P.causal && o < -31) || (far >= P.window + 31 && j0 >= P.sinks);
+  const bool whole = bits == ~0u && j0 + 31 < P.nk && (!P.causal || o >= 31) &&
+                     (far < P.window - 31 || j0 + 31 < P.sinks);
+  const int side = P.w == nullptr || o - 31 >= P.D ? 1 : o + 31 <= -P.D ? -1 : 0;
+  return (hidden ? kHidden : whole ? kWhole : kPartial) | (side + 1) << 2;
 }
-// Class of the block of 32 queries at p0 and 32 keys at j0 whose mask bits are `bits`.
-DFS_DEV uint8_t block_class(const AttnParams& P, int p0, int j0, uint32_t bits) {
-  const int p1 = p0 + 31, j1 = j0 + 31;
-  const bool out = p0 - j1 >= P.window || j0 - p1 >= P.window;  // of the window, every pair
-  const bool hidden = bits == 0 || j0 >= P.nk || (P.causal && p1 < j0) || (out && j0 >= P.sinks);
-  const int kind = hidden ? kHidden : bits == ~0u && block_visible(P, p0, j0) ? kWhole : kPartial;
-  return static_cast<uint8_t>(kind | ((P.w ? block_side(P, p0, j0) : 1) + 1) << 2);
-}
-// What the producer (a full warp) says of the tile of np queries at p0 and nj keys at j0 with the given mask bits.
-DFS_DEV void describe_tile(const AttnParams& P, TileInfo& f, int at, int head, int p0, int j0, int np, int nj,
-                           const uint32_t (&bits)[4], int lane) {
-  const int nc = nj / 32;  // blocks along the keys: cls[query block * nc + key block]
-  const uint32_t own = bits[0] * (lane % nc == 0) + bits[1] * (lane % nc == 1) + bits[2] * (lane % nc == 2) +
-                       bits[3] * (lane % nc == 3);
-  if (at >= 0 && lane < np / 32 * nc) f.cls[lane] = block_class(P, p0 + lane / nc * 32, j0 + lane % nc * 32, own);
+// The tiles of 32 NP queries x 32 NJ keys that are plain, the key mask apart, by o = (first query's position) -
+// (first key): all distances beyond the bias table, all inside the window.  Two comparisons a tile keep the
+// producer's chain of instructions shorter than a tile's work; it runs alone, without the instruction cache to
+// itself, and classing every tile's blocks (600 clocks) held everybody up.
+template <int NP, int NJ>
+struct PlainTiles {
+  int a1, b1, a2, b2;
+  DFS_DEV explicit PlainTiles(const AttnParams& P) {
+    const int w = P.window - 1, low = P.w ? P.D : P.causal ? 0 : -w;
+    a1 = low + 32 * NJ - 1;        // beyond the far end (or anywhere, without a bias)
+    b1 = w - (32 * NP - 1);
+    a2 = -w + 32 * NJ - 1;         // beyond the other end
+    b2 = P.w && !P.causal ? -P.D - (32 * NP - 1) : a2 - 1;
+  }
+  DFS_DEV int side(int o) const { return o >= a1 && o <= b1 ? 1 : o >= a2 && o <= b2 ? -1 : 0; }  // 0: not plain
+};
+
+// What the producer (a full warp) says of the tile of 32 NP queries from position p0 and 32 NJ keys from j0 with
+// the given mask bits (all ones if `whole`); -1 for `at`: the end.  A lane per block, joined by votes.
+template <int NP, int NJ>
+DFS_DEV void describe_tile(const AttnParams& P, const PlainTiles<NP, NJ>& plain, TileInfo& f, int at, int head, int p0,
+                           int j0, bool whole_mask, const uint32_t (&bits)[4], int lane) {
+  static_assert(NP * NJ <= 16, "blocks of a tile");
+  int side = plain.side(p0 - j0);
+  const bool easy = at < 0 || (side != 0 && whole_mask && j0 + 32 * NJ <= P.nk);
+  if (!easy) {
+    const int jb = lane % NJ, pb = lane / NJ % NP;
+    uint32_t own = bits[0];
+#pragma unroll
+    for (int w = 1; w < NJ; ++w) own = jb == w ? bits[w] : own;
+    const int jl = j0 + 32 * jb, cls = block_class(P, p0 + 32 * pb - jl, jl, own);
+    if (lane < NP * NJ) f.cls[lane] = static_cast<uint8_t>(cls);  // (the other lanes repeat blocks)
+    if (lane < NJ) f.bits[lane] = own;
+    side = __all_sync(0xffffffffu, (cls >> 2) == 2) ? 1 : __all_sync(0xffffffffu, (cls >> 2) == 0) ? -1 : 0;
+  }
   if (lane == 0) {
     f.at = at;
     f.head = head;
-    f.side = P.w ? block_side(P, p0, j0, np, nj) : 1;
-    bool all = true;
-    for (int w = 0; w < nc; ++w) all = all && bits[w] == ~0u;
-    f.plain = all && f.side != 0 && block_visible(P, p0, j0, np, nj);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) f.bits[w] = bits[w];
+    f.side = side;
+    f.plain = easy;
   }
   __syncwarp();
 }

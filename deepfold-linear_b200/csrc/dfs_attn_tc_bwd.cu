@@ -106,8 +106,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
         mbar_init(&S.own_full, 1);
         for (int s = 0; s < kStages; ++s) mbar_init(&S.full[s], 1), mbar_init(&S.empty[s], 1);
         mbar_init(&S.s_full, 1);
-        mbar_init(&S.s_free, kWork);
-        mbar_init(&S.ds_ready, kWork);
+        mbar_init(&S.s_free, kWork / 32);
+        mbar_init(&S.ds_ready, kWork / 32);
         mbar_init(&S.acc_done, 1);
         fence_mbar_init();
       }
@@ -120,10 +120,12 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
         tma_load_4d(sQ, &T.q, 0, i0, h, b, smem_u32(&S.own_full));
         tma_load_4d(sO, &T.d_o, 0, i0, h, b, smem_u32(&S.own_full));
       }
+      const PlainTiles<4, 2> plain(P);
+      const int count = tiles.count();
+      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
       int t = 0;
-      for (int x = 0; x <= tiles.count(); ++x) {
-        const int j0 = x < tiles.count() ? tiles[x] * kTcHalf : -1;
-        uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+      for (int x = 0; x <= count; ++x) {
+        const int j0 = x < count ? tiles[x] * kTcHalf : -1;
         if (j0 >= 0 && mask != nullptr) {
           key_bits(mask, j0, P.nk, lane, bits);
           if ((bits[0] | bits[1]) == 0) continue;
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
           tma_load_4d(sK + s * kHalfBytes, &T.k, 0, j0, hk, b, smem_u32(&S.full[s]));
           tma_load_4d(sV + s * kHalfBytes, &T.v, 0, j0, hk, b, smem_u32(&S.full[s]));
         }
-        describe_tile(P, S.info[t % kInfo], j0, h, p0, j0, kTcRows, kTcHalf, bits, lane);
+        describe_tile(P, plain, S.info[t % kInfo], j0, h, p0, j0, (bits[0] & bits[1]) == ~0u, bits, lane);
         if (lane == 0) mbar_arrive(&S.full[s]);
         ++t;
       }
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
         if (!tc_wait(&S.full[s], (t / kStages) & 1)) return false;
         const TileInfo& f = S.info[t % kInfo];
         end = f.at < 0;
-        if (!end && P.mask != nullptr) {
+        if (!end && P.mask != nullptr && !f.plain) {
           // a hidden key's K may hold anything, and 0 x NaN is NaN in dS K: zero its row
           unsigned char* kt = gen + 2 * kTcTileBytes + s * kHalfBytes;
 #pragma unroll
@@ -254,7 +256,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
       tmem_wait_ld(sr);
       tmem_wait_ld(dr);
       tc_fence_before();
-      mbar_arrive(&S.s_free);
+      warp_arrive(&S.s_free, lane);
       uint32_t pk[16];
       if (kPlain || live) {
         if (!kPlain && side == 0) {
@@ -288,7 +290,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
       tmem_st16(tm + lanes + kColDS + 16 * cg, pk);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&S.ds_ready);
+      warp_arrive(&S.ds_ready, lane);
       return true;
     };
     int t = 0;
@@ -383,8 +385,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
         mbar_init(&S.own_full, 1);
         for (int s = 0; s < kStages; ++s) mbar_init(&S.full[s], 1), mbar_init(&S.empty[s], 1);
         mbar_init(&S.s_full, 1);
-        mbar_init(&S.s_free, kWork);
-        mbar_init(&S.ds_ready, kWork);
+        mbar_init(&S.s_free, kWork / 32);
+        mbar_init(&S.ds_ready, kWork / 32);
         mbar_init(&S.acc_done, 1);
         fence_mbar_init();
       }
@@ -398,32 +400,37 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
         tma_load_4d(sK, &T.k, 0, j0, hk, b, smem_u32(&S.own_full));
         tma_load_4d(sV, &T.v, 0, j0, hk, b, smem_u32(&S.own_full));
       }
-      for (int t = 0; t <= total; ++t) {
-        const int s = t % kStages;
-        const int g = t < total ? (first + t) / per : 0, h = hk * P.G + g;
-        const int i0 = t < total ? (i_lo + (first + t) % per) * kTcHalf : -1;
-        float st[2][2];
-        if (i0 >= 0) {
-          const size_t at = (static_cast<size_t>(b) * P.H + h) * P.nq;
+      const PlainTiles<2, 4> plain(P);
+      const bool whole = (bits[0] & bits[1] & bits[2] & bits[3]) == ~0u;
+      int g = total > 0 ? first / per : 0, it = total > 0 ? first - g * per : 0;  // head and query tile of the step
+      float st[2][2];
+      auto load_stats = [&](int g, int it) {  // -lse and -D of two queries a lane, a step ahead
+        const size_t at = (static_cast<size_t>(b) * P.H + hk * P.G + g) * P.nq;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int i = i0 + 2 * lane + e;
-            st[0][e] = i < P.nq ? -P.lse[at + i] : -INFINITY;
-            st[1][e] = i < P.nq ? -P.dsum[at + i] : 0.0f;
-          }
+        for (int e = 0; e < 2; ++e) {
+          const int i = (i_lo + it) * kTcHalf + 2 * lane + e;
+          st[0][e] = i < P.nq ? -P.lse[at + i] : -INFINITY;
+          st[1][e] = i < P.nq ? -P.dsum[at + i] : 0.0f;
         }
+      };
+      if (total > 0) load_stats(g, it);
+      for (int t = 0; t <= total; ++t) {
+        const int s = t % kStages, i0 = t < total ? (i_lo + it) * kTcHalf : -1, now = g;
         if (!tc_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
         if (i0 >= 0) {
           if (lane == 0) {
-            mbar_expect_tx(smem_u32(&S.full[s]), 2 * kHalfBytes);
-            tma_load_4d(sQ + s * kHalfBytes, &T.q, 0, i0, h, b, smem_u32(&S.full[s]));
-            tma_load_4d(sO + s * kHalfBytes, &T.d_o, 0, i0, h, b, smem_u32(&S.full[s]));
+            const uint32_t bar = smem_u32(&S.full[s]);
+            mbar_expect_tx(bar, 2 * kHalfBytes);
+            tma_load_4d(sQ + s * kHalfBytes, &T.q, 0, i0, hk * P.G + g, b, bar);
+            tma_load_4d(sO + s * kHalfBytes, &T.d_o, 0, i0, hk * P.G + g, b, bar);
           }
 #pragma unroll
           for (int k = 0; k < 2; ++k)
             *reinterpret_cast<float2*>(&S.stat[s][k][2 * lane]) = make_float2(st[k][0], st[k][1]);
+          if (++it == per) it = 0, ++g;
+          if (t + 1 < total) load_stats(g, it);
         }
-        describe_tile(P, S.info[t % kInfo], i0, g, i0 + P.qs, j0, kTcHalf, kTcRows, bits, lane);
+        describe_tile(P, plain, S.info[t % kInfo], i0, now, i0 + P.qs, j0, whole, bits, lane);
         if (lane == 0) mbar_arrive(&S.full[s]);
       }
     } else if (warp == kMmaWarp) {  // ---- MMA
@@ -613,7 +620,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
       }
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&S.ds_ready);
+      warp_arrive(&S.ds_ready, lane);
       if (!dw) continue;
       if (tile_side != 0) {
         if (tile_side > 0) hi += sum.x + sum.y;
