@@ -31,6 +31,12 @@ struct AttnParams {
   float scale, scale2;  // scale; scale * log2(e)
 };
 
+// Programmatic dependent launches: a kernel's blocks may be set up while the one before it ends.  Nothing of
+// global memory is read or written before wait_previous(); allow_next() comes after a block's TMEM allocation, so
+// that the next kernel's blocks, which wait for this one to end, cannot hold the columns that it still needs.
+DFS_DEV void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+DFS_DEV void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Visible apart from the mask.  A window of "all" is INT_MAX/2 by the host.
 DFS_DEV bool key_near(int delta, int j, int causal, int window, int sinks) {
   if (causal ? delta < 0 : false) return false;

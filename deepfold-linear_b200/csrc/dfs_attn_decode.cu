@@ -73,6 +73,14 @@ __global__ void __launch_bounds__(kThreads) decode_mma_kernel(const __grid_const
   const int tid = threadIdx.x, warp = warp_index(), lane = tid % 32, rank = blockIdx.x, split = T.split;
   const int hk = blockIdx.y / T.chunks, g0 = blockIdx.y % T.chunks * kHeads, b = blockIdx.z;
   const int ng = min(kHeads, P.G - g0), h0 = hk * P.G + g0;
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(&S.full[s], 1), mbar_init(&S.empty[s], 4);
+    fence_mbar_init();
+    prefetch_tmap(&T.k);
+    prefetch_tmap(&T.v);
+  }
+  allow_next();
+  wait_previous();
   const int len = min(max(P.lengths[b], 0), P.nk), p = len - 1;
   const int lo = max(0, len - P.window), ns = min(P.sinks, lo);  // keys [0, ns) and [lo, len) are visible
   const int w0 = lo / kTcRows, sink_tiles = min((ns + kTcRows - 1) / kTcRows, w0);
@@ -81,10 +89,6 @@ __global__ void __launch_bounds__(kThreads) decode_mma_kernel(const __grid_const
   auto tile_key = [&](int t) { return (t < sink_tiles ? t : w0 + (t - sink_tiles)) * kTcRows; };
   const int ksteps = (P.d + 15) / 16;
   bool err = false;
-  if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&S.full[s], 1), mbar_init(&S.empty[s], 4);
-    fence_mbar_init();
-  }
   __syncthreads();
   const int t_near = t1 - 1;  // the run's newest tile
   const bool near_run = P.w && t1 > t0 && p - min(tile_key(t_near) + kTcRows - 1, p) < P.D;
@@ -318,13 +322,15 @@ cudaError_t launch(const AttnParams& P, cudaStream_t st) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = T.split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = T.split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = T.split > 1 ? 1 : 0;
+  cfg.numAttrs = T.split > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, decode_mma_kernel<E>, T);
 }
 

@@ -30,7 +30,6 @@ constexpr int kHalfBytes = kTcTileBytes / 2;  // a tile of 64 keys
 constexpr float kLag = 8.0f;
 // below any sum with a visible key in it (which holds a term of at least 2^-8)
 constexpr float kNone = 1e-30f;
-constexpr int kPolyEvery = 4;
 
 struct FwdShared {
   uint64_t q_full, full[kStages], empty[kStages];
@@ -72,6 +71,7 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
       }
       __syncwarp();
       setup_arrive<kFwdThreads>();
+      wait_previous();
       const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
       const TcKeyTiles<kTcHalf> tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
       if (lane == 0) {
@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
       }
     } else if (warp == kMmaWarp) {  // ---- MMA
       tmem_alloc(&S.tmem, 128);
+      allow_next();
       tc_fence_before();
       setup_wait<kFwdThreads>();
       tc_fence_after();
@@ -161,6 +162,7 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
     tc_fence_after();
     regs_up<kElementRegs>();
     const uint32_t tm = S.tmem;
+    wait_previous();
     if (P.w) {
       load_bias_ext(tab, P, h, threadIdx.x, 128);
       asm volatile("bar.sync 5, 128;" ::: "memory");
@@ -234,8 +236,9 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             float2 x = make_float2(__uint_as_float(sr[u][2 * c]), __uint_as_float(sr[u][2 * c + 1]));
-            x = exp2_pair<kPolyEvery>(fma2(x, mu, off), c);
-            l = add2_ftz(l, x);
+            x = fma2(x, mu, off);
+            x = make_float2(ex2(x.x), ex2(x.y));
+            l = add2(l, x);
             pk[c] = pack16<BF16>(x.x, x.y);
           }
         } else {
@@ -328,11 +331,7 @@ cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st) 
       !tc_tmap(&T.v, P.v, bf16, P.d, P.nk, P.Hkv, P.B, kTcHalf))
     return cudaErrorInvalidValue;
   T.d_o = T.q;
-  if (bf16)
-    tc_fwd_kernel<true><<<grid, kFwdThreads, smem, st>>>(T);
-  else
-    tc_fwd_kernel<false><<<grid, kFwdThreads, smem, st>>>(T);
-  return cudaGetLastError();
+  return launch_dependent(bf16 ? tc_fwd_kernel<true> : tc_fwd_kernel<false>, grid, kFwdThreads, smem, st, T);
 }
 
 }  // namespace dfs

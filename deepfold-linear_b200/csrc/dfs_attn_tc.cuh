@@ -150,55 +150,11 @@ DFS_DEV float2 unpack16(uint32_t x) {
   return __half22float2(h);
 }
 
-// Packed fp32 pairs.  Products and the sums of exponentials flush denormals, so that
-// an exponential that underflowed counts as 0.
+// Packed fp32 pairs.
 DFS_DEV float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 DFS_DEV float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
-DFS_DEV float2 add2_ftz(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, w;\n\t"
-      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-      "add.rn.ftz.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-DFS_DEV float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, w;\n\t"
-      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-      "mul.rn.ftz.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
+DFS_DEV float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
 DFS_DEV float2 both(float x) { return make_float2(x, x); }
-
-// 2^x of a pair on the FMA pipes (the MUFU gives 16 a clock per SM, and these
-// kernels wait for it): x = j + f, j = round(x) by adding 1.5 * 2^23 (j lands in
-// the low mantissa bits), 2^f on [-1/2, 1/2] by a degree-4 polynomial (relative
-// minimax fit by reweighted least squares: 2.7e-6 off at most, far below the
-// 16-bit rounding of what it feeds), 2^j by adding j to the exponent.  At and
-// below -126 the result is a denormal (2^f there is just under 1), which the packed operations above take as
-// 0; NaN stays non-finite.
-DFS_DEV float2 exp2_poly(float2 x) {
-  float2 c;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c.x) : "f"(x.x), "f"(-126.0f));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c.y) : "f"(x.y), "f"(-126.0f));
-  const float2 t = add2(c, both(12582912.0f));
-  const float2 f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), c);
-  float2 p = fma2(both(0.00957009662f), f, both(0.0559178591f));
-  p = fma2(p, f, both(0.240247443f));
-  p = fma2(p, f, both(0.693121791f));
-  p = fma2(p, f, both(0.999999285f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
-// Pair number c of a row's chunk of 16 pairs: about one in three on the FMA pipes.
-template <int kEvery>
-DFS_DEV float2 exp2_pair(float2 x, int c) {
-  return kEvery > 0 && c % kEvery == kEvery - 1 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
-}
 
 // Wait for the phase with the given parity; false after some seconds (each try
 // sleeps for a while by itself).  No clock is read and the loop is short: warps

@@ -18,7 +18,7 @@
 // warps the same work took about twice as long.  Warps 0-7 work element by element
 // (a TMEM row and half of a tile's columns per thread: blocks of 32 x 32 per warp,
 // skipped where all is hidden), warp 8 issues the MMAs, warp 9 stages tiles by TMA
-// and announces them.  Part of the exponentials go to the FMA pipes.
+// and announces them. 
 #include <type_traits>
 
 #include "dfs_attn_tc.cuh"
@@ -32,7 +32,6 @@ constexpr int kElementRegs = 104, kOtherRegs = 32;
 static_assert(256 * kElementRegs + 128 * kOtherRegs <= kBwdThreads * 80, "register shares");
 constexpr int kWork = 256;     // threads of the element warps
 constexpr int kMmaWarp = 8, kTmaWarp = 9;
-constexpr int kPolyEvery = 3;
 constexpr int kStages = 3, kInfo = 4;
 constexpr int kHalfBytes = kTcTileBytes / 2;  // a streamed tile
 
@@ -113,6 +112,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
       }
       __syncwarp();
       setup_arrive<kBwdThreads>();
+      wait_previous();
       const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
       const TcKeyTiles<kTcHalf> tiles(P, p0, min(i0 + kTcRows, P.nq) - 1 + P.qs);
       if (lane == 0) {
@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
       }
     } else if (warp == kMmaWarp) {  // ---- MMA
       tmem_alloc(&S.tmem, 256);
+      allow_next();
       tc_fence_before();
       setup_wait<kBwdThreads>();
       tc_fence_after();
@@ -206,6 +207,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
     tc_fence_after();
     regs_up<kElementRegs>();
     const uint32_t tm = S.tmem;
+    wait_previous();
     if (P.w) load_bias_ext(tab, P, h, threadIdx.x, kWork);  // read after the barrier below
     const int wq = warp % 4, cg = warp / 4, row = wq * 32 + lane, i = i0 + row, p = p0 + row;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
@@ -278,7 +280,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
         for (int c = 0; c < 16; ++c) {
           const float2 s = make_float2(__uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1]));
           const float2 dp = make_float2(__uint_as_float(dr[2 * c]), __uint_as_float(dr[2 * c + 1]));
-          const float2 ds = mul2(exp2_pair<kPolyEvery>(fma2(s, mul_2, off), c), add2(dp, both(-D)));
+          const float2 x = fma2(s, mul_2, off);
+          const float2 ds = mul2(make_float2(ex2(x.x), ex2(x.y)), add2(dp, both(-D)));
           rest = add2(rest, ds);
           pk[c] = pack16<BF16>(ds.x, ds.y);
         }
@@ -392,6 +395,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
       }
       __syncwarp();
       setup_arrive<kBwdThreads>();
+      wait_previous();
       uint32_t bits[4];
       key_bits(P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr, j0, P.nk, lane, bits);
       const int total = (bits[0] | bits[1] | bits[2] | bits[3]) == 0 ? 0 : last - first;
@@ -435,6 +439,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
       }
     } else if (warp == kMmaWarp) {  // ---- MMA
       tmem_alloc(&S.tmem, 256);
+      allow_next();
       tc_fence_before();
       setup_wait<kBwdThreads>();
       tc_fence_after();
@@ -484,6 +489,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
     tc_fence_after();
     regs_up<kElementRegs>();
     const uint32_t tm = S.tmem;
+    wait_previous();
     const int wq = warp % 4, cg = warp / 4, row = wq * 32 + lane, j = j0 + row, tid = threadIdx.x;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
     const int E = bias_ext(P.D);
@@ -564,7 +570,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
             const int e = 16 * hf + 2 * (c + u);
             const float2 s = make_float2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
             const float2 dp = make_float2(__uint_as_float(dr[e]), __uint_as_float(dr[e + 1]));
-            const float2 x = exp2_pair<kPolyEvery>(fma2(s, mul_2, add2(l2, far_2)), 8 * hf + c + u);
+            float2 x = fma2(s, mul_2, add2(l2, far_2));
+            x = make_float2(ex2(x.x), ex2(x.y));
             const float2 ds = mul2(x, add2(dp, d2));
             sum = add2(sum, ds);
             pp[c + u] = pack16<BF16>(x.x, x.y);
@@ -704,6 +711,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
 // grid (sink tiles, key heads, batch), a thread per value of a row at a time.
 template <bool BF16>
 __global__ void __launch_bounds__(256) sink_join_kernel(AttnParams P) {
+  wait_previous();
+  allow_next();
   const int tile = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, j0 = tile * kTcRows;
   const int rows = min(min(P.sinks, P.nk) - j0, kTcRows), pitch = min(P.sinks, kTcRows) * 128;
   const float* src = P.sink_part +
@@ -738,14 +747,13 @@ static cudaError_t launch_bwd(const AttnParams& P, cudaStream_t st) {
   if (e == cudaSuccess) e = prepare_kernel<tc_dkv_kernel<BF16>>(smem, kBwdThreads, share);
   if (e != cudaSuccess) return e;
   if (!maps(kTcRows, kTcHalf)) return cudaErrorInvalidValue;
-  tc_dq_kernel<BF16><<<tc_grid(P.nq, P.H, P.B), kBwdThreads, smem, st>>>(T);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  e = launch_dependent(tc_dq_kernel<BF16>, tc_grid(P.nq, P.H, P.B), kBwdThreads, smem, st, T);
+  if (e != cudaSuccess) return e;
   if (!maps(kTcHalf, kTcRows)) return cudaErrorInvalidValue;
   const unsigned units = (P.nk + kTcRows - 1) / kTcRows + P.sink_tiles * P.far_segs;
-  tc_dkv_kernel<BF16><<<units * P.Hkv * P.B, kBwdThreads, smem, st>>>(T);
-  if ((e = cudaGetLastError()) != cudaSuccess || P.far_segs == 0) return e;
-  sink_join_kernel<BF16><<<dim3(P.sink_tiles, P.Hkv, P.B), 256, 0, st>>>(P);
-  return cudaGetLastError();
+  e = launch_dependent(tc_dkv_kernel<BF16>, units * P.Hkv * P.B, kBwdThreads, smem, st, T);
+  if (e != cudaSuccess || P.far_segs == 0) return e;
+  return launch_dependent(sink_join_kernel<BF16>, dim3(P.sink_tiles, P.Hkv, P.B), 256, 0, st, P);
 }
 
 cudaError_t launch_attn_tc_bwd(const AttnParams& P, int dtype, cudaStream_t st) {

@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "dfs_attn.cuh"
+#include "dfs_tma.cuh"
 
 namespace dfs {
 namespace {
@@ -29,6 +30,8 @@ __global__ void __cluster_dims__(kBucketCtas) __launch_bounds__(kBucketThreads)
   const float* src = part + static_cast<size_t>(h) * parts * W;
   const uint32_t first = dsmem_addr(smem_u32(acc), 0);
   cluster_sync();  // the first CTA's memory exists
+  allow_next();
+  wait_previous();
   for (int x0 = rank * 32; x0 < W; x0 += kBucketCtas * 32) {
     const int x = x0 + cx;
     float s = 0.0f;
@@ -63,19 +66,19 @@ cudaError_t launch_bucket_sums(const float* part, int H, int parts, int D, const
   const size_t sm = (2 * D + 1) * sizeof(float);
   const int grid = H * kBucketCtas;
   if (dtype == DFS_F32)
-    bucket_sums_kernel<float><<<grid, kBucketThreads, sm, st>>>(part, parts, D, lut, nb, static_cast<float*>(out));
-  else if (dtype == DFS_BF16)
-    bucket_sums_kernel<__nv_bfloat16><<<grid, kBucketThreads, sm, st>>>(part, parts, D, lut, nb,
-                                                                       static_cast<__nv_bfloat16*>(out));
-  else
-    bucket_sums_kernel<__half><<<grid, kBucketThreads, sm, st>>>(part, parts, D, lut, nb, static_cast<__half*>(out));
-  return cudaGetLastError();
+    return launch_dependent(bucket_sums_kernel<float>, grid, kBucketThreads, sm, st, part, parts, D, lut, nb,
+                            static_cast<float*>(out));
+  if (dtype == DFS_BF16)
+    return launch_dependent(bucket_sums_kernel<__nv_bfloat16>, grid, kBucketThreads, sm, st, part, parts, D, lut, nb,
+                            static_cast<__nv_bfloat16*>(out));
+  return launch_dependent(bucket_sums_kernel<__half>, grid, kBucketThreads, sm, st, part, parts, D, lut, nb,
+                          static_cast<__half*>(out));
 }
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kRelThreads = 256;
+constexpr int kRelWarps = kRelThreads / 32;
 
 struct RelParams {
   const void* w;
@@ -91,18 +94,20 @@ struct RelParams {
 // value; others are looked up in the head's table in shared memory.
 // X threads side by side, 256 / X rows at once; grid (row tiles x column tiles, H).
 template <typename U>
-__global__ void __launch_bounds__(kThreads) relbias_fwd_kernel(RelParams P, U* out, int log2x) {
+__global__ void __launch_bounds__(kRelThreads) relbias_fwd_kernel(RelParams P, U* out, int log2x) {
   extern __shared__ unsigned char raw[];
   constexpr int V = 16 / sizeof(U);
   U* tab = reinterpret_cast<U*>(raw);
   const int h = blockIdx.y, tid = threadIdx.x;
+  allow_next();
+  wait_previous();
   const U* w = static_cast<const U*>(P.w) + static_cast<size_t>(h) * P.nb;
-  for (int x = tid; x < 2 * P.D + 1; x += kThreads) tab[x] = w[min(max(P.lut[x], 0), P.nb - 1)];
+  for (int x = tid; x < 2 * P.D + 1; x += kRelThreads) tab[x] = w[min(max(P.lut[x], 0), P.nb - 1)];
   __syncthreads();
   const int c = ((blockIdx.x % P.col_tiles) << log2x) + (tid & ((1 << log2x) - 1));
   const int i1 = min(P.nq, static_cast<int>(blockIdx.x / P.col_tiles + 1) * P.rows);
   const U ends[2] = {tab[0], tab[2 * P.D]};
-  for (int i = blockIdx.x / P.col_tiles * P.rows + (tid >> log2x); i < i1; i += kThreads >> log2x) {
+  for (int i = blockIdx.x / P.col_tiles * P.rows + (tid >> log2x); i < i1; i += kRelThreads >> log2x) {
     U* row = out + (static_cast<size_t>(h) * P.nq + i) * P.nk;
     const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(row) / sizeof(U) % V);
     const int64_t j64 = static_cast<int64_t>(c) * V - mis;  // the piece's first column
@@ -173,20 +178,22 @@ DFS_DEV void unpack(uint4 q, float (&x)[16 / sizeof(T)]) {
 // strip's last column is complete.  Strips beyond the table's ends need no
 // diagonals, one sum serves.  grid (row tiles x column tiles, H).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) relbias_bwd_kernel(RelParams P, const T* dB, float* part) {
+__global__ void __launch_bounds__(kRelThreads) relbias_bwd_kernel(RelParams P, const T* dB, float* part) {
   constexpr int V = 16 / sizeof(T), C = 32 * V;
   extern __shared__ float sm[];
   const int D = P.D, W = 2 * D + 1, tid = threadIdx.x, warp = tid / 32, lane = tid % 32, h = blockIdx.y;
   float* acc = sm;                       // W
-  float* strips = sm + W;                // [kWarps][rows + C - 1]: a strip's diagonals
-  __shared__ float ends[2][kWarps];
-  __shared__ int is_near[kWarps];
+  float* strips = sm + W;                // [kRelWarps][rows + C - 1]: a strip's diagonals
+  __shared__ float ends[2][kRelWarps];
+  __shared__ int is_near[kRelWarps];
   const int len = P.rows + C - 1;
   const int i0 = blockIdx.x / P.col_tiles * P.rows, i1 = min(P.nq, i0 + P.rows);
-  const int J0 = blockIdx.x % P.col_tiles * (kWarps * C), s0 = J0 + warp * C, j = s0 + lane * V;
+  const int J0 = blockIdx.x % P.col_tiles * (kRelWarps * C), s0 = J0 + warp * C, j = s0 + lane * V;
   const T* head = dB + static_cast<size_t>(h) * P.nq * P.nk;
   const T* end = dB + static_cast<size_t>(P.H) * P.nq * P.nk;
-  for (int x = tid; x < W; x += kThreads) acc[x] = 0.0f;
+  for (int x = tid; x < W; x += kRelThreads) acc[x] = 0.0f;
+  allow_next();
+  wait_previous();
 
   // V elements of row i from column j on, zeros outside the row
   auto fetch = [&](int i) -> uint4 {
@@ -297,11 +304,11 @@ __global__ void __launch_bounds__(kThreads) relbias_bwd_kernel(RelParams P, cons
   }
   __syncthreads();
   // the near strips' diagonals, by distance: one thread each, the strips in order
-  const int e0 = i0 - (J0 + kWarps * C - 1);
-  for (int e = e0 + tid; e <= i1 - 1 - J0; e += kThreads) {
+  const int e0 = i0 - (J0 + kRelWarps * C - 1);
+  for (int e = e0 + tid; e <= i1 - 1 - J0; e += kRelThreads) {
     float s = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kRelWarps; ++w) {
       const int slot = e - (i0 - (J0 + w * C + C - 1));
       if (is_near[w] && slot >= 0 && slot < i1 - i0 + C - 1) s += strips[w * len + slot];
     }
@@ -318,12 +325,12 @@ __global__ void __launch_bounds__(kThreads) relbias_bwd_kernel(RelParams P, cons
   if (tid < 2 && (D > 0 || tid == 1)) {
     float s = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) s += ends[tid][w];
+    for (int w = 0; w < kRelWarps; ++w) s += ends[tid][w];
     acc[tid == 0 ? 0 : 2 * D] = s;
   }
   __syncthreads();
   float* dst = part + (static_cast<size_t>(h) * gridDim.x + blockIdx.x) * W;
-  for (int x = tid; x < W; x += kThreads) dst[x] = acc[x];
+  for (int x = tid; x < W; x += kRelThreads) dst[x] = acc[x];
 }
 
 bool bias_ok(const dfs_relbias* b) {
@@ -340,7 +347,7 @@ int elem_size(int dtype) { return dtype == DFS_F32 ? 4 : 2; }
 // Backward tiles: 8 strips of 512 bytes of columns; as many rows (a multiple of 32 up to 256, so that partial
 // sums stay a small part of what is read) as leave about four CTAs an SM.
 void bwd_tiles(int H, int nq, int nk, int dtype, RelParams& P) {
-  P.col_tiles = static_cast<int>(ceil_div(nk, kWarps * 512 / elem_size(dtype)));
+  P.col_tiles = static_cast<int>(ceil_div(nk, kRelWarps * 512 / elem_size(dtype)));
   P.rows = 256;
   while (P.rows > 32 && H * ceil_div(nq, P.rows) * P.col_tiles < 4 * 148) P.rows /= 2;
   P.row_tiles = static_cast<int>(ceil_div(nq, P.rows));
@@ -362,17 +369,17 @@ extern "C" int dfs_relbias_fwd(int H, int n_q, int n_k, int q_start, const dfs_r
   while (log2x < 8 && (int64_t{1} << log2x) < pieces) ++log2x;
   P.col_tiles = static_cast<int>(ceil_div(pieces, int64_t{1} << log2x));
   // rows of a CTA: 32 passes of its threads at most, fewer while there are not eight CTAs an SM
-  P.rows = 32 * (kThreads >> log2x);
-  while (P.rows > (kThreads >> log2x) && H * ceil_div(n_q, P.rows) * P.col_tiles < 8 * 148) P.rows /= 2;
+  P.rows = 32 * (kRelThreads >> log2x);
+  while (P.rows > (kRelThreads >> log2x) && H * ceil_div(n_q, P.rows) * P.col_tiles < 8 * 148) P.rows /= 2;
   P.row_tiles = static_cast<int>(ceil_div(n_q, P.rows));
   if (H > 65535 || static_cast<int64_t>(P.row_tiles) * P.col_tiles > INT_MAX) return DFS_ERR_UNSUPPORTED;
   const dim3 grid(P.row_tiles * P.col_tiles, H);
   const size_t sm = (2 * P.D + 1) * size;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (size == 4)
-    relbias_fwd_kernel<uint32_t><<<grid, kThreads, sm, st>>>(P, static_cast<uint32_t*>(out), log2x);
+    relbias_fwd_kernel<uint32_t><<<grid, kRelThreads, sm, st>>>(P, static_cast<uint32_t*>(out), log2x);
   else
-    relbias_fwd_kernel<uint16_t><<<grid, kThreads, sm, st>>>(P, static_cast<uint16_t*>(out), log2x);
+    relbias_fwd_kernel<uint16_t><<<grid, kRelThreads, sm, st>>>(P, static_cast<uint16_t*>(out), log2x);
   return cudaGetLastError() == cudaSuccess ? DFS_OK : DFS_ERR_CUDA;
 }
 
@@ -396,15 +403,15 @@ extern "C" int dfs_relbias_bwd(int H, int n_q, int n_k, int q_start, const dfs_r
   if (parts > 0) {
     if (work_bytes < dfs_relbias_bwd_work(H, n_q, n_k, b)) return DFS_ERR_WORKSPACE;
     const dim3 grid(static_cast<unsigned>(parts), H);
-    const size_t sm = (2 * P.D + 1 + kWarps * (P.rows + 512 / elem_size(b->dtype) - 1)) * sizeof(float);
+    const size_t sm = (2 * P.D + 1 + kRelWarps * (P.rows + 512 / elem_size(b->dtype) - 1)) * sizeof(float);
     float* part = static_cast<float*>(work);
     if (b->dtype == DFS_F32)
-      relbias_bwd_kernel<float><<<grid, kThreads, sm, st>>>(P, static_cast<const float*>(d_bias), part);
+      relbias_bwd_kernel<float><<<grid, kRelThreads, sm, st>>>(P, static_cast<const float*>(d_bias), part);
     else if (b->dtype == DFS_BF16)
-      relbias_bwd_kernel<__nv_bfloat16><<<grid, kThreads, sm, st>>>(P, static_cast<const __nv_bfloat16*>(d_bias),
+      relbias_bwd_kernel<__nv_bfloat16><<<grid, kRelThreads, sm, st>>>(P, static_cast<const __nv_bfloat16*>(d_bias),
                                                                     part);
     else
-      relbias_bwd_kernel<__half><<<grid, kThreads, sm, st>>>(P, static_cast<const __half*>(d_bias), part);
+      relbias_bwd_kernel<__half><<<grid, kRelThreads, sm, st>>>(P, static_cast<const __half*>(d_bias), part);
     if (cudaGetLastError() != cudaSuccess) return DFS_ERR_CUDA;
   }
   return launch_bucket_sums(static_cast<const float*>(work), H, static_cast<int>(parts), b->max_distance, b->lut,
