@@ -83,7 +83,8 @@ KeyUnits key_units(const dfs_attn_problem* p, int tile, int q_tile) {
   KeyUnits u{(p->n_k + tile - 1) / tile, 0, 0, 0};
   if (p->window == 0 || p->sinks == 0 || q_tile == 0 || p->H_kv == 0) return u;
   const int64_t G = p->H / p->H_kv, q_tiles = (p->n_q + q_tile - 1) / q_tile;
-  const int64_t near_end = std::min<int64_t>(std::max<int64_t>(int64_t{std::min(tile, p->n_k)} - 1 + p->window - p->q_start, 0), p->n_q);
+  const int64_t last = std::min(tile, p->n_k) - 1;  // key of the first tile
+  const int64_t near_end = std::clamp<int64_t>(last + p->window - p->q_start, 0, p->n_q);
   const int64_t far = (q_tiles - (near_end + q_tile - 1) / q_tile) * G;  // of the first tile, the most
   const int64_t len = std::max<int64_t>(std::min<int64_t>((int64_t{tile} + p->window) / q_tile + 1, q_tiles) * G, 8);
   if (far < 2 * len) return u;
@@ -103,15 +104,15 @@ constexpr int kSimtTile = 64;
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool staged(const dfs_strided& s, int n, int heads, int B) {
   auto ok = [](int64_t stride, int extent) { return extent <= 1 || (stride > 0 && stride % 8 == 0); };
-  return aligned16(s.ptr) && ok(s.stride_n, n) && ok(s.stride_h, heads) &&
-         ok(s.stride_b, B);
+  return aligned16(s.ptr) && ok(s.stride_n, n) && ok(s.stride_h, heads) && ok(s.stride_b, B);
 }
 // The tensor-core kernels: 16-bit operands that TMA can stage.  fp32 operands keep all their bits on the
 // SIMT kernels; a scale that is not positive would turn the running maximum of raw products around.
 bool tensor_cores(const dfs_attn_problem* p, const dfs_attn_args* a) {
   const int64_t tiles = (std::max(p->n_q, p->n_k) + kTcRows - 1) / kTcRows + (p->n_q + kTcHalf - 1) / kTcHalf;
   return tiles * p->B * p->H < (int64_t{1} << 31) && p->dtype != DFS_F32 && p->d % 8 == 0 && p->scale > 0.0f &&
-         p->n_q > 0 && p->n_k > 0 && tmap_available() && aligned16(a->o_lo) && staged(a->q, p->n_q, p->H, p->B) && staged(a->o, p->n_q, p->H, p->B) &&
+         p->n_q > 0 && p->n_k > 0 && tmap_available() && aligned16(a->o_lo) &&
+         staged(a->q, p->n_q, p->H, p->B) && staged(a->o, p->n_q, p->H, p->B) &&
          staged(a->k, p->n_k, p->H_kv, p->B) && staged(a->v, p->n_k, p->H_kv, p->B);
 }
 int rc(cudaError_t e) { return e == cudaSuccess ? DFS_OK : DFS_ERR_CUDA; }
@@ -188,7 +189,7 @@ extern "C" int dfs_window_attn_decode(const dfs_attn_problem* p, const dfs_attn_
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // cache tiles staged by TMA, 4-byte reads of q
   const bool rows = p->dtype != DFS_F32 && p->d % 8 == 0 && p->n_k > 0 && tmap_available() &&
-                    staged(a->q, 1, p->H, p->B) &&
-                    staged(a->k, p->n_k, p->H_kv, p->B) && staged(a->v, p->n_k, p->H_kv, p->B);
+                    staged(a->q, 1, p->H, p->B) && staged(a->k, p->n_k, p->H_kv, p->B) &&
+                    staged(a->v, p->n_k, p->H_kv, p->B);
   return rc(rows ? launch_decode_mma(P, p->dtype, st) : launch_decode(P, p->dtype, st));
 }

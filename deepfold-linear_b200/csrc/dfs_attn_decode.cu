@@ -49,11 +49,13 @@ DFS_DEV void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
 template <bool BF16>
 DFS_DEV void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -131,7 +133,8 @@ __global__ void __launch_bounds__(kThreads) decode_mma_kernel(const __grid_const
     const int bk = min(max(P.lut[2 * P.D], 0), P.nb - 1);
 #pragma unroll
     for (int r = 0; r < 2; ++r)
-      if (g + 8 * r < ng) far[r] = load_as_f32<void>(P.w, static_cast<size_t>(h0 + g + 8 * r) * P.nb + bk, P.wdtype) * kLog2e;
+      if (g + 8 * r < ng)
+        far[r] = load_as_f32<void>(P.w, static_cast<size_t>(h0 + g + 8 * r) * P.nb + bk, P.wdtype) * kLog2e;
   }
   if (near_run && warp < 4) asm volatile("bar.sync 1, 128;" ::: "memory");
 

@@ -51,7 +51,7 @@ DFS_DEV void load_tile(const Strided& s, int b, int h, int n0, int n, int d, con
   for (int x = tid; x < kT * kT; x += kNT) {
     const int r = x / kT, c = x % kT, row = n0 + r;
     float v = 0.0f;
-    if (row >= 0 && row < n && c < d && (mask == nullptr || mask[row] != 0)) v = to_f32<E>(row_ptr<E>(s, b, h, row)[c]);
+    if (row < n && c < d && (mask == nullptr || mask[row] != 0)) v = to_f32<E>(row_ptr<E>(s, b, h, row)[c]);
     if (T) T[c * kLd + r] = v;
     if (R) R[r * kLd + c] = v;
   }
@@ -159,9 +159,10 @@ __global__ void __launch_bounds__(kNT) simt_fwd_kernel(AttnParams P) {
 }
 
 // dQ of 64 queries, and D_i for the key pass.  Here D_i = sum_c dO_ic O_ic comes
-// from O (with what its rounding took, where the forward kept that); the key pass gets D_i + sum_j dS_ij, which is sum_j p_ij dP_ij
-// in fp32 (sum_j p_ij = 1).  The sums of dS by bucket need that: they cancel
-// within a row, and from a bfloat16 O alone they were 4e-3 off.
+// from O (with what its rounding took, where the forward kept that); the key pass
+// gets D_i + sum_j dS_ij, which is sum_j p_ij dP_ij in fp32 (sum_j p_ij = 1).  The
+// sums of dS by bucket need that: they cancel within a row, and from a bfloat16 O
+// alone they were 4e-3 off.
 template <typename E>
 __global__ void __launch_bounds__(kNT) simt_dq_kernel(AttnParams P) {
   extern __shared__ __align__(16) float sm[];
@@ -180,7 +181,8 @@ __global__ void __launch_bounds__(kNT) simt_dq_kernel(AttnParams P) {
     const int i = i0 + tid;
     if (i < P.nq) {
       const E* orow = row_ptr<E>(P.o, b, h, i);
-      const E* rest = P.o_lo ? reinterpret_cast<const E*>(P.o_lo) + (orow - reinterpret_cast<const E*>(P.o.p)) : nullptr;
+      const E* rest = nullptr;
+      if (P.o_lo) rest = reinterpret_cast<const E*>(P.o_lo) + (orow - reinterpret_cast<const E*>(P.o.p));
       for (int c = 0; c < P.d; ++c)
         s = fmaf(dOt[c * kLd + tid], to_f32<E>(orow[c]) + (rest ? to_f32<E>(rest[c]) : 0.0f), s);
     }
@@ -212,7 +214,8 @@ __global__ void __launch_bounds__(kNT) simt_dq_kernel(AttnParams P) {
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float p = exp2f(logit2(P, P.w ? tab : nullptr, mask, s[r][c], i0 + 4 * ty + r, j0 + 4 * tx + c) - lse[r]);
+        const int i = i0 + 4 * ty + r, j = j0 + 4 * tx + c;
+        const float p = exp2f(logit2(P, P.w ? tab : nullptr, mask, s[r][c], i, j) - lse[r]);
         const float ds = p * (dp[r][c] - Di[r]);
         rest[r] += ds;
         dSt[(4 * tx + c) * kLd + 4 * ty + r] = ds;
@@ -348,8 +351,8 @@ size_t table_bytes(const AttnParams& P) { return P.w ? (2 * P.D + 1) * sizeof(fl
 
 template <typename E>
 cudaError_t fwd(const AttnParams& P, cudaStream_t st) {
-  return launch(simt_fwd_kernel<E>, dim3((P.nq + kT - 1) / kT, P.H, P.B), 4 * kTile * sizeof(float) + table_bytes(P), st,
-                P);
+  return launch(simt_fwd_kernel<E>, dim3((P.nq + kT - 1) / kT, P.H, P.B),
+                4 * kTile * sizeof(float) + table_bytes(P), st, P);
 }
 template <typename E>
 cudaError_t bwd(const AttnParams& P, cudaStream_t st) {
@@ -360,8 +363,8 @@ cudaError_t bwd(const AttnParams& P, cudaStream_t st) {
     if (e != cudaSuccess) return e;
   }
   if (P.nk == 0) return cudaSuccess;
-  return launch(simt_dkv_kernel<E>, dim3((P.nk + kT - 1) / kT, P.Hkv, P.B), 8 * kTile * sizeof(float) + table_bytes(P) + acc,
-                st, P);
+  return launch(simt_dkv_kernel<E>, dim3((P.nk + kT - 1) / kT, P.Hkv, P.B),
+                8 * kTile * sizeof(float) + table_bytes(P) + acc, st, P);
 }
 
 }  // namespace

@@ -9,9 +9,9 @@
 
 namespace dfs {
 
-constexpr int kTcRows = 128;              // tile edge, queries and keys
+constexpr int kTcRows = 128;              // rows of a CTA's own tile
 constexpr int kTcTileBytes = 128 * 128;   // 128 rows of 64 16-bit elements, 128-byte swizzle
-constexpr int kTcHalf = 64;               // rows of the backward's streamed tiles
+constexpr int kTcHalf = 64;               // rows of the tiles it walks
 
 struct TcParams {
   CUtensorMap q, k, v, d_o;
@@ -50,7 +50,8 @@ DFS_DEV float max32u(const uint32_t (&v)[32]) {
   for (int i = 0; i < 3; ++i)
     a[i] = fmax3(__uint_as_float(v[3 * i]), __uint_as_float(v[3 * i + 1]), __uint_as_float(v[3 * i + 2]));
 #pragma unroll
-  for (int i = 9; i + 1 < 32; i += 2) a[(i / 2) % 3] = fmax3(a[(i / 2) % 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+  for (int i = 9; i + 1 < 32; i += 2)
+    a[(i / 2) % 3] = fmax3(a[(i / 2) % 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
   return fmaxf(fmax3(a[0], a[1], a[2]), __uint_as_float(v[31]));
 }
 
@@ -69,7 +70,7 @@ DFS_DEV int warp_index() { return __shfl_sync(0xffffffffu, static_cast<int>(thre
 // +2 in the address field), or as the contraction index (16 rows: +128).
 DFS_DEV uint64_t tc_desc(uint32_t s) { return sw128_desc(s, 1024, 1024); }
 
-// 128 x 128 product over d of two tiles
+// Product over d of two tiles whose rows are the M and N indices
 DFS_DEV void tc_mma_kk(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, int ksteps) {
 #pragma unroll
   for (int k = 0; k < 4; ++k)
@@ -84,17 +85,6 @@ DFS_DEV void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t id
     mma_f16_ts(d_tmem, a_tmem + (kSpread ? 32 * (k / 2) + 8 * (k % 2) : 8 * k), b + 128 * k, idesc, accum || k > 0);
 }
 
-DFS_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
 DFS_DEV void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
@@ -111,18 +101,9 @@ DFS_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
           taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-}
-DFS_DEV void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-DFS_DEV void tmem_wait_ld16(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 DFS_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -156,9 +137,9 @@ DFS_DEV float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 DFS_DEV float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
 DFS_DEV float2 both(float x) { return make_float2(x, x); }
 
-// Wait for the phase with the given parity; false after some seconds (each try
-// sleeps for a while by itself).  No clock is read and the loop is short: warps
-// wait most of the time, and their tries take issue slots from the others.
+// Wait for the phase with the given parity; false after some seconds (2^27 tries,
+// each of which sleeps for a while by itself).  No clock is read and the loop is
+// short, for warps wait much of the time.
 DFS_DEV bool tc_wait(uint64_t* bar, uint32_t parity) {
   const uint32_t addr = smem_u32(bar);
   for (int tries = 1 << 27; tries > 0; --tries) {
@@ -226,9 +207,10 @@ inline size_t bias_ext_bytes(const AttnParams& P) { return P.w ? (2 * (P.D + 255
 
 // One tile as the producer announces it: first key (or query) row, -1 for the
 // end; whether it is plain (all pairs visible, one bias for all) and where its
-// distances lie (1 beyond the bias table's far end, -1 beyond the other, 0 in it); the key mask's bits; and for a tile that is not
-// plain, the class of each of its blocks of 32 x 32, so that the element warps
-// need no look at positions for most of them.
+// distances lie (1 beyond the bias table's far end, -1 beyond the other, 0 in
+// it); for a tile that is not plain, the key mask's bits and the class of each of
+// its blocks of 32 x 32, so that the element warps need no look at positions for
+// most of them.
 enum { kHidden = 0, kWhole = 1, kPartial = 2 };
 struct TileInfo {
   int at, plain, side, head;
@@ -336,7 +318,9 @@ bool tc_tmap(CUtensorMap* tm, const Strided& s, bool bf16, int d, int n, int hea
 // the CTAs with the most tiles to walk start first, over all heads.  (Tiles
 // fastest left a head's longest CTA among the last: 35 % of SM time idle at
 // N = 4096, causal.)
-inline unsigned tc_grid(int n, int heads, int B) { return static_cast<unsigned>((n + kTcRows - 1) / kTcRows) * heads * B; }
+inline unsigned tc_grid(int n, int heads, int B) {
+  return static_cast<unsigned>((n + kTcRows - 1) / kTcRows) * heads * B;
+}
 
 // Dynamic shared memory of kernel K, raised once per device to the largest asked for (the call costs host
 // time); and, where the kernel splits its registers, that the shares fit what it is launched with (an increase

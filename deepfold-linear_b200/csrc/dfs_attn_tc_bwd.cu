@@ -3,8 +3,9 @@
 // Two passes, neither with atomics, so gradients repeat bit for bit:
 //   dQ pass   one CTA per 128 queries of a head, over the key tiles they see:
 //             S = Q K^T, dP = dO V^T, p = 2^(S - lse), dS = p (dP - D), dQ += dS K;
-//             D comes from O (and what its rounding took), and D + sum_j dS_ij = sum_j p_ij dP_ij (in
-//             fp32) goes to the key pass, whose bias sums cancel within a row;
+//             D = sum_c dO O comes from O and what its rounding took, and D + sum_j dS_ij,
+//             which is sum_j p_ij dP_ij in fp32, goes to the key pass, whose bias sums
+//             cancel within a row;
 //   dK/dV pass  one CTA per 128 keys of a key head, over the query tiles (of every
 //             head of the group) that see them, on transposed tiles: S^T = K Q^T,
 //             dP^T = V dO^T, dV += P^T dO, dK += dS^T Q; and the sums of dS by distance.
@@ -18,7 +19,7 @@
 // warps the same work took about twice as long.  Warps 0-7 work element by element
 // (a TMEM row and half of a tile's columns per thread: blocks of 32 x 32 per warp,
 // skipped where all is hidden), warp 8 issues the MMAs, warp 9 stages tiles by TMA
-// and announces them. 
+// and announces them.
 #include <type_traits>
 
 #include "dfs_attn_tc.cuh"
@@ -73,8 +74,8 @@ DFS_DEV void store_row32(const Strided& s, int b, int h, int row, int c0, int d,
       uint32_t r[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        r[u] = zero ? 0u
-                    : pack16<BF16>(__uint_as_float(v[8 * e + 2 * u]) * mul, __uint_as_float(v[8 * e + 2 * u + 1]) * mul);
+        r[u] = zero ? 0u : pack16<BF16>(__uint_as_float(v[8 * e + 2 * u]) * mul,
+                                        __uint_as_float(v[8 * e + 2 * u + 1]) * mul);
       *reinterpret_cast<uint4*>(dst + 8 * e) = make_uint4(r[0], r[1], r[2], r[3]);
     }
 }
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
         __syncwarp();
         end = next_end;
       }
-    } else if (warp != kMmaWarp) {  // ---- the warpgroup's idle warps
+    } else {  // ---- the warpgroup's idle warps
       setup_wait<kBwdThreads>();
     }
   } else {  // ---- elements: warp w has TMEM lanes 32 (w % 4).. and columns 32 (w / 4)..
@@ -223,7 +224,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (c0 + 8 * e < P.d) {
-          const uint4 x = *reinterpret_cast<const uint4*>(orow + 8 * e), y = *reinterpret_cast<const uint4*>(drow + 8 * e);
+          const uint4 x = *reinterpret_cast<const uint4*>(orow + 8 * e);
+          const uint4 y = *reinterpret_cast<const uint4*>(drow + 8 * e);
           const uint4 z = rest ? *reinterpret_cast<const uint4*>(rest + 8 * e) : make_uint4(0, 0, 0, 0);
           const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
@@ -388,7 +390,6 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
         mbar_init(&S.own_full, 1);
         for (int s = 0; s < kStages; ++s) mbar_init(&S.full[s], 1), mbar_init(&S.empty[s], 1);
         mbar_init(&S.s_full, 1);
-        mbar_init(&S.s_free, kWork / 32);
         mbar_init(&S.ds_ready, kWork / 32);
         mbar_init(&S.acc_done, 1);
         fence_mbar_init();
@@ -481,7 +482,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
         }
         __syncwarp();
       }
-    } else if (warp != kMmaWarp) {  // ---- the warpgroup's idle warps
+    } else {  // ---- the warpgroup's idle warps
       setup_wait<kBwdThreads>();
     }
   } else {  // ---- elements: a key row and half of the tile's queries per thread

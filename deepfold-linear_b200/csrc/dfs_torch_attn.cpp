@@ -176,8 +176,8 @@ Tensor run_forward(const Problem& r, bool keep, Tensor* lse, Tensor* o_lo) {
 
 struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
   static Tensor forward(AutogradContext* ctx, Tensor Q, Tensor K, Tensor V, optional<Tensor> weight,
-                        optional<Tensor> mask, optional<Tensor> lut, int64_t max_distance, int64_t window, int64_t sinks, bool causal,
-                        int64_t q_start, double scale) {
+                        optional<Tensor> mask, optional<Tensor> lut, int64_t max_distance, int64_t window,
+                        int64_t sinks, bool causal, int64_t q_start, double scale) {
     const Problem r = make_problem(Q, K, V, mask, weight, lut, max_distance, window, sinks, causal, q_start, scale);
     Tensor lse, o_lo;
     Tensor o = run_forward(r, true, &lse, &o_lo);
@@ -234,8 +234,8 @@ Tensor window_attn(Tensor Q, Tensor K, Tensor V, optional<Tensor> mask, optional
   if (grad)
     return WindowAttnFn::apply(Q, K, V, has_w ? weight : c10::nullopt, mask, lut, max_distance, window, sinks,
                                causal, q_start, scale);
-  return run_forward(make_problem(Q, K, V, mask, weight, lut, max_distance, window, sinks, causal, q_start, scale), false,
-                     nullptr, nullptr);
+  return run_forward(make_problem(Q, K, V, mask, weight, lut, max_distance, window, sinks, causal, q_start, scale),
+                     false, nullptr, nullptr);
 }
 
 Tensor window_attn_decode(Tensor q, Tensor K, Tensor V, Tensor lengths, optional<Tensor> weight, optional<Tensor> lut,

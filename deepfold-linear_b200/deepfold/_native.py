@@ -24,8 +24,8 @@ LIB_DIR = os.path.join(PKG_DIR, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libdfsink.so")
 SOURCES = ["dfs_abi.cu", "dfs_fwd.cu", "dfs_bwd.cu", "dfs_stream.cu", "dfs_stream_bwd.cu", "dfs_stream_tma.cu",
            "dfs_stream_bwd_tma.cu", "dfs_selftest.cu", "dfs_noalloc.cu", "dfs_pad.cu", "dfs_dense.cu",
-           "dfs_dense_grad.cu", "dfs_peer.cu", "dfs_relbias.cu", "dfs_attn_simt.cu", "dfs_attn_tc.cu", "dfs_attn_tc_bwd.cu", "dfs_attn_decode.cu",
-           "dfs_attn.cu"]
+           "dfs_dense_grad.cu", "dfs_peer.cu", "dfs_relbias.cu", "dfs_attn_simt.cu", "dfs_attn_tc.cu",
+           "dfs_attn_tc_bwd.cu", "dfs_attn_decode.cu", "dfs_attn.cu"]
 HEADERS = ["dfs_device.cuh", "dfs_kernels.cuh", "dfs_slab.cuh", "dfs_tma.cuh", "dfs_attn.cuh", "dfs_attn_tc.cuh"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",

@@ -83,8 +83,8 @@ def flash_window_attn(Q, K, V, window: int | None = None, sinks: int = 0, causal
         raise ValueError("Q must be (B, H, n_q, d) or (H, n_q, d), K and V alike")
     window, scale, lut, distance = _options(Q.shape[-1], window, sinks, scale, pos_weight, buckets, Q.device)
     q_start = K.shape[2] - Q.shape[2] if q_start is None else int(q_start)
-    out = nat.ext().window_attn(Q, K, V, mask, pos_weight, lut, distance, window, min(int(sinks), 1 << 30), bool(causal), q_start,
-                                scale)
+    out = nat.ext().window_attn(Q, K, V, mask, pos_weight, lut, distance, window, min(int(sinks), 1 << 30),
+                                bool(causal), q_start, scale)
     return out.squeeze(0) if unbatched else out
 
 
@@ -107,5 +107,5 @@ def window_attn_decode(q, k_cache, v_cache, lengths, window: int | None = None, 
         raise NotImplementedError("window_attn_decode is forward only: call it under torch.no_grad(), or "
                                   "flash_window_attn for gradients")
     window, scale, lut, distance = _options(q.shape[-1], window, sinks, scale, pos_weight, buckets, q.device)
-    return nat.ext().window_attn_decode(q, k_cache, v_cache, lengths, pos_weight, lut, distance, window, min(int(sinks), 1 << 30),
-                                        scale)
+    return nat.ext().window_attn_decode(q, k_cache, v_cache, lengths, pos_weight, lut, distance, window,
+                                        min(int(sinks), 1 << 30), scale)
