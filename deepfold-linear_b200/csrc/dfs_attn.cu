@@ -102,8 +102,8 @@ constexpr int kSimtTile = 64;
 // Whether an operand can be staged by TMA (and stored in 16-byte pieces): its address and the strides of
 // its extents above 1 are multiples of 16 bytes.
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-bool staged(const dfs_strided& s, int n, int heads, int B) {
-  auto ok = [](int64_t stride, int extent) { return extent <= 1 || (stride > 0 && stride % 8 == 0); };
+bool staged(const dfs_strided& s, int n, int heads, int B, int piece = 8) {  // piece: elements of 16 bytes
+  auto ok = [=](int64_t stride, int extent) { return extent <= 1 || (stride > 0 && stride % piece == 0); };
   return aligned16(s.ptr) && ok(s.stride_n, n) && ok(s.stride_h, heads) && ok(s.stride_b, B);
 }
 // The tensor-core kernels: 16-bit operands that TMA can stage.  fp32 operands keep all their bits on the
@@ -114,6 +114,11 @@ bool tensor_cores(const dfs_attn_problem* p, const dfs_attn_args* a) {
          p->n_q > 0 && p->n_k > 0 && tmap_available() && aligned16(a->o_lo) &&
          staged(a->q, p->n_q, p->H, p->B) && staged(a->o, p->n_q, p->H, p->B) &&
          staged(a->k, p->n_k, p->H_kv, p->B) && staged(a->v, p->n_k, p->H_kv, p->B);
+}
+// fp32 operands whose rows the other kernels read in 16-byte pieces
+bool vector_rows(const dfs_attn_problem* p, const dfs_attn_args* a) {
+  return p->dtype == DFS_F32 && p->d % 4 == 0 && staged(a->k, p->n_k, p->H_kv, p->B, 4) &&
+         staged(a->v, p->n_k, p->H_kv, p->B, 4);
 }
 int rc(cudaError_t e) { return e == cudaSuccess ? DFS_OK : DFS_ERR_CUDA; }
 
@@ -127,7 +132,8 @@ extern "C" int dfs_window_attn_fwd(const dfs_attn_problem* p, const dfs_attn_arg
   if (!a->q.ptr || !a->o.ptr || (p->n_k > 0 && (!a->k.ptr || !a->v.ptr))) return DFS_ERR_INVALID_ARGUMENT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const AttnParams P = params(p, a);
-  return rc(tensor_cores(p, a) ? launch_attn_tc_fwd(P, p->dtype, st) : launch_attn_simt_fwd(P, p->dtype, st));
+  if (tensor_cores(p, a)) return rc(launch_attn_tc_fwd(P, p->dtype, st));
+  return rc(launch_attn_simt_fwd(P, p->dtype, vector_rows(p, a) && staged(a->q, p->n_q, p->H, p->B, 4), st));
 }
 
 extern "C" size_t dfs_window_attn_bwd_work(const dfs_attn_problem* p, const dfs_relbias* b) {
@@ -167,7 +173,8 @@ extern "C" int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_arg
   P.sink_part = reinterpret_cast<float*>(at);
   if (dw) P.dw_part = reinterpret_cast<float*>(at + round256(sink_part_bytes(p, u)));
   if (p->n_q > 0 || p->n_k > 0) {
-    const int r = rc(tc ? launch_attn_tc_bwd(P, p->dtype, st) : launch_attn_simt_bwd(P, p->dtype, st));
+    const bool vec = vector_rows(p, a) && staged(a->q, p->n_q, p->H, p->B, 4) && staged(a->d_o, p->n_q, p->H, p->B, 4);
+    const int r = rc(tc ? launch_attn_tc_bwd(P, p->dtype, st) : launch_attn_simt_bwd(P, p->dtype, vec, st));
     if (r != DFS_OK) return r;
   }
   if (!dw) return DFS_OK;
@@ -191,5 +198,6 @@ extern "C" int dfs_window_attn_decode(const dfs_attn_problem* p, const dfs_attn_
   const bool rows = p->dtype != DFS_F32 && p->d % 8 == 0 && p->n_k > 0 && tmap_available() &&
                     staged(a->q, 1, p->H, p->B) && staged(a->k, p->n_k, p->H_kv, p->B) &&
                     staged(a->v, p->n_k, p->H_kv, p->B);
-  return rc(rows ? launch_decode_mma(P, p->dtype, st) : launch_decode(P, p->dtype, st));
+  if (rows) return rc(launch_decode_mma(P, p->dtype, st));
+  return rc(launch_decode_any(P, p->dtype, vector_rows(p, a), st));
 }

@@ -90,9 +90,10 @@ DFS_DEV void load_bias_table(float* tab, const void* w, const int32_t* lut, int 
 // launchers (host)
 cudaError_t launch_bucket_sums(const float* part, int H, int parts, int D, const int32_t* lut, int nb, int dtype,
                                void* out, cudaStream_t st);
-cudaError_t launch_attn_simt_fwd(const AttnParams& P, int dtype, cudaStream_t st);
-cudaError_t launch_attn_simt_bwd(const AttnParams& P, int dtype, cudaStream_t st);
-cudaError_t launch_decode(const AttnParams& P, int dtype, cudaStream_t st);
-cudaError_t launch_decode_mma(const AttnParams& P, int dtype, cudaStream_t st);  // 16-bit, 16-byte rows
+// vec: fp32 rows on 16-byte boundaries
+cudaError_t launch_attn_simt_fwd(const AttnParams& P, int dtype, bool vec, cudaStream_t st);
+cudaError_t launch_attn_simt_bwd(const AttnParams& P, int dtype, bool vec, cudaStream_t st);
+cudaError_t launch_decode_mma(const AttnParams& P, int dtype, cudaStream_t st);  // 16-bit, staged by TMA
+cudaError_t launch_decode_any(const AttnParams& P, int dtype, bool vec, cudaStream_t st);
 
 }  // namespace dfs

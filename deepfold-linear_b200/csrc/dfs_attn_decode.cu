@@ -25,11 +25,17 @@ constexpr int kStages = 2;         // of K and V tiles: 64 KB, three CTAs an SM
 constexpr int kHeads = 16;         // query heads of a CTA: the rows of an m16n8k16 product
 constexpr int kMaxSplit = 8;
 
+// What a CTA found, read by its cluster: maxima, sums and sums of P V
+template <int N>
+struct Found {
+  float m[N], l[N];
+  float o[N][68];
+};
+
 struct DecodeShared {
   uint64_t full[kStages], empty[kStages];
   float m[4][kHeads], l[4][kHeads];       // the warps' maxima and sums
-  float cm[kHeads], cl[kHeads];           // the CTA's, read by the cluster
-  float o[kHeads][68];                    // the CTA's sums of P V, read by the cluster
+  Found<kHeads> found;
 };
 
 struct DecodeParams {
@@ -61,6 +67,32 @@ DFS_DEV void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t 
 }
 // Byte of 16-byte piece c of row r of a tile (128-byte rows, 128-byte swizzle)
 DFS_DEV uint32_t piece_at(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+
+// Joins the cluster's CTAs in order, and writes the outputs: this one finishes every split-th head.
+template <typename E, int N, int kBlock>
+DFS_DEV void join_cluster(const AttnParams& P, const Found<N>& F, int b, int h0, int ng, int rank, int split) {
+  if (split > 1) cluster_sync();
+  for (int x = threadIdx.x; x < ng * P.d; x += kBlock) {
+    const int head = x / P.d, c = x % P.d;
+    if (head % split != rank) continue;
+    float top = -INFINITY, sum = 0.0f, acc = 0.0f;
+    if (split == 1) {
+      sum = F.l[head];
+      acc = F.o[head][c];
+    } else {
+      const uint32_t am = smem_u32(&F.m[head]), al = smem_u32(&F.l[head]), ao = smem_u32(&F.o[head][c]);
+      for (int r = 0; r < split; ++r) top = fmaxf(top, dsmem_ld(dsmem_addr(am, r)));
+      const float ref = top == -INFINITY ? 0.0f : top;
+      for (int r = 0; r < split; ++r) {
+        const float k = exp2f(dsmem_ld(dsmem_addr(am, r)) - ref);
+        sum += dsmem_ld(dsmem_addr(al, r)) * k;
+        acc += dsmem_ld(dsmem_addr(ao, r)) * k;
+      }
+    }
+    row_ptr<E>(P.o, b, h0 + head, 0)[c] = from_f32<E>(sum > 0.0f ? acc / sum : 0.0f);
+  }
+  if (split > 1) cluster_sync();  // nobody leaves while its memory is read
+}
 
 // grid (split, key heads x head chunks, batch), clusters of `split` CTAs
 template <typename E>
@@ -256,11 +288,11 @@ __global__ void __launch_bounds__(kThreads) decode_mma_kernel(const __grid_const
     const float ref = top == -INFINITY ? 0.0f : top;
     f[r] = ex2(m[r] - ref);
     if (warp == 0 && lane % 4 == 0) {
-      S.cm[row] = top;
+      S.found.m[row] = top;
       float sum = 0.0f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) sum += S.l[w][row] * ex2(S.m[w][row] - ref);
-      S.cl[row] = sum;
+      S.found.l[row] = sum;
     }
   }
 #pragma unroll
@@ -270,35 +302,192 @@ __global__ void __launch_bounds__(kThreads) decode_mma_kernel(const __grid_const
       for (int n = 0; n < 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float* at = &S.o[g + 8 * (e >> 1)][8 * n + q2 + (e & 1)];
+          float* at = &S.found.o[g + 8 * (e >> 1)][8 * n + q2 + (e & 1)];
           const float v = o[n][e] * f[e >> 1];
           *at = w == 0 ? v : *at + v;
         }
     __syncthreads();
   }
-  // join the CTAs: this one finishes every split-th head
-  if (split > 1) cluster_sync();
-  for (int x = tid; x < ng * P.d; x += kThreads) {
-    const int head = x / P.d, c = x % P.d;
-    if (head % split != rank) continue;
-    float top = -INFINITY, sum = 0.0f, acc = 0.0f;
-    if (split == 1) {
-      sum = S.cl[head];
-      acc = S.o[head][c];
-    } else {
-      const uint32_t am = smem_u32(&S.cm[head]), al = smem_u32(&S.cl[head]), ao = smem_u32(&S.o[head][c]);
-      for (int r = 0; r < split; ++r) top = fmaxf(top, dsmem_ld(dsmem_addr(am, r)));
-      const float ref = top == -INFINITY ? 0.0f : top;
-      for (int r = 0; r < split; ++r) {
-        const float k = ex2(dsmem_ld(dsmem_addr(am, r)) - ref);
-        sum += dsmem_ld(dsmem_addr(al, r)) * k;
-        acc += dsmem_ld(dsmem_addr(ao, r)) * k;
-      }
-    }
-    row_ptr<E>(P.o, b, h0 + head, 0)[c] = from_f32<E>(sum > 0.0f ? acc / sum : 0.0f);
-  }
   if (err) report_timeout(P.status);
-  if (split > 1) cluster_sync();  // nobody leaves while its memory is read
+  join_cluster<E, kHeads, kThreads>(P, S.found, b, h0, ng, rank, split);
+}
+
+// The same for every type and any strides, on the fp32 pipes: fp32 operands, and 16-bit ones that TMA cannot
+// stage.  Sixteen lanes take a key at a time, four columns each, for four query heads; of four keys' products the
+// sixteen sums end one to a lane (reduced and scattered together, a shuffle a sum), so a lane has one exponential.
+// kVec: fp32 rows on 16-byte boundaries.  Measured (fp32): 64 sequences of 16 / 4 heads, 4096 keys of 512 bytes each:
+// 112 us, 4.8 TB/s; 8 of 32 / 8 heads over 16384 keys: 96 us, 5.6 TB/s.
+constexpr int kAnyThreads = 128, kAnyHeads = 4, kAnyKeys = 4;
+constexpr int kAnyTeams = kAnyThreads / 16, kAnyStep = kAnyTeams * kAnyKeys;  // keys of the CTA at once
+
+template <typename E, bool kVec>
+__global__ void __launch_bounds__(kAnyThreads, 4) decode_any_kernel(AttnParams P, int split, int chunks) {
+  extern __shared__ float tab[];  // [heads][D + 1] bias of delta = 0 .. D
+  __shared__ Found<kAnyHeads> F;
+  __shared__ float tm[kAnyTeams][kAnyHeads], tl[kAnyTeams][kAnyHeads];
+  const int tid = threadIdx.x, lane = tid % 32, team = tid / 16, at = tid % 16, rank = blockIdx.x;
+  const int hk = blockIdx.y / chunks, g0 = blockIdx.y % chunks * kAnyHeads, b = blockIdx.z;
+  const int ng = min(kAnyHeads, P.G - g0), h0 = hk * P.G + g0;
+  const int head = at % kAnyHeads, key = at / kAnyHeads;  // of the sum that ends in this lane
+  allow_next();
+  wait_previous();
+  const int len = min(max(P.lengths[b], 0), P.nk), p = len - 1;
+  const int lo = max(0, len - P.window), ns = min(P.sinks, lo), total = ns + len - lo;  // keys [0, ns), [lo, len)
+  const int per = ((total + split - 1) / split + kAnyStep - 1) / kAnyStep * kAnyStep;
+  const int x0 = static_cast<int>(min(static_cast<int64_t>(rank) * per, static_cast<int64_t>(total)));
+  const int x1 = static_cast<int>(min(static_cast<int64_t>(x0) + per, static_cast<int64_t>(total)));
+  auto key_at = [&](int x) { return x < ns ? x : lo + (x - ns); };
+  auto col = [&](int e) { return kVec ? 4 * at + e : at + 16 * e; };
+  float far = 0.0f;
+  bool near_run = false;
+  if (P.w) {
+    near_run = x1 > x0 && p - key_at(x1 - 1) < P.D;
+    auto weight = [&](int r, int x) {
+      const int bk = min(max(P.lut[P.D + x], 0), P.nb - 1);
+      return load_as_f32<void>(P.w, static_cast<size_t>(h0 + r) * P.nb + bk, P.wdtype) * kLog2e;
+    };
+    if (near_run)
+      for (int x = tid; x < ng * (P.D + 1); x += kAnyThreads) tab[x] = weight(x / (P.D + 1), x % (P.D + 1));
+    far = weight(min(head, ng - 1), P.D);
+  }
+  float q[kAnyHeads][4], o[kAnyHeads][4];
+#pragma unroll
+  for (int h = 0; h < kAnyHeads; ++h)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[h][e] = 0.0f;
+      q[h][e] = h < ng && col(e) < P.d ? to_f32<E>(row_ptr<E>(P.q, b, h0 + h, 0)[col(e)]) : 0.0f;
+    }
+  __syncthreads();
+  float m = -INFINITY, l = 0.0f;
+  auto row4 = [&](const Strided& s, int j, bool on, float (&v)[4]) {  // zeros for a key that is not visible
+    const E* row = row_ptr<E>(s, b, hk, j);
+    if (kVec) {
+      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (on && 4 * at < P.d) x = __ldcs(reinterpret_cast<const float4*>(row) + at);
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = on && col(e) < P.d ? to_f32<E>(row[col(e)]) : 0.0f;
+    }
+  };
+  for (int xb = x0; xb < x1; xb += kAnyStep) {
+    const int xt = xb + team * kAnyKeys;
+    float k[kAnyKeys][4], v[kAnyKeys][4];
+#pragma unroll
+    for (int r = 0; r < kAnyKeys; ++r) row4(P.k, key_at(min(xt + r, x1 - 1)), xt + r < x1, k[r]);
+#pragma unroll
+    for (int r = 0; r < kAnyKeys; ++r) row4(P.v, key_at(min(xt + r, x1 - 1)), xt + r < x1, v[r]);
+    float s[16];
+#pragma unroll
+    for (int r = 0; r < kAnyKeys; ++r)
+#pragma unroll
+      for (int h = 0; h < kAnyHeads; ++h) {
+        float t = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t = fmaf(q[h][e], k[r][e], t);
+        s[r * kAnyHeads + h] = t;
+      }
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+      for (int i = 0; i < w; ++i) {
+        const bool up = at & w;
+        const float keep = up ? s[i + w] : s[i], send = up ? s[i] : s[i + w];
+        s[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+      }
+    const int x = xt + key;
+    float val = -INFINITY;
+    if (x < x1)
+      val = fmaf(s[0], P.scale2,
+                 near_run ? tab[min(head, ng - 1) * (P.D + 1) + min(p - key_at(x), P.D)] : far);
+    float top = fmaxf(val, __shfl_xor_sync(0xffffffffu, val, 4));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.0f : mn;
+    if (__any_sync(0xffffffffu, mn != m)) {
+      const float shrink = exp2f(m - ref);
+      l *= shrink;
+#pragma unroll
+      for (int h = 0; h < kAnyHeads; ++h) {
+        const float f = __shfl_sync(0xffffffffu, shrink, h, 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[h][e] *= f;
+      }
+      m = mn;
+    }
+    const float pr = exp2f(val - ref);
+    l += pr;
+#pragma unroll
+    for (int r = 0; r < kAnyKeys; ++r)
+#pragma unroll
+      for (int h = 0; h < kAnyHeads; ++h) {
+        const float f = __shfl_sync(0xffffffffu, pr, r * kAnyHeads + h, 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[h][e] = fmaf(f, v[r][e], o[h][e]);
+      }
+  }
+  // join the teams: two of a warp by a shuffle, the warps in turn
+  l += __shfl_xor_sync(0xffffffffu, l, 4);
+  l += __shfl_xor_sync(0xffffffffu, l, 8);
+  if (key == 0) tm[team][head] = m, tl[team][head] = l;
+  __syncthreads();
+  float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int t = 0; t < kAnyTeams; ++t) top = fmaxf(top, tm[t][head]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+  for (int t = 0; t < kAnyTeams; ++t) sum += tl[t][head] * exp2f(tm[t][head] - ref);
+  if (tid < kAnyHeads) F.m[head] = top, F.l[head] = sum;
+  const float scale = exp2f(m - ref);
+#pragma unroll
+  for (int h = 0; h < kAnyHeads; ++h) {
+    const float f = __shfl_sync(0xffffffffu, scale, h, 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[h][e] *= f;
+      o[h][e] += __shfl_xor_sync(0xffffffffu, o[h][e], 16);
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < kAnyThreads / 32; ++w) {
+    if (tid / 32 == w && lane < 16)
+#pragma unroll
+      for (int h = 0; h < kAnyHeads; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) F.o[h][col(e)] = w == 0 ? o[h][e] : F.o[h][col(e)] + o[h][e];
+    __syncthreads();
+  }
+  join_cluster<E, kAnyHeads, kAnyThreads>(P, F, b, h0, ng, rank, split);
+}
+
+// How many CTAs share a (sequence, key head): until there are twice the CTAs that fit at once (`resident` an SM),
+// so that ragged lengths even out, while each has 128 keys; short batches are split and large ones are not.
+int split_of(const AttnParams& P, int chunks, int resident) {
+  const long problems = static_cast<long>(P.B) * P.Hkv * chunks;
+  const long tiles = (std::min<long>(static_cast<long>(P.window) + P.sinks, P.nk) + kTcRows - 1) / kTcRows;
+  int split = 1;
+  while (split < kMaxSplit && split * problems < 2 * resident * 148 && 2 * split <= tiles) split *= 2;
+  return split;
+}
+
+template <typename... A>
+cudaError_t launch_split(void (*kern)(A...), int split, int heads, int B, int threads, size_t smem, cudaStream_t st,
+                         const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(split, heads, B);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
 template <typename E>
@@ -309,38 +498,30 @@ cudaError_t launch(const AttnParams& P, cudaStream_t st) {
   if (!tc_tmap(&T.k, P.k, bf16, P.d, P.nk, P.Hkv, P.B) || !tc_tmap(&T.v, P.v, bf16, P.d, P.nk, P.Hkv, P.B))
     return cudaErrorInvalidValue;
   T.chunks = (P.G + kHeads - 1) / kHeads;
-  // Splits: until there are twice the CTAs that fit at once (three an SM), so that ragged lengths even out,
-  // while each has a tile of keys; short batches are split and large ones are not.
-  const long problems = static_cast<long>(P.B) * P.Hkv * T.chunks;
-  const long seen = std::min<long>(static_cast<long>(P.window) + P.sinks, P.nk);
-  const long tiles = (seen + kTcRows - 1) / kTcRows;
-  T.split = 1;
-  while (T.split < kMaxSplit && T.split * problems < 6 * 148 && 2 * T.split <= tiles) T.split *= 2;
+  T.split = split_of(P, T.chunks, 3);
   const size_t smem = 1024 + kStages * 2 * kTcTileBytes + sizeof(DecodeShared) +
                       (P.w ? std::min(P.G, kHeads) * (P.D + 1) * sizeof(float) : 0);
   const cudaError_t e = prepare_kernel<decode_mma_kernel<E>>(smem);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(T.split, P.Hkv * T.chunks, P.B);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = T.split;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = T.split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, decode_mma_kernel<E>, T);
+  return launch_split(decode_mma_kernel<E>, T.split, P.Hkv * T.chunks, P.B, kThreads, smem, st, T);
+}
+
+template <typename E, bool kVec>
+cudaError_t launch_any(const AttnParams& P, cudaStream_t st) {
+  const int chunks = (P.G + kAnyHeads - 1) / kAnyHeads, split = split_of(P, chunks, 4);
+  const size_t smem = P.w ? kAnyHeads * (P.D + 1) * sizeof(float) : 0;
+  return launch_split(decode_any_kernel<E, kVec>, split, P.Hkv * chunks, P.B, kAnyThreads, smem, st, P, split, chunks);
 }
 
 }  // namespace
 
 cudaError_t launch_decode_mma(const AttnParams& P, int dtype, cudaStream_t st) {
   return dtype == DFS_BF16 ? launch<__nv_bfloat16>(P, st) : launch<__half>(P, st);
+}
+
+cudaError_t launch_decode_any(const AttnParams& P, int dtype, bool vec, cudaStream_t st) {
+  if (dtype == DFS_F32) return vec ? launch_any<float, true>(P, st) : launch_any<float, false>(P, st);
+  return dtype == DFS_BF16 ? launch_any<__nv_bfloat16, false>(P, st) : launch_any<__half, false>(P, st);
 }
 
 }  // namespace dfs
