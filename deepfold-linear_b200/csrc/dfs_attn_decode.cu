@@ -2,7 +2,7 @@
 // (bf16, fp16 whose rows can be copied in 16-byte pieces).
 //
 // Reading the visible cache rows is all the time there is: 256 bytes of K and V
-// a key at d = 64 for 4 d operations a query head.  A cluster of up to 8 CTAs
+// a key at d = 64 for 4 d operations a query head.  A cluster of up to 16 CTAs
 // shares one key head of one sequence and splits the tiles of 128 keys that hold
 // visible ones (the sinks' and the window's) into equal runs.  In a CTA one warp
 // keeps TMA copies in flight through a ring of stages and four warps take 32 keys
@@ -23,7 +23,6 @@ namespace {
 constexpr int kThreads = 160;      // four warps of products, one of copies
 constexpr int kStages = 2;         // of K and V tiles: 64 KB, three CTAs an SM
 constexpr int kHeads = 16;         // query heads of a CTA: the rows of an m16n8k16 product
-constexpr int kMaxSplit = 8;
 
 // What a CTA found, read by its cluster: maxima, sums and sums of P V
 template <int N>
@@ -461,18 +460,24 @@ __global__ void __launch_bounds__(kAnyThreads, 4) decode_any_kernel(AttnParams P
 }
 
 // How many CTAs share a (sequence, key head): until there are twice the CTAs that fit at once (`resident` an SM),
-// so that ragged lengths even out, while each has 128 keys; short batches are split and large ones are not.
+// so that ragged lengths even out, while each has 128 keys; short batches are split and large ones are not.  Sixteen
+// only while no SM gets more than two, for they have to find room together (bfloat16, d = 64, 32768 keys: 8 key heads
+// 38 -> 26 us with sixteen, 32 key heads 51 -> 58).
 int split_of(const AttnParams& P, int chunks, int resident) {
   const long problems = static_cast<long>(P.B) * P.Hkv * chunks;
   const long tiles = (std::min<long>(static_cast<long>(P.window) + P.sinks, P.nk) + kTcRows - 1) / kTcRows;
   int split = 1;
-  while (split < kMaxSplit && split * problems < 2 * resident * 148 && 2 * split <= tiles) split *= 2;
-  return split;
+  while (split < 8 && split * problems < 2 * resident * 148 && 2 * split <= tiles) split *= 2;
+  return split == 8 && 16 * problems <= 2 * 148 && 16 <= tiles ? 16 : split;
 }
 
 template <typename... A>
 cudaError_t launch_split(void (*kern)(A...), int split, int heads, int B, int threads, size_t smem, cudaStream_t st,
                          const A&... args) {
+  if (split > 8) {  // beyond what every device has: opted in
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(split, heads, B);
   cfg.blockDim = dim3(threads);

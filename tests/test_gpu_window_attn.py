@@ -378,3 +378,14 @@ def test_refusals():
             window_attn_decode(q[:, :, 0], k, v, lengths)
     with pytest.raises(NotImplementedError):
         window_attn_decode(q[:, :, 0].requires_grad_(), k, v, one)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_decode_of_one_long_sequence(dtype):
+    """Sixteen blocks join, and runs of keys end inside a tile."""
+    x = inputs(1, 4, 2, 1, 5003, 64, dtype, 31, nb=32)
+    got = window_attn_decode(x["q"][:, :, 0], x["k"], x["v"], torch.tensor([4990], device="cuda"),
+                             pos_weight=x["w"], buckets=BUCKETS["log"])
+    want = orc.window_attn(f64(x["q"]), f64(x["k"][:, :, :4990]), f64(x["v"][:, :, :4990]), weight=f64(x["w"]),
+                           table=BUCKETS["log"].table)
+    close(got[:, :, None], want, dtype, 2)
