@@ -72,26 +72,36 @@ size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 size_t dsum_bytes(const dfs_attn_problem* p) {
   return round256(sizeof(float) * static_cast<size_t>(p->B) * p->H * p->n_q);
 }
-// The backward's key pass: units of work of a batch element and key head.  Every query sees the sinks, so the
-// CTAs of their key tiles would walk all query tiles, with the others done long before; where the queries beyond
-// the window are many, they are cut into segments of their own of about an ordinary tile's length.
+// The backward's key pass: units of work of a batch element and key head, each a CTA that walks steps of (head of
+// the group, query tile).  Every query sees the sinks, so the CTAs of their key tiles would walk all query tiles,
+// with the others done long before; where the queries beyond the window are many, they are cut into segments of
+// their own of about an ordinary tile's length.  And where few key heads leave SMs idle, every tile's steps are cut
+// into segments of at least four, up to two CTAs an SM (16 / 2 heads, 2048 tokens: see the key pass).
 struct KeyUnits {
-  int tiles, sink_tiles, far_segs, far_len;
-  int count() const { return tiles + sink_tiles * far_segs; }
+  int tiles, sink_tiles, far_segs, far_len, near_segs;
+  int count() const { return tiles * near_segs + sink_tiles * far_segs; }
 };
 KeyUnits key_units(const dfs_attn_problem* p, int tile, int q_tile) {
-  KeyUnits u{(p->n_k + tile - 1) / tile, 0, 0, 0};
-  if (p->window == 0 || p->sinks == 0 || q_tile == 0 || p->H_kv == 0) return u;
+  KeyUnits u{(p->n_k + tile - 1) / tile, 0, 0, 0, 1};
+  if (q_tile == 0 || p->H_kv == 0 || u.tiles == 0) return u;
   const int64_t G = p->H / p->H_kv, q_tiles = (p->n_q + q_tile - 1) / q_tile;
+  const int64_t seen = p->window == 0 ? q_tiles : (int64_t{tile} + p->window) / q_tile + 1;
+  const int64_t steps = std::min<int64_t>(seen, q_tiles) * G;  // of an ordinary tile
+  const int64_t ctas = int64_t{u.tiles} * p->H_kv * std::max(p->B, 1);
+  u.near_segs = static_cast<int>(std::clamp<int64_t>(std::min<int64_t>(2 * 148 / ctas, steps / 4), 1, 32));
+  if (p->window == 0 || p->sinks == 0) return u;
   const int64_t last = std::min(tile, p->n_k) - 1;  // key of the first tile
   const int64_t near_end = std::clamp<int64_t>(last + p->window - p->q_start, 0, p->n_q);
   const int64_t far = (q_tiles - (near_end + q_tile - 1) / q_tile) * G;  // of the first tile, the most
-  const int64_t len = std::max<int64_t>(std::min<int64_t>((int64_t{tile} + p->window) / q_tile + 1, q_tiles) * G, 8);
+  const int64_t len = std::max<int64_t>(steps / u.near_segs, 8);
   if (far < 2 * len) return u;
   u.sink_tiles = static_cast<int>((std::min(p->sinks, p->n_k) + tile - 1) / tile);
   u.far_segs = static_cast<int>((far + len - 1) / len);
   u.far_len = static_cast<int>(len);
   return u;
+}
+size_t near_part_bytes(const dfs_attn_problem* p, const KeyUnits& u) {
+  return u.near_segs == 1 ? 0 : sizeof(float) * kTcRows * 128 * p->B * p->H_kv * u.tiles * u.near_segs;
 }
 size_t sink_part_bytes(const dfs_attn_problem* p, const KeyUnits& u) {
   return sizeof(float) * 128 * static_cast<size_t>(std::min<int>(p->sinks, kTcRows)) * p->B * p->H_kv * u.sink_tiles *
@@ -139,7 +149,7 @@ extern "C" int dfs_window_attn_fwd(const dfs_attn_problem* p, const dfs_attn_arg
 extern "C" size_t dfs_window_attn_bwd_work(const dfs_attn_problem* p, const dfs_relbias* b) {
   if (problem_status(p, b) != DFS_OK) return 0;
   const KeyUnits u = key_units(p, kTcRows, kTcHalf);
-  size_t n = dsum_bytes(p) + round256(sink_part_bytes(p, u));
+  size_t n = dsum_bytes(p) + round256(sink_part_bytes(p, u)) + near_part_bytes(p, u);
   if (b && b->weight) {
     const int units = std::max(u.count(), key_units(p, kSimtTile, 0).count());  // whichever kernels run
     n += sizeof(float) * static_cast<size_t>(p->H) * p->B * units * (2 * b->max_distance + 1);
@@ -169,9 +179,12 @@ extern "C" int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_arg
   P.sink_tiles = u.sink_tiles;
   P.far_segs = u.far_segs;
   P.far_len = u.far_len;
+  P.near_segs = u.near_segs;
   char* at = static_cast<char*>(work) + dsum_bytes(p);
   P.sink_part = reinterpret_cast<float*>(at);
-  if (dw) P.dw_part = reinterpret_cast<float*>(at + round256(sink_part_bytes(p, u)));
+  at += round256(sink_part_bytes(p, u));
+  P.near_part = reinterpret_cast<float*>(at);
+  if (dw) P.dw_part = reinterpret_cast<float*>(at + near_part_bytes(p, u));
   if (p->n_q > 0 || p->n_k > 0) {
     const bool vec = vector_rows(p, a) && staged(a->q, p->n_q, p->H, p->B, 4) && staged(a->d_o, p->n_q, p->H, p->B, 4);
     const int r = rc(tc ? launch_attn_tc_bwd(P, p->dtype, st) : launch_attn_simt_bwd(P, p->dtype, vec, st));

@@ -21,7 +21,9 @@ struct AttnParams {
   const int32_t* lut;   // (2 D + 1)
   float* dw_part;       // (H, parts, 2 D + 1) sums of dS by distance, or null
   float* sink_part;     // fp32 parts of the sink keys' gradients, or null
+  float* near_part;     // fp32 parts of key tiles' gradients, or null
   int sink_tiles, far_segs, far_len;  // key tiles that hold sinks; segments of queries beyond the window, steps of each
+  int near_segs;        // segments of every key tile's other steps
   int32_t* status;
   const int32_t* lengths;  // decode: (B,)
   int nb, D, wdtype;

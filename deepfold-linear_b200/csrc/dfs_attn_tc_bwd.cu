@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
   // only; without them those tiles' CTAs would walk every query tile), then the key tiles.
   const int far_units = P.sink_tiles * P.far_segs;
   const bool far_unit = unit < far_units;
-  const int tile = far_unit ? unit / P.far_segs : unit - far_units, j0 = tile * kTcRows;
+  const int near = unit - far_units, tile = far_unit ? unit / P.far_segs : near / P.near_segs, j0 = tile * kTcRows;
   const int sink_rows = P.far_segs > 0 ? min(max(P.sinks - j0, 0), kTcRows) : 0;  // rows that are joined afterwards
   bool err = false;
 
@@ -376,8 +376,9 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
     i_hi = (P.nq + kTcHalf - 1) / kTcHalf;
   }
   const int per = max(0, i_hi - i_lo);
-  const int first = far_unit ? min(unit % P.far_segs * P.far_len, per * P.G) : 0;
-  const int last = far_unit ? min(first + P.far_len, per * P.G) : per * P.G;
+  const int len = far_unit ? P.far_len : (per * P.G + P.near_segs - 1) / P.near_segs;
+  const int first = min((far_unit ? unit % P.far_segs : near % P.near_segs) * len, per * P.G);
+  const int last = min(first + len, per * P.G);
 
   if (warp >= kMmaWarp) {
     regs_down<kOtherRegs>();  // one instruction for the whole warpgroup
@@ -686,7 +687,18 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
           tmem_wait_ld(v);
         }
         if (j >= P.nk) continue;
-        if (row < sink_rows) {
+        if (!far_unit && P.near_segs > 1) {
+          // joined in 32 bits: [key head][key tile][segment][row][dV, dK][64]
+          const size_t head = static_cast<size_t>(b) * P.Hkv + hk, per_head = (P.nk + kTcRows - 1) / kTcRows * P.near_segs;
+          float* dst = P.near_part + ((head * per_head + near) * kTcRows + row) * 128 + 64 * which + c0;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            if (c0 + e < P.d)
+              *reinterpret_cast<float4*>(dst + e) =
+                  t > 0 ? make_float4(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), __uint_as_float(v[e + 2]),
+                                      __uint_as_float(v[e + 3]))
+                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        } else if (row < sink_rows) {
           // joined in 32 bits: [key head][sink tile][key tile, segments][sink row][dV, dK][64]
           const size_t seg = far_unit ? unit % P.far_segs + 1 : 0;
           float* dst = P.sink_part +
@@ -708,24 +720,43 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
   if (warp == kMmaWarp) tmem_dealloc(S.tmem, 256);
 }
 
-// Joins a sink row's parts (the key tile's own and the far segments', in order).
-// grid (sink tiles, key heads, batch), a thread per value of a row at a time.
+// Joins the parts of a row's dV and dK in order: those of its tile's segments, and a sink's far segments (where
+// tiles have one segment, sinks' own tiles are part 0 of the latter).  grid (32 rows each, key heads, batch), four
+// values of a row a thread at a time.
+constexpr int kJoinRows = 32;
 template <bool BF16>
-__global__ void __launch_bounds__(256) sink_join_kernel(AttnParams P) {
+__global__ void __launch_bounds__(256) join_kernel(AttnParams P) {
   wait_previous();
   allow_next();
-  const int tile = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, j0 = tile * kTcRows;
-  const int rows = min(min(P.sinks, P.nk) - j0, kTcRows), pitch = min(P.sinks, kTcRows) * 128;
-  const float* src = P.sink_part +
-                     ((static_cast<size_t>(b) * P.Hkv + hk) * P.sink_tiles + tile) * (P.far_segs + 1) * pitch;
-  for (int x = threadIdx.x; x < rows * 128; x += 256) {
-    const int row = x / 128, which = x % 128 / 64, c = x % 64;
-    if (c >= P.d) continue;
-    float s = 0.0f;
+  const int tile = blockIdx.x / (kTcRows / kJoinRows), r0 = blockIdx.x % (kTcRows / kJoinRows) * kJoinRows;
+  const int hk = blockIdx.y, b = blockIdx.z, j0 = tile * kTcRows, tiles = (P.nk + kTcRows - 1) / kTcRows;
+  const size_t head = static_cast<size_t>(b) * P.Hkv + hk;
+  const bool near = P.near_segs > 1;
+  const int sinks = tile < P.sink_tiles ? min(min(P.sinks, P.nk) - j0, kTcRows) : 0;
+  const int rows = near ? min(P.nk - j0, kTcRows) : sinks, pitch = min(P.sinks, kTcRows) * 128;
+  const float* np = P.near_part + (head * tiles + tile) * P.near_segs * (kTcRows * 128);
+  const float* sp = P.sink_part + (head * P.sink_tiles + tile) * (P.far_segs + 1) * pitch;
+  for (int x = threadIdx.x; x < kJoinRows * 32; x += 256) {
+    const int row = r0 + x / 32, which = x % 32 / 16, c = x % 16 * 4;
+    if (row >= rows || c >= P.d) continue;
+    const int at = row * 128 + 64 * which + c;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](const float* part) {
+      const float4 v = *reinterpret_cast<const float4*>(part + at);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    };
+    if (near) {
+#pragma unroll 4
+      for (int k = 0; k < P.near_segs; ++k) add(np + static_cast<size_t>(k) * (kTcRows * 128));
+    }
+    if (row < sinks) {
 #pragma unroll 8
-    for (int k = 0; k <= P.far_segs; ++k) s += src[static_cast<size_t>(k) * pitch + x];
+      for (int k = near; k <= P.far_segs; ++k) add(sp + static_cast<size_t>(k) * pitch);
+    }
     using T16 = typename E16<BF16>::T;
-    row_ptr<T16>(which ? P.d_k : P.d_v, b, hk, j0 + row)[c] = from_f32<T16>(which ? s * P.scale : s);
+    const float mul = which ? P.scale : 1.0f;
+    T16* out = row_ptr<T16>(which ? P.d_k : P.d_v, b, hk, j0 + row) + c;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack16<BF16>(s.x * mul, s.y * mul), pack16<BF16>(s.z * mul, s.w * mul));
   }
 }
 
@@ -751,10 +782,11 @@ static cudaError_t launch_bwd(const AttnParams& P, cudaStream_t st) {
   e = launch_dependent(tc_dq_kernel<BF16>, tc_grid(P.nq, P.H, P.B), kBwdThreads, smem, st, T);
   if (e != cudaSuccess) return e;
   if (!maps(kTcHalf, kTcRows)) return cudaErrorInvalidValue;
-  const unsigned units = (P.nk + kTcRows - 1) / kTcRows + P.sink_tiles * P.far_segs;
+  const unsigned tiles = (P.nk + kTcRows - 1) / kTcRows, units = tiles * P.near_segs + P.sink_tiles * P.far_segs;
   e = launch_dependent(tc_dkv_kernel<BF16>, units * P.Hkv * P.B, kBwdThreads, smem, st, T);
-  if (e != cudaSuccess || P.far_segs == 0) return e;
-  return launch_dependent(sink_join_kernel<BF16>, dim3(P.sink_tiles, P.Hkv, P.B), 256, 0, st, P);
+  const unsigned joined = P.near_segs > 1 ? tiles : P.sink_tiles;
+  if (e != cudaSuccess || joined == 0) return e;
+  return launch_dependent(join_kernel<BF16>, dim3(joined * (kTcRows / kJoinRows), P.Hkv, P.B), 256, 0, st, P);
 }
 
 cudaError_t launch_attn_tc_bwd(const AttnParams& P, int dtype, cudaStream_t st) {

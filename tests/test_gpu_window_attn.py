@@ -389,3 +389,17 @@ def test_decode_of_one_long_sequence(dtype):
     want = orc.window_attn(f64(x["q"]), f64(x["k"][:, :, :4990]), f64(x["v"][:, :, :4990]), weight=f64(x["w"]),
                            table=BUCKETS["log"].table)
     close(got[:, :, None], want, dtype, 2)
+
+
+@pytest.mark.parametrize("causal,window,sinks,n,H,H_kv,d", [
+    (True, None, 0, 900, 8, 1, 64),       # one key head: its tiles' steps are spread over many blocks
+    (True, 150, 5, 1600, 8, 1, 40),       # with the sinks' far queries apart
+    (False, 64, 140, 1100, 6, 1, 32),     # sinks over two key tiles, the keys' last tile ragged
+])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gradients_of_few_key_heads(causal, window, sinks, n, H, H_kv, d, dtype):
+    x = inputs(1, H, H_kv, n, n, d, dtype, 37, "bnhd", 32)
+    mask = prefix_mask([n - 130], n) if sinks == 5 else None
+    _, first = check(x, dtype, BUCKETS["log"], mask, causal=causal, window=window, sinks=sinks)
+    _, again = check(x, dtype, BUCKETS["log"], mask, causal=causal, window=window, sinks=sinks)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
