@@ -471,30 +471,6 @@ int split_of(const AttnParams& P, int chunks, int resident) {
   return split == 8 && 16 * problems <= 2 * 148 && 16 <= tiles ? 16 : split;
 }
 
-template <typename... A>
-cudaError_t launch_split(void (*kern)(A...), int split, int heads, int B, int threads, size_t smem, cudaStream_t st,
-                         const A&... args) {
-  if (split > 8) {  // beyond what every device has: opted in
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(split, heads, B);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = split;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kern, args...);
-}
-
 template <typename E>
 cudaError_t launch(const AttnParams& P, cudaStream_t st) {
   DecodeParams T;
@@ -508,14 +484,15 @@ cudaError_t launch(const AttnParams& P, cudaStream_t st) {
                       (P.w ? std::min(P.G, kHeads) * (P.D + 1) * sizeof(float) : 0);
   const cudaError_t e = prepare_kernel<decode_mma_kernel<E>>(smem);
   if (e != cudaSuccess) return e;
-  return launch_split(decode_mma_kernel<E>, T.split, P.Hkv * T.chunks, P.B, kThreads, smem, st, T);
+  return launch_clusters(decode_mma_kernel<E>, dim3(T.split, P.Hkv * T.chunks, P.B), T.split, kThreads, smem, st, T);
 }
 
 template <typename E, bool kVec>
 cudaError_t launch_any(const AttnParams& P, cudaStream_t st) {
   const int chunks = (P.G + kAnyHeads - 1) / kAnyHeads, split = split_of(P, chunks, 4);
   const size_t smem = P.w ? kAnyHeads * (P.D + 1) * sizeof(float) : 0;
-  return launch_split(decode_any_kernel<E, kVec>, split, P.Hkv * chunks, P.B, kAnyThreads, smem, st, P, split, chunks);
+  return launch_clusters(decode_any_kernel<E, kVec>, dim3(split, P.Hkv * chunks, P.B), split, kAnyThreads, smem, st, P,
+                         split, chunks);
 }
 
 }  // namespace

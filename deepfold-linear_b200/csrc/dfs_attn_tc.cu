@@ -11,6 +11,7 @@
 // At d <= 64 the exponentials bound it (8192 a tile at 16 a clock: 512 clocks, the
 // two products 320), if the chain S -> P -> O of one tile after the other does not:
 // so the tiles are narrow (64 + 64 TMEM columns), and four CTAs share an SM.
+#include <algorithm>
 #include <type_traits>
 
 #include "dfs_attn_tc.cuh"
@@ -41,7 +42,17 @@ struct FwdShared {
 // TMEM columns (128 allocated): S, and P over its first half; O
 constexpr uint32_t kColS = 0, kColO = 64;
 
-template <bool BF16>
+// Parts of a tile whose keys a cluster shares, over the staged tiles once all products are done
+constexpr int kPartPitch = 68;
+struct FwdPart {
+  float o[kTcRows * kPartPitch];  // not normalised
+  float m[kTcRows], l[kTcRows];
+};
+static_assert(sizeof(FwdPart) <= kTcTileBytes + 2 * kStages * kHalfBytes, "parts over the staged tiles");
+
+// kSplit: a cluster of T.split CTAs shares each tile of queries, a run of the key tiles for each, joined in order
+// through distributed shared memory.
+template <bool BF16, bool kSplit>
 __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_constant__ TcParams T) {
   extern __shared__ unsigned char raw[];
   const AttnParams& P = T.a;
@@ -51,8 +62,10 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
   FwdShared& S = *reinterpret_cast<FwdShared*>(gen + kTcTileBytes + 2 * kStages * kHalfBytes);
   float* tab = reinterpret_cast<float*>(&S + 1);
   const int warp = warp_index(), lane = threadIdx.x % 32;
-  const int h = blockIdx.x % P.H, b = blockIdx.x / P.H % P.B, hk = h / P.G;
-  const int i0 = ((P.nq - 1) / kTcRows - static_cast<int>(blockIdx.x / P.H / P.B)) * kTcRows;  // causal: longest first
+  const int split = kSplit ? T.split : 1, rank = blockIdx.x % split;
+  const unsigned unit = blockIdx.x / split;
+  const int h = unit % P.H, b = unit / P.H % P.B, hk = h / P.G;
+  const int i0 = ((P.nq - 1) / kTcRows - static_cast<int>(unit / P.H / P.B)) * kTcRows;  // causal: longest first
   const int p0 = i0 + P.qs;
   bool err = false;
   if (warp >= kMmaWarp) {
@@ -79,11 +92,11 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
         tma_load_4d(sQ, &T.q, 0, i0, h, b, smem_u32(&S.q_full));
       }
       const PlainTiles<4, 2> plain(P);
-      const int count = tiles.count();
+      const int count = tiles.count(), x1 = count * (rank + 1) / split;
       uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
       int t = 0;
-      for (int x = 0; x <= count; ++x) {
-        const int j0 = x < count ? tiles[x] * kTcHalf : -1;
+      for (int x = count * rank / split; x <= x1; ++x) {
+        const int j0 = x < x1 ? tiles[x] * kTcHalf : -1;
         if (j0 >= 0 && mask != nullptr) {
           key_bits(mask, j0, P.nk, lane, bits);
           if ((bits[0] | bits[1]) == 0) continue;
@@ -156,6 +169,11 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
       }
     } else {  // ---- the warpgroup's idle warps
       setup_wait<kFwdThreads>();
+    }
+    if (kSplit) {
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
     }
   } else {  // ---- elements: a query row per thread
     setup_wait<kFwdThreads>();
@@ -272,8 +290,58 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
     const bool none = !(total > kNone) && total == total;
     const float inv = 1.0f / total;
     using E16 = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+    if (kSplit) {
+      FwdPart& part = *reinterpret_cast<FwdPart*>(gen);
 #pragma unroll
-    for (int c0 = 0; c0 < 64; c0 += 32) {
+      for (int c0 = 0; c0 < 64; c0 += 32) {
+        if (c0 >= P.d) break;
+        uint32_t o[32] = {};
+        if (t > 0) {
+          tmem_ld32_async(tm + lanes + kColO + c0, o);
+          tmem_wait_ld(o);
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+          *reinterpret_cast<uint4*>(&part.o[row * kPartPitch + c0 + e]) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+      }
+      part.m[row] = m;
+      part.l[row] = total;
+      __syncwarp();
+      cluster_sync();
+      const int rows = kTcRows / split, r0 = rank * rows;  // this CTA's share of the rows
+      for (int x = threadIdx.x; x < rows * 16; x += 128) {
+        const int r = r0 + x / 16, c = x % 16 * 4, at = i0 + r;
+        if (at >= P.nq || c >= P.d) continue;
+        const uint32_t am = smem_u32(&part.m[r]), al = smem_u32(&part.l[r]), ao = smem_u32(&part.o[r * kPartPitch + c]);
+        float top = -INFINITY, sum = 0.0f;
+        for (int k = 0; k < split; ++k) top = fmaxf(top, dsmem_ld(dsmem_addr(am, k)));
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = 0; k < split; ++k) {
+          const float f = ex2(dsmem_ld(dsmem_addr(am, k)) - ref);
+          const float4 v = dsmem_ld4(dsmem_addr(ao, k));
+          sum = fmaf(dsmem_ld(dsmem_addr(al, k)), f, sum);
+          acc = make_float4(fmaf(v.x, f, acc.x), fmaf(v.y, f, acc.y), fmaf(v.z, f, acc.z), fmaf(v.w, f, acc.w));
+        }
+        const bool empty = !(sum > kNone) && sum == sum;
+        const float g = empty ? 0.0f : 1.0f / sum;
+        acc = make_float4(acc.x * g, acc.y * g, acc.z * g, acc.w * g);
+        const uint2 out = make_uint2(pack16<BF16>(acc.x, acc.y), pack16<BF16>(acc.z, acc.w));
+        E16* dst = row_ptr<E16>(P.o, b, h, at) + c;
+        *reinterpret_cast<uint2*>(dst) = out;
+        if (P.o_lo) {
+          const float2 lo = unpack16<BF16>(out.x), hi = unpack16<BF16>(out.y);
+          *reinterpret_cast<uint2*>(reinterpret_cast<E16*>(P.o_lo) + (dst - reinterpret_cast<E16*>(P.o.p))) =
+              make_uint2(pack16<BF16>(acc.x - lo.x, acc.y - lo.y), pack16<BF16>(acc.z - hi.x, acc.w - hi.y));
+        }
+        if (P.lse && c == 0)
+          P.lse[(static_cast<size_t>(b) * P.H + h) * P.nq + at] = empty ? INFINITY : top + lg2(sum);
+      }
+      __syncwarp();
+      cluster_sync();  // nobody leaves while its memory is read
+    }
+#pragma unroll
+    for (int c0 = 0; c0 < 64 && !kSplit; c0 += 32) {
       if (c0 >= P.d) break;
       uint32_t o[32];
       if (t > 0) {  // warp-collective
@@ -300,7 +368,7 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
           }
       }
     }
-    if (P.lse && i < P.nq)
+    if (!kSplit && P.lse && i < P.nq)
       P.lse[(static_cast<size_t>(b) * P.H + h) * P.nq + i] = none ? INFINITY : m + lg2(total);
   }
   if (err) report_timeout(P.status);
@@ -322,16 +390,26 @@ cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st) 
   T.a = P;
   const size_t smem = 1024 + kTcTileBytes + 2 * kStages * kHalfBytes + sizeof(FwdShared) + bias_ext_bytes(P);
   const int share = 128 * kElementRegs + 128 * kOtherRegs;
+  // Few queries over many keys: a cluster of CTAs shares them, until every SM has four and while each has four tiles
+  // (bfloat16, d = 64: 5 queries of 16 heads over 8192 keys 110 -> 28 us, 8 heads of 1024 18.6 -> 15.6)
   const unsigned grid = tc_grid(P.nq, P.H, P.B);
-  const cudaError_t e = bf16 ? prepare_kernel<tc_fwd_kernel<true>>(smem, kFwdThreads, share)
-                             : prepare_kernel<tc_fwd_kernel<false>>(smem, kFwdThreads, share);
-  if (e != cudaSuccess) return e;
-  if (!tc_tmap(&T.q, P.q, bf16, P.d, P.nq, P.H, P.B) ||
-      !tc_tmap(&T.k, P.k, bf16, P.d, P.nk, P.Hkv, P.B, kTcHalf) ||
-      !tc_tmap(&T.v, P.v, bf16, P.d, P.nk, P.Hkv, P.B, kTcHalf))
-    return cudaErrorInvalidValue;
-  T.d_o = T.q;
-  return launch_dependent(bf16 ? tc_fwd_kernel<true> : tc_fwd_kernel<false>, grid, kFwdThreads, smem, st, T);
+  const int64_t seen = std::min<int64_t>(P.nk, int64_t{P.window} * (P.causal ? 1 : 2) + kTcRows + P.sinks) / kTcHalf;
+  T.split = 1;
+  while (T.split < 8 && 2u * T.split * grid <= 4 * 148 && 8 * T.split <= seen) T.split *= 2;
+  auto run = [&](auto kern, cudaError_t e) {
+    if (e != cudaSuccess) return e;
+    if (!tc_tmap(&T.q, P.q, bf16, P.d, P.nq, P.H, P.B) ||
+        !tc_tmap(&T.k, P.k, bf16, P.d, P.nk, P.Hkv, P.B, kTcHalf) ||
+        !tc_tmap(&T.v, P.v, bf16, P.d, P.nk, P.Hkv, P.B, kTcHalf))
+      return cudaErrorInvalidValue;
+    T.d_o = T.q;
+    return launch_clusters(kern, grid * T.split, T.split, kFwdThreads, smem, st, T);
+  };
+  if (T.split > 1)
+    return bf16 ? run(tc_fwd_kernel<true, true>, prepare_kernel<tc_fwd_kernel<true, true>>(smem, kFwdThreads, share))
+                : run(tc_fwd_kernel<false, true>, prepare_kernel<tc_fwd_kernel<false, true>>(smem, kFwdThreads, share));
+  return bf16 ? run(tc_fwd_kernel<true, false>, prepare_kernel<tc_fwd_kernel<true, false>>(smem, kFwdThreads, share))
+              : run(tc_fwd_kernel<false, false>, prepare_kernel<tc_fwd_kernel<false, false>>(smem, kFwdThreads, share));
 }
 
 }  // namespace dfs

@@ -16,6 +16,7 @@ constexpr int kTcHalf = 64;               // rows of the tiles it walks
 struct TcParams {
   CUtensorMap q, k, v, d_o;
   AttnParams a;
+  int split = 1;  // CTAs that share a tile of queries
 };
 
 // instruction descriptor, kind::f16; b_mn: B is stored with its N index contiguous
@@ -63,6 +64,12 @@ DFS_DEV bool elect_one() {
   asm volatile(
       "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
+}
+DFS_DEV float4 dsmem_ld4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
 }
 DFS_DEV int warp_index() { return __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x / 32), 0); }
 
@@ -341,6 +348,31 @@ cudaError_t prepare_kernel(size_t smem, int threads = 0, int share = 0) {
   e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e == cudaSuccess && dev < kMaxDevices) ready[dev].store(smem, std::memory_order_relaxed);
   return e;
+}
+
+// A dependent launch (launch_dependent) whose blocks come in clusters of `size` along x.
+template <typename... Params, typename... Args>
+cudaError_t launch_clusters(void (*kern)(Params...), dim3 grid, int size, int threads, size_t smem, cudaStream_t st,
+                            const Args&... args) {
+  if (size > 8) {  // beyond what every device has: opted in
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = size;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = size > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
 cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st);

@@ -403,3 +403,27 @@ def test_gradients_of_few_key_heads(causal, window, sinks, n, H, H_kv, d, dtype)
     _, first = check(x, dtype, BUCKETS["log"], mask, causal=causal, window=window, sinks=sinks)
     _, again = check(x, dtype, BUCKETS["log"], mask, causal=causal, window=window, sinks=sinks)
     assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("causal,window,sinks,n_q,n_k,H,H_kv,d", [
+    (True, None, 0, 5, 3001, 4, 2, 64),      # a few new tokens over a long past
+    (True, None, 3, 1, 2048, 2, 2, 40),
+    (True, 900, 4, 200, 4000, 3, 1, 32),
+    (False, 700, 0, 130, 2100, 2, 2, 64),
+    (True, None, 0, 1000, 1000, 1, 1, 64),   # the first tiles have fewer keys than there are blocks
+])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_few_queries_over_many_keys(causal, window, sinks, n_q, n_k, H, H_kv, d, dtype):
+    x = inputs(2, H, H_kv, n_q, n_k, d, dtype, 41, "bnhd", 32)
+    mask = prefix_mask([n_k, n_k // 3], n_k)
+    if n_q > 1:
+        mask[1, :n_k // 4] = False
+    check(x, dtype, BUCKETS["log"], mask, causal=causal, window=window, sinks=sinks)
+    check(x, dtype, BUCKETS["log"], None, causal=causal, window=window, sinks=sinks, grad=False)
+
+
+def test_few_queries_that_see_nothing():
+    x = inputs(1, 2, 1, 40, 2048, 64, BF16, 43, nb=32)
+    mask = torch.zeros(1, 2048, dtype=torch.bool, device="cuda")
+    o, grads = check(x, BF16, BUCKETS["log"], mask, causal=True)
+    assert (o == 0).all() and all((g == 0).all() for g in grads)
