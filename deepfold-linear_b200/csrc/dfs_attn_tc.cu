@@ -9,8 +9,14 @@
 // nothing for a block of 32 x 32 pairs that are all hidden.
 //
 // At d <= 64 the exponentials bound it (8192 a tile at 16 a clock: 512 clocks, the
-// two products 320), if the chain S -> P -> O of one tile after the other does not:
-// so the tiles are narrow (64 + 64 TMEM columns), and four CTAs share an SM.
+// two products 320), if the chain S -> P -> O of one tile after the other does not
+// (1600 clocks for a CTA alone): so the tiles are narrow (64 + 64 TMEM columns), and
+// four CTAs share an SM.  Measured (bfloat16, d = 64): 8192 tokens of 16 / 4 heads,
+// window 4096, 155 us, 660 TFLOP/s, an exponential pipe 60 % busy; 8 x 1024 of 16
+// heads, window 256 in both directions, 32 us.  Slower at the same sizes: 128-key
+// tiles with 256 or 512 threads, two S buffers and two CTAs an SM (155 to 170 us),
+// part of the exponentials as a polynomial on the FMA pipes, and long rows shared by
+// CTAs where the grid fills the GPU anyway (171 us).
 #include <algorithm>
 #include <type_traits>
 

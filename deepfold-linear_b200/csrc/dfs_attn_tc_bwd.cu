@@ -20,6 +20,14 @@
 // (a TMEM row and half of a tile's columns per thread: blocks of 32 x 32 per warp,
 // skipped where all is hidden), warp 8 issues the MMAs, warp 9 stages tiles by TMA
 // and announces them.
+//
+// Measured (bfloat16, d = 64, 8192 tokens of 16 heads, window 1024, a bias): dQ pass
+// 95 us, dK/dV pass 143 us, together 340 TFLOP/s of the 10 d a visible pair needs.
+// No pipe is more than half busy; a tile's chain through TMEM is what is waited for,
+// and TMEM holds two CTAs' accumulators.  (dK/dV with one CTA an SM, two groups of
+// element warps and three buffers: 20 us slower.)  Where few key heads would leave
+// SMs idle, the key pass spreads a tile's steps over CTAs and joins them in 32 bits
+// (16 / 2 heads of 2048 tokens: 351 -> 108 us).
 #include <type_traits>
 
 #include "dfs_attn_tc.cuh"

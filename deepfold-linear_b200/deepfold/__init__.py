@@ -1,10 +1,14 @@
 """B200-native drop-in for the flash-Sinkhorn path of DeepFold-Linear.
 
-Mirrors the reference package layout for that path only:
+Mirrors the reference package layout for that path, with local attention beside it:
 
 * ``deepfold.model.kernels.flash_sinkhorn_attn.flash_sinkhorn_attn``
 * ``deepfold.model.kernels.sinkhorn_kernel.flash_sinkhorn``
 * ``deepfold.model.sinkhorn.sinkhorn_solve``
+* ``deepfold.model.kernels.flash_window_attn.flash_window_attn`` /
+  ``window_attn_decode`` and ``deepfold.model.position_encoding.
+  relative_position_bias`` -- local softmax attention and its position bias
+  (no counterpart in the reference)
 * ``deepfold.utils.cg.conjugate_gradient`` / ``steihaug_cg``
 * ``deepfold.sharding`` -- multi-GPU (batch, head) and row sharding
 

@@ -1,1 +1,1 @@
-"""Sinkhorn attention operators backed by libdfsink.so."""
+"""Sinkhorn and local attention operators backed by libdfsink.so."""

@@ -464,7 +464,8 @@ typedef struct {
   /* backward only: gradients of o (in) and of q, k, v, bias.weight (out; d_weight may be NULL) */
   dfs_strided d_o, d_q, d_k, d_v;
   void* d_weight;
-  int32_t* status;         /* device int32, error bits OR-ed in; or NULL                        */
+  int32_t* status;         /* int32 that the device can write (mapped host memory will do): a      */
+                           /* bounded wait that gave up stores DFS_ERR_DEVICE_TIMEOUT; or NULL    */
 } dfs_attn_args;
 
 int dfs_window_attn_fwd(const dfs_attn_problem* p, const dfs_attn_args* a, void* stream);
