@@ -93,9 +93,11 @@ KeyUnits key_units(const dfs_attn_problem* p, int tile, int q_tile) {
   const int64_t last = std::min(tile, p->n_k) - 1;  // key of the first tile
   const int64_t near_end = std::clamp<int64_t>(last + p->window - p->q_start, 0, p->n_q);
   const int64_t far = (q_tiles - (near_end + q_tile - 1) / q_tile) * G;  // of the first tile, the most
-  const int64_t len = std::max<int64_t>(steps / u.near_segs, 8);
+  const int64_t sink_tiles = (std::min(p->sinks, p->n_k) + tile - 1) / tile;
+  // (with many sinks longer ones, so that their parts are no more than the key tiles)
+  const int64_t len = std::max<int64_t>({steps / u.near_segs, 8, (far * sink_tiles + u.tiles - 1) / u.tiles});
   if (far < 2 * len) return u;
-  u.sink_tiles = static_cast<int>((std::min(p->sinks, p->n_k) + tile - 1) / tile);
+  u.sink_tiles = static_cast<int>(sink_tiles);
   u.far_segs = static_cast<int>((far + len - 1) / len);
   u.far_len = static_cast<int>(len);
   return u;

@@ -427,3 +427,44 @@ def test_few_queries_that_see_nothing():
     mask = torch.zeros(1, 2048, dtype=torch.bool, device="cuda")
     o, grads = check(x, BF16, BUCKETS["log"], mask, causal=True)
     assert (o == 0).all() and all((g == 0).all() for g in grads)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_every_key_is_a_sink(dtype):
+    """Sinks over all key tiles: their far queries outnumber the near ones everywhere."""
+    n = 1900
+    x = inputs(1, 2, 1, n, n, 32, dtype, 47, nb=32)
+    check(x, dtype, BUCKETS["log"], causal=True, window=16, sinks=n)
+
+
+def test_captured_in_a_graph():
+    """A decoding step, and a forward with gradients, replayed on new inputs."""
+    x = inputs(2, 4, 2, 260, 260, 64, BF16, 53, nb=32)
+    kw = dict(window=100, sinks=4, buckets=BUCKETS["log"])
+    q, k, v, w = (x[n].detach().clone().requires_grad_() for n in ("q", "k", "v", "w"))
+    lengths = torch.tensor([260, 31], device="cuda", dtype=torch.int32)
+
+    def work():
+        with torch.no_grad():
+            one = window_attn_decode(q[:, :, 0], k, v, lengths, pos_weight=w, **kw)
+            few = flash_window_attn(q[:, :, :3], k, v, causal=False, pos_weight=w, **kw)
+        o = flash_window_attn(q, k, v, pos_weight=w, **kw)
+        return (one, few, o.detach(), *torch.autograd.grad(o, (q, k, v, w), x["d_o"]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    fresh = inputs(2, 4, 2, 260, 260, 64, BF16, 54, nb=32)
+    with torch.no_grad():
+        for t, n in ((q, "q"), (k, "k"), (v, "v"), (w, "w")):
+            t.copy_(fresh[n])
+        lengths.copy_(torch.tensor([7, 200]))
+    graph.replay()
+    got = [t.clone() for t in got]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, work()))
+    del graph

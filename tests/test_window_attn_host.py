@@ -152,3 +152,15 @@ def test_python_surface_refuses_on_the_host():
         relative_position_bias(torch.zeros(2, 64), [0, 1, 2], 4, 4)
     with pytest.raises(ValueError):
         relative_position_bias(torch.zeros(2, 65), RelativeBuckets.clip(), -1, 4)
+
+
+@pytest.mark.parametrize("n,window,sinks,H,H_kv,B", [
+    (65536, 16, 65536, 16, 16, 1), (65536, 16, 4, 16, 2, 1), (65536, 0, 0, 16, 16, 2), (2048, 0, 0, 32, 1, 1),
+    (20000, 1, 300, 8, 8, 3)])
+def test_backward_workspace_stays_in_proportion(n, window, sinks, H, H_kv, B):
+    """At most a float a query and, where blocks share key tiles, 1 KB a key and block (sinks: a block more at most
+    per key tile; few key heads: up to two blocks an SM)."""
+    p = attn(B=B, H=H, H_kv=H_kv, n_q=n, n_k=n, d=64, window=window, sinks=sinks)
+    work = nat.lib().dfs_window_attn_bwd_work(p, None)
+    sink_rows = min(sinks, 128) * (n // 128 + min(sinks, n) // 128 + 2) * B * H_kv
+    assert 4 * B * H * n <= work <= 4 * B * H * n + 512 * sink_rows + 2 * 148 * 128 * 512 + 1024
