@@ -367,7 +367,8 @@ __global__ void __launch_bounds__(kNT, 2) simt_dkv_kernel(AttnParams P) {
 #pragma unroll
         for (int r = 0; r < kR; ++r) {
           const int j = j0 + ty + 8 * r;
-          const float x = side != 0 ? fmaf(p[r][c], P.scale2, far) : logit2(P, P.w ? tab : nullptr, mask, p[r][c], i, j);
+          const float x =
+              side != 0 ? fmaf(p[r][c], P.scale2, far) : logit2(P, P.w ? tab : nullptr, mask, p[r][c], i, j);
           p[r][c] = exp2f(x - ls);
           Pt[(ty + 8 * r) * kLd + tx + 16 * c] = p[r][c];
         }

@@ -308,7 +308,8 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
         }
 #pragma unroll
         for (int e = 0; e < 32; e += 4)
-          *reinterpret_cast<uint4*>(&part.o[row * kPartPitch + c0 + e]) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          *reinterpret_cast<uint4*>(&part.o[row * kPartPitch + c0 + e]) =
+              make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
       }
       part.m[row] = m;
       part.l[row] = total;

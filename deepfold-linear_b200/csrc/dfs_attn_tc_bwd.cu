@@ -697,8 +697,9 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
         if (j >= P.nk) continue;
         if (!far_unit && P.near_segs > 1) {
           // joined in 32 bits: [key head][key tile][segment][row][dV, dK][64]
-          const size_t head = static_cast<size_t>(b) * P.Hkv + hk, per_head = (P.nk + kTcRows - 1) / kTcRows * P.near_segs;
-          float* dst = P.near_part + ((head * per_head + near) * kTcRows + row) * 128 + 64 * which + c0;
+          const size_t per_head = static_cast<size_t>((P.nk + kTcRows - 1) / kTcRows) * P.near_segs;
+          float* dst = P.near_part + ((static_cast<size_t>(b) * P.Hkv + hk) * per_head + near) * (kTcRows * 128) +
+                       row * 128 + 64 * which + c0;
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
             if (c0 + e < P.d)

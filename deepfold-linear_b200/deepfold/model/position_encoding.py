@@ -23,6 +23,8 @@ current CUDA device and the result returned on the CPU (there is no CPU path).
 
 from __future__ import annotations
 
+from array import array
+
 import torch
 
 from deepfold import _native as nat
@@ -58,7 +60,7 @@ class RelativeBuckets:
     """
 
     def __init__(self, table, num_buckets: int | None = None, device=None):
-        table = [int(x) for x in table]
+        table = list(map(int, table))
         if len(table) % 2 != 1 or len(table) > 2 * nat.DFS_MAX_BUCKET_DISTANCE + 1:
             raise ValueError("table must list the buckets of -D .. D: an odd number of them, D up to "
                              f"{nat.DFS_MAX_BUCKET_DISTANCE}")
@@ -105,7 +107,7 @@ class RelativeBuckets:
         """The table as int32 on ``device``."""
         t = self._on.get(device)
         if t is None:
-            t = torch.tensor(self.table, dtype=torch.int32, device=device)
+            t = torch.frombuffer(array("i", self.table), dtype=torch.int32).to(device)  # quicker than from a list
             self._on[t.device] = self._on[device] = t
         return t
 
