@@ -645,19 +645,28 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
         continue;
       }
       // Diagonals of this warp's block of 32 keys x 32 queries: the running sum of a diagonal moves one lane up
-      // as the query advances, and is complete once lane 31 has added its element.
+      // as the query advances, and is complete once lane 31 has added its element.  Two chains, of the first and of
+      // the last 16 queries, halve the way of dependent shuffles; the first one's sums then go on where the
+      // second one's diagonals are.
       float* out = S.diag[strip][warp];
       float run = 0.0f;
       if (live) {
+        float up = 0.0f;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          run += __uint_as_float(dr[c]);
-          if (c < 31) {
-            if (lane == 31) out[c] = run;
+        for (int c = 0; c < 16; ++c) {
+          up += __uint_as_float(dr[c]);
+          run += __uint_as_float(dr[c + 16]);
+          if (c < 15) {
+            if (lane == 31) out[c] = up, out[c + 16] = run;
+            up = __shfl_up_sync(0xffffffffu, up, 1);
             run = __shfl_up_sync(0xffffffffu, run, 1);
-            if (lane == 0) run = 0.0f;
+            if (lane == 0) up = run = 0.0f;
           }
         }
+        __syncwarp();
+        if (lane >= 16) out[46 - lane] = lane == 31 ? up : out[46 - lane] + up;
+        up = __shfl_up_sync(0xffffffffu, up, 16);
+        if (lane >= 16) run += up;
       } else {
         out[lane] = 0.0f;  // slots 0..30 (slot 31 is lane 31's below)
         __syncwarp();
