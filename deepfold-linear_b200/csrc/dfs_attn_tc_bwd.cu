@@ -56,7 +56,7 @@ struct BwdShared {
   alignas(16) float stat[kStages][2][kTcHalf];  // dK/dV pass: -lse and -D of the stage's queries
   float part[2][kTcRows];           // dQ pass: a row's two partial sums
   float ends[2][kWork / 32];
-  float diag[2][kWork / 32][64];    // dK/dV pass: the diagonals of a warp's block, two tiles in turn
+  float diag[kWork / 32][32];       // dK/dV pass: diagonals of a warp's block that ended at lane 31
   uint32_t tmem;
 };
 
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
   BwdShared& S = *reinterpret_cast<BwdShared*>(gen + 2 * kTcTileBytes + 2 * kStages * kHalfBytes);
   float* tab = reinterpret_cast<float*>(&S + 1);
   const int W = 2 * P.D + 1;
-  float* acc = tab + (P.w ? 2 * bias_ext(P.D) + 1 : 0);  // W sums by distance
+  float* acc = tab + (P.w ? 2 * bias_ext(P.D) + 1 : 0);  // a table of W sums by distance for each element warp
   const int warp = warp_index(), lane = threadIdx.x % 32;
   const int hk = blockIdx.x % P.Hkv, b = blockIdx.x / P.Hkv % P.B, unit = blockIdx.x / P.Hkv / P.B;
   // Units: first the far segments of the sinks' tiles (the queries beyond their window, which see the sinks
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
     const int E = bias_ext(P.D);
     const bool dw = P.dw_part != nullptr;
     float lo = 0.0f, hi = 0.0f;  // sums of dS beyond the table's ends
-    int head = -1, strip = 0;
+    int head = -1;
     float far_hi = 0.0f, far_lo = 0.0f;
     auto dw_row = [&](int g) {
       return P.dw_part + (static_cast<size_t>(hk * P.G + g) * P.parts + b * (P.parts / P.B) + unit) * W;
@@ -523,7 +523,12 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
       }
       work_barrier();
       float* dst = dw_row(head);
-      for (int x = tid; x < W; x += kWork) dst[x] = acc[x];
+      for (int x = tid; x < W; x += kWork) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWork / 32; ++w) s += acc[w * W + x];
+        dst[x] = s;
+      }
       lo = hi = 0.0f;
     };
     // heads that have no tile here: their sums are zero
@@ -611,7 +616,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
         head = g;
         if (P.w) load_bias_ext(tab, P, hk * P.G + g, tid, kWork);
         if (dw)
-          for (int x = tid; x < W; x += kWork) acc[x] = 0.0f;
+          for (int x = tid; x < kWork / 32 * W; x += kWork) acc[x] = 0.0f;
         work_barrier();
         if (P.w) far_hi = tab[E + P.D], far_lo = tab[E - P.D];
       }
@@ -644,49 +649,38 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
         else lo += sum.x + sum.y;
         continue;
       }
+      if (!live) continue;
       // Diagonals of this warp's block of 32 keys x 32 queries: the running sum of a diagonal moves one lane up
       // as the query advances, and is complete once lane 31 has added its element.  Two chains, of the first and of
       // the last 16 queries, halve the way of dependent shuffles; the first one's sums then go on where the
-      // second one's diagonals are.
-      float* out = S.diag[strip][warp];
-      float run = 0.0f;
-      if (live) {
-        float up = 0.0f;
+      // second one's diagonals are.  The sums go to a table of this warp's own, while it would wait for the next
+      // tile's S: with one table and a join of the warps a tile, such tiles took half as long again.
+      float* out = S.diag[warp];
+      float up = 0.0f, run = 0.0f;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          up += __uint_as_float(dr[c]);
-          run += __uint_as_float(dr[c + 16]);
-          if (c < 15) {
-            if (lane == 31) out[c] = up, out[c + 16] = run;
-            up = __shfl_up_sync(0xffffffffu, up, 1);
-            run = __shfl_up_sync(0xffffffffu, run, 1);
-            if (lane == 0) up = run = 0.0f;
-          }
+      for (int c = 0; c < 16; ++c) {
+        up += __uint_as_float(dr[c]);
+        run += __uint_as_float(dr[c + 16]);
+        if (c < 15) {
+          if (lane == 31) out[c] = up, out[c + 16] = run;  // slot x + 31 for diagonal x = query - key of the block
+          up = __shfl_up_sync(0xffffffffu, up, 1);
+          run = __shfl_up_sync(0xffffffffu, run, 1);
+          if (lane == 0) up = run = 0.0f;
         }
-        __syncwarp();
-        if (lane >= 16) out[46 - lane] = lane == 31 ? up : out[46 - lane] + up;
-        up = __shfl_up_sync(0xffffffffu, up, 16);
-        if (lane >= 16) run += up;
-      } else {
-        out[lane] = 0.0f;  // slots 0..30 (slot 31 is lane 31's below)
-        __syncwarp();
       }
-      out[62 - lane] = run;  // slot x + 31 for diagonal x = query - key of the block
-      work_barrier();
-      if (tid < kTcRows + kTcHalf - 1) {
-        const int e = tid - (kTcRows - 1);  // query - key within the tile
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWork / 32; ++w) {
-          const int x = e - 32 * (w / 4) + 32 * (w % 4) + 31;
-          if (x >= 0 && x < 63) s += S.diag[strip][w][x];
-        }
-        const int delta = p0 - j0 + e;
-        if (delta <= -P.D) lo += s;
-        else if (delta >= P.D) hi += s;
-        else acc[delta + P.D] += s;
-      }
-      strip ^= 1;
+      __syncwarp();
+      const float done = lane < 15 ? out[lane] : lane < 16 ? 0.0f : lane == 31 ? up : out[46 - lane] + up;
+      up = __shfl_up_sync(0xffffffffu, up, 16);
+      if (lane >= 16) run += up;
+      float* mine = acc + warp * W;
+      auto add = [&](int slot, float v) {
+        const int delta = pw - (j0 + 32 * wq) + slot - 31;
+        if (delta <= -P.D) lo += v;
+        else if (delta >= P.D) hi += v;
+        else mine[delta + P.D] += v;
+      };
+      if (lane != 15) add(lane < 15 ? lane : 46 - lane, done);
+      add(62 - lane, run);
     }
     if (dw) {
       if (head >= 0) flush();
@@ -790,18 +784,19 @@ static cudaError_t launch_bwd(const AttnParams& P, cudaStream_t st) {
            tc_tmap(&T.k, P.k, BF16, P.d, P.nk, P.Hkv, P.B, k_rows) &&
            tc_tmap(&T.v, P.v, BF16, P.d, P.nk, P.Hkv, P.B, k_rows);
   };
-  const size_t smem = 1024 + 2 * kTcTileBytes + 2 * kStages * kHalfBytes + sizeof(BwdShared) + bias_ext_bytes(P) +
-                      (P.w ? (2 * P.D + 1) * sizeof(float) : 0);
+  const size_t smem = 1024 + 2 * kTcTileBytes + 2 * kStages * kHalfBytes + sizeof(BwdShared) + bias_ext_bytes(P);
+  // Tables of distances up to some 400 leave room for two CTAs an SM
+  const size_t smem_keys = smem + (P.dw_part ? kWork / 32 * (2 * P.D + 1) * sizeof(float) : 0);
   const int share = 256 * kElementRegs + 128 * kOtherRegs;
   cudaError_t e = prepare_kernel<tc_dq_kernel<BF16>>(smem, kBwdThreads, share);
-  if (e == cudaSuccess) e = prepare_kernel<tc_dkv_kernel<BF16>>(smem, kBwdThreads, share);
+  if (e == cudaSuccess) e = prepare_kernel<tc_dkv_kernel<BF16>>(smem_keys, kBwdThreads, share);
   if (e != cudaSuccess) return e;
   if (!maps(kTcRows, kTcHalf)) return cudaErrorInvalidValue;
   e = launch_dependent(tc_dq_kernel<BF16>, tc_grid(P.nq, P.H, P.B), kBwdThreads, smem, st, T);
   if (e != cudaSuccess) return e;
   if (!maps(kTcHalf, kTcRows)) return cudaErrorInvalidValue;
   const unsigned tiles = (P.nk + kTcRows - 1) / kTcRows, units = tiles * P.near_segs + P.sink_tiles * P.far_segs;
-  e = launch_dependent(tc_dkv_kernel<BF16>, units * P.Hkv * P.B, kBwdThreads, smem, st, T);
+  e = launch_dependent(tc_dkv_kernel<BF16>, units * P.Hkv * P.B, kBwdThreads, smem_keys, st, T);
   const unsigned joined = P.near_segs > 1 ? tiles : P.sink_tiles;
   if (e != cudaSuccess || joined == 0) return e;
   return launch_dependent(join_kernel<BF16>, dim3(joined * (kTcRows / kJoinRows), P.Hkv, P.B), 256, 0, st, P);
