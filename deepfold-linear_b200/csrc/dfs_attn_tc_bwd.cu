@@ -181,14 +181,10 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
         }
         if (t > 0 && !tc_wait(&S.s_free, (t - 1) & 1)) return false;
         tc_fence_after();
-        if (elect_one()) {
-          if (end) {
-            mbar_arrive(&S.s_full);
-          } else {
-            tc_mma_kk(tm + kColS, tc_desc(sQ), tc_desc(sK + s * kHalfBytes), id_s, dp / 16);
-            tc_mma_kk(tm + kColDP, tc_desc(sO), tc_desc(sV + s * kHalfBytes), id_s, dp / 16);
-            mma_commit(&S.s_full);
-          }
+        if (!end && elect_one()) {
+          tc_mma_kk(tm + kColS, tc_desc(sQ), tc_desc(sK + s * kHalfBytes), id_s, dp / 16);
+          tc_mma_kk(tm + kColDP, tc_desc(sO), tc_desc(sV + s * kHalfBytes), id_s, dp / 16);
+          mma_commit(&S.s_full);
         }
         __syncwarp();
         return true;
@@ -308,13 +304,15 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
     };
     int t = 0;
     for (;; ++t) {
-      if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
+      // what the producer says of the tile, while its S and dP are computed
+      if (!tc_wait(&S.full[t % kStages], (t / kStages) & 1)) { err = true; break; }
       const TileInfo& f = S.info[t % kInfo];
       const int at = f.at, j0 = at + 32 * cg;
       if (at < 0) break;
       const int plain = f.plain, tile_side = f.side;
       const uint32_t bits = f.bits[cg];
       const int cls = f.cls[2 * wq + cg];
+      if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
       tc_fence_after();
       uint32_t sr[32], dr[32];
       tmem_ld32_async(tm + lanes + kColS + 32 * cg, sr);
@@ -462,19 +460,15 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
         end = S.info[t % kInfo].at < 0;
         return true;
       };
-      auto start = [&](int t, bool end) {  // one lane: tile t's S and dP, or the end
+      auto start = [&](int t) {  // one lane: tile t's S and dP
         const int s = t % kStages;
-        if (end) {
-          mbar_arrive(&S.s_full);
-        } else {
-          tc_mma_kk(tm + kColS, tc_desc(sK), tc_desc(sQ + s * kHalfBytes), id_s, dp / 16);
-          tc_mma_kk(tm + kColDP, tc_desc(sV), tc_desc(sO + s * kHalfBytes), id_s, dp / 16);
-          mma_commit(&S.s_full);
-        }
+        tc_mma_kk(tm + kColS, tc_desc(sK), tc_desc(sQ + s * kHalfBytes), id_s, dp / 16);
+        tc_mma_kk(tm + kColDP, tc_desc(sV), tc_desc(sO + s * kHalfBytes), id_s, dp / 16);
+        mma_commit(&S.s_full);
       };
       bool end = false;
       if (!err) err = !wait_tile(0, end);
-      if (!err && elect_one()) start(0, end);
+      if (!err && !end && elect_one()) start(0);
       __syncwarp();
       for (int t = 0; !end && !err; ++t) {
         if (!wait_tile(t + 1, end) || !tc_wait(&S.ds_ready, t & 1)) { err = true; break; }
@@ -487,7 +481,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
           mma_commit(&S.acc_done);
           // The next S and dP overwrite the P and dS that these products read: MMAs of one thread execute in
           // the order of their issue, and the commit below covers all of them.
-          start(t + 1, end);
+          if (!end) start(t + 1);
         }
         __syncwarp();
       }
@@ -540,16 +534,14 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
     };
     // One block, S^T and dP^T on their way to sr and dr: P and dS to TMEM, over S and dP, and the block's sum of dS
     // to `sum`; a block that is not plain also leaves dS in dr.
-    auto step = [&](auto is_plain, int t, uint32_t (&sr)[32], uint32_t (&dr)[32], int pw, uint32_t kbits, int cls,
+    auto step = [&](auto is_plain, int t, uint32_t (&sr)[32], uint32_t (&dr)[32], int pw, uint32_t vis, int cls,
                     float far, float2& sum) {
       constexpr bool kPlain = decltype(is_plain)::value;
       const float* lse = S.stat[t % kStages][0] + 32 * cg;
       const float* Dv = S.stat[t % kStages][1] + 32 * cg;
       float mul = P.scale2;
-      uint32_t vis = ~0u;
       if (!kPlain) {
         const int side = (cls >> 2) - 1;
-        if ((cls & 3) == kPartial) vis = (kbits >> lane) & 1u ? query_word(P, j, pw) : 0u;
         far = side == 1 ? far_hi : side == -1 ? far_lo : 0.0f;
         if (side == 0) mul = 1.0f;
       }
@@ -603,7 +595,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
     };
     int t = 0;
     for (;; ++t) {
-      if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
+      // what the producer says of the tile, while its S and dP are computed
+      if (!tc_wait(&S.full[t % kStages], (t / kStages) & 1)) { err = true; break; }
       const TileInfo& f = S.info[t % kInfo];
       const int i0 = f.at, g = f.head;
       if (i0 < 0) break;
@@ -624,16 +617,18 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
       const uint32_t kbits = f.bits[wq];
       const int p0 = i0 + P.qs, pw = p0 + 32 * cg;
       const bool live = plain || (cls & 3) != kHidden;
+      const uint32_t vis = (kbits >> lane) & 1u ? query_word(P, j, pw) : 0u;
       float2 sum = both(0.0f);
       uint32_t sr[32], dr[32];
+      if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
       if (live) {
         tc_fence_after();
         tmem_ld32_async(tm + lanes + kColS + 32 * cg, sr);
         tmem_ld32_async(tm + lanes + kColDP + 32 * cg, dr);
         if (plain)
-          step(std::true_type(), t, sr, dr, pw, kbits, cls, tile_side > 0 ? far_hi : far_lo, sum);
+          step(std::true_type(), t, sr, dr, pw, vis, cls, tile_side > 0 ? far_hi : far_lo, sum);
         else
-          step(std::false_type(), t, sr, dr, pw, kbits, cls, 0.0f, sum);
+          step(std::false_type(), t, sr, dr, pw, vis, cls, 0.0f, sum);
       } else {
         const uint32_t none[16] = {};
         tc_fence_after();
