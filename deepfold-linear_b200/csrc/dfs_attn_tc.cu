@@ -56,6 +56,60 @@ struct FwdPart {
 };
 static_assert(sizeof(FwdPart) <= kTcTileBytes + 2 * kStages * kHalfBytes, "parts over the staged tiles");
 
+// This CTA's share of the joined rows, 16 lanes a row (whole rows of the other CTAs' memory at once).  The remote
+// reads of 8 / N rows are on their way together; one after the other they took as long as several tiles.
+template <bool BF16, int N>
+DFS_DEV void join_rows(const AttnParams& P, const FwdPart& part, int b, int h, int i0, int rank) {
+  using E16 = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  constexpr int kRows = 8 / N;  // rows of a thread at a time; 8 rows of the CTA's 128 / N at once
+  const int c = threadIdx.x % 16 * 4;
+#pragma unroll 1
+  for (int r0 = rank * (kTcRows / N) + threadIdx.x / 16; r0 < (rank + 1) * (kTcRows / N); r0 += 8 * kRows) {
+    float m[kRows][N], l[kRows][N];
+    float4 v[kRows][N];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int r = r0 + 8 * u;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        m[u][k] = dsmem_ld(dsmem_addr(smem_u32(&part.m[r]), k));
+        l[u][k] = dsmem_ld(dsmem_addr(smem_u32(&part.l[r]), k));
+        v[u][k] = dsmem_ld4(dsmem_addr(smem_u32(&part.o[r * kPartPitch + c]), k));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int at = i0 + r0 + 8 * u;
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < N; ++k) top = fmaxf(top, m[u][k]);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float f = ex2(m[u][k] - ref);
+        sum = fmaf(l[u][k], f, sum);
+        acc = make_float4(fmaf(v[u][k].x, f, acc.x), fmaf(v[u][k].y, f, acc.y), fmaf(v[u][k].z, f, acc.z),
+                          fmaf(v[u][k].w, f, acc.w));
+      }
+      if (at >= P.nq || c >= P.d) continue;
+      const bool none = !(sum > kNone) && sum == sum;
+      const float inv = none ? 0.0f : 1.0f / sum;
+      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      const uint2 out = make_uint2(pack16<BF16>(acc.x, acc.y), pack16<BF16>(acc.z, acc.w));
+      E16* dst = row_ptr<E16>(P.o, b, h, at) + c;
+      *reinterpret_cast<uint2*>(dst) = out;
+      if (P.o_lo) {
+        const float2 lo = unpack16<BF16>(out.x), hi = unpack16<BF16>(out.y);
+        *reinterpret_cast<uint2*>(reinterpret_cast<E16*>(P.o_lo) + (dst - reinterpret_cast<E16*>(P.o.p))) =
+            make_uint2(pack16<BF16>(acc.x - lo.x, acc.y - lo.y), pack16<BF16>(acc.z - hi.x, acc.w - hi.y));
+      }
+      if (P.lse && c == 0)
+        P.lse[(static_cast<size_t>(b) * P.H + h) * P.nq + at] = none ? INFINITY : top + lg2(sum);
+    }
+  }
+}
+
 // kSplit: a cluster of T.split CTAs shares each tile of queries, a run of the key tiles for each, joined in order
 // through distributed shared memory.
 template <bool BF16, bool kSplit>
@@ -315,35 +369,9 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
       part.l[row] = total;
       __syncwarp();
       cluster_sync();
-      const int rows = kTcRows / split, r0 = rank * rows;  // this CTA's share of the rows
-      for (int x = threadIdx.x; x < rows * 16; x += 128) {
-        const int r = r0 + x / 16, c = x % 16 * 4, at = i0 + r;
-        if (at >= P.nq || c >= P.d) continue;
-        const uint32_t am = smem_u32(&part.m[r]), al = smem_u32(&part.l[r]), ao = smem_u32(&part.o[r * kPartPitch + c]);
-        float top = -INFINITY, sum = 0.0f;
-        for (int k = 0; k < split; ++k) top = fmaxf(top, dsmem_ld(dsmem_addr(am, k)));
-        const float ref = top == -INFINITY ? 0.0f : top;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k = 0; k < split; ++k) {
-          const float f = ex2(dsmem_ld(dsmem_addr(am, k)) - ref);
-          const float4 v = dsmem_ld4(dsmem_addr(ao, k));
-          sum = fmaf(dsmem_ld(dsmem_addr(al, k)), f, sum);
-          acc = make_float4(fmaf(v.x, f, acc.x), fmaf(v.y, f, acc.y), fmaf(v.z, f, acc.z), fmaf(v.w, f, acc.w));
-        }
-        const bool empty = !(sum > kNone) && sum == sum;
-        const float g = empty ? 0.0f : 1.0f / sum;
-        acc = make_float4(acc.x * g, acc.y * g, acc.z * g, acc.w * g);
-        const uint2 out = make_uint2(pack16<BF16>(acc.x, acc.y), pack16<BF16>(acc.z, acc.w));
-        E16* dst = row_ptr<E16>(P.o, b, h, at) + c;
-        *reinterpret_cast<uint2*>(dst) = out;
-        if (P.o_lo) {
-          const float2 lo = unpack16<BF16>(out.x), hi = unpack16<BF16>(out.y);
-          *reinterpret_cast<uint2*>(reinterpret_cast<E16*>(P.o_lo) + (dst - reinterpret_cast<E16*>(P.o.p))) =
-              make_uint2(pack16<BF16>(acc.x - lo.x, acc.y - lo.y), pack16<BF16>(acc.z - hi.x, acc.w - hi.y));
-        }
-        if (P.lse && c == 0)
-          P.lse[(static_cast<size_t>(b) * P.H + h) * P.nq + at] = empty ? INFINITY : top + lg2(sum);
-      }
+      if (split == 2) join_rows<BF16, 2>(P, part, b, h, i0, rank);
+      else if (split == 4) join_rows<BF16, 4>(P, part, b, h, i0, rank);
+      else join_rows<BF16, 8>(P, part, b, h, i0, rank);
       __syncwarp();
       cluster_sync();  // nobody leaves while its memory is read
     }
