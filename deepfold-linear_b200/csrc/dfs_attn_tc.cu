@@ -13,10 +13,11 @@
 // (1600 clocks for a CTA alone): so the tiles are narrow (64 + 64 TMEM columns), and
 // four CTAs share an SM.  Measured (bfloat16, d = 64): 8192 tokens of 16 / 4 heads,
 // window 4096, 155 us, 660 TFLOP/s, an exponential pipe 60 % busy; 8 x 1024 of 16
-// heads, window 256 in both directions, 32 us.  Slower at the same sizes: 128-key
-// tiles with 256 or 512 threads, two S buffers and two CTAs an SM (155 to 170 us),
-// part of the exponentials as a polynomial on the FMA pipes, and long rows shared by
-// CTAs where the grid fills the GPU anyway (171 us).
+// heads, window 256 in both directions, 32 us.  While all SMs have four CTAs a tile
+// takes 560 clocks of each; the rest is the last wave, whose rows are of unequal
+// length.  Slower at the same sizes: 128-key tiles with 256 or 512 threads, two S
+// buffers and two CTAs an SM (155 to 170 us), part of the exponentials as a
+// polynomial on the FMA pipes, and every row shared by two CTAs (157 us).
 #include <algorithm>
 #include <type_traits>
 
@@ -425,12 +426,15 @@ cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st) 
   T.a = P;
   const size_t smem = 1024 + kTcTileBytes + 2 * kStages * kHalfBytes + sizeof(FwdShared) + bias_ext_bytes(P);
   const int share = 128 * kElementRegs + 128 * kOtherRegs;
-  // Few queries over many keys: a cluster of CTAs shares them, until every SM has four and while each has four tiles
-  // (bfloat16, d = 64: 5 queries of 16 heads over 8192 keys 110 -> 28 us, 8 heads of 1024 18.6 -> 15.6)
+  // Few queries over many keys: a cluster of CTAs shares them, until every SM has four and while each has four
+  // tiles; with sixteen each, until every SM has had eight (a wave that is not full ends with its longest CTA).
+  // Measured (bfloat16, d = 64, causal): 5 queries of 16 heads over 8192 keys 110 -> 28 us, 8 heads of 1024 18.6 ->
+  // 12.7; 16 heads of 4096 97 -> 62, but 32 heads of 2048 with a window of 512, ten tiles a CTA, 29 -> 36.
   const unsigned grid = tc_grid(P.nq, P.H, P.B);
   const int64_t seen = std::min<int64_t>(P.nk, int64_t{P.window} * (P.causal ? 1 : 2) + kTcRows + P.sinks) / kTcHalf;
   T.split = 1;
-  while (T.split < 8 && 2u * T.split * grid <= 4 * 148 && 8 * T.split <= seen) T.split *= 2;
+  while (T.split < 8 && 8 * T.split <= seen && 2u * T.split * grid <= (32 * T.split <= seen ? 8u : 4u) * 148)
+    T.split *= 2;
   auto run = [&](auto kern, cudaError_t e) {
     if (e != cudaSuccess) return e;
     if (!tc_tmap(&T.q, P.q, bf16, P.d, P.nq, P.H, P.B) ||
