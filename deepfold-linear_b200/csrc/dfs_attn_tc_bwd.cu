@@ -181,10 +181,14 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
         }
         if (t > 0 && !tc_wait(&S.s_free, (t - 1) & 1)) return false;
         tc_fence_after();
-        if (!end && elect_one()) {
-          tc_mma_kk(tm + kColS, tc_desc(sQ), tc_desc(sK + s * kHalfBytes), id_s, dp / 16);
-          tc_mma_kk(tm + kColDP, tc_desc(sO), tc_desc(sV + s * kHalfBytes), id_s, dp / 16);
-          mma_commit(&S.s_full);
+        if (elect_one()) {
+          if (end) {
+            mbar_arrive(&S.s_full);
+          } else {
+            tc_mma_kk(tm + kColS, tc_desc(sQ), tc_desc(sK + s * kHalfBytes), id_s, dp / 16);
+            tc_mma_kk(tm + kColDP, tc_desc(sO), tc_desc(sV + s * kHalfBytes), id_s, dp / 16);
+            mma_commit(&S.s_full);
+          }
         }
         __syncwarp();
         return true;
@@ -304,15 +308,13 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
     };
     int t = 0;
     for (;; ++t) {
-      // what the producer says of the tile, while its S and dP are computed
-      if (!tc_wait(&S.full[t % kStages], (t / kStages) & 1)) { err = true; break; }
+      if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
       const TileInfo& f = S.info[t % kInfo];
       const int at = f.at, j0 = at + 32 * cg;
       if (at < 0) break;
       const int plain = f.plain, tile_side = f.side;
       const uint32_t bits = f.bits[cg];
       const int cls = f.cls[2 * wq + cg];
-      if (!tc_wait(&S.s_full, t & 1)) { err = true; break; }
       tc_fence_after();
       uint32_t sr[32], dr[32];
       tmem_ld32_async(tm + lanes + kColS + 32 * cg, sr);
