@@ -22,10 +22,14 @@
 // and announces them.
 //
 // Measured (bfloat16, d = 64, 8192 tokens of 16 heads, window 1024, a bias): dQ pass
-// 95 us, dK/dV pass 143 us, together 340 TFLOP/s of the 10 d a visible pair needs.
-// No pipe is more than half busy; a tile's chain through TMEM is what is waited for,
-// and TMEM holds two CTAs' accumulators.  (dK/dV with one CTA an SM, two groups of
-// element warps and three buffers: 20 us slower.)  Where few key heads would leave
+// 95 us, dK/dV pass 133 us, together 350 TFLOP/s of the 10 d a visible pair needs.
+// No pipe is more than half busy.  A key tile's step is a chain of about 2500 clocks:
+// 650 for the four products (their operands' way out of shared memory, not the
+// tensor cores), 450 through TMEM, 900 of arithmetic, the rest waits' wake-ups; two
+// CTAs, which is what TMEM holds, overlap theirs.  Slower: one CTA an SM with two
+// groups of element warps and three buffers (20 us), and P and dS handed over one
+// after the other, so that half of the products run behind the other half's
+// arithmetic (13 us: twice the waits and reads).  Where few key heads would leave
 // SMs idle, the key pass spreads a tile's steps over CTAs and joins them in 32 bits
 // (16 / 2 heads of 2048 tokens: 351 -> 108 us).
 #include <type_traits>
