@@ -164,10 +164,14 @@ extern "C" int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_arg
   if (!a) return DFS_ERR_INVALID_ARGUMENT;
   const int s = problem_status(p, &a->bias);
   if (s != DFS_OK) return s;
-  if (p->B == 0 || p->H == 0) return DFS_OK;
+  if (p->H == 0) return DFS_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool dw = a->d_weight != nullptr && a->bias.weight != nullptr;
   if (a->d_weight && !a->bias.weight) return DFS_ERR_INVALID_ARGUMENT;
+  if (p->B == 0)  // d_weight alone has elements: sums of nothing
+    return !dw ? DFS_OK
+               : rc(launch_bucket_sums(nullptr, p->H, 0, a->bias.max_distance, a->bias.lut, a->bias.num_buckets,
+                                       a->bias.dtype, a->d_weight, st));
   if ((p->n_q > 0 && (!a->q.ptr || !a->o.ptr || !a->d_o.ptr || !a->d_q.ptr || !a->lse || !work)) ||
       (p->n_k > 0 && (!a->k.ptr || !a->v.ptr || !a->d_k.ptr || !a->d_v.ptr)))
     return DFS_ERR_INVALID_ARGUMENT;

@@ -1,0 +1,40 @@
+"""Local attention and its position bias at the edges of what a call may be given: empty problems, values that are
+not finite or very large, derivatives that it does not have, other threads.  Tolerances as in test_gpu_window_attn.py
+unless a test derives its own."""
+
+import pytest
+import torch
+
+from deepfold import _native as nat
+from deepfold.model.kernels.flash_window_attn import flash_window_attn
+
+from test_gpu_window_attn import BF16, BUCKETS, F32
+
+pytestmark = pytest.mark.gpu
+
+
+def poison(*shape, dtype=F32):
+    """Leaves blocks of NaN of this size in the allocator's cache, for the call's outputs to be made in."""
+    spare = [torch.full(shape, float("nan"), device="cuda", dtype=dtype) for _ in range(8)]
+    torch.cuda.synchronize()
+    del spare
+
+
+def test_bias_gradient_of_an_empty_batch_is_zero():
+    w = torch.ones(3, 32, device="cuda", requires_grad=True)
+    q = torch.zeros(0, 3, 5, 16, device="cuda", dtype=BF16)
+    poison(3, 32)
+    (d_w,) = torch.autograd.grad(flash_window_attn(q, q, q, pos_weight=w, buckets=BUCKETS["log"]).sum(), [w])
+    assert (d_w == 0).all()
+
+
+@pytest.mark.parametrize("dtype,code", [(F32, nat.DFS_F32), (BF16, nat.DFS_BF16)])
+def test_c_entry_writes_the_bias_gradient_of_an_empty_batch(dtype, code):
+    lut = torch.zeros(3, device="cuda", dtype=torch.int32)
+    w = torch.ones(2, 5, device="cuda", dtype=dtype)
+    d_w = torch.full_like(w, float("nan"))
+    p = nat.DfsAttnProblem(B=0, H=2, H_kv=1, n_q=4, n_k=4, d=16, dtype=code, causal=1, scale=1.0)
+    bias = nat.DfsRelBias(weight=w.data_ptr(), lut=lut.data_ptr(), num_buckets=5, max_distance=1, dtype=code)
+    a = nat.DfsAttnArgs(bias=bias, d_weight=d_w.data_ptr())
+    assert nat.lib().dfs_window_attn_bwd(p, a, None, 0, nat.stream_ptr(w.device)) == nat.DFS_OK
+    assert (d_w == 0).all()
