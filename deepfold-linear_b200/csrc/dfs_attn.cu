@@ -123,7 +123,7 @@ bool staged(const dfs_strided& s, int n, int heads, int B, int piece = 8) {  // 
 bool tensor_cores(const dfs_attn_problem* p, const dfs_attn_args* a) {
   const int64_t tiles = (std::max(p->n_q, p->n_k) + kTcRows - 1) / kTcRows + (p->n_q + kTcHalf - 1) / kTcHalf;
   return tiles * p->B * p->H < (int64_t{1} << 31) && p->dtype != DFS_F32 && p->d % 8 == 0 && p->scale > 0.0f &&
-         p->n_q > 0 && p->n_k > 0 && tmap_available() && aligned16(a->o_lo) &&
+         p->H > 0 && p->n_q > 0 && p->n_k > 0 && tmap_available() && aligned16(a->o_lo) &&
          staged(a->q, p->n_q, p->H, p->B) && staged(a->o, p->n_q, p->H, p->B) &&
          staged(a->k, p->n_k, p->H_kv, p->B) && staged(a->v, p->n_k, p->H_kv, p->B);
 }
@@ -164,7 +164,7 @@ extern "C" int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_arg
   if (!a) return DFS_ERR_INVALID_ARGUMENT;
   const int s = problem_status(p, &a->bias);
   if (s != DFS_OK) return s;
-  if (p->H == 0) return DFS_OK;
+  if (p->H == 0 && (p->B == 0 || p->H_kv == 0 || p->n_k == 0)) return DFS_OK;  // (else d_k and d_v are zeros)
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool dw = a->d_weight != nullptr && a->bias.weight != nullptr;
   if (a->d_weight && !a->bias.weight) return DFS_ERR_INVALID_ARGUMENT;
@@ -172,7 +172,7 @@ extern "C" int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_arg
     return !dw ? DFS_OK
                : rc(launch_bucket_sums(nullptr, p->H, 0, a->bias.max_distance, a->bias.lut, a->bias.num_buckets,
                                        a->bias.dtype, a->d_weight, st));
-  if ((p->n_q > 0 && (!a->q.ptr || !a->o.ptr || !a->d_o.ptr || !a->d_q.ptr || !a->lse || !work)) ||
+  if ((p->n_q > 0 && p->H > 0 && (!a->q.ptr || !a->o.ptr || !a->d_o.ptr || !a->d_q.ptr || !a->lse || !work)) ||
       (p->n_k > 0 && (!a->k.ptr || !a->v.ptr || !a->d_k.ptr || !a->d_v.ptr)))
     return DFS_ERR_INVALID_ARGUMENT;
   if (work_bytes < dfs_window_attn_bwd_work(p, dw ? &a->bias : nullptr)) return DFS_ERR_WORKSPACE;
@@ -196,7 +196,7 @@ extern "C" int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_arg
     const int r = rc(tc ? launch_attn_tc_bwd(P, p->dtype, st) : launch_attn_simt_bwd(P, p->dtype, vec, st));
     if (r != DFS_OK) return r;
   }
-  if (!dw) return DFS_OK;
+  if (!dw || p->H == 0) return DFS_OK;
   return rc(launch_bucket_sums(P.dw_part, p->H, P.parts, P.D, P.lut, P.nb, P.wdtype, a->d_weight, st));
 }
 

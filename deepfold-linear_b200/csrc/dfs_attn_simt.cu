@@ -441,7 +441,7 @@ cudaError_t fwd(const AttnParams& P, cudaStream_t st) {
 template <typename E, bool kVec>
 cudaError_t bwd(const AttnParams& P, cudaStream_t st) {
   const size_t acc = P.dw_part ? (2 * P.D + 1) * sizeof(float) : 0;
-  if (P.nq > 0) {
+  if (P.nq > 0 && P.H > 0) {
     const cudaError_t e = launch(simt_dq_kernel<E, kVec>, dim3((P.nq + kT - 1) / kT, P.H, P.B),
                                  5 * kTile * sizeof(float) + table_bytes(P), st, P);
     if (e != cudaSuccess) return e;

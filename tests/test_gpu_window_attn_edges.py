@@ -38,3 +38,15 @@ def test_c_entry_writes_the_bias_gradient_of_an_empty_batch(dtype, code):
     a = nat.DfsAttnArgs(bias=bias, d_weight=d_w.data_ptr())
     assert nat.lib().dfs_window_attn_bwd(p, a, None, 0, nat.stream_ptr(w.device)) == nat.DFS_OK
     assert (d_w == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_key_gradients_without_query_heads_are_zero(dtype):
+    q = torch.zeros(2, 0, 5, 16, device="cuda", dtype=dtype, requires_grad=True)
+    k, v = (torch.ones(2, 3, 70, 16, device="cuda", dtype=dtype, requires_grad=True) for _ in range(2))
+    w = torch.ones(0, 32, device="cuda", requires_grad=True)
+    for kw, leaves in ((dict(), [k, v]), (dict(pos_weight=w, buckets=BUCKETS["log"], window=4, sinks=1), [k, v, w])):
+        o = flash_window_attn(q, k, v, **kw)
+        poison(2, 3, 70, 16, dtype=dtype)
+        grads = torch.autograd.grad(o.sum(), leaves)
+        assert all(g.shape == t.shape and (g == 0).all() for g, t in zip(grads, leaves))
