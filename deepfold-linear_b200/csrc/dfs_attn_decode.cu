@@ -95,7 +95,8 @@ DFS_DEV void join_cluster(const AttnParams& P, const Found<N>& F, int b, int h0,
         acc += dsmem_ld(dsmem_addr(ao, r)) * k;
       }
     }
-    row_ptr<E>(P.o, b, h0 + head, 0)[c] = from_f32<E>(sum > 0.0f ? acc / sum : 0.0f);
+    // nothing visible: 0 exactly; a sum that is NaN (a NaN, or a logit of +inf) stays one
+    row_ptr<E>(P.o, b, h0 + head, 0)[c] = from_f32<E>(sum == 0.0f ? 0.0f : acc / sum);
   }
   if (split > 1) cluster_sync();  // nobody leaves while its memory is read
 }

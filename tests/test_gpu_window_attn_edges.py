@@ -6,9 +6,9 @@ import pytest
 import torch
 
 from deepfold import _native as nat
-from deepfold.model.kernels.flash_window_attn import flash_window_attn
+from deepfold.model.kernels.flash_window_attn import flash_window_attn, window_attn_decode
 
-from test_gpu_window_attn import BF16, BUCKETS, F32
+from test_gpu_window_attn import BF16, BUCKETS, F16, F32, inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,31 @@ def test_key_gradients_without_query_heads_are_zero(dtype):
         poison(2, 3, 70, 16, dtype=dtype)
         grads = torch.autograd.grad(o.sum(), leaves)
         assert all(g.shape == t.shape and (g == 0).all() for g, t in zip(grads, leaves))
+
+
+def plain(q, k, v, w, table):
+    """Causal attention with a bias as float64 softmax: what is not finite spreads as the formula has it."""
+    q, k, v, w = (t.detach().double().cpu() for t in (q, k, v, w))
+    G, (n_q, n_k), D = q.shape[1] // k.shape[1], (q.shape[2], k.shape[2]), len(table) // 2
+    k, v = (t.repeat_interleave(G, 1) for t in (k, v))
+    delta = (torch.arange(n_q) + n_k - n_q)[:, None] - torch.arange(n_k)[None]
+    bias = w[:, torch.tensor(table)[delta.clamp(-D, D) + D]]
+    s = (q @ k.mT * q.shape[-1] ** -0.5 + bias).masked_fill(delta < 0, float("-inf"))
+    p = torch.softmax(s, -1).masked_fill(delta < 0, 0.0)
+    return (p @ v).cuda()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n", [40, 5003])  # one block, and sixteen that join
+@pytest.mark.parametrize("what", ["q", "k", "v", "w", "logit"])
+def test_what_is_not_finite_shows_in_the_token(what, n, dtype):
+    """NaN in q, in a visible key, value or weight, or a logit of +inf: NaN where the formula has it, as the forward."""
+    x = inputs(2, 4, 2, 1, n, 32, dtype, 61, nb=32)
+    at = {"q": x["q"][0, 1, 0], "k": x["k"][0, 0, n - 2], "v": x["v"][0, 0, n - 2], "w": x["w"][1]}
+    at.get(what, x["w"][1])[0] = float("inf") if what == "logit" else float("nan")
+    kw = dict(pos_weight=x["w"], buckets=BUCKETS["log"])
+    one = window_attn_decode(x["q"][:, :, 0], x["k"], x["v"], torch.tensor([n, n], device="cuda"), **kw)
+    full = flash_window_attn(x["q"], x["k"], x["v"], **kw)[:, :, 0]
+    want = plain(x["q"], x["k"], x["v"], x["w"], BUCKETS["log"].table)[:, :, 0]
+    assert torch.isnan(want).any() and not torch.isnan(want).all()
+    assert torch.equal(torch.isnan(one), torch.isnan(want)) and torch.equal(torch.isnan(full), torch.isnan(want))
