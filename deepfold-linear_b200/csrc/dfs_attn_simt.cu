@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kNT, 3) simt_fwd_kernel(AttnParams P) {
   for (int r = 0; r < kR; ++r) {
     const int i = i0 + ty + 8 * r;
     if (i >= P.nq) continue;
-    const float inv = l[r] > 0.0f ? 1.0f / l[r] : 0.0f;
+    const float inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];  // a sum that is NaN stays one, here and in lse
     E* row = row_ptr<E>(P.o, b, h, i);
     E* rest = P.o_lo ? reinterpret_cast<E*>(P.o_lo) + (row - reinterpret_cast<E*>(P.o.p)) : nullptr;
 #pragma unroll
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kNT, 3) simt_fwd_kernel(AttnParams P) {
         if (rest) rest[4 * tx + c] = from_f32<E>(v - to_f32<E>(from_f32<E>(v)));
       }
     if (P.lse && tx == 0)
-      P.lse[(static_cast<size_t>(b) * P.H + h) * P.nq + i] = l[r] > 0.0f ? m[r] + log2f(l[r]) : INFINITY;
+      P.lse[(static_cast<size_t>(b) * P.H + h) * P.nq + i] = l[r] == 0.0f ? INFINITY : m[r] + log2f(l[r]);
   }
 }
 

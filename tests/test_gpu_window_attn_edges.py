@@ -78,3 +78,21 @@ def test_what_is_not_finite_shows_in_the_token(what, n, dtype):
     want = plain(x["q"], x["k"], x["v"], x["w"], BUCKETS["log"].table)[:, :, 0]
     assert torch.isnan(want).any() and not torch.isnan(want).all()
     assert torch.equal(torch.isnan(one), torch.isnan(want)) and torch.equal(torch.isnan(full), torch.isnan(want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("what", ["k", "w"])
+def test_gradients_of_a_row_that_is_not_finite(what, dtype):
+    """A query whose softmax is NaN gives every key that it sees a NaN gradient, not that of a query that sees none."""
+    x = inputs(1, 2, 1, 150, 150, 32, dtype, 67, nb=32)
+    if what == "k":
+        x["k"][0, 0, 60, 1] = float("nan")   # seen from query 60 on
+    else:
+        x["w"][:, 3] = float("inf")          # the bucket of delta = 3: every query from 3 on
+    leaves = [x[n].detach().requires_grad_() for n in ("q", "k", "v")]
+    o = flash_window_attn(*leaves, pos_weight=x["w"], buckets=BUCKETS["log"])
+    d_q, d_k, d_v = torch.autograd.grad(o, leaves, x["d_o"])
+    first = 60 if what == "k" else 3
+    assert torch.isnan(o[:, :, first:]).all() and torch.isfinite(o[:, :, :first]).all()
+    assert torch.isnan(d_q[:, :, first:]).all()
+    assert torch.isnan(d_k).all() and torch.isnan(d_v).all()  # the last query sees every key
