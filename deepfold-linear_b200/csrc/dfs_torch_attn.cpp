@@ -8,6 +8,7 @@
 // nothing for them: the next call reads the word.
 #include <ATen/cuda/CUDAContext.h>
 
+#include <initializer_list>
 #include <limits>
 #include <mutex>
 
@@ -60,6 +61,14 @@ int32_t narrow32(int64_t v, const char* what) {
 bool float_type(const Tensor& t) {
   const auto s = t.scalar_type();
   return s == at::kBFloat16 || s == at::kHalf || s == at::kFloat;
+}
+
+// No kernel computes a tangent: a call on dual tensors (forward-mode derivatives) that went on would drop theirs,
+// which reads as a derivative of 0.
+void refuse_tangents(std::initializer_list<optional<Tensor>> operands) {
+  for (const auto& t : operands)
+    require(!t.has_value() || !t->defined() || !t->_fw_grad(/*level=*/0).defined(),
+            "deepfold B200 attention and position bias have no forward-mode derivatives");
 }
 
 // The tensor itself where the kernels can walk it (unit stride along d, no row
@@ -227,6 +236,7 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
 
 Tensor window_attn(Tensor Q, Tensor K, Tensor V, optional<Tensor> mask, optional<Tensor> weight, optional<Tensor> lut,
                    int64_t max_distance, int64_t window, int64_t sinks, bool causal, int64_t q_start, double scale) {
+  refuse_tangents({Q, K, V, weight});
   const bool has_w = weight.has_value() && weight->defined();
   const bool grad = at::GradMode::is_enabled() && (Q.requires_grad() || K.requires_grad() || V.requires_grad() ||
                                                    (has_w && weight->requires_grad()));
@@ -240,6 +250,7 @@ Tensor window_attn(Tensor Q, Tensor K, Tensor V, optional<Tensor> mask, optional
 
 Tensor window_attn_decode(Tensor q, Tensor K, Tensor V, Tensor lengths, optional<Tensor> weight, optional<Tensor> lut,
                           int64_t max_distance, int64_t window, int64_t sinks, double scale) {
+  refuse_tangents({q, K, V, weight});
   require(q.dim() == 3, "q must be (B, H, d)");
   const Problem r = make_problem(q, K, V, c10::nullopt, weight, lut, max_distance, window, sinks, true, 0,
                                  scale);
@@ -303,6 +314,7 @@ struct RelBiasFn : public torch::autograd::Function<RelBiasFn> {
 };
 
 Tensor relative_position_bias(Tensor w, Tensor lut, int64_t max_distance, int64_t n_q, int64_t n_k, int64_t q_start) {
+  refuse_tangents({w});
   if (at::GradMode::is_enabled() && w.requires_grad())
     return RelBiasFn::apply(w, lut, max_distance, n_q, n_k, q_start);
   return relbias_forward(w, lut, max_distance, n_q, n_k, q_start);

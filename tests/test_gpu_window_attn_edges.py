@@ -4,9 +4,11 @@ unless a test derives its own."""
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from deepfold import _native as nat
 from deepfold.model.kernels.flash_window_attn import flash_window_attn, window_attn_decode
+from deepfold.model.position_encoding import relative_position_bias
 
 from test_gpu_window_attn import BF16, BUCKETS, F16, F32, inputs
 
@@ -96,3 +98,21 @@ def test_gradients_of_a_row_that_is_not_finite(what, dtype):
     assert torch.isnan(o[:, :, first:]).all() and torch.isfinite(o[:, :, :first]).all()
     assert torch.isnan(d_q[:, :, first:]).all()
     assert torch.isnan(d_k).all() and torch.isnan(d_v).all()  # the last query sees every key
+
+
+def test_forward_mode_derivatives_are_refused():
+    x = inputs(1, 2, 2, 20, 20, 16, F32, 71, nb=32)
+    q, k, v, w, b = x["q"], x["k"], x["v"], x["w"], BUCKETS["log"]
+    one = torch.tensor([20], device="cuda")
+    with forward_ad.dual_level():
+        d = {n: forward_ad.make_dual(x[n], torch.ones_like(x[n])) for n in ("q", "k", "v", "w")}
+        for call in (lambda: flash_window_attn(d["q"], k, v), lambda: flash_window_attn(q, d["k"], v),
+                     lambda: flash_window_attn(q, k, d["v"]),
+                     lambda: flash_window_attn(q, k, v, pos_weight=d["w"], buckets=b),
+                     lambda: window_attn_decode(d["q"][:, :, 0], k, v, one),
+                     lambda: window_attn_decode(q[:, :, 0], k, v, one, pos_weight=d["w"], buckets=b),
+                     lambda: relative_position_bias(d["w"], b, 4, 4)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()

@@ -1,0 +1,21 @@
+"""Local attention's edges that need no GPU: what its calls refuse and keep on the host."""
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from deepfold import _native as nat
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Before anything else, with or without gradients: a tangent that is dropped reads as a derivative of 0."""
+    x, w, lut = torch.ones(1, 2, 4, 8), torch.ones(2, 3), torch.zeros(3, dtype=torch.int32)
+    ext = nat.ext()
+    with forward_ad.dual_level():
+        dual, dual_w = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, w))
+        for call in (lambda: ext.window_attn(dual, x, x, None, None, None, 0, 0, 0, True, 0, 1.0),
+                     lambda: ext.window_attn(x, x, x, None, dual_w, lut, 1, 0, 0, True, 0, 1.0),
+                     lambda: ext.window_attn_decode(x[:, :, 0], x, dual, torch.ones(1), None, None, 0, 0, 0, 1.0),
+                     lambda: ext.relative_position_bias(dual_w, lut, 1, 4, 4, 0)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
