@@ -7,6 +7,7 @@
 // straight into one word of mapped host memory per device, so a call pays
 // nothing for them: the next call reads the word.
 #include <ATen/cuda/CUDAContext.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <initializer_list>
 #include <limits>
@@ -69,6 +70,22 @@ void refuse_tangents(std::initializer_list<optional<Tensor>> operands) {
   for (const auto& t : operands)
     require(!t.has_value() || !t->defined() || !t->_fw_grad(/*level=*/0).defined(),
             "deepfold B200 attention and position bias have no forward-mode derivatives");
+}
+
+// What a backward returns.  Where it is itself recorded (create_graph) its gradients carry an error in place of the
+// second derivative that the kernels lack: without a history they would count as constants.
+variable_list once_differentiable(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list in;
+  for (const Tensor& g : grads)
+    if (g.defined()) in.push_back(g.detach().requires_grad_());
+  const auto n = static_cast<int64_t>(in.size());
+  variable_list out = torch::autograd::DelayedError(
+      "deepfold B200 attention and position bias are differentiable once only", n).apply(std::move(in));
+  auto next = out.begin();
+  for (Tensor& g : grads)
+    if (g.defined()) g = *next++;
+  return grads;
 }
 
 // The tensor itself where the kernels can walk it (unit stride along d, no row
@@ -230,7 +247,7 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
     out[1] = dk;
     out[2] = dv;
     if (want_w) out[3] = dw;
-    return out;
+    return once_differentiable(out);
   }
 };
 
@@ -309,7 +326,7 @@ struct RelBiasFn : public torch::autograd::Function<RelBiasFn> {
                              dw.data_ptr(), bytes ? work.data_ptr() : nullptr, bytes, stream_of(g)),
              "dfs_relbias_bwd");
     out[0] = dw;
-    return out;
+    return once_differentiable(out);
   }
 };
 

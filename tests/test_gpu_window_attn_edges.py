@@ -116,3 +116,17 @@ def test_forward_mode_derivatives_are_refused():
                 call()
             with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+def test_second_derivatives_are_refused():
+    """Under create_graph the gradients are what they are without it; to differentiate them again raises."""
+    x = inputs(1, 2, 1, 20, 20, 16, F32, 73, nb=32)
+    q, k, v, w = leaves = [x[n].requires_grad_() for n in ("q", "k", "v", "w")]
+    b = BUCKETS["log"]
+    for out, of in ((flash_window_attn(q, k, v, pos_weight=w, buckets=b), leaves), (relative_position_bias(w, b, 9, 9), [w])):
+        plain_grads = torch.autograd.grad(out.square().sum(), of, retain_graph=True)
+        grads = torch.autograd.grad(out.square().sum(), of, create_graph=True)
+        for t, g, want in zip(of, grads, plain_grads):
+            assert g.requires_grad and not want.requires_grad and torch.equal(g, want)
+            with pytest.raises(RuntimeError, match="once"):
+                (t.sum() + g.square().sum()).backward(retain_graph=True)
