@@ -107,7 +107,9 @@ class RelativeBuckets:
         """The table as int32 on ``device``."""
         t = self._on.get(device)
         if t is None:
-            t = torch.frombuffer(array("i", self.table), dtype=torch.int32).to(device)  # quicker than from a list
+            # an inference tensor, kept from a first call in inference mode, could not be saved for a later backward
+            with torch.inference_mode(False):
+                t = torch.frombuffer(array("i", self.table), dtype=torch.int32).to(device)  # quicker than from a list
             self._on[t.device] = self._on[device] = t
         return t
 

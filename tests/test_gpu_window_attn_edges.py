@@ -8,7 +8,7 @@ from torch.autograd import forward_ad
 
 from deepfold import _native as nat
 from deepfold.model.kernels.flash_window_attn import flash_window_attn, window_attn_decode
-from deepfold.model.position_encoding import relative_position_bias
+from deepfold.model.position_encoding import RelativeBuckets, relative_position_bias
 
 from test_gpu_window_attn import BF16, BUCKETS, F16, F32, inputs
 
@@ -130,3 +130,14 @@ def test_second_derivatives_are_refused():
             assert g.requires_grad and not want.requires_grad and torch.equal(g, want)
             with pytest.raises(RuntimeError, match="once"):
                 (t.sum() + g.square().sum()).backward(retain_graph=True)
+
+
+def test_training_after_a_first_call_in_inference_mode():
+    x = inputs(1, 2, 1, 20, 20, 16, F32, 79, nb=32)
+    b = RelativeBuckets(BUCKETS["log"].table)
+    with torch.inference_mode():
+        first = flash_window_attn(x["q"], x["k"], x["v"], pos_weight=x["w"], buckets=b)
+    w = x["w"].requires_grad_()
+    o = flash_window_attn(x["q"], x["k"], x["v"], pos_weight=w, buckets=b)
+    (o.sum() + relative_position_bias(w, b, 7, 7).sum()).backward()
+    assert torch.equal(o.detach(), first) and torch.isfinite(w.grad).all()

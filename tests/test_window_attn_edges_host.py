@@ -5,6 +5,7 @@ import torch
 from torch.autograd import forward_ad
 
 from deepfold import _native as nat
+from deepfold.model.position_encoding import RelativeBuckets
 
 
 def test_forward_mode_derivatives_are_refused():
@@ -19,3 +20,12 @@ def test_forward_mode_derivatives_are_refused():
                      lambda: ext.relative_position_bias(dual_w, lut, 1, 4, 4, 0)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+def test_a_table_first_used_in_inference_mode_serves_training():
+    b = RelativeBuckets.log(16, 40)
+    with torch.inference_mode():
+        first = b.on(torch.device("cpu"))
+        made = RelativeBuckets.clip(4, device="cpu").on(torch.device("cpu"))
+    assert not first.is_inference() and not made.is_inference()
+    assert b.on(torch.device("cpu")) is first and first.tolist() == list(b.table)
