@@ -2,6 +2,8 @@
 // rule of which key a query sees, element types, and the expanded bias table.
 #pragma once
 
+#include <atomic>
+
 #include "dfs_device.cuh"
 
 namespace dfs {
@@ -87,6 +89,29 @@ DFS_DEV void load_bias_table(float* tab, const void* w, const int32_t* lut, int 
     const int b = min(max(lut[x], 0), nb - 1);
     tab[x] = load_as_f32<void>(w, static_cast<size_t>(h) * nb + b, wdtype) * mul;
   }
+}
+
+// Raises kernel K's limit of dynamic shared memory to `most`, what it needs with the largest bias table (D =
+// DFS_MAX_BUCKET_DISTANCE): once per device, for the call costs host time, and to the same value in every call, so
+// that no host thread can lower it between another's check and its launch.  And, where the kernel splits its
+// registers, checks that the shares fit what it is launched with (an increase that the block's own registers cannot
+// serve would wait forever).
+template <auto K>
+cudaError_t prepare_kernel(size_t most, int threads = 0, int share = 0) {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<bool> ready[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < kMaxDevices && ready[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  if (share > 0) {
+    cudaFuncAttributes at;
+    if ((e = cudaFuncGetAttributes(&at, K)) != cudaSuccess) return e;
+    if ((at.numRegs + 7) / 8 * 8 * threads < share) return cudaErrorInvalidConfiguration;
+  }
+  e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+  if (e == cudaSuccess && dev < kMaxDevices) ready[dev].store(true, std::memory_order_release);
+  return e;
 }
 
 // launchers (host)

@@ -488,9 +488,10 @@ cudaError_t launch(const AttnParams& P, cudaStream_t st) {
     return cudaErrorInvalidValue;
   T.chunks = (P.G + kHeads - 1) / kHeads;
   T.split = split_of(P, T.chunks, 3);
-  const size_t smem = 1024 + kStages * 2 * kTcTileBytes + sizeof(DecodeShared) +
-                      (P.w ? std::min(P.G, kHeads) * (P.D + 1) * sizeof(float) : 0);
-  const cudaError_t e = prepare_kernel<decode_mma_kernel<E>>(smem);
+  const size_t fixed = 1024 + kStages * 2 * kTcTileBytes + sizeof(DecodeShared);
+  const size_t smem = fixed + (P.w ? std::min(P.G, kHeads) * (P.D + 1) * sizeof(float) : 0);
+  const cudaError_t e =
+      prepare_kernel<decode_mma_kernel<E>>(fixed + kHeads * (DFS_MAX_BUCKET_DISTANCE + 1) * sizeof(float));
   if (e != cudaSuccess) return e;
   return launch_clusters(decode_mma_kernel<E>, dim3(T.split, P.Hkv * T.chunks, P.B), T.split, kThreads, smem, st, T);
 }

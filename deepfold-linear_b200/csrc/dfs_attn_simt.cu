@@ -423,32 +423,31 @@ __global__ void __launch_bounds__(kNT, 2) simt_dkv_kernel(AttnParams P) {
   }
 }
 
-template <typename... A>
-cudaError_t launch(void (*kern)(A...), dim3 grid, size_t smem, cudaStream_t st, A... args) {
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+// K over a grid with `tiles` tiles and `tables` bias tables (or sums by distance) in shared memory; most: the tables
+// that it can have
+template <auto K>
+cudaError_t launch(dim3 grid, int tiles, int tables, int most, cudaStream_t st, const AttnParams& P) {
+  auto bytes = [=](int n, int D) { return (tiles * kTile + n * (2 * D + 1)) * sizeof(float); };
+  const cudaError_t e = prepare_kernel<K>(bytes(most, DFS_MAX_BUCKET_DISTANCE));
   if (e != cudaSuccess) return e;
-  kern<<<grid, kNT, smem, st>>>(args...);
+  K<<<grid, kNT, bytes(tables, P.D), st>>>(P);
   return cudaGetLastError();
 }
 
-size_t table_bytes(const AttnParams& P) { return P.w ? (2 * P.D + 1) * sizeof(float) : 0; }
-
 template <typename E, bool kVec>
 cudaError_t fwd(const AttnParams& P, cudaStream_t st) {
-  return launch(simt_fwd_kernel<E, kVec>, dim3((P.nq + kT - 1) / kT, P.H, P.B),
-                4 * kTile * sizeof(float) + table_bytes(P), st, P);
+  return launch<simt_fwd_kernel<E, kVec>>(dim3((P.nq + kT - 1) / kT, P.H, P.B), 4, P.w != nullptr, 1, st, P);
 }
 template <typename E, bool kVec>
 cudaError_t bwd(const AttnParams& P, cudaStream_t st) {
-  const size_t acc = P.dw_part ? (2 * P.D + 1) * sizeof(float) : 0;
+  const int table = P.w != nullptr, sums = P.dw_part != nullptr;
   if (P.nq > 0 && P.H > 0) {
-    const cudaError_t e = launch(simt_dq_kernel<E, kVec>, dim3((P.nq + kT - 1) / kT, P.H, P.B),
-                                 5 * kTile * sizeof(float) + table_bytes(P), st, P);
+    const cudaError_t e =
+        launch<simt_dq_kernel<E, kVec>>(dim3((P.nq + kT - 1) / kT, P.H, P.B), 5, table, 1, st, P);
     if (e != cudaSuccess) return e;
   }
   if (P.nk == 0) return cudaSuccess;
-  return launch(simt_dkv_kernel<E, kVec>, dim3((P.nk + kT - 1) / kT, P.Hkv, P.B),
-                6 * kTile * sizeof(float) + table_bytes(P) + acc, st, P);
+  return launch<simt_dkv_kernel<E, kVec>>(dim3((P.nk + kT - 1) / kT, P.Hkv, P.B), 6, table + sums, 2, st, P);
 }
 
 }  // namespace

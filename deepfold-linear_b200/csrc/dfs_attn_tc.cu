@@ -424,7 +424,8 @@ cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st) 
   const bool bf16 = dtype == DFS_BF16;
   TcParams T;
   T.a = P;
-  const size_t smem = 1024 + kTcTileBytes + 2 * kStages * kHalfBytes + sizeof(FwdShared) + bias_ext_bytes(P);
+  const size_t fixed = 1024 + kTcTileBytes + 2 * kStages * kHalfBytes + sizeof(FwdShared);
+  const size_t smem = fixed + bias_ext_bytes(P), most = fixed + ext_table_bytes(DFS_MAX_BUCKET_DISTANCE);
   const int share = 128 * kElementRegs + 128 * kOtherRegs;
   // Few queries over many keys: a cluster of CTAs shares them, until every SM has four and while each has four
   // tiles; with sixteen each, until every SM has had eight (a wave that is not full ends with its longest CTA).
@@ -445,10 +446,10 @@ cudaError_t launch_attn_tc_fwd(const AttnParams& P, int dtype, cudaStream_t st) 
     return launch_clusters(kern, grid * T.split, T.split, kFwdThreads, smem, st, T);
   };
   if (T.split > 1)
-    return bf16 ? run(tc_fwd_kernel<true, true>, prepare_kernel<tc_fwd_kernel<true, true>>(smem, kFwdThreads, share))
-                : run(tc_fwd_kernel<false, true>, prepare_kernel<tc_fwd_kernel<false, true>>(smem, kFwdThreads, share));
-  return bf16 ? run(tc_fwd_kernel<true, false>, prepare_kernel<tc_fwd_kernel<true, false>>(smem, kFwdThreads, share))
-              : run(tc_fwd_kernel<false, false>, prepare_kernel<tc_fwd_kernel<false, false>>(smem, kFwdThreads, share));
+    return bf16 ? run(tc_fwd_kernel<true, true>, prepare_kernel<tc_fwd_kernel<true, true>>(most, kFwdThreads, share))
+                : run(tc_fwd_kernel<false, true>, prepare_kernel<tc_fwd_kernel<false, true>>(most, kFwdThreads, share));
+  return bf16 ? run(tc_fwd_kernel<true, false>, prepare_kernel<tc_fwd_kernel<true, false>>(most, kFwdThreads, share))
+              : run(tc_fwd_kernel<false, false>, prepare_kernel<tc_fwd_kernel<false, false>>(most, kFwdThreads, share));
 }
 
 }  // namespace dfs

@@ -2,8 +2,6 @@
 // staging, TMEM operands, tile information, bias tables.
 #pragma once
 
-#include <atomic>
-
 #include "dfs_attn.cuh"
 #include "dfs_tma.cuh"
 
@@ -210,7 +208,8 @@ DFS_DEV void load_bias_ext(float* tab, const AttnParams& P, int h, int tid, int 
       if (x0 + u * nthreads < W) tab[x0 + u * nthreads] = v[u] * kLog2e;
   }
 }
-inline size_t bias_ext_bytes(const AttnParams& P) { return P.w ? (2 * (P.D + 255) + 1) * sizeof(float) : 0; }
+constexpr size_t ext_table_bytes(int D) { return (2 * (D + 255) + 1) * sizeof(float); }
+inline size_t bias_ext_bytes(const AttnParams& P) { return P.w ? ext_table_bytes(P.D) : 0; }
 
 // One tile as the producer announces it: first key (or query) row, -1 for the
 // end; whether it is plain (all pairs visible, one bias for all) and where its
@@ -327,27 +326,6 @@ bool tc_tmap(CUtensorMap* tm, const Strided& s, bool bf16, int d, int n, int hea
 // N = 4096, causal.)
 inline unsigned tc_grid(int n, int heads, int B) {
   return static_cast<unsigned>((n + kTcRows - 1) / kTcRows) * heads * B;
-}
-
-// Dynamic shared memory of kernel K, raised once per device to the largest asked for (the call costs host
-// time); and, where the kernel splits its registers, that the shares fit what it is launched with (an increase
-// that the block's own registers cannot serve would wait forever).
-template <auto K>
-cudaError_t prepare_kernel(size_t smem, int threads = 0, int share = 0) {
-  constexpr int kMaxDevices = 64;
-  static std::atomic<size_t> ready[kMaxDevices];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < kMaxDevices && ready[dev].load(std::memory_order_relaxed) >= smem) return cudaSuccess;
-  if (share > 0) {
-    cudaFuncAttributes at;
-    if ((e = cudaFuncGetAttributes(&at, K)) != cudaSuccess) return e;
-    if ((at.numRegs + 7) / 8 * 8 * threads < share) return cudaErrorInvalidConfiguration;
-  }
-  e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (e == cudaSuccess && dev < kMaxDevices) ready[dev].store(smem, std::memory_order_relaxed);
-  return e;
 }
 
 // A dependent launch (launch_dependent) whose blocks come in clusters of `size` along x.

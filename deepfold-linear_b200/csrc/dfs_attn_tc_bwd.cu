@@ -785,12 +785,16 @@ static cudaError_t launch_bwd(const AttnParams& P, cudaStream_t st) {
            tc_tmap(&T.k, P.k, BF16, P.d, P.nk, P.Hkv, P.B, k_rows) &&
            tc_tmap(&T.v, P.v, BF16, P.d, P.nk, P.Hkv, P.B, k_rows);
   };
-  const size_t smem = 1024 + 2 * kTcTileBytes + 2 * kStages * kHalfBytes + sizeof(BwdShared) + bias_ext_bytes(P);
+  const size_t fixed = 1024 + 2 * kTcTileBytes + 2 * kStages * kHalfBytes + sizeof(BwdShared);
+  const size_t smem = fixed + bias_ext_bytes(P);
   // Tables of distances up to some 400 leave room for two CTAs an SM
-  const size_t smem_keys = smem + (P.dw_part ? kWork / 32 * (2 * P.D + 1) * sizeof(float) : 0);
+  auto sums = [](int D) { return kWork / 32 * (2 * D + 1) * sizeof(float); };
+  const size_t smem_keys = smem + (P.dw_part ? sums(P.D) : 0);
+  const size_t most = fixed + ext_table_bytes(DFS_MAX_BUCKET_DISTANCE);
   const int share = 256 * kElementRegs + 128 * kOtherRegs;
-  cudaError_t e = prepare_kernel<tc_dq_kernel<BF16>>(smem, kBwdThreads, share);
-  if (e == cudaSuccess) e = prepare_kernel<tc_dkv_kernel<BF16>>(smem_keys, kBwdThreads, share);
+  cudaError_t e = prepare_kernel<tc_dq_kernel<BF16>>(most, kBwdThreads, share);
+  if (e == cudaSuccess)
+    e = prepare_kernel<tc_dkv_kernel<BF16>>(most + sums(DFS_MAX_BUCKET_DISTANCE), kBwdThreads, share);
   if (e != cudaSuccess) return e;
   if (!maps(kTcRows, kTcHalf)) return cudaErrorInvalidValue;
   e = launch_dependent(tc_dq_kernel<BF16>, tc_grid(P.nq, P.H, P.B), kBwdThreads, smem, st, T);

@@ -2,6 +2,8 @@
 not finite or very large, derivatives that it does not have, other threads.  Tolerances as in test_gpu_window_attn.py
 unless a test derives its own."""
 
+import threading
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -141,3 +143,43 @@ def test_training_after_a_first_call_in_inference_mode():
     o = flash_window_attn(x["q"], x["k"], x["v"], pos_weight=w, buckets=b)
     (o.sum() + relative_position_bias(w, b, 7, 7).sum()).backward()
     assert torch.equal(o.detach(), first) and torch.isfinite(w.grad).all()
+
+
+@pytest.mark.parametrize("dtype,code", [(F32, nat.DFS_F32), (BF16, nat.DFS_BF16)])
+def test_threads_with_tables_of_different_sizes(dtype, code):
+    """The C entries from two host threads at once, one with the smallest table and one with the largest: neither
+    thread's call takes the shared memory that the other's launch needs."""
+    lib, failed = nat.lib(), []
+
+    def worker(D, steps=2000):
+        n, d, H = 64, 32, 2
+        t = {name: torch.ones(1, H, n, d, device="cuda", dtype=dtype) for name in
+             ("q", "k", "v", "o", "d_o", "d_q", "d_k", "d_v")}
+        lse = torch.empty(1, H, n, device="cuda")
+        w, d_w = (torch.ones(H, 4, device="cuda", dtype=dtype) for _ in range(2))
+        lut = torch.zeros(2 * D + 1, dtype=torch.int32, device="cuda")
+        length = torch.tensor([n], dtype=torch.int32, device="cuda")
+        at = {name: nat.DfsStrided(ptr=x.data_ptr(), stride_b=H * n * d, stride_h=n * d, stride_n=d)
+              for name, x in t.items()}
+        bias = nat.DfsRelBias(weight=w.data_ptr(), lut=lut.data_ptr(), num_buckets=4, max_distance=D, dtype=code)
+        a = nat.DfsAttnArgs(**at, lse=lse.data_ptr(), bias=bias, d_weight=d_w.data_ptr())
+        p = nat.DfsAttnProblem(B=1, H=H, H_kv=H, n_q=n, n_k=n, d=d, dtype=code, causal=1, scale=0.2)
+        one = nat.DfsAttnProblem(B=1, H=H, H_kv=H, n_q=1, n_k=n, d=d, dtype=code, causal=1, scale=0.2)
+        size = lib.dfs_window_attn_bwd_work(p, bias)
+        work = torch.empty(size, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        stream = torch.cuda.Stream()
+        for _ in range(steps):
+            rc = (lib.dfs_window_attn_fwd(p, a, stream.cuda_stream),
+                  lib.dfs_window_attn_bwd(p, a, work.data_ptr(), size, stream.cuda_stream),
+                  lib.dfs_window_attn_decode(one, a, length.data_ptr(), stream.cuda_stream))
+            if any(rc):
+                failed.append((D, rc))
+                break
+        stream.synchronize()
+    threads = [threading.Thread(target=worker, args=(D,)) for D in (0, 1024)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
