@@ -200,8 +200,7 @@ extern "C" int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_arg
   return rc(launch_bucket_sums(P.dw_part, p->H, P.parts, P.D, P.lut, P.nb, P.wdtype, a->d_weight, st));
 }
 
-extern "C" int dfs_window_attn_decode(const dfs_attn_problem* p, const dfs_attn_args* a, const int32_t* lengths,
-                                      void* stream) {
+static int decode(const dfs_attn_problem* p, const dfs_attn_args* a, const void* lengths, bool wide, void* stream) {
   if (!a) return DFS_ERR_INVALID_ARGUMENT;
   const int s = problem_status(p, &a->bias);
   if (s != DFS_OK) return s;
@@ -212,6 +211,7 @@ extern "C" int dfs_window_attn_decode(const dfs_attn_problem* p, const dfs_attn_
   P.causal = 1;
   P.mask = nullptr;
   P.lengths = lengths;
+  P.wide_lengths = wide;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // cache tiles staged by TMA, 4-byte reads of q
   const bool rows = p->dtype != DFS_F32 && p->d % 8 == 0 && p->n_k > 0 && tmap_available() &&
@@ -219,4 +219,13 @@ extern "C" int dfs_window_attn_decode(const dfs_attn_problem* p, const dfs_attn_
                     staged(a->v, p->n_k, p->H_kv, p->B);
   if (rows) return rc(launch_decode_mma(P, p->dtype, st));
   return rc(launch_decode_any(P, p->dtype, vector_rows(p, a), st));
+}
+
+extern "C" int dfs_window_attn_decode(const dfs_attn_problem* p, const dfs_attn_args* a, const int32_t* lengths,
+                                      void* stream) {
+  return decode(p, a, lengths, false, stream);
+}
+extern "C" int dfs_window_attn_decode_i64(const dfs_attn_problem* p, const dfs_attn_args* a, const int64_t* lengths,
+                                          void* stream) {
+  return decode(p, a, lengths, true, stream);
 }

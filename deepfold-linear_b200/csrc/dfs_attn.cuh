@@ -27,7 +27,8 @@ struct AttnParams {
   int sink_tiles, far_segs, far_len;  // key tiles that hold sinks; segments of queries beyond the window, steps of each
   int near_segs;        // segments of every key tile's other steps
   int32_t* status;
-  const int32_t* lengths;  // decode: (B,)
+  const void* lengths;  // decode: (B,) int32, or int64 if wide_lengths
+  int wide_lengths;
   int nb, D, wdtype;
   int parts;            // rows of dw_part per head: key tiles (and far segments) of all batch elements
   int B, H, Hkv, G, nq, nk, d;
@@ -45,6 +46,13 @@ DFS_DEV void allow_next() { asm volatile("griddepcontrol.launch_dependents;" :::
 DFS_DEV bool key_near(int delta, int j, int causal, int window, int sinks) {
   if (causal ? delta < 0 : false) return false;
   return (delta < window && -delta < window) || j < sinks;
+}
+
+// Keys of sequence b's cache that hold a token, [0, n_k].
+DFS_DEV int seq_length(const AttnParams& P, int b) {
+  const int64_t n = P.wide_lengths ? static_cast<const int64_t*>(P.lengths)[b]
+                                   : static_cast<const int32_t*>(P.lengths)[b];
+  return static_cast<int>(min(max(n, int64_t{0}), static_cast<int64_t>(P.nk)));
 }
 
 // Keys [lo, hi) that positions p0..p1 may see through the window (sinks apart).

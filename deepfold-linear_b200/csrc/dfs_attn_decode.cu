@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kThreads) decode_mma_kernel(const __grid_const
   }
   allow_next();
   wait_previous();
-  const int len = min(max(P.lengths[b], 0), P.nk), p = len - 1;
+  const int len = seq_length(P, b), p = len - 1;
   const int lo = max(0, len - P.window), ns = min(P.sinks, lo);  // keys [0, ns) and [lo, len) are visible
   const int w0 = lo / kTcRows, sink_tiles = min((ns + kTcRows - 1) / kTcRows, w0);
   const int tiles = len > 0 ? sink_tiles + (len + kTcRows - 1) / kTcRows - w0 : 0;
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kAnyThreads, 4) decode_any_kernel(AttnParams P
   const int head = at % kAnyHeads, key = at / kAnyHeads;  // of the sum that ends in this lane
   allow_next();
   wait_previous();
-  const int len = min(max(P.lengths[b], 0), P.nk), p = len - 1;
+  const int len = seq_length(P, b), p = len - 1;
   const int lo = max(0, len - P.window), ns = min(P.sinks, lo), total = ns + len - lo;  // keys [0, ns), [lo, len)
   const int per = ((total + split - 1) / split + kAnyStep - 1) / kAnyStep * kAnyStep;
   const int x0 = static_cast<int>(min(static_cast<int64_t>(rank) * per, static_cast<int64_t>(total)));

@@ -274,12 +274,15 @@ Tensor window_attn_decode(Tensor q, Tensor K, Tensor V, Tensor lengths, optional
   require(lengths.is_cuda() && lengths.device() == q.device() && lengths.dim() == 1 && lengths.size(0) == q.size(0) &&
               (lengths.scalar_type() == at::kInt || lengths.scalar_type() == at::kLong),
           "lengths must be (B,) int32 or int64 on the operands' device");
-  const Tensor len = lengths.contiguous().to(at::kInt);
+  const Tensor len = lengths.contiguous();
   const DeviceSwitch guard(q.device());
   Tensor o = at::empty(q.sizes(), q.options());
   dfs_attn_args a = args_of(r, o, Tensor(), Tensor());
   a.status = checked_status(q.device());
-  check_rc(dfs_window_attn_decode(&r.p, &a, len.data_ptr<int32_t>(), stream_of(q)), "dfs_window_attn_decode");
+  check_rc(len.scalar_type() == at::kInt
+               ? dfs_window_attn_decode(&r.p, &a, len.data_ptr<int32_t>(), stream_of(q))
+               : dfs_window_attn_decode_i64(&r.p, &a, len.data_ptr<int64_t>(), stream_of(q)),
+           "dfs_window_attn_decode");
   return o;
 }
 

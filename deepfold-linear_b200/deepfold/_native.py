@@ -122,7 +122,7 @@ EXPORTED_SYMBOLS = ("dfs_abi_version", "dfs_status_string", "dfs_max_n", "dfs_wo
                     "dfs_dense_iterate", "dfs_dense_work_bytes", "dfs_dense_solve_bwd", "dfs_dense_solve_bwd_scratch",
                     "dfs_dense_transport_bwd", "dfs_relbias_fwd", "dfs_relbias_bwd", "dfs_relbias_bwd_work",
                     "dfs_window_attn_fwd", "dfs_window_attn_bwd", "dfs_window_attn_bwd_work",
-                    "dfs_window_attn_decode")
+                    "dfs_window_attn_decode", "dfs_window_attn_decode_i64")
 
 # phases of the streamed path for row-sharded runs (include/dfsink.h)
 DFS_OP_FWD_INIT, DFS_OP_FWD_ROWS, DFS_OP_FWD_COLS, DFS_OP_FWD_OUT = 0, 1, 2, 3
@@ -320,8 +320,9 @@ def lib() -> ctypes.CDLL:
             L.dfs_window_attn_bwd_work.argtypes = [_AP, _RB]
             L.dfs_window_attn_bwd.restype = ctypes.c_int
             L.dfs_window_attn_bwd.argtypes = [_AP, _AA, _P, ctypes.c_size_t, _P]
-            L.dfs_window_attn_decode.restype = ctypes.c_int
-            L.dfs_window_attn_decode.argtypes = [_AP, _AA, _P, _P]
+            for f in (L.dfs_window_attn_decode, L.dfs_window_attn_decode_i64):
+                f.restype = ctypes.c_int
+                f.argtypes = [_AP, _AA, _P, _P]
             L.dfs_selftest_mma.restype = ctypes.c_int
             L.dfs_selftest_mma.argtypes = [ctypes.c_int, _P, _P, _P, ctypes.c_int, ctypes.c_int,
                                            ctypes.c_int, _P]

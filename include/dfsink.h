@@ -478,6 +478,8 @@ int dfs_window_attn_bwd(const dfs_attn_problem* p, const dfs_attn_args* a, void*
  * Reads the cache rows of the sinks and the window only; causal, q_start, lse,
  * mask and the gradients are ignored. */
 int dfs_window_attn_decode(const dfs_attn_problem* p, const dfs_attn_args* a, const int32_t* lengths, void* stream);
+/* The same with 64-bit lengths, clamped as they are. */
+int dfs_window_attn_decode_i64(const dfs_attn_problem* p, const dfs_attn_args* a, const int64_t* lengths, void* stream);
 
 /* TEST-ONLY entry point, not part of the operator surface: runs one of the
  * three tcgen05 MMA operand layouts the kernels use on caller-provided data

@@ -183,3 +183,11 @@ def test_threads_with_tables_of_different_sizes(dtype, code):
     for t in threads:
         t.join()
     assert not failed
+
+
+def test_lengths_beyond_32_bits_are_clamped():
+    x = inputs(5, 2, 2, 1, 50, 16, F32, 83)
+    lengths = torch.tensor([2 ** 32 + 5, 2 ** 40, -2 ** 40, 2 ** 31, -2 ** 31 - 7], device="cuda")
+    got = window_attn_decode(x["q"][:, :, 0], x["k"], x["v"], lengths)
+    want = window_attn_decode(x["q"][:, :, 0], x["k"], x["v"], torch.tensor([50, 50, 0, 50, 0], device="cuda"))
+    assert torch.equal(got, want)

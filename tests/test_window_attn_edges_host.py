@@ -29,3 +29,13 @@ def test_a_table_first_used_in_inference_mode_serves_training():
         made = RelativeBuckets.clip(4, device="cpu").on(torch.device("cpu"))
     assert not first.is_inference() and not made.is_inference()
     assert b.on(torch.device("cpu")) is first and first.tolist() == list(b.table)
+
+
+def test_the_entry_for_64_bit_lengths_refuses_as_the_other_does():
+    lib, none = nat.lib(), nat.DfsAttnArgs()
+    p = nat.DfsAttnProblem(B=2, H=4, H_kv=2, n_q=1, n_k=8, d=32, dtype=nat.DFS_BF16, causal=1, scale=0.2)
+    for call in (lib.dfs_window_attn_decode, lib.dfs_window_attn_decode_i64):
+        assert call(p, none, None, None) == call(p, None, None, None) == nat.DFS_ERR_INVALID_ARGUMENT
+        p.B = 0
+        assert call(p, none, None, None) == nat.DFS_OK
+        p.B = 2
