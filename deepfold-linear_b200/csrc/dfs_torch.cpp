@@ -140,9 +140,8 @@ void check_device_status(const at::Device& dev) { g_seen.fetch_or(poll_device_st
 // For Python: the status bits of the current device (see poll_device_status)
 // together with the bits kept by the checks inside calls; all are cleared.
 int take_status(bool wait) {
-  const at::Device dev(at::kCUDA, c10::cuda::current_device());
-  const int v = poll_device_status(dev, wait);
-  return v | g_seen.exchange(0) | attn_take_status(dev);
+  const int v = poll_device_status(at::Device(at::kCUDA, c10::cuda::current_device()), wait);
+  return v | g_seen.exchange(0);
 }
 
 // DFS_TERM_* bits of the optional inputs a call passes (the streamed kernels

@@ -47,9 +47,7 @@ struct DeviceSwitch {
   DeviceSwitch& operator=(const DeviceSwitch&) = delete;
 };
 
-// dfs_torch_attn.cpp: the local attention's functions, and the device error
-// bits of its calls so far (cleared).
+// dfs_torch_attn.cpp: the local attention's functions.
 void bind_window_attn(pybind11::module_& m);
-int attn_take_status(const at::Device& dev);
 
 }  // namespace dfs_torch

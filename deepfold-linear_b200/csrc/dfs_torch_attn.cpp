@@ -5,7 +5,8 @@
 //
 // Device errors (a bounded wait that gave up) are written by the kernels
 // straight into one word of mapped host memory per device, so a call pays
-// nothing for them: the next call reads the word.
+// nothing for them: the next attention call (or its check_status) reads the
+// word, which the other operators' calls leave alone.
 #include <ATen/cuda/CUDAContext.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
@@ -340,14 +341,13 @@ Tensor relative_position_bias(Tensor w, Tensor lut, int64_t max_distance, int64_
   return relbias_forward(w, lut, max_distance, n_q, n_k, q_start);
 }
 
-}  // namespace
-
-int attn_take_status(const at::Device& dev) {
-  const int i = dev.index();
-  if (i < 0 || i >= kMaxDevices) return 0;
-  std::lock_guard<std::mutex> lock(g_mu);
-  return g_word[i] ? __atomic_exchange_n(g_word[i], 0, __ATOMIC_RELAXED) : 0;
+// For Python: raises for an error that an attention call on the current device left (wait: any made so far).
+void check_status(bool wait) {
+  require(!wait || cudaDeviceSynchronize() == cudaSuccess, "cudaDeviceSynchronize failed");
+  checked_status(at::Device(at::kCUDA, c10::cuda::current_device()));
 }
+
+}  // namespace
 
 void bind_window_attn(pybind11::module_& m) {
   m.def("window_attn", &window_attn, "sliding-window softmax attention with sinks and a bucketed position bias",
@@ -357,6 +357,11 @@ void bind_window_attn(pybind11::module_& m) {
   m.def("window_attn_decode", &window_attn_decode, "the same for one query per sequence over a cache", py::arg("q"),
         py::arg("K"), py::arg("V"), py::arg("lengths"), py::arg("weight"), py::arg("lut"), py::arg("max_distance"),
         py::arg("window"), py::arg("sinks"), py::arg("scale"));
+  m.def("window_attn_check_status", &check_status, "raise for a device error of an earlier window attention call",
+        py::arg("wait") = true);
+  m.def("window_attn_plant_status", [](int code) {
+    *status_word(at::Device(at::kCUDA, c10::cuda::current_device())) = code;
+  }, "TEST-ONLY: the status that a kernel of the current device would leave", py::arg("code"));
   m.def("relative_position_bias", &relative_position_bias, "(H, n_q, n_k) bias by distance buckets", py::arg("weight"),
         py::arg("lut"), py::arg("max_distance"), py::arg("n_q"), py::arg("n_k"), py::arg("q_start"));
 }

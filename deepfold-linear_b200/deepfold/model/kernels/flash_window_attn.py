@@ -22,6 +22,8 @@ Head dims 1 to 64; any strides with unit stride along d.  Head counts may differ
 (H a multiple of H_kv: shared key heads, whose gradients are summed over the
 group in a fixed order).  Results are bitwise reproducible.
 
+A device error raises from the next attention call, or from ``check_status``.
+
 CPU tensors are computed on the current CUDA device and the results returned on
 the CPU; without a CUDA device the calls raise (there is no CPU path).
 """
@@ -35,7 +37,15 @@ import torch
 from deepfold import _native as nat
 from deepfold.model.position_encoding import RelativeBuckets, check_buckets
 
-__all__ = ["flash_window_attn", "window_attn_decode"]
+__all__ = ["flash_window_attn", "window_attn_decode", "check_status"]
+
+
+def check_status(wait: bool = True) -> None:
+    """RuntimeError if an attention call made so far on the current device met a
+    device error (a bounded wait of a kernel that gave up); without ``wait`` only
+    if a call that has finished did.  The next attention call raises by itself;
+    this makes the check immediate."""
+    nat.ext().window_attn_check_status(bool(wait))
 
 
 def _gpu(t):

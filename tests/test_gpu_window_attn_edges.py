@@ -9,7 +9,8 @@ import torch
 from torch.autograd import forward_ad
 
 from deepfold import _native as nat
-from deepfold.model.kernels.flash_window_attn import flash_window_attn, window_attn_decode
+from deepfold.model.kernels.flash_window_attn import check_status, flash_window_attn, window_attn_decode
+from deepfold.model.kernels import sinkhorn_kernel
 from deepfold.model.position_encoding import RelativeBuckets, relative_position_bias
 
 from test_gpu_window_attn import BF16, BUCKETS, F16, F32, inputs
@@ -191,3 +192,20 @@ def test_lengths_beyond_32_bits_are_clamped():
     got = window_attn_decode(x["q"][:, :, 0], x["k"], x["v"], lengths)
     want = window_attn_decode(x["q"][:, :, 0], x["k"], x["v"], torch.tensor([50, 50, 0, 50, 0], device="cuda"))
     assert torch.equal(got, want)
+
+
+def test_a_device_error_is_reported_to_the_attention_that_met_it():
+    """Not by the Sinkhorn operators' check, which neither raises for it nor takes it away; and once."""
+    x = inputs(1, 2, 2, 20, 20, 16, F32, 89)
+    q, k, v = x["q"], x["k"], x["v"]
+    one = torch.tensor([20], device="cuda")
+    want = flash_window_attn(q, k, v)
+    torch.cuda.synchronize()
+    for call in (check_status, lambda: check_status(wait=False), lambda: flash_window_attn(q, k, v),
+                 lambda: window_attn_decode(q[:, :, 0], k, v, one)):
+        nat.ext().window_attn_plant_status(nat.DFS_ERR_DEVICE_TIMEOUT)
+        sinkhorn_kernel.check_status()
+        with pytest.raises(RuntimeError, match="previous window attention call"):
+            call()
+        check_status()
+        assert torch.equal(flash_window_attn(q, k, v), want)
