@@ -3,6 +3,7 @@
 #pragma once
 
 #include <atomic>
+#include <cfloat>
 
 #include "dfs_device.cuh"
 
@@ -90,13 +91,24 @@ DFS_DEV T* row_ptr(const Strided& s, int b, int h, int64_t n) {
   return reinterpret_cast<T*>(s.p) + b * s.sb + h * s.sh + n * s.sn;
 }
 
-// tab[delta + D] = weight[h, lut[delta + D]] * mul for the whole table (a block's threads).
-DFS_DEV void load_bias_table(float* tab, const void* w, const int32_t* lut, int D, int nb, int wdtype, int h,
-                             float mul, int tid, int nthreads) {
-  for (int x = tid; x < 2 * D + 1; x += nthreads) {
-    const int b = min(max(lut[x], 0), nb - 1);
-    tab[x] = load_as_f32<void>(w, static_cast<size_t>(h) * nb + b, wdtype) * mul;
-  }
+// A bias weight in log2 units, the finite ones within +-32000.  A type's lowest value, with which a table may hide
+// distances, would overflow to -inf here, and a row that sees such keys only would count as one that sees none; and
+// with -1e9 such a row's log-sum m + log2(l) would no longer hold log2(l), so that the backward's p were l times too
+// large.  At 32000 logits and log-sums keep steps of 2^-9, so those rows are right to 2^-10; beside any other key such a
+// key's p is 0 all the same.
+constexpr float kBiasLimit = 32000.0f;
+DFS_DEV float bias_log2(float w) {
+  const float x = w * kLog2e;
+  return fabsf(w) <= FLT_MAX ? fminf(fmaxf(x, -kBiasLimit), kBiasLimit) : x;  // infinities and NaN as they are
+}
+// Weight of head h's bucket b.
+DFS_DEV float bias_weight(const AttnParams& P, int h, int b) {
+  return bias_log2(load_as_f32<void>(P.w, static_cast<size_t>(h) * P.nb + min(max(b, 0), P.nb - 1), P.wdtype));
+}
+
+// tab[delta + D] = weight[h, lut[delta + D]] in log2 units for the whole table (a block's threads).
+DFS_DEV void load_bias_table(float* tab, const AttnParams& P, int h, int tid, int nthreads) {
+  for (int x = tid; x < 2 * P.D + 1; x += nthreads) tab[x] = bias_weight(P, h, P.lut[x]);
 }
 
 // Raises kernel K's limit of dynamic shared memory to `most`, what it needs with the largest bias table (D =

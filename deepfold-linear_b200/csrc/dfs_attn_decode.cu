@@ -149,10 +149,9 @@ __global__ void __launch_bounds__(kThreads) decode_mma_kernel(const __grid_const
   // the table where this run comes near the query (the copies are on their way)
   if (near_run && warp < 4)
     for (int x = tid; x <= P.D; x += 128) {
-      const int bk = min(max(P.lut[P.D + x], 0), P.nb - 1);
+      const int bk = P.lut[P.D + x];
 #pragma unroll 4
-      for (int r = 0; r < ng; ++r)
-        tab[r * (P.D + 1) + x] = load_as_f32<void>(P.w, static_cast<size_t>(h0 + r) * P.nb + bk, P.wdtype) * kLog2e;
+      for (int r = 0; r < ng; ++r) tab[r * (P.D + 1) + x] = bias_weight(P, h0 + r, bk);
     }
 
   // Q as the A operand: rows lane / 4 and + 8, columns 2 (lane % 4).. of each k step
@@ -169,11 +168,10 @@ __global__ void __launch_bounds__(kThreads) decode_mma_kernel(const __grid_const
   // the far bias of this thread's two heads; the table where this run comes near the query
   float far[2] = {0.0f, 0.0f};
   if (P.w) {
-    const int bk = min(max(P.lut[2 * P.D], 0), P.nb - 1);
+    const int bk = P.lut[2 * P.D];
 #pragma unroll
     for (int r = 0; r < 2; ++r)
-      if (g + 8 * r < ng)
-        far[r] = load_as_f32<void>(P.w, static_cast<size_t>(h0 + g + 8 * r) * P.nb + bk, P.wdtype) * kLog2e;
+      if (g + 8 * r < ng) far[r] = bias_weight(P, h0 + g + 8 * r, bk);
   }
   if (near_run && warp < 4) asm volatile("bar.sync 1, 128;" ::: "memory");
 
@@ -349,10 +347,7 @@ __global__ void __launch_bounds__(kAnyThreads, 4) decode_any_kernel(AttnParams P
   bool near_run = false;
   if (P.w) {
     near_run = x1 > x0 && p - key_at(x1 - 1) < P.D;
-    auto weight = [&](int r, int x) {
-      const int bk = min(max(P.lut[P.D + x], 0), P.nb - 1);
-      return load_as_f32<void>(P.w, static_cast<size_t>(h0 + r) * P.nb + bk, P.wdtype) * kLog2e;
-    };
+    auto weight = [&](int r, int x) { return bias_weight(P, h0 + r, P.lut[P.D + x]); };
     if (near_run)
       for (int x = tid; x < ng * (P.D + 1); x += kAnyThreads) tab[x] = weight(x / (P.D + 1), x % (P.D + 1));
     far = weight(min(head, ng - 1), P.D);

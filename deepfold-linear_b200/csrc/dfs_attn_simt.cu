@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kNT, 3) simt_fwd_kernel(AttnParams P) {
   const int i0 = (gridDim.x - 1 - blockIdx.x) * kT, dk = (P.d + 3) / 4 * 4;  // causal: longest first
   if (P.w) {
     tab = Pr + kTile;
-    load_bias_table(tab, P.w, P.lut, P.D, P.nb, P.wdtype, h, kLog2e, tid, kNT);
+    load_bias_table(tab, P, h, tid, kNT);
   }
   const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
   load_tile<E, kVec>(P.q, b, h, i0, P.nq, P.d, nullptr, Q, tid);
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kNT, 2) simt_dq_kernel(AttnParams P) {
   __shared__ float Drow[kT];
   const int h = blockIdx.y, b = blockIdx.z, hk = h / P.G, tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
   const int i0 = (gridDim.x - 1 - blockIdx.x) * kT, dk = (P.d + 3) / 4 * 4;  // causal: longest first
-  if (P.w) load_bias_table(tab, P.w, P.lut, P.D, P.nb, P.wdtype, h, kLog2e, tid, kNT);
+  if (P.w) load_bias_table(tab, P, h, tid, kNT);
   const uint8_t* mask = P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr;
   load_tile<E, kVec>(P.q, b, h, i0, P.nq, P.d, nullptr, Q, tid);
   load_tile<E, kVec>(P.d_o, b, h, i0, P.nq, P.d, nullptr, dO, tid);
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kNT, 2) simt_dkv_kernel(AttnParams P) {
     const int h = hk * P.G + g;
     if (P.w) {
       __syncthreads();
-      load_bias_table(tab, P.w, P.lut, P.D, P.nb, P.wdtype, h, kLog2e, tid, kNT);
+      load_bias_table(tab, P, h, tid, kNT);
     }
     if (dw)
       for (int x = tid; x < W; x += kNT) acc[x] = 0.0f;

@@ -201,11 +201,10 @@ DFS_DEV void load_bias_ext(float* tab, const AttnParams& P, int h, int tid, int 
       b[u] = P.lut[at];
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      v[u] = load_as_f32<void>(P.w, static_cast<size_t>(h) * P.nb + min(max(b[u], 0), P.nb - 1), P.wdtype);
+    for (int u = 0; u < 4; ++u) v[u] = bias_weight(P, h, b[u]);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (x0 + u * nthreads < W) tab[x0 + u * nthreads] = v[u] * kLog2e;
+      if (x0 + u * nthreads < W) tab[x0 + u * nthreads] = v[u];
   }
 }
 constexpr size_t ext_table_bytes(int D) { return (2 * (D + 255) + 1) * sizeof(float); }

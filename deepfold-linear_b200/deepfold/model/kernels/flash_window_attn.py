@@ -77,7 +77,8 @@ def flash_window_attn(Q, K, V, window: int | None = None, sinks: int = 0, causal
     """Softmax attention over a sliding window and the first ``sinks`` keys.
 
     Q (B,H,n_q,d), K and V (B,H_kv,n_k,d); unbatched inputs drop B.  pos_weight
-    (H, num_buckets) with ``buckets``: the learned bias.  mask (B,n_k) or (n_k,),
+    (H, num_buckets) with ``buckets``: the learned bias (-inf hides a bucket; finite
+    ones count up to 22180 either way, far beyond where a softmax tells them apart).  mask (B,n_k) or (n_k,),
     nonzero = real key.  q_start: position of query 0, default n_k - n_q (queries
     end where the keys end).  scale: default d ** -0.5.  Returns O like Q.
     """

@@ -4,6 +4,7 @@ unless a test derives its own."""
 
 import threading
 
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -12,8 +13,9 @@ from deepfold import _native as nat
 from deepfold.model.kernels.flash_window_attn import check_status, flash_window_attn, window_attn_decode
 from deepfold.model.kernels import sinkhorn_kernel
 from deepfold.model.position_encoding import RelativeBuckets, relative_position_bias
+from oracle import window_attn_oracle as orc
 
-from test_gpu_window_attn import BF16, BUCKETS, F16, F32, inputs
+from test_gpu_window_attn import BF16, BUCKETS, F16, F32, ROUND, f64, inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -209,3 +211,38 @@ def test_a_device_error_is_reported_to_the_attention_that_met_it():
             call()
         check_status()
         assert torch.equal(flash_window_attn(q, k, v), want)
+
+
+LOWEST = [(F32, -1e9), (F32, torch.finfo(F32).min), (F32, 1e9), (BF16, -1e9), (BF16, torch.finfo(BF16).min),
+          (F16, torch.finfo(F16).min)]
+
+
+@pytest.mark.parametrize("dtype,low", LOWEST)
+def test_rows_that_see_only_keys_of_one_very_large_bias(dtype, low):
+    """A bias that all of a row's keys have changes nothing, whatever its size.  Logits and log-sums are held in steps
+    of 2^-9 there: each p is off by 2^-10 of itself at most for either, beside the roundings of the type."""
+    x = inputs(1, 2, 1, 150, 150, 32, dtype, 97, nb=32)
+    x["w"][:] = low
+    kw = dict(pos_weight=x["w"], buckets=BUCKETS["log"], window=70)
+    leaves = [x[n].detach().requires_grad_() for n in ("q", "k", "v")]
+    o = flash_window_attn(*leaves, **kw)
+    got = (o, *torch.autograd.grad(o, leaves, x["d_o"]),
+           window_attn_decode(x["q"][:, :, -1], x["k"], x["v"], torch.tensor([150], device="cuda"), **kw))
+    want = orc.window_attn(f64(x["q"]), f64(x["k"]), f64(x["v"]), window=70, d_o=f64(x["d_o"]))[:4]
+    tol = 2 * 2.0 ** -10 + 2 * 3 * ROUND.get(dtype, 0.0) + 1e-5
+    for a, b in zip(got, (*want, want[0][:, :, -1])):
+        assert np.linalg.norm(f64(a) - b) <= tol * np.linalg.norm(b)
+
+
+@pytest.mark.parametrize("dtype,low", LOWEST)
+def test_a_very_low_bias_beside_others_hides(dtype, low):
+    x = inputs(1, 2, 1, 150, 150, 32, dtype, 101, nb=32)
+    x["w"][:, 9:] = -abs(low)   # a distance of 0 to 8 is seen by every query
+    grads = []
+    for w in (x["w"], torch.where(x["w"] == x["w"][0, 9], float("-inf"), x["w"])):
+        leaves = [x[n].detach().requires_grad_() for n in ("q", "k", "v")]
+        o = flash_window_attn(*leaves, pos_weight=w, buckets=BUCKETS["log"])
+        one = window_attn_decode(x["q"][:, :, -1], x["k"], x["v"], torch.tensor([150], device="cuda"), pos_weight=w,
+                                 buckets=BUCKETS["log"])
+        grads.append((o, one, *torch.autograd.grad(o, leaves, x["d_o"])))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
