@@ -142,12 +142,12 @@ DFS_DEV float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 DFS_DEV float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
 DFS_DEV float2 both(float x) { return make_float2(x, x); }
 
-// Wait for the phase with the given parity; false after some seconds (2^27 tries,
-// each of which sleeps for a while by itself).  No clock is read and the loop is
-// short, for warps wait much of the time.
+// Wait for the phase with the given parity; false after some seconds (2^20 tries,
+// each of which sleeps for 1.5 to 4 us by itself: measured).  No clock is read
+// and the loop is short, for warps wait much of the time.
 DFS_DEV bool tc_wait(uint64_t* bar, uint32_t parity) {
   const uint32_t addr = smem_u32(bar);
-  for (int tries = 1 << 27; tries > 0; --tries) {
+  for (int tries = 1 << 20; tries > 0; --tries) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"

@@ -25,7 +25,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libdfsink.so")
 SOURCES = ["dfs_abi.cu", "dfs_fwd.cu", "dfs_bwd.cu", "dfs_stream.cu", "dfs_stream_bwd.cu", "dfs_stream_tma.cu",
            "dfs_stream_bwd_tma.cu", "dfs_selftest.cu", "dfs_noalloc.cu", "dfs_pad.cu", "dfs_dense.cu",
            "dfs_dense_grad.cu", "dfs_peer.cu", "dfs_relbias.cu", "dfs_attn_simt.cu", "dfs_attn_tc.cu",
-           "dfs_attn_tc_bwd.cu", "dfs_attn_decode.cu", "dfs_attn.cu"]
+           "dfs_attn_tc_bwd.cu", "dfs_attn_decode.cu", "dfs_attn.cu", "dfs_attn_selftest.cu"]
 HEADERS = ["dfs_device.cuh", "dfs_kernels.cuh", "dfs_slab.cuh", "dfs_tma.cuh", "dfs_attn.cuh", "dfs_attn_tc.cuh"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
@@ -116,7 +116,7 @@ class DfsPeerSet(ctypes.Structure):
 
 
 EXPORTED_SYMBOLS = ("dfs_abi_version", "dfs_status_string", "dfs_max_n", "dfs_workspace_size",
-                    "dfs_fwd", "dfs_bwd", "dfs_selftest_mma", "dfs_fwd_static", "dfs_stream_op",
+                    "dfs_fwd", "dfs_bwd", "dfs_selftest_mma", "dfs_selftest_wait", "dfs_fwd_static", "dfs_stream_op",
                     "dfs_peer_alloc", "dfs_peer_open", "dfs_peer_close", "dfs_peer_free", "dfs_stream_op_peer",
                     "dfs_compute_bins", "dfs_peer_gather_rows", "dfs_stream_cg_loop_peer",
                     "dfs_dense_iterate", "dfs_dense_work_bytes", "dfs_dense_solve_bwd", "dfs_dense_solve_bwd_scratch",
@@ -323,6 +323,8 @@ def lib() -> ctypes.CDLL:
             for f in (L.dfs_window_attn_decode, L.dfs_window_attn_decode_i64):
                 f.restype = ctypes.c_int
                 f.argtypes = [_AP, _AA, _P, _P]
+            L.dfs_selftest_wait.restype = ctypes.c_int
+            L.dfs_selftest_wait.argtypes = [_I, _P, _P]
             L.dfs_selftest_mma.restype = ctypes.c_int
             L.dfs_selftest_mma.argtypes = [ctypes.c_int, _P, _P, _P, ctypes.c_int, ctypes.c_int,
                                            ctypes.c_int, _P]

@@ -488,6 +488,10 @@ int dfs_window_attn_decode_i64(const dfs_attn_problem* p, const dfs_attn_args* a
 int dfs_selftest_mma(int which, const float* A, const float* B, float* D,
                      int M, int N, int K, void* stream);
 
+/* TEST-ONLY: the attention kernels' bounded waits where they run out, in one block.  which 0: a wait for a phase
+ * that nothing completes, which stores DFS_ERR_DEVICE_TIMEOUT to `status` and returns. */
+int dfs_selftest_wait(int which, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,6 +3,7 @@ not finite or very large, derivatives that it does not have, other threads.  Tol
 unless a test derives its own."""
 
 import threading
+import time
 
 import numpy as np
 import pytest
@@ -246,3 +247,19 @@ def test_a_very_low_bias_beside_others_hides(dtype, low):
                                  buckets=BUCKETS["log"])
         grads.append((o, one, *torch.autograd.grad(o, leaves, x["d_o"])))
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def run_out(which):
+    """(seconds, status) of a block whose wait cannot succeed."""
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    start = time.monotonic()
+    nat.check(nat.lib().dfs_selftest_wait(which, status.data_ptr(), nat.stream_ptr(status.device)), "dfs_selftest_wait")
+    torch.cuda.synchronize()
+    return time.monotonic() - start, int(status.item())
+
+
+def test_a_wait_that_runs_out_ends_in_seconds():
+    seconds, status = run_out(0)
+    assert status == nat.DFS_ERR_DEVICE_TIMEOUT
+    assert 1.0 < seconds < 10.0  # far above any wait of a kernel that works; bounded all the same

@@ -39,3 +39,8 @@ def test_the_entry_for_64_bit_lengths_refuses_as_the_other_does():
         p.B = 0
         assert call(p, none, None, None) == nat.DFS_OK
         p.B = 2
+
+
+def test_the_wait_check_refuses_what_it_does_not_know():
+    for which, status in ((-1, 16), (9, 16), (0, None)):
+        assert nat.lib().dfs_selftest_wait(which, status, None) == nat.DFS_ERR_INVALID_ARGUMENT
