@@ -66,6 +66,19 @@ struct BwdShared {
 
 DFS_DEV void work_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
+// Barriers of a key-pass element warp up to a head's first tile, as the `entered`-th of its unit: two a head for the
+// tables, and with sums by distance two for the flush of each head before it.
+__host__ __device__ constexpr int barriers_before(int entered, bool dw) {
+  return entered == 0 ? 0 : 2 * entered + (dw ? 2 * (entered - 1) : 0);
+}
+// Those that are left, the last head's flush among them, for a unit of `heads`
+__host__ __device__ constexpr int barriers_left(int heads, int entered, bool dw) {
+  return barriers_before(heads, dw) + (dw && heads > 0 ? 2 : 0) - barriers_before(entered, dw);
+}
+static_assert(barriers_left(0, 0, true) == 0 && barriers_left(3, 0, true) == 12 && barriers_left(3, 3, true) == 2 &&
+                  barriers_left(3, 1, false) == 4 && barriers_left(3, 3, false) == 0,
+              "as the key pass's loop has them");
+
 template <bool BF16>
 struct E16 {
   using T = __half;
@@ -683,7 +696,15 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
       if (lane != 15) add(lane < 15 ? lane : 46 - lane, done);
       add(62 - lane, run);
     }
-    if (dw) {
+    if (err) {
+      // A wait of this warp gave up, where the others' may not have: it takes part in the barriers that are left, the
+      // same number for every warp, so that nobody waits for it for good.
+      uint32_t bits[4];
+      key_bits(P.mask ? P.mask + static_cast<size_t>(b) * P.nk : nullptr, j0, P.nk, lane, bits);
+      const int g0 = per > 0 ? first / per : 0;
+      const int heads = (bits[0] | bits[1] | bits[2] | bits[3]) != 0 && last > first ? (last - 1) / per - g0 + 1 : 0;
+      for (int n = barriers_left(heads, head < 0 ? 0 : head - g0 + 1, dw); n > 0; --n) work_barrier();
+    } else if (dw) {
       if (head >= 0) flush();
       zero_heads(head + 1, P.G);
     }
