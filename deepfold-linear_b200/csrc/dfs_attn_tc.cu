@@ -41,9 +41,10 @@ constexpr float kNone = 1e-30f;
 
 struct FwdShared {
   uint64_t q_full, full[kStages], empty[kStages];
-  uint64_t s_full, p_ready, o_done;
+  uint64_t s_full, p_ready, o_done, products;
   TileInfo info[kInfo];
   uint32_t tmem;
+  int uses;  // of the ring of stages
 };
 
 // TMEM columns (128 allocated): S, and P over its first half; O
@@ -141,6 +142,7 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
         mbar_init(&S.s_full, 1);
         mbar_init(&S.p_ready, 4);
         mbar_init(&S.o_done, 1);
+        mbar_init(&S.products, 1);
         fence_mbar_init();
       }
       __syncwarp();
@@ -174,6 +176,7 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
         if (lane == 0) mbar_arrive(&S.full[s]);
         ++t;
       }
+      if (lane == 0) S.uses = t;
     } else if (warp == kMmaWarp) {  // ---- MMA
       tmem_alloc(&S.tmem, 128);
       allow_next();
@@ -407,10 +410,7 @@ __global__ void __launch_bounds__(kFwdThreads, 4) tc_fwd_kernel(const __grid_con
     if (!kSplit && P.lse && i < P.nq)
       P.lse[(static_cast<size_t>(b) * P.H + h) * P.nq + i] = none ? INFINITY : m + lg2(total);
   }
-  if (err) report_timeout(P.status);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  end_block<kStages>(err, P.status, warp == kTmaWarp, warp == kMmaWarp, &S.q_full, S.full, S.uses, &S.products);
   if (warp == kMmaWarp) tmem_dealloc(S.tmem, 128);
 }
 

@@ -167,17 +167,43 @@ DFS_DEV void warp_arrive(uint64_t* bar, int lane) {
   if (lane == 0) mbar_arrive(bar);
 }
 
+// A wait that gave up: tell the host (status may be mapped host memory: a plain store)
+DFS_DEV void report_timeout(int32_t* status) {
+  if (status != nullptr) *reinterpret_cast<volatile int32_t*>(status) = DFS_ERR_DEVICE_TIMEOUT;
+}
+
+// A block that some wait of its warps made give up must not end before what it has started, for its shared memory and
+// TMEM go to the next one: copies into the last stages of a ring of kStages (uses 0 .. n - 1 of it) ...
+template <int kStages>
+DFS_DEV void land_copies(uint64_t* full, int n) {
+  for (int u = max(0, n - kStages); u < n; ++u) tc_wait(&full[u % kStages], (u / kStages) & 1);
+}
+// ... and the products that this warp's elected lane has issued.  (Where none gave up, somebody waited for all of them.)
+DFS_DEV void end_products(uint64_t* bar) {
+  if (elect_one()) mma_commit(bar);
+  __syncwarp();
+  tc_wait(bar, 0);
+}
+// The end of a block: err: a wait of this thread gave up; `uses` of the ring, written by the TMA warp.
+template <int kStages>
+DFS_DEV void end_block(bool err, int32_t* status, bool tma, bool mma, uint64_t* own, uint64_t* full, const int& uses,
+                       uint64_t* products) {
+  tc_fence_before();
+  if (__syncthreads_or(err)) {
+    if (err) report_timeout(status);
+    if (tma) tc_wait(own, 0), land_copies<kStages>(full, uses);
+    if (mma) end_products(products);
+    __syncthreads();
+  }
+  tc_fence_after();
+}
+
 // Registers of this warpgroup (four warps) from here on.  The shares of a block
 // must not add up to more than it was launched with.
 template <int N>
 DFS_DEV void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 DFS_DEV void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
-// A wait that gave up: tell the host (status may be mapped host memory: a plain store)
-DFS_DEV void report_timeout(int32_t* status) {
-  if (status != nullptr) *reinterpret_cast<volatile int32_t*>(status) = DFS_ERR_DEVICE_TIMEOUT;
-}
 
 // Bits c of [0, 128) with a <= c < b, as four words
 DFS_DEV uint32_t range_word(int a, int b, int w) {

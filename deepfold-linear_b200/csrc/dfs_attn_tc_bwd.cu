@@ -55,13 +55,14 @@ constexpr uint32_t kColDS = 192;              // dQ pass
 
 struct BwdShared {
   uint64_t own_full, full[kStages], empty[kStages];
-  uint64_t s_full, s_free, ds_ready, acc_done;
+  uint64_t s_full, s_free, ds_ready, acc_done, products;
   TileInfo info[kInfo];
   alignas(16) float stat[kStages][2][kTcHalf];  // dK/dV pass: -lse and -D of the stage's queries
   float part[2][kTcRows];           // dQ pass: a row's two partial sums
   float ends[2][kWork / 32];
   float diag[kWork / 32][32];       // dK/dV pass: diagonals of a warp's block that ended at lane 31
   uint32_t tmem;
+  int uses;  // of the ring of stages
 };
 
 DFS_DEV void work_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -134,6 +135,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
         mbar_init(&S.s_free, kWork / 32);
         mbar_init(&S.ds_ready, kWork / 32);
         mbar_init(&S.acc_done, 1);
+        mbar_init(&S.products, 1);
         fence_mbar_init();
       }
       __syncwarp();
@@ -167,6 +169,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
         if (lane == 0) mbar_arrive(&S.full[s]);
         ++t;
       }
+      if (lane == 0) S.uses = t;
     } else if (warp == kMmaWarp) {  // ---- MMA
       tmem_alloc(&S.tmem, 256);
       allow_next();
@@ -358,10 +361,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dq_kernel(const __grid_cons
     if (cg == 0 && i < P.nq)
       P.dsum[stat] = D + (S.part[0][row] + S.part[1][row]);
   }
-  if (err) report_timeout(P.status);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  end_block<kStages>(err, P.status, warp == kTmaWarp, warp == kMmaWarp, &S.own_full, S.full, S.uses, &S.products);
   if (warp == kMmaWarp) tmem_dealloc(S.tmem, 256);
 }
 
@@ -418,6 +418,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
         mbar_init(&S.s_full, 1);
         mbar_init(&S.ds_ready, kWork / 32);
         mbar_init(&S.acc_done, 1);
+        mbar_init(&S.products, 1);
         fence_mbar_init();
       }
       __syncwarp();
@@ -445,7 +446,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
         }
       };
       if (total > 0) load_stats(g, it);
-      for (int t = 0; t <= total; ++t) {
+      int t = 0;
+      for (; t <= total; ++t) {
         const int s = t % kStages, i0 = t < total ? (i_lo + it) * kTcHalf : -1, now = g;
         if (!tc_wait(&S.empty[s], ((t / kStages) & 1) ^ 1)) { err = true; break; }
         if (i0 >= 0) {
@@ -464,6 +466,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
         describe_tile(P, plain, S.info[t % kInfo], i0, now, i0 + P.qs, j0, whole, bits, lane);
         if (lane == 0) mbar_arrive(&S.full[s]);
       }
+      if (lane == 0) S.uses = t;
     } else if (warp == kMmaWarp) {  // ---- MMA
       tmem_alloc(&S.tmem, 256);
       allow_next();
@@ -747,10 +750,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) tc_dkv_kernel(const __grid_con
       }
     }
   }
-  if (err) report_timeout(P.status);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  end_block<kStages>(err, P.status, warp == kTmaWarp, warp == kMmaWarp, &S.own_full, S.full, S.uses, &S.products);
   if (warp == kMmaWarp) tmem_dealloc(S.tmem, 256);
 }
 

@@ -489,7 +489,8 @@ int dfs_selftest_mma(int which, const float* A, const float* B, float* D,
                      int M, int N, int K, void* stream);
 
 /* TEST-ONLY: the attention kernels' bounded waits where they run out, in one block.  which 0: a wait for a phase
- * that nothing completes, which stores DFS_ERR_DEVICE_TIMEOUT to `status` and returns. */
+ * that nothing completes, which stores DFS_ERR_DEVICE_TIMEOUT to `status` and returns; 1: copies on their way when a
+ * block gives up, where `status` counts the 16-byte pieces of them that have not landed at its end. */
 int dfs_selftest_wait(int which, int32_t* status, void* stream);
 
 #ifdef __cplusplus

@@ -263,3 +263,7 @@ def test_a_wait_that_runs_out_ends_in_seconds():
     seconds, status = run_out(0)
     assert status == nat.DFS_ERR_DEVICE_TIMEOUT
     assert 1.0 < seconds < 10.0  # far above any wait of a kernel that works; bounded all the same
+
+
+def test_copies_land_before_a_block_that_gave_up_ends():
+    assert run_out(1)[1] == 0
