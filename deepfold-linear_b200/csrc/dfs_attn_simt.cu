@@ -17,8 +17,6 @@
 // 25 TFLOP/s of 74; with both gradients 7.1 ms.  (Transposed copies in shared
 // memory and 4 x 4 pairs a thread: 2.1 and 11.3 ms.)  A third of the instructions
 // are not products, and 12 warps an SM leave half of the issue slots empty.
-#include <climits>
-
 #include "dfs_attn.cuh"
 
 namespace dfs {
@@ -136,7 +134,8 @@ DFS_DEV int plain_side(const AttnParams& P, int p0, int j0, bool rows) {
   return P.w == nullptr || lo >= P.D ? 1 : hi <= -P.D ? -1 : 0;
 }
 
-// Key tiles of 64 seen by positions p0..p1: the sink tiles [0, ns), then the window's [t0, t1).
+// Key tiles of 64 seen by positions p0..p1: the sink tiles [0, ns), then the window's [t0, t1), which go on to the last
+// sink where the sinks reach into them or (without causality) past them.
 struct KeyTiles {
   int ns, t0, t1;
   DFS_DEV KeyTiles(const AttnParams& P, int p0, int p1) {
@@ -144,7 +143,8 @@ struct KeyTiles {
     near_keys(P, p0, p1, lo, hi);
     t0 = lo / kT;
     t1 = hi > lo ? (hi + kT - 1) / kT : t0;
-    ns = min((sink_keys(P, p1) + kT - 1) / kT, hi > lo ? t0 : INT_MAX);
+    ns = (sink_keys(P, p1) + kT - 1) / kT;
+    if (hi > lo && ns > t0) t1 = max(t1, ns), ns = t0;
   }
   DFS_DEV int count() const { return ns + (t1 - t0); }
   DFS_DEV int operator[](int x) const { return x < ns ? x : t0 + (x - ns); }

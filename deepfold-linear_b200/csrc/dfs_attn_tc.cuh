@@ -262,7 +262,8 @@ DFS_DEV void key_bits(const uint8_t* mask, int j0, int nk, int lane, uint32_t (&
   for (int w = 0; w < 4; ++w) bits[w] = __reduce_or_sync(0xffffffffu, (lane >> 3) == w ? part : 0u);
 }
 
-// Key tiles of kRows seen by positions p0..p1: the sink tiles [0, ns), then the window's [t0, t1).
+// Key tiles of kRows seen by positions p0..p1: the sink tiles [0, ns), then the window's [t0, t1), which go on to the
+// last sink where the sinks reach into them or (without causality) past them.
 template <int kRows>
 struct TcKeyTiles {
   int ns, t0, t1;
@@ -272,7 +273,7 @@ struct TcKeyTiles {
     t0 = lo / kRows;
     t1 = hi > lo ? (hi + kRows - 1) / kRows : t0;
     ns = (sink_keys(P, p1) + kRows - 1) / kRows;
-    if (hi > lo) ns = min(ns, t0);
+    if (hi > lo && ns > t0) t1 = max(t1, ns), ns = t0;
   }
   DFS_DEV int count() const { return ns + (t1 - t0); }
   DFS_DEV int operator[](int x) const { return x < ns ? x : t0 + (x - ns); }

@@ -16,7 +16,7 @@ from deepfold.model.kernels import sinkhorn_kernel
 from deepfold.model.position_encoding import RelativeBuckets, relative_position_bias
 from oracle import window_attn_oracle as orc
 
-from test_gpu_window_attn import BF16, BUCKETS, F16, F32, ROUND, f64, inputs
+from test_gpu_window_attn import BF16, BUCKETS, F16, F32, ROUND, check, f64, inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -267,3 +267,16 @@ def test_a_wait_that_runs_out_ends_in_seconds():
 
 def test_copies_land_before_a_block_that_gave_up_ends():
     assert run_out(1)[1] == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("window,sinks,n_q,n_k,q_start", [
+    (10, 148, 339, 339, None),    # the first queries' windows end tiles before the last sink
+    (3, 700, 130, 900, 200),
+    (1, 300, 70, 300, -5),
+    (20, 64, 40, 400, -30),       # some queries stand before the first key
+])
+def test_sinks_ahead_of_the_window(window, sinks, n_q, n_k, q_start, dtype):
+    """Without causality a query also sees the sinks that lie beyond its window's end."""
+    x = inputs(2, 4, 2, n_q, n_k, 32, dtype, 103, nb=32)
+    check(x, dtype, BUCKETS["log2"], causal=False, window=window, sinks=sinks, q_start=q_start)
