@@ -13,7 +13,7 @@
 // without a second launch.
 //
 // Measured: 12 sequences of 32 / 8 heads over up to 32768 keys (float16, d = 64)
-// 111 us, 5.8 TB/s; 64 ragged sequences of 16 / 4 heads, window 4096, 46 us, 4.3
+// 111 us, 5.8 TB/s; 64 ragged sequences of 16 / 4 heads, window 4096, 47 us, 4.3
 // TB/s (a run of eight tiles hardly fills the ring before it drains); one sequence,
 // window 1024, 8 us, of which the launch is most.  (Copies by the threads
 // themselves, 16 bytes each, cost 440 instructions a warp per 64 keys and held the

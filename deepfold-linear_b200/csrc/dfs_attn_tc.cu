@@ -14,8 +14,8 @@
 // four CTAs share an SM.  Measured (bfloat16, d = 64): 8192 tokens of 16 / 4 heads,
 // window 4096, 155 us, 660 TFLOP/s, an exponential pipe 60 % busy; 8 x 1024 of 16
 // heads, window 256 in both directions, 32 us.  While all SMs have four CTAs a tile
-// takes 560 clocks of each; the rest is the last wave, whose rows are of unequal
-// length.  Slower at the same sizes: 128-key tiles with 256 or 512 threads, two S
+// takes 560 clocks of each: 76 us of the 155 for the first wave, and 44 for the longest
+// row of the second, alone.  Where the other 35 go has not been measured.  Slower at the same sizes: 128-key tiles with 256 or 512 threads, two S
 // buffers and two CTAs an SM (155 to 170 us), part of the exponentials as a
 // polynomial on the FMA pipes, and every row shared by two CTAs (157 us).
 #include <algorithm>

@@ -8,7 +8,7 @@ Mirrors the reference package layout for that path, with local attention beside 
 * ``deepfold.model.kernels.flash_window_attn.flash_window_attn`` /
   ``window_attn_decode`` and ``deepfold.model.position_encoding.
   relative_position_bias`` -- local softmax attention and its position bias
-  (no counterpart in the reference)
+  (new here: not drop-ins for the reference's softmax attention)
 * ``deepfold.utils.cg.conjugate_gradient`` / ``steihaug_cg``
 * ``deepfold.sharding`` -- multi-GPU (batch, head) and row sharding
 

@@ -6,8 +6,9 @@ visible (sinks), and a learned relative position bias by buckets.
 * ``window_attn_decode``: the same attention for the newest token of each
   sequence over a cache.
 
-Both have no counterpart in the reference, whose trunk runs dense softmax
-attention beside the Sinkhorn transport.  With delta = i + q_start - j, a key j
+Neither is a drop-in for the reference's own softmax attention
+(src/deepfold/model/kernels/flash_diffusion_attn.py, with its 68-bin bias;
+flash_atom_attn.py, over a local window).  With delta = i + q_start - j, a key j
 is visible to a query i when its ``mask`` entry is nonzero, it is not in the
 future (``causal``: delta >= 0), and it is near (0 <= delta < window; without
 ``causal`` |delta| < window) or one of the first ``sinks`` keys.  A query that
@@ -16,13 +17,17 @@ never used, whatever they hold (padding may be NaN); keys hidden by the window
 or by causality must be finite, as any real token's are.
 
 Types: bfloat16 and float16 (tensor-core products, softmax statistics and all
-sums in fp32, the probabilities rounded to the operands' type for the product
-with V, as the operands themselves are) and float32 (fp32 products throughout).
+sums in fp32; the probabilities and, in the backward, the logits' gradients are
+rounded to the operands' type for the products that they enter, so an output is
+about 1.3 and a gradient 1.5 times as far off as the exact one rounded once) and
+float32 (fp32 products throughout).  With float16, upstream gradients much below
+1e-4 meet the type's smallest values in those products: scale the loss.
 Head dims 1 to 64; any strides with unit stride along d.  Head counts may differ
 (H a multiple of H_kv: shared key heads, whose gradients are summed over the
 group in a fixed order).  Results are bitwise reproducible.
 
-A device error raises from the next attention call, or from ``check_status``.
+The gradients are first ones in reverse mode: a second differentiation and
+forward-mode derivatives raise.  A device error raises from the next attention call, or from ``check_status``.
 
 CPU tensors are computed on the current CUDA device and the results returned on
 the CPU; without a CUDA device the calls raise (there is no CPU path).

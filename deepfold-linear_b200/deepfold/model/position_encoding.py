@@ -1,11 +1,11 @@
 """Position encodings on the GPU: the 68-bin position / bond code, and a learned
 relative position bias by buckets.
 
-``relative_position_bias`` (no counterpart in the reference) gives the dense
-bias ``pos_weight[h, bucket(i + q_start - j)]`` and its gradient, e.g. to add to
-the cost of ``sinkhorn_solve``; ``flash_window_attn`` takes the same weights and
-buckets and never builds the matrix.  ``RelativeBuckets`` holds the bucket of
-every distance.
+``relative_position_bias`` (not in the reference, whose kernels look their 68
+bins up themselves) gives the dense bias ``pos_weight[h, bucket(i + q_start - j)]``
+and its gradient, e.g. to add to the cost of ``sinkhorn_solve``;
+``flash_window_attn`` takes the same weights and buckets and never builds the
+matrix.  ``RelativeBuckets`` holds the bucket of every distance.
 
 ``compute_bins``: drop-in for ``deepfold.model.position_encoding.compute_bins`` of the reference
 (src/deepfold/model/position_encoding.py:7-52): same arguments, same (N, N) or

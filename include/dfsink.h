@@ -411,7 +411,8 @@ int dfs_stream_cg_loop_peer(const dfs_problem* p, const dfs_cg_params* cg, const
  * A query i stands at position p = i + q_start, a key j at position j; delta =
  * p - j.  The bias of a pair is weight[h, lut[clamp(delta, -D, D) + D]] with D =
  * max_distance: `lut` holds the bucket of every distance, the ends stand for all
- * distances beyond them.
+ * distances beyond them.  In the attention a weight of -inf hides its pairs, and
+ * finite ones count up to 22180 either way.
  * --------------------------------------------------------------------------- */
 #define DFS_MAX_BUCKET_DISTANCE 1024
 typedef struct {
